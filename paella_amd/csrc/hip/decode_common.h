@@ -1,0 +1,130 @@
+#pragma once
+// What the operators of a decoding step share: element types, 16-byte loads, write-through stores, page lookups.
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "paella_decode.h"
+#include "paella_ops.h"
+#include <llis/job/finished_block_notifier.h>
+
+#include "launch.h"
+#include "out_store.h"
+
+namespace paella {
+
+using Notifier = llis::job::FinishedBlockNotifier;
+
+struct F32 { static constexpr int bytes = 4; };
+struct Bf16 { static constexpr int bytes = 2; };
+struct F16 { static constexpr int bytes = 2; };
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// By value: a bit cast of a vector's element in place reads element 0.
+__device__ __forceinline__ float as_float(unsigned w) { return __builtin_bit_cast(float, w); }
+__device__ __forceinline__ unsigned as_word(float f) { return __builtin_bit_cast(unsigned, f); }
+
+// Two neighbouring 16-bit values of a word, and back (one rounding, to nearest even).
+template <typename T> __device__ __forceinline__ f32x2 unpack2(unsigned w);
+template <> __device__ __forceinline__ f32x2 unpack2<Bf16>(unsigned w) {
+    return f32x2{as_float(w << 16), as_float(w & 0xFFFF0000u)};
+}
+template <> __device__ __forceinline__ f32x2 unpack2<F16>(unsigned w) { return __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2); }
+
+template <typename T> __device__ __forceinline__ unsigned pack2(float a, float b);
+template <> __device__ __forceinline__ unsigned pack2<Bf16>(float a, float b) {
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+template <> __device__ __forceinline__ unsigned pack2<F16>(float a, float b) {
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, f16x2));
+}
+
+__device__ __forceinline__ float wave_sum_f(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+__device__ __forceinline__ float wave_max_f(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+    return v;
+}
+
+// A descriptor over everything behind `base` (uniform over the wave); offsets are 32-bit, sc1 = 16 writes through / reads past this XCD's caches.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(const void* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0xFFFFFFFFu, 0x00027000);
+}
+constexpr int kThrough = 16;
+
+// The sequence of row t and its index j among the sequence's new tokens, found by every wave for itself with one load per 64 sequences;
+// false for rows that belong to none.  t is uniform over the wave.
+__device__ __forceinline__ bool row_owner(const int* __restrict__ starts, int sequences, int max_new, int t, int lane, int* seq, int* j) {
+    if (!starts) {
+        *seq = t / max_new;
+        *j = t - *seq * max_new;
+        return *seq < sequences;
+    }
+    int b = 0;
+    for (int at = 0; at < sequences; at += 64) {
+        const int i = at + lane;
+        const unsigned long long begun = __ballot(i < sequences && starts[i + 1] <= t);
+        b += __popcll(begun);
+        if (begun != ~0ull) break;
+    }
+    *seq = b;
+    if (b >= sequences) return false;
+    *j = t - starts[b];
+    return *j >= 0 && *j < max_new;
+}
+
+// Host side: what every entry point asks of a cache and a batch.  `tables`: the batch's device pointers are needed too.
+inline int element_bytes(int dtype) { return dtype == PAELLA_F32 ? 4 : 2; }
+
+inline bool cache_extents_ok(const paella_kv_cache* c) {
+    if (!c || c->dtype < PAELLA_F32 || c->dtype > PAELLA_F16 || c->num_pages <= 0 || c->kv_heads <= 0 || c->page_size <= 0 || c->head_dim <= 0) return false;
+    if (c->page_size % 8 || c->head_dim % 8 || c->head_dim > 512) return false;
+    return (double)c->kv_heads * c->page_size * c->head_dim * element_bytes(c->dtype) < 2147483648.0;
+}
+inline bool cache_ok(const paella_kv_cache* c) { return cache_extents_ok(c) && c->k && c->v && (((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0; }
+
+inline bool batch_extents_ok(const paella_kv_batch* b) {
+    if (!b || b->sequences <= 0 || b->max_new <= 0 || b->tokens <= 0 || b->max_pages <= 0 || b->prefix_len < 0) return false;
+    // rows and positions are 32-bit numbers
+    return (double)b->sequences * b->max_new < 2147483648.0 && (double)b->sequences * b->max_pages < 2147483648.0 && b->prefix_len < (1 << 30);
+}
+inline bool batch_ok(const paella_kv_batch* b) {
+    if (!batch_extents_ok(b) || !b->past || !b->tables) return false;
+    return b->starts != nullptr || (double)b->sequences * b->max_new == (double)b->tokens;
+}
+
+inline bool overlap(const void* a, double a_bytes, const void* b, double b_bytes) {
+    const double x = (double)(uintptr_t)a, y = (double)(uintptr_t)b;
+    return x < y + b_bytes && y < x + a_bytes;
+}
+
+inline void set_launch_dims(paella_launch_dims* d, unsigned grid, unsigned block, unsigned lds, unsigned vgprs) {
+    d->grid = grid;
+    d->block = block;
+    d->lds_bytes = lds;
+    d->vgprs = vgprs;
+}
+
+// Register count and static LDS of the kernel that a launch takes, where there is a device to ask; *dims is left as planned elsewhere.
+inline void loaded_dims(const void* kernel, paella_launch_dims* dims) {
+    hipFuncAttributes attr;
+    if (hipFuncGetAttributes(&attr, kernel) != hipSuccess) {
+        (void)hipGetLastError();
+        return;
+    }
+    dims->vgprs = (unsigned)attr.numRegs;
+    dims->lds_bytes += (unsigned)attr.sharedSizeBytes;
+}
+
+}  // namespace paella

@@ -27,6 +27,14 @@ extern const char paella_hsaco_conv_begin[];
 extern const char paella_hsaco_conv_end[];
 extern const char paella_hsaco_misc_begin[];
 extern const char paella_hsaco_misc_end[];
+extern const char paella_hsaco_decode_begin[];
+extern const char paella_hsaco_decode_end[];
+extern const char paella_hsaco_attention_f32_begin[];
+extern const char paella_hsaco_attention_f32_end[];
+extern const char paella_hsaco_attention_bf16_begin[];
+extern const char paella_hsaco_attention_bf16_end[];
+extern const char paella_hsaco_attention_f16_begin[];
+extern const char paella_hsaco_attention_f16_end[];
 }
 
 namespace paella {
@@ -145,6 +153,10 @@ bool init_runtime_locked() {
     hsa_amd_agent_iterate_memory_pools(g_rt.gpu, find_device_pool, nullptr);
     if (!load_code_object(paella_hsaco_conv_begin, paella_hsaco_conv_end, "load conv code object")) return false;
     if (!load_code_object(paella_hsaco_misc_begin, paella_hsaco_misc_end, "load misc code object")) return false;
+    if (!load_code_object(paella_hsaco_decode_begin, paella_hsaco_decode_end, "load decode code object")) return false;
+    if (!load_code_object(paella_hsaco_attention_f32_begin, paella_hsaco_attention_f32_end, "load attention code object (fp32)")) return false;
+    if (!load_code_object(paella_hsaco_attention_bf16_begin, paella_hsaco_attention_bf16_end, "load attention code object (bf16)")) return false;
+    if (!load_code_object(paella_hsaco_attention_f16_begin, paella_hsaco_attention_f16_end, "load attention code object (fp16)")) return false;
     return true;
 }
 

@@ -1,0 +1,138 @@
+// Attention of a decoding step: planning and launch (the kernels: prefix_attention.h).
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "prefix_attention.h"
+
+namespace {
+
+using namespace paella;
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+AttentionKernel kernel_of(const paella_prefix_attention_plan* p) {
+    const int rp = p->prefix_rows / 16, ro = p->own_rows / 16;
+    return p->dtype == PAELLA_F32 ? attention_kernel_f32(p->head_dim, rp, ro)
+                                  : p->dtype == PAELLA_BF16 ? attention_kernel_bf16(p->head_dim, rp, ro) : attention_kernel_f16(p->head_dim, rp, ro);
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct Grid {
+    int64_t prefix_tiles, own_tiles, prefix_items, own_items;
+};
+
+Grid grid_of(const paella_prefix_attention_plan* p) {
+    const int64_t per_kv = p->heads / p->kv_heads;
+    Grid g;
+    g.prefix_tiles = p->prefix_len ? ceil_div(p->tokens * per_kv, p->prefix_rows) : 0;
+    g.own_tiles = ceil_div(p->max_new * per_kv, p->own_rows);
+    g.prefix_items = g.prefix_tiles * p->kv_heads * p->prefix_splits;
+    g.own_items = p->sequences * g.own_tiles * p->kv_heads * p->own_splits;
+    return g;
+}
+
+bool extents_ok(const paella_prefix_attention_plan* p) {
+    if (p->heads <= 0 || p->kv_heads <= 0 || p->heads % p->kv_heads) return false;
+    // 32-bit offsets of outputs and parts
+    return (double)p->tokens * p->heads * p->head_dim < 1073741824.0 && (double)p->max_new * p->heads < 1073741824.0;
+}
+
+bool plan_ok(const paella_prefix_attention_plan* p) {
+    if (!p || p->dtype < PAELLA_F32 || p->dtype > PAELLA_F16 || p->page_size <= 0 || p->page_size % 8 || p->sequences <= 0 || p->max_new <= 0 || p->tokens <= 0 ||
+        p->max_pages <= 0 || p->prefix_len < 0 || !(p->scale >= 0.f) || !(p->scale < INFINITY) || !extents_ok(p) || !kernel_of(p))
+        return false;
+    if (p->own_splits <= 0 || p->own_splits > 64 || p->prefix_splits < 0 || p->prefix_splits > 64 || (p->prefix_splits > 0) != (p->prefix_len > 0)) return false;
+    const Grid g = grid_of(p);
+    return (double)g.prefix_items + (double)g.own_items < 1e9;
+}
+
+size_t workspace_of(const paella_prefix_attention_plan* p) {
+    const size_t parts = (size_t)p->prefix_splits + p->own_splits, rows = (size_t)p->tokens * p->heads;
+    return parts == 1 ? 0 : up256(rows * 4) + up256(parts * rows * 8) + parts * rows * p->head_dim * 4;
+}
+
+}  // namespace
+
+extern "C" {
+
+int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_batch* b, int heads, float scale, paella_prefix_attention_plan* p) {
+    if (!p || !cache_extents_ok(c) || !batch_extents_ok(b) || heads <= 0 || heads % c->kv_heads || !(scale >= 0.f) || !(scale < INFINITY)) return PAELLA_EINVAL;
+    *p = paella_prefix_attention_plan{};
+    p->dtype = c->dtype; p->heads = heads; p->kv_heads = c->kv_heads; p->head_dim = c->head_dim; p->page_size = c->page_size;
+    p->sequences = b->sequences; p->max_new = b->max_new; p->tokens = b->tokens; p->max_pages = b->max_pages; p->prefix_len = b->prefix_len;
+    p->scale = scale > 0.f ? scale : 1.f / std::sqrt((float)c->head_dim);
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return PAELLA_ENOSUP;
+    if (!extents_ok(p)) return PAELLA_ENOSUP;
+    const int64_t per_kv = heads / c->kv_heads, size = element_bytes(c->dtype), row_bytes = c->head_dim * size;
+    // rows of a tile: as many as there are, up to what the registers hold beside a step of keys
+    const int most = row_bytes <= 256 ? 64 : row_bytes <= 512 && c->head_dim <= 128 ? 32 : 16;
+    auto rows = [&](int64_t n) { return n <= 16 || most == 16 ? 16 : n <= 32 || most == 32 ? 32 : 64; };
+    p->own_rows = rows(b->max_new * per_kv);
+    p->prefix_rows = p->prefix_len ? rows(b->tokens * per_kv) : p->own_rows;
+    if (p->prefix_rows < p->own_rows) p->prefix_rows = p->own_rows;
+    // A row's keys are shared by as many workgroups as fill the device twice, each with two steps per wave at least.
+    const int step = size == 4 ? 16 : 32;
+    auto splits = [&](int64_t others, int64_t keys) {
+        const int64_t want = ceil_div(512, others), least = ceil_div(ceil_div(keys, step), 8);
+        const int64_t n = want < least ? want : least;
+        return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    };
+    p->own_splits = 1;
+    Grid g = grid_of(p);
+    if (p->prefix_len) p->prefix_splits = splits(g.prefix_tiles * c->kv_heads, p->prefix_len);
+    p->own_splits = splits(b->sequences * g.own_tiles * c->kv_heads, (int64_t)b->max_pages * c->page_size);
+    if (!plan_ok(p)) return PAELLA_ENOSUP;
+    g = grid_of(p);
+    p->workspace_bytes = workspace_of(p);
+    set_launch_dims(&p->dims, (unsigned)(g.prefix_items + g.own_items), 256, 0, 256);
+    const double keys = (double)b->max_pages * c->page_size;
+    p->flops = 4.0 * c->head_dim * b->tokens * heads * (p->prefix_len + keys);
+    p->bytes = 2.0 * (p->prefix_len + b->sequences * keys) * c->kv_heads * row_bytes + 2.0 * b->tokens * heads * row_bytes;
+    return 0;
+}
+
+int paella_prefix_attention_dims(const paella_prefix_attention_plan* p, paella_launch_dims* dims) {
+    if (!plan_ok(p) || !dims) return PAELLA_EINVAL;
+    const Grid g = grid_of(p);
+    set_launch_dims(dims, (unsigned)(g.prefix_items + g.own_items), 256, 0, 256);
+    loaded_dims((const void*)kernel_of(p), dims);
+    return 0;
+}
+
+int paella_prefix_attention_launch(const paella_prefix_attention_plan* p, const paella_kv_cache* c, const paella_kv_batch* b, const void* q, int64_t q_stride,
+                                   void* out, void* workspace, void* stream, uint32_t job_id, void* notifier) {
+    if (!plan_ok(p) || !cache_ok(c) || !batch_ok(b) || !q || !out) return PAELLA_EINVAL;
+    if (c->dtype != p->dtype || c->kv_heads != p->kv_heads || c->head_dim != p->head_dim || c->page_size != p->page_size || b->sequences != p->sequences ||
+        b->max_new != p->max_new || b->tokens != p->tokens || b->max_pages != p->max_pages || b->prefix_len != p->prefix_len)
+        return PAELLA_EINVAL;
+    if (p->prefix_len && !b->prefix_table) return PAELLA_EINVAL;
+    const int64_t size = element_bytes(c->dtype), row = (int64_t)p->heads * c->head_dim;
+    if (q_stride < row || q_stride % 8 || (((uintptr_t)q | (uintptr_t)out) & 15)) return PAELLA_EINVAL;
+    if (overlap(q, ((double)(b->tokens - 1) * q_stride + row) * size, out, (double)b->tokens * row * size)) return PAELLA_EINVAL;
+    const size_t need = workspace_of(p);
+    if (need && (!workspace || ((uintptr_t)workspace & 15))) return PAELLA_EINVAL;
+    const Grid g = grid_of(p);
+    AttentionArgs a;
+    a.q = (const char*)q; a.k_cache = (const char*)c->k; a.v_cache = (const char*)c->v; a.out = (char*)out;
+    a.starts = b->starts; a.past = b->past; a.tables = b->tables; a.prefix_table = b->prefix_table;
+    a.q_stride = q_stride * size;
+    a.sequences = b->sequences; a.max_new = b->max_new; a.tokens = b->tokens; a.max_pages = b->max_pages; a.prefix_len = b->prefix_len;
+    a.heads = p->heads; a.kv_heads = p->kv_heads; a.per_kv = p->heads / p->kv_heads; a.page_size = c->page_size; a.num_pages = c->num_pages;
+    a.page_blocks = (unsigned)c->page_size / 8;
+    a.page_blocks_inv = a.page_blocks == 1 ? 0xFFFFFFFFu : (unsigned)(0x100000000ull / a.page_blocks);
+    a.scale_log2 = p->scale * 1.44269504088896340736f;
+    a.prefix_tiles = (int)g.prefix_tiles; a.prefix_splits = p->prefix_splits; a.own_tiles = (int)g.own_tiles; a.own_splits = p->own_splits;
+    a.prefix_items = (unsigned)g.prefix_items;
+    const size_t parts = (size_t)p->prefix_splits + p->own_splits, rows = (size_t)p->tokens * p->heads;
+    a.counters = need ? (unsigned*)workspace : nullptr;
+    a.ml = need ? (f32x2*)((char*)workspace + up256(rows * 4)) : nullptr;
+    a.acc = need ? (float*)((char*)a.ml + up256(parts * rows * 8)) : nullptr;
+    a.job_id = job_id; a.notifier = (Notifier*)notifier;
+    launch(kernel_of(p), dim3((unsigned)(g.prefix_items + g.own_items)), dim3(256), 0, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+}  // extern "C"

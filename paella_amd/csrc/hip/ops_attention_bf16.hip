@@ -1,0 +1,6 @@
+// Attention over a shared prefix, bf16 (prefix_attention.h).
+#include "prefix_attention.h"
+
+namespace paella {
+AttentionKernel attention_kernel_bf16(int dim, int rp, int ro) { return attention_kernel<Bf16>(dim, rp, ro); }
+}  // namespace paella

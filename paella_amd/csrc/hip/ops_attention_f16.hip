@@ -1,0 +1,6 @@
+// Attention over a shared prefix, f16 (prefix_attention.h).
+#include "prefix_attention.h"
+
+namespace paella {
+AttentionKernel attention_kernel_f16(int dim, int rp, int ro) { return attention_kernel<F16>(dim, rp, ro); }
+}  // namespace paella

@@ -1,0 +1,704 @@
+// Operators of a decoding step over a paged cache, all bounded by memory traffic or latency: appending keys and values
+// (with norms and rotation), beam search's selection, and the reordering of the beams' caches.
+
+#include <hip/hip_runtime.h>
+
+#include <climits>
+#include <cmath>
+
+#include "decode_common.h"
+
+namespace {
+
+using namespace paella;
+
+// ------------------------------------------------------------------------------------------ append
+// Per new token: x' = x / sqrt(mean(x^2) + eps) * w for each query and key head, pairs (a, b) turned by the angle p * f_i:
+// (a cos - b sin, b cos + a sin); keys and values to the slot that the page table names.  One pass over the data: a workgroup per token,
+// 16 bytes (8 values of 16 bits; two loads in 32 bits) per lane, a head per group of lanes that a few shuffles norm and pair up.
+struct AppendArgs {
+    const char *q, *k, *v;
+    char *q_out, *k_cache, *v_cache;
+    const float *q_weight, *k_weight, *inv_freq;
+    const int *starts, *past, *tables;
+    int64_t q_stride, k_stride, v_stride;  // bytes
+    int sequences, max_new, max_pages, prefix_len;
+    int heads, kv_heads, dim, page_size, num_pages, rotary, interleaved, group_log2;  // a head's group of lanes: 2^group_log2 of 8 values each
+    float eps;
+    uint32_t job_id;
+    Notifier* notifier;
+};
+
+template <typename T>
+struct Eight {  // eight values of a head as they lie in memory
+    u32x4 raw[T::bytes / 2];
+    __device__ __forceinline__ void load(const char* p) {
+#pragma unroll
+        for (int i = 0; i < T::bytes / 2; ++i) raw[i] = *reinterpret_cast<const u32x4*>(p + 16 * i);
+    }
+    __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t to, unsigned at) const {
+#pragma unroll
+        for (int i = 0; i < T::bytes / 2; ++i) __builtin_amdgcn_raw_buffer_store_b128(raw[i], to, (int)(at + 16 * i), 0, kThrough);
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        if constexpr (T::bytes == 4) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = as_float(raw[e / 4][e % 4]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const f32x2 v = unpack2<T>(raw[0][e]);
+                x[2 * e] = v.x;
+                x[2 * e + 1] = v.y;
+            }
+        }
+    }
+    __device__ __forceinline__ void set(const float (&x)[8]) {
+        if constexpr (T::bytes == 4) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) raw[e / 4][e % 4] = as_word(x[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) raw[0][e] = pack2<T>(x[2 * e], x[2 * e + 1]);
+        }
+    }
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
+    hook_entry(a.notifier, a.job_id);
+    __shared__ f32x2 turn[256];  // (cos, sin) of each pair's angle
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int t = blockIdx.x;
+    int seq, j;
+    if (row_owner(a.starts, a.sequences, a.max_new, t, lane, &seq, &j)) {
+        const int group = 1 << a.group_log2, li = lane & (group - 1);
+        const int per_wave = 64 >> a.group_log2;
+        const int total = a.heads + 2 * a.kv_heads;
+        const int head_bytes = a.dim * T::bytes;
+        const bool in_head = li * 8 < a.dim;
+        constexpr int AHEAD = 4;  // heads of a lane that are requested together: all of them up to 4 * 4 * (64 / group), 64 at 128 values
+        Eight<T> x[AHEAD];
+        auto fetch = [&](int first) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int h = first + (u * 4 + wave) * per_wave + (lane >> a.group_log2);
+                if (!in_head || h >= total) continue;
+                const char* row = h < a.heads                ? a.q + t * a.q_stride + h * head_bytes
+                                  : h < a.heads + a.kv_heads ? a.k + t * a.k_stride + (h - a.heads) * head_bytes
+                                                             : a.v + t * a.v_stride + (h - a.heads - a.kv_heads) * head_bytes;
+                x[u].load(row + li * 8 * T::bytes);
+            }
+        };
+        fetch(0);
+        // where the token goes; a place outside the table or the cache is none
+        const unsigned own = (unsigned)max(a.past[seq], 0) + (unsigned)j;
+        const unsigned column = own / (unsigned)a.page_size, slot = own - column * (unsigned)a.page_size;
+        int page = -1;
+        if (column < (unsigned)a.max_pages) page = a.tables[(size_t)seq * a.max_pages + column];
+        page = __builtin_amdgcn_readfirstlane(page);  // (descriptors are built from it)
+        const bool placed = (unsigned)page < (unsigned)a.num_pages;
+        // The angle in revolutions, reduced to half a turn in 64 bits: in 32 bits a position of 100000 would be off by 0.006 radians.  (Each pair once
+        // per token, by one lane; 16 heads' worth of lanes read it from LDS.)
+        for (int i = threadIdx.x; i < a.rotary / 2; i += 256) {
+            const double turns = ((double)a.prefix_len + (double)own) * (double)a.inv_freq[i] * 0.15915494309189533577;
+            float s, c;
+            sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+            turn[i] = f32x2{c, s};
+        }
+        __syncthreads();
+        const size_t page_bytes = (size_t)a.kv_heads * a.page_size * head_bytes;
+        const __amdgpu_buffer_rsrc_t to_q = descriptor(a.q_out + (size_t)t * a.heads * head_bytes);
+        const __amdgpu_buffer_rsrc_t to_k = descriptor(a.k_cache + (placed ? page : 0) * page_bytes);
+        const __amdgpu_buffer_rsrc_t to_v = descriptor(a.v_cache + (placed ? page : 0) * page_bytes);
+        const int half = a.rotary >> 1;
+        for (int first = 0; first < total; first += AHEAD * 4 * per_wave) {
+            if (first) fetch(first);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int at = first + (u * 4 + wave) * per_wave;
+                if (at >= total) break;  // whole waves
+                const int h = at + (lane >> a.group_log2);
+                const bool live = in_head && h < total;
+                const bool is_q = h < a.heads, is_v = h >= a.heads + a.kv_heads;
+                float f[8];
+                x[u].get(f);
+                if (!live) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] = 0.f;
+                }
+                const float* weight = is_q ? a.q_weight : a.k_weight;
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum += f[e] * f[e];
+                for (int off = group >> 1; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+                if (weight && live && !is_v) {
+                    const float r = 1.f / sqrtf(sum / (float)a.dim + a.eps);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] = f[e] * r * weight[li * 8 + e];
+                }
+                if (a.rotary) {
+                    const int d0 = li * 8;  // rotary_dim is a multiple of 16: a lane's values are all in one half, or none is rotated
+                    if (a.interleaved) {
+                        if (d0 < a.rotary) {
+#pragma unroll
+                            for (int e = 0; e < 8; e += 2) {
+                                const f32x2 cs = turn[(d0 + e) >> 1];
+                                const float p = f[e], q = f[e + 1];
+                                f[e] = p * cs.x - q * cs.y;
+                                f[e + 1] = q * cs.x + p * cs.y;
+                            }
+                        }
+                    } else {
+                        const bool lower = d0 < half;
+                        const int other = (lane & ~(group - 1)) + (lower ? li + (half >> 3) : li - (half >> 3));
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float partner = __shfl(f[e], other & 63, 64);
+                            if (d0 < a.rotary) {
+                                const f32x2 cs = turn[lower ? d0 + e : d0 - half + e];
+                                f[e] = lower ? f[e] * cs.x - partner * cs.y : f[e] * cs.x + partner * cs.y;
+                            }
+                        }
+                    }
+                }
+                if (!live) continue;
+                if (is_q) {
+                    x[u].set(f);
+                    x[u].store(to_q, (unsigned)(h * head_bytes + li * 8 * T::bytes));
+                } else if (placed) {
+                    const int hk = is_v ? h - a.heads - a.kv_heads : h - a.heads;
+                    const unsigned to = ((unsigned)hk * a.page_size + slot) * head_bytes + li * 8 * T::bytes;
+                    if (is_v) {
+                        x[u].store(to_v, to);  // as it came
+                    } else {
+                        x[u].set(f);
+                        x[u].store(to_k, to);
+                    }
+                }
+            }
+        }
+    }
+    hook_exit(a.notifier, a.job_id);
+}
+
+// ------------------------------------------------------------------------------------------ beam selection
+// value(w, t) = scores[w] + x - lse_w: within a beam the order of the logits is the order of the values, so one pass over the logits takes each
+// workgroup's running maximum, its sum of exponentials and its `count` largest logits; the workgroup that arrives last in a group puts the beams'
+// logarithms together and merges the lists.  Bounded by reading the logits once.
+//
+// A logit as a number whose order is the logits' (-0 and 0 alike, NaN as -inf), with its index behind it such that the larger of two is the one to
+// take; 0 is no candidate.
+__device__ __forceinline__ unsigned order_key(float v) {
+    const unsigned b = as_word(v + 0.f);
+    return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ float key_value(unsigned k) { return as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
+constexpr unsigned kLowestKey = 0x00800000u;  // order_key(-FLT_MAX); -inf lies right below
+__device__ __forceinline__ unsigned long long entry(unsigned key, unsigned index) { return (unsigned long long)key << 32 | (0xFFFFFFFFu - index); }
+
+constexpr int kMostLists = 2048;     // beams * splits
+constexpr int kWaveCandidates = 128;  // of one wave's logits that go on to the workgroup's ranking
+
+struct SelectArgs {
+    const char* logits;
+    int64_t row_stride;  // bytes
+    const float* scores;
+    const unsigned char* finished;
+    int pad_token, groups, beams, vocab, count, splits;
+    unsigned long long* sums;     // [groups * beams * splits]: maximum and sum of exponentials
+    unsigned long long* entries;  // [groups * beams * splits][count], best first
+    unsigned* counters;           // [groups], zero between launches
+    float* out_scores;
+    int *out_parents, *out_tokens;
+    uint32_t job_id;
+    Notifier* notifier;
+};
+
+__device__ __forceinline__ void put64(unsigned long long* p, unsigned long long v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ unsigned long long get64(const unsigned long long* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// 16 bytes from an address on a value's boundary (rows of an odd number of logits begin anywhere).
+__device__ __forceinline__ u32x4 load_unaligned(const char* p) {
+    u32x4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+
+template <typename T, int VALUES>
+__device__ __forceinline__ void load_logits(const char* row, int first, int vocab, unsigned (&key)[VALUES]) {
+    constexpr int VEC = 16 / T::bytes;
+#pragma unroll
+    for (int i = 0; i < VALUES / VEC; ++i) {
+        const int at = first + (i * 256 + (int)threadIdx.x) * VEC;
+        float f[VEC];
+        if (at + VEC <= vocab) {
+            const u32x4 w = load_unaligned(row + (size_t)at * T::bytes);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (T::bytes == 4) {
+                    f[e] = as_float(w[e]);
+                } else {
+                    const f32x2 two = unpack2<T>(w[e]);
+                    f[2 * e] = two.x;
+                    f[2 * e + 1] = two.y;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                f[e] = -INFINITY;
+                if (at + e < vocab) {
+                    if constexpr (T::bytes == 4) f[e] = reinterpret_cast<const float*>(row)[at + e];
+                    else f[e] = unpack2<T>(reinterpret_cast<const unsigned short*>(row)[at + e]).x;
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) key[i * VEC + e] = order_key(f[e] == f[e] ? f[e] : -INFINITY);
+    }
+}
+
+template <typename T, int VALUES>
+__global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
+    hook_entry(a.notifier, a.job_id);
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ float wave_top[4], wave_total[4];
+    __shared__ unsigned found, arrived;
+    __shared__ double row_lse[32];
+    constexpr int VEC = 16 / T::bytes;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row = blockIdx.x / a.splits, split = blockIdx.x - row * a.splits;
+    const int group = row / a.beams;
+    const int K = a.count;
+
+    if (!a.finished || !a.finished[row]) {
+        unsigned long long* const cand = reinterpret_cast<unsigned long long*>(lds);
+        const int first = split * 256 * VALUES;
+        unsigned key[VALUES];
+        load_logits<T, VALUES>(a.logits + (size_t)row * a.row_stride, first, a.vocab, key);
+        if (threadIdx.x == 0) found = 0;
+        unsigned mine = 0;
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) mine = max(mine, key[i]);
+        const float top = wave_max_f(key_value(mine));
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        constexpr float kLog2e = 1.44269504088896340736f;
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) sum += __builtin_amdgcn_exp2f((key_value(key[i]) - base) * kLog2e);
+        sum = wave_sum_f(sum);
+        if (lane == 0) {
+            wave_top[wave] = top;
+            wave_total[wave] = sum;
+        }
+        // A bound that at least K of the wave's logits reach: the K-th largest of the lanes' own maxima, found bit by bit.  Few others reach it.
+        unsigned bound = 0;
+#pragma unroll
+        for (int bit = 31; bit >= 0; --bit) {
+            const unsigned trial = bound | (1u << bit);
+            if (__popcll(__ballot(mine >= trial)) >= K) bound = trial;
+        }
+        bound = max(bound, kLowestKey);
+        int over = 0;
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) over += __popcll(__ballot(key[i] >= bound));
+        unsigned last = 0xFFFFFFFFu;  // of the logits equal to the bound, the index of the last one taken
+        if (over > kWaveCandidates) {  // equal logits, or the best ones in few lanes: the K-th of all of the wave's logits, ties by index
+            unsigned exact = 0;
+            for (int bit = 31; bit >= 0; --bit) {
+                const unsigned trial = exact | (1u << bit);
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < VALUES; ++i) n += __popcll(__ballot(key[i] >= trial));
+                if (n >= K) exact = trial;
+            }
+            bound = max(exact, kLowestKey);
+            int larger = 0;
+#pragma unroll
+            for (int i = 0; i < VALUES; ++i) larger += __popcll(__ballot(key[i] > bound));
+            last = 0;
+            for (int bit = 19; bit >= 0; --bit) {  // the largest index with fewer than the wanted number of equals below it
+                const unsigned trial = last | (1u << bit);
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < VALUES; ++i) {
+                    const unsigned index = first + (i / VEC * 256 + threadIdx.x) * VEC + i % VEC;
+                    n += __popcll(__ballot(key[i] == bound && index < trial));
+                }
+                if (n < K - larger) last = trial;
+            }
+            over = larger;
+#pragma unroll
+            for (int i = 0; i < VALUES; ++i) {
+                const unsigned index = first + (i / VEC * 256 + threadIdx.x) * VEC + i % VEC;
+                over += __popcll(__ballot(key[i] == bound && index <= last));
+            }
+        }
+        __syncthreads();
+        unsigned at = 0;
+        if (lane == 0) at = atomicAdd(&found, (unsigned)over);  // (the order of the waves' entries does not matter: they are ranked)
+        at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) {
+            const unsigned index = first + (i / VEC * 256 + threadIdx.x) * VEC + i % VEC;
+            const bool take = key[i] > bound || (key[i] == bound && index <= last);
+            const unsigned long long who = __ballot(take);
+            if (who) {
+                if (take) cand[at + __popcll(who & ((1ull << lane) - 1))] = entry(key[i], index);
+                at += __popcll(who);
+            }
+        }
+        __syncthreads();
+        const int n = (int)found;
+        unsigned long long* const to = a.entries + (size_t)blockIdx.x * K;
+        for (int c = threadIdx.x; c < n; c += 256) {
+            const unsigned long long e = cand[c];
+            int rank = 0;
+            for (int o = 0; o < n; ++o) rank += cand[o] > e;
+            if (rank < K) put64(to + rank, e);
+        }
+        for (int c = n + threadIdx.x; c < K; c += 256) put64(to + c, 0);
+        if (threadIdx.x == 0) {
+            const float m = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
+            double s = 0.;
+            if (fabsf(m) < INFINITY) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    if (wave_total[w] > 0.f) s += (double)wave_total[w] * (double)__builtin_amdgcn_exp2f((wave_top[w] - m) * kLog2e);
+            }
+            put64(a.sums + blockIdx.x, (unsigned long long)as_word(m) << 32 | as_word((float)s));
+        }
+    }
+
+    // The last workgroup of the group merges.  As in the convs' split reductions: the stores above go through to memory ahead of the count.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const int lists = a.beams * a.splits;
+    if (threadIdx.x == 0) arrived = __hip_atomic_fetch_add(a.counters + group, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(arrived) == (unsigned)lists - 1) {
+        // LDS: each list's best value and flat index w * vocab + t, then the lists taken, then the candidates
+        double* const head = reinterpret_cast<double*>(lds);
+        f32x2* const ms = reinterpret_cast<f32x2*>(head + lists);
+        unsigned* const flat = reinterpret_cast<unsigned*>(ms + lists);
+        int* const taken = reinterpret_cast<int*>(flat + lists + (lists & 1));
+        const int most = min(K, lists);
+        double* const value = reinterpret_cast<double*>(taken + K + (K & 1));
+        unsigned* const where = reinterpret_cast<unsigned*>(value + most * K);
+        const int first_list = group * lists;
+        auto ended = [&](int w) { return a.finished && a.finished[group * a.beams + w]; };
+        for (int l = threadIdx.x; l < lists; l += 256) {
+            const int w = l / a.splits;
+            unsigned long long s = 0, e = 0;
+            if (!ended(w)) {
+                s = get64(a.sums + first_list + l);
+                e = get64(a.entries + (size_t)(first_list + l) * K);
+            }
+            ms[l] = f32x2{as_float((unsigned)(s >> 32)), as_float((unsigned)s)};
+            head[l] = e ? (double)key_value((unsigned)(e >> 32)) : -INFINITY;
+            flat[l] = e ? (unsigned)w * a.vocab + (0xFFFFFFFFu - (unsigned)e) : 0xFFFFFFFFu - (unsigned)l;
+        }
+        if (threadIdx.x == 0) found = 0;
+        __syncthreads();
+        if ((int)threadIdx.x < a.beams) {
+            const int w = threadIdx.x;
+            float m = -INFINITY;
+            for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ms[w * a.splits + s].x);
+            double total = 0.;
+            for (int s = 0; s < a.splits; ++s) {
+                const f32x2 p = ms[w * a.splits + s];
+                if (p.y > 0.f) total += (double)p.y * exp((double)p.x - (double)m);
+            }
+            row_lse[w] = m == INFINITY ? INFINITY : (double)m + log(total);
+        }
+        __syncthreads();
+        // in 64 bits: 32 would make equals of neighbours, and the lower index would win
+        auto worth = [&](int w, double logit) {
+            const double v = (double)a.scores[group * a.beams + w] + (logit - row_lse[w]);
+            return v > -INFINITY && v < INFINITY ? v : -INFINITY;
+        };
+        for (int l = threadIdx.x; l < lists; l += 256) {
+            const int w = l / a.splits;
+            if (ended(w)) {
+                if (l == w * a.splits) {
+                    const double v = (double)a.scores[group * a.beams + w];
+                    head[l] = v > -INFINITY && v < INFINITY ? v : -INFINITY;
+                    if (head[l] > -INFINITY) flat[l] = (unsigned)w * a.vocab + (unsigned)a.pad_token;
+                }
+            } else if (head[l] > -INFINITY) {
+                head[l] = worth(w, head[l]);
+            }
+        }
+        __syncthreads();
+        // The K lists with the best heads: no other holds one of the K best.
+        for (int l = threadIdx.x; l < lists; l += 256) {
+            const double v = head[l];
+            const unsigned f = flat[l];
+            int rank = 0;
+            for (int o = 0; o < lists; ++o) rank += head[o] > v || (head[o] == v && flat[o] < f);
+            if (rank < K) taken[rank] = l;
+        }
+        __syncthreads();
+        const double least = lists >= K ? head[taken[K - 1]] : -INFINITY;
+        for (int c = threadIdx.x; c < most * K; c += 256) {
+            const int r = c / K, i = c - r * K, l = taken[r], w = l / a.splits;
+            double v = -INFINITY;
+            unsigned f = 0;
+            if (i == 0) {
+                v = head[l];
+                f = flat[l];
+            } else if (!ended(w)) {
+                const unsigned long long e = get64(a.entries + (size_t)(first_list + l) * K + i);
+                if (e) {
+                    v = worth(w, (double)key_value((unsigned)(e >> 32)));
+                    f = (unsigned)w * a.vocab + (0xFFFFFFFFu - (unsigned)e);
+                }
+            }
+            if (v > -INFINITY && v >= least) {
+                const unsigned at = atomicAdd(&found, 1u);
+                value[at] = v;
+                where[at] = f;
+            }
+        }
+        __syncthreads();
+        const int n = (int)found;
+        const size_t out = (size_t)group * K;
+        for (int c = threadIdx.x; c < n; c += 256) {
+            const double v = value[c];
+            const unsigned f = where[c];
+            int rank = 0;
+            for (int o = 0; o < n; ++o) rank += value[o] > v || (value[o] == v && where[o] < f);
+            if (rank < K) {
+                const unsigned w = f / (unsigned)a.vocab;
+                store_out(a.out_scores + out + rank, (float)v);
+                __hip_atomic_store(a.out_parents + out + rank, (int)w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(a.out_tokens + out + rank, (int)(f - w * (unsigned)a.vocab), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        for (int c = n + threadIdx.x; c < K; c += 256) {
+            store_out(a.out_scores + out + c, -INFINITY);
+            __hip_atomic_store(a.out_parents + out + c, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(a.out_tokens + out + c, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        if (threadIdx.x == 0) __hip_atomic_store(a.counters + group, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    hook_exit(a.notifier, a.job_id);
+}
+
+// ------------------------------------------------------------------------------------------ reordering of the beams' caches
+// A workgroup per child and key head: the tokens that the parent's last page holds lie side by side for a head, keys and values each one run of
+// bytes.  Nothing is copied for a parent's first child; the first head's workgroup writes the child's row of the table.
+struct ReorderArgs {
+    char *k_cache, *v_cache;
+    const int *parents, *past, *tables, *spare;
+    int *tables_out, *past_out;
+    int groups, beams, count, max_pages, num_pages, kv_heads, page_size, head_bytes;
+    uint32_t job_id;
+    Notifier* notifier;
+};
+
+__global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
+    hook_entry(a.notifier, a.job_id);
+    const int lane = threadIdx.x & 63;
+    const int row = blockIdx.x / a.kv_heads, head = blockIdx.x - row * a.kv_heads;
+    const int group = row / a.count, child = row - group * a.count;
+    const int parent = a.parents[row];
+    const int spare = __builtin_amdgcn_readfirstlane(a.spare[row]);
+    bool first = true;
+    for (int c = 0; c < child && first; c += 64) first = !__any(c + lane < child && a.parents[group * a.count + c + lane] == parent);
+    if ((unsigned)parent < (unsigned)a.beams) {
+        const int source = group * a.beams + parent;
+        const unsigned past = (unsigned)max(a.past[source], 0);
+        const unsigned full = past / (unsigned)a.page_size, rest = past - full * (unsigned)a.page_size;
+        const int* const from = a.tables + (size_t)source * a.max_pages;
+        const bool inside = full < (unsigned)a.max_pages;
+        int last = -1;
+        if (inside && rest) last = __builtin_amdgcn_readfirstlane(from[full]);
+        if (head == 0) {
+            int* const to = a.tables_out + (size_t)row * a.max_pages;
+            const int whole = (int)min(full, (unsigned)a.max_pages);
+            for (int i = threadIdx.x; i < whole; i += 256) __hip_atomic_store(to + i, from[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (threadIdx.x == 0) {
+                if (inside) __hip_atomic_store(to + full, first && rest ? last : spare, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(a.past_out + row, (int)past, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        if (!first && (unsigned)last < (unsigned)a.num_pages && (unsigned)spare < (unsigned)a.num_pages) {
+            const size_t run = (size_t)a.page_size * a.head_bytes, page_bytes = run * a.kv_heads;
+            const unsigned bytes = rest * (unsigned)a.head_bytes;
+            const size_t src = last * page_bytes + head * run, dst = spare * page_bytes + head * run;
+            const __amdgpu_buffer_rsrc_t to_k = descriptor(a.k_cache + dst), to_v = descriptor(a.v_cache + dst);
+            for (unsigned at = threadIdx.x * 16; at < bytes; at += 4096) {
+                const u32x4 x = *reinterpret_cast<const u32x4*>(a.k_cache + src + at);
+                const u32x4 y = *reinterpret_cast<const u32x4*>(a.v_cache + src + at);
+                __builtin_amdgcn_raw_buffer_store_b128(x, to_k, (int)at, 0, kThrough);
+                __builtin_amdgcn_raw_buffer_store_b128(y, to_v, (int)at, 0, kThrough);
+            }
+        }
+    } else if (head == 0 && threadIdx.x == 0) {
+        __hip_atomic_store(a.past_out + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    hook_exit(a.notifier, a.job_id);
+}
+
+using AppendKernel = void (*)(AppendArgs);
+AppendKernel append_kernel(int dtype) {
+    return dtype == PAELLA_F32 ? kv_append_kernel<F32> : dtype == PAELLA_BF16 ? kv_append_kernel<Bf16> : kv_append_kernel<F16>;
+}
+
+using SelectKernel = void (*)(SelectArgs);
+SelectKernel select_kernel(int dtype, int values) {
+    if (values == 8) return dtype == PAELLA_F32 ? beam_select_kernel<F32, 8> : dtype == PAELLA_BF16 ? beam_select_kernel<Bf16, 8> : beam_select_kernel<F16, 8>;
+    return dtype == PAELLA_F32 ? beam_select_kernel<F32, 32> : dtype == PAELLA_BF16 ? beam_select_kernel<Bf16, 32> : beam_select_kernel<F16, 32>;
+}
+
+int append_check(const paella_kv_append_desc* d, const paella_kv_cache* c, const paella_kv_batch* b) {
+    if (!d || !cache_extents_ok(c) || !batch_extents_ok(b)) return PAELLA_EINVAL;
+    if (d->heads < 0 || d->heads > 65536 || d->rotary_dim < 0 || d->rotary_dim % 16 || d->rotary_dim > c->head_dim || !(d->eps >= 0.f)) return PAELLA_EINVAL;
+    return 0;
+}
+
+// LDS of a selection: the wave's candidates of the pass over the logits, and the merge's lists, in the same place.
+unsigned select_lds(const paella_beam_select_plan* p) {
+    const unsigned lists = p->beams * p->splits, most = (unsigned)p->count < lists ? p->count : lists;
+    const unsigned merge = lists * 20 + (lists & 1) * 4 + (p->count + (p->count & 1)) * 4 + most * p->count * 12;
+    const unsigned pass = 4 * kWaveCandidates * 8;
+    return ((merge > pass ? merge : pass) + 15) / 16 * 16;
+}
+
+bool select_plan_ok(const paella_beam_select_plan* p) {
+    if (!p || p->dtype < PAELLA_F32 || p->dtype > PAELLA_F16 || p->groups <= 0 || p->beams <= 0 || p->beams > 32 || p->vocab <= 0 || p->vocab > 524288) return false;
+    if (p->count <= 0 || p->count > 64 || (p->values != 8 && p->values != 32)) return false;
+    const int splits = (p->vocab + 256 * p->values - 1) / (256 * p->values);
+    return p->splits == splits && p->beams * splits <= kMostLists && (double)p->groups * p->beams * splits < 1e9;
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+extern "C" {
+
+int paella_kv_append_dims(const paella_kv_append_desc* desc, const paella_kv_cache* cache, const paella_kv_batch* batch, paella_launch_dims* dims) {
+    if (int rc = append_check(desc, cache, batch)) return rc;
+    if (!dims) return PAELLA_EINVAL;
+    set_launch_dims(dims, (unsigned)batch->tokens, 256, 0, 64);
+    loaded_dims((const void*)append_kernel(cache->dtype), dims);
+    return 0;
+}
+
+int paella_kv_append_launch(const paella_kv_append_desc* d, const paella_kv_cache* c, const paella_kv_batch* b, const void* q, const void* k, const void* v,
+                            const float* q_weight, const float* k_weight, const float* inv_freq, void* q_out, void* stream, uint32_t job_id,
+                            void* notifier) {
+    if (int rc = append_check(d, c, b)) return rc;
+    if (!cache_ok(c) || !batch_ok(b) || !k || !v || (d->heads > 0) != (q != nullptr) || (d->heads > 0) != (q_out != nullptr)) return PAELLA_EINVAL;
+    if (d->rotary_dim && !inv_freq) return PAELLA_EINVAL;
+    const int64_t size = element_bytes(c->dtype), kv_row = (int64_t)c->kv_heads * c->head_dim, q_row = (int64_t)d->heads * c->head_dim;
+    if (d->k_stride < kv_row || d->v_stride < kv_row || d->k_stride % 8 || d->v_stride % 8) return PAELLA_EINVAL;
+    if (d->heads && (d->q_stride < q_row || d->q_stride % 8 || q_row * size >= (int64_t)1 << 31)) return PAELLA_EINVAL;
+    if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out) & 15) != 0) return PAELLA_EINVAL;
+    if (d->heads && overlap(q, (double)(b->tokens - 1) * d->q_stride * size + q_row * size, q_out, (double)b->tokens * q_row * size) &&
+        !(q == q_out && d->q_stride == q_row))
+        return PAELLA_EINVAL;
+    AppendArgs a;
+    a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v;
+    a.q_out = (char*)q_out; a.k_cache = (char*)c->k; a.v_cache = (char*)c->v;
+    a.q_weight = q_weight; a.k_weight = k_weight; a.inv_freq = inv_freq;
+    a.starts = b->starts; a.past = b->past; a.tables = b->tables;
+    a.q_stride = d->q_stride * size; a.k_stride = d->k_stride * size; a.v_stride = d->v_stride * size;
+    a.sequences = b->sequences; a.max_new = b->max_new; a.max_pages = b->max_pages; a.prefix_len = b->prefix_len;
+    a.heads = d->heads; a.kv_heads = c->kv_heads; a.dim = c->head_dim; a.page_size = c->page_size; a.num_pages = c->num_pages;
+    a.rotary = d->rotary_dim; a.interleaved = d->interleaved; a.eps = d->eps;
+    a.group_log2 = 0;
+    while ((8 << a.group_log2) < c->head_dim) ++a.group_log2;
+    a.job_id = job_id; a.notifier = (Notifier*)notifier;
+    launch(append_kernel(c->dtype), dim3(b->tokens), dim3(256), 0, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+int paella_beam_select_plan_make(int dtype, int groups, int beams, int vocab, int count, paella_beam_select_plan* p) {
+    if (!p || dtype < PAELLA_F32 || dtype > PAELLA_F16 || groups <= 0 || beams <= 0 || vocab <= 0 || count <= 0) return PAELLA_EINVAL;
+    if (beams > 32 || vocab > 524288 || count > 64) return PAELLA_ENOSUP;
+    *p = paella_beam_select_plan{};
+    p->dtype = dtype; p->groups = groups; p->beams = beams; p->vocab = vocab; p->count = count;
+    // 32 logits per thread where that still gives two workgroups per compute unit, else 8 (up to the 64 lists per beam that the merge takes)
+    const int long_splits = (vocab + 8191) / 8192, short_splits = (vocab + 2047) / 2048;
+    p->values = (double)groups * beams * long_splits >= 512 || short_splits > 64 ? 32 : 8;
+    p->splits = p->values == 32 ? long_splits : short_splits;
+    if (!select_plan_ok(p)) return PAELLA_ENOSUP;
+    const size_t lists = (size_t)groups * beams * p->splits;
+    p->workspace_bytes = up256((size_t)groups * 4) + up256(lists * 8) + lists * count * 8;
+    set_launch_dims(&p->dims, (unsigned)lists, 256, select_lds(p), 64);
+    p->flops = 4.0 * groups * beams * vocab;
+    p->bytes = (double)groups * beams * vocab * element_bytes(dtype) + groups * (beams * 4.0 + count * 12.0);
+    return 0;
+}
+
+int paella_beam_select_dims(const paella_beam_select_plan* p, paella_launch_dims* dims) {
+    if (!select_plan_ok(p) || !dims) return PAELLA_EINVAL;
+    set_launch_dims(dims, (unsigned)(p->groups * p->beams * p->splits), 256, select_lds(p), 64);
+    loaded_dims((const void*)select_kernel(p->dtype, p->values), dims);
+    return 0;
+}
+
+int paella_beam_select_launch(const paella_beam_select_plan* p, const void* logits, int64_t row_stride, const float* scores, const uint8_t* finished,
+                              int pad_token, float* out_scores, int32_t* out_parents, int32_t* out_tokens, void* workspace, void* stream,
+                              uint32_t job_id, void* notifier) {
+    if (!select_plan_ok(p) || !logits || !scores || !out_scores || !out_parents || !out_tokens || !workspace) return PAELLA_EINVAL;
+    if (row_stride < p->vocab || (finished && (pad_token < 0 || pad_token >= p->vocab))) return PAELLA_EINVAL;
+    const int size = element_bytes(p->dtype);
+    if (((uintptr_t)logits & (size - 1)) || ((uintptr_t)workspace & 15)) return PAELLA_EINVAL;
+    const size_t lists = (size_t)p->groups * p->beams * p->splits;
+    SelectArgs a;
+    a.logits = (const char*)logits; a.row_stride = row_stride * size; a.scores = scores; a.finished = finished;
+    a.pad_token = pad_token; a.groups = p->groups; a.beams = p->beams; a.vocab = p->vocab; a.count = p->count; a.splits = p->splits;
+    a.counters = (unsigned*)workspace;
+    a.sums = (unsigned long long*)((char*)workspace + up256((size_t)p->groups * 4));
+    a.entries = (unsigned long long*)((char*)a.sums + up256(lists * 8));
+    a.out_scores = out_scores; a.out_parents = out_parents; a.out_tokens = out_tokens;
+    a.job_id = job_id; a.notifier = (Notifier*)notifier;
+    const unsigned lds = select_lds(p);
+    const SelectKernel kernel = select_kernel(p->dtype, p->values);
+    if (lds > 65536) {
+        if (hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds)) return (int)e;
+    }
+    launch(kernel, dim3((unsigned)lists), dim3(256), lds, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+static int reorder_check(const paella_beam_reorder_desc* d, const paella_kv_cache* c) {
+    if (!d || !cache_extents_ok(c) || d->groups <= 0 || d->beams <= 0 || d->count <= 0 || d->max_pages <= 0) return PAELLA_EINVAL;
+    const double rows = (double)d->groups * (d->count > d->beams ? d->count : d->beams);
+    return rows * c->kv_heads < 2147483648.0 ? 0 : PAELLA_EINVAL;
+}
+
+int paella_beam_reorder_dims(const paella_beam_reorder_desc* d, const paella_kv_cache* c, paella_launch_dims* dims) {
+    if (int rc = reorder_check(d, c)) return rc;
+    if (!dims) return PAELLA_EINVAL;
+    set_launch_dims(dims, (unsigned)(d->groups * d->count * c->kv_heads), 256, 0, 32);
+    loaded_dims((const void*)beam_reorder_kernel, dims);
+    return 0;
+}
+
+int paella_beam_reorder_launch(const paella_beam_reorder_desc* d, const paella_kv_cache* c, const int32_t* parents, const int32_t* past, const int32_t* tables,
+                               const int32_t* spare, int32_t* tables_out, int32_t* past_out, void* stream, uint32_t job_id, void* notifier) {
+    if (int rc = reorder_check(d, c)) return rc;
+    if (!cache_ok(c) || !parents || !past || !tables || !spare || !tables_out || !past_out) return PAELLA_EINVAL;
+    const double in = (double)d->groups * d->beams * 4, out = (double)d->groups * d->count * 4;
+    if (overlap(tables, in * d->max_pages, tables_out, out * d->max_pages) || overlap(past, in, past_out, out) || overlap(parents, out, past_out, out) ||
+        overlap(spare, out, tables_out, out * d->max_pages))
+        return PAELLA_EINVAL;
+    ReorderArgs a;
+    a.k_cache = (char*)c->k; a.v_cache = (char*)c->v;
+    a.parents = parents; a.past = past; a.tables = tables; a.spare = spare; a.tables_out = tables_out; a.past_out = past_out;
+    a.groups = d->groups; a.beams = d->beams; a.count = d->count; a.max_pages = d->max_pages;
+    a.num_pages = c->num_pages; a.kv_heads = c->kv_heads; a.page_size = c->page_size; a.head_bytes = c->head_dim * element_bytes(c->dtype);
+    a.job_id = job_id; a.notifier = (Notifier*)notifier;
+    launch(beam_reorder_kernel, dim3((unsigned)(d->groups * d->count * c->kv_heads)), dim3(256), 0, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+}  // extern "C"

@@ -1,0 +1,236 @@
+"""Functional front-end over the operators of a decoding step (include/paella_decode.h): a paged cache of keys and values, attention for
+sequences that share a prefix, beam search.
+
+As in `ops`: tensors are torch CUDA tensors, everything runs on the calling thread's current torch stream unless a stream handle is
+given, arguments that do not fit raise AssertionError here and RuntimeError from the library.  One step of a batch:
+
+    cache = KVCache.empty(num_pages, kv_heads, page_size, head_dim, torch.bfloat16)      # one per layer
+    batch = KVBatch(past, tables, prefix_table=shared, prefix_len=len_of_prefix)         # past, tables: int32 device tensors
+    attend = PrefixAttention(heads, cache, batch)
+    q = kv_append(cache, batch, k, v, q=q, q_norm=wq, k_norm=wk, inv_freq=freq)          # per layer
+    out = attend(q, cache, batch)
+    past += 1
+
+Lengths and tables are read on the device at every launch, so a captured step may be replayed while they change.
+"""
+import ctypes
+
+import torch
+
+from . import _abi
+from ._abi import LaunchDims, check
+from ._abi_decode import BeamReorderDesc, BeamSelectPlan, KvAppendDesc, KvBatch, KvCache, PrefixAttentionPlan
+from .ops import _stream, _torch_stream
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _on_device(*tensors):
+    """Launches go to the current device: every tensor has to live there."""
+    device = torch.cuda.current_device()
+    for t in tensors:
+        assert t is None or (t.is_cuda and t.device.index == device), "tensors of the current device are needed"
+
+
+def _ints(t, *shape):
+    assert t.dtype == torch.int32 and t.is_contiguous() and tuple(t.shape) == shape, ("contiguous int32 of shape %s" % (shape,), t.dtype, tuple(t.shape))
+    return t.data_ptr()
+
+
+def _floats(t, n):
+    if t is None:
+        return None
+    assert t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n, ("%d contiguous float32" % n, t.dtype, tuple(t.shape))
+    return t.data_ptr()
+
+
+def _rows(t, heads, cache):
+    """Address and row stride of [tokens, heads, head_dim] whose heads lie side by side."""
+    assert t.dtype == cache.dtype and t.dim() == 3 and t.shape[1:] == (heads, cache.head_dim), (t.dtype, tuple(t.shape))
+    assert t.stride(2) == 1 and (heads == 1 or t.stride(1) == cache.head_dim), "heads have to lie side by side: strides %s" % (t.stride(),)
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else heads * cache.head_dim
+
+
+class _Workspaces:
+    """Scratch memory that starts out zeroed, one per stream, so that calls on different streams do not meet in it.  A call under graph capture gets one of
+    its own in the graph's memory: graphs that were captured from one plan may run at once."""
+
+    def __init__(self, nbytes):
+        self.nbytes = nbytes
+        self.of_stream = {}
+
+    def __call__(self, stream, device):
+        if not self.nbytes:
+            return None
+        if torch.cuda.is_current_stream_capturing():
+            return torch.zeros(self.nbytes // 4 + 1, dtype=torch.int32, device=device)
+        key = (device, stream)
+        w = self.of_stream.get(key)
+        if w is None:
+            w = self.of_stream[key] = torch.zeros(self.nbytes // 4 + 1, dtype=torch.int32, device=device)
+            if stream != _torch_stream():  # the fill ran on torch's stream
+                torch.cuda.current_stream().synchronize()
+        return w
+
+
+class KVCache:
+    """Keys and values of one layer: two tensors [num_pages, kv_heads, page_size, head_dim] of one type (float32, bfloat16, float16)."""
+
+    def __init__(self, k, v):
+        assert k.dtype in _DTYPES and k.dim() == 4 and k.is_contiguous() and k.shape == v.shape and v.dtype == k.dtype and v.is_contiguous() and v.device == k.device
+        self.k, self.v = k, v
+        self.dtype = k.dtype
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        self.desc = KvCache(k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], *k.shape)
+        self.ref = ctypes.byref(self.desc)
+
+    @classmethod
+    def empty(cls, num_pages, kv_heads, page_size, head_dim, dtype=torch.float32, device="cuda:0"):
+        return cls(*(torch.zeros((num_pages, kv_heads, page_size, head_dim), dtype=dtype, device=device) for _ in range(2)))
+
+
+class KVBatch:
+    """The new tokens of a step.  past: int32 [sequences], own tokens in the cache so far; tables: int32 [sequences, max_pages]; prefix_table: int32, the pages of
+    the prefix that all sequences share, prefix_len its tokens.  Every sequence has max_new new tokens, or, with starts (int32 [sequences + 1]), rows starts[b] to
+    starts[b + 1] of the `tokens` rows.  The tensors are read at every launch, not here."""
+
+    def __init__(self, past, tables, max_new=1, starts=None, tokens=None, prefix_table=None, prefix_len=0):
+        assert past.dim() == 1 and tables.dim() == 2 and max_new >= 1
+        n = past.shape[0]
+        _on_device(past, tables, starts, prefix_table)
+        if starts is None:
+            assert tokens is None or tokens == n * max_new, "without starts every sequence has max_new tokens"
+            tokens = n * max_new
+        else:
+            assert tokens is not None and tokens >= 1, "the number of rows, which starts alone does not tell the host"
+        assert prefix_len >= 0 and (prefix_len == 0 or prefix_table is not None)
+        self.past, self.tables, self.starts, self.prefix_table = past, tables, starts, prefix_table
+        self.tokens, self.prefix_len = tokens, prefix_len
+        self.desc = KvBatch(n, max_new, tokens, tables.shape[1], prefix_len, None if starts is None else _ints(starts, n + 1), _ints(past, n), _ints(tables, n, tables.shape[1]),
+                            _ints(prefix_table, prefix_table.numel()) if prefix_len else None)
+        self.prefix_pages = prefix_table.numel() if prefix_len else 0
+        self.ref = ctypes.byref(self.desc)
+
+    def check_prefix(self, cache):
+        assert self.prefix_pages * cache.page_size >= self.prefix_len, "the prefix's table has too few pages"
+
+
+def kv_append(cache, batch, k, v, q=None, q_norm=None, k_norm=None, eps=1e-6, inv_freq=None, interleaved=False, out=None, stream=None, job_id=0, notifier=None):
+    """Stores the new tokens' k and v ([tokens, kv_heads, head_dim]) in the cache, k normed per head (k_norm: float32 [head_dim]) and rotated (inv_freq: float32, one
+    per rotated pair) on the way; returns q ([tokens, heads, head_dim]) normed and rotated likewise, in `out` where given (which may be q)."""
+    lib = _abi.ops()
+    _on_device(cache.k, k, v, q, q_norm, k_norm, inv_freq, out)
+    heads = 0 if q is None else q.shape[1]
+    kp, ks = _rows(k, cache.kv_heads, cache)
+    vp, vs = _rows(v, cache.kv_heads, cache)
+    assert k.shape[0] == v.shape[0] == batch.tokens, (k.shape[0], v.shape[0], batch.tokens)
+    qp = op = None
+    qs = 0
+    if q is not None:
+        qp, qs = _rows(q, heads, cache)
+        assert q.shape[0] == batch.tokens
+        if out is None:
+            out = q.new_empty(q.shape)
+        assert out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()
+        op = out.data_ptr()
+    rotary = 0 if inv_freq is None else 2 * inv_freq.numel()
+    desc = KvAppendDesc(heads, rotary, int(interleaved), eps, qs, ks, vs)
+    rc = lib.paella_kv_append_launch(ctypes.byref(desc), cache.ref, batch.ref, qp, kp, vp, _floats(q_norm, cache.head_dim), _floats(k_norm, cache.head_dim),
+                                     _floats(inv_freq, rotary // 2), op, _stream(stream), job_id, notifier)
+    if rc:
+        check(rc, "paella_kv_append_launch")
+    return out
+
+
+class PrefixAttention:
+    """Planned attention of a batch: every new token over the shared prefix and its own sequence's tokens up to itself.  The plan holds for every cache and batch of these
+    extents (layers, steps); scale: 1 / sqrt(head_dim) unless given."""
+
+    def __init__(self, heads, cache, batch, scale=0.0):
+        self.lib = _abi.ops()
+        self.plan = PrefixAttentionPlan()
+        check(self.lib.paella_prefix_attention_plan_make(cache.ref, batch.ref, heads, scale, ctypes.byref(self.plan)), "paella_prefix_attention_plan_make")
+        self._ref = ctypes.byref(self.plan)
+        self._launch = self.lib.paella_prefix_attention_launch
+        self.heads = heads
+        self.workspaces = _Workspaces(self.plan.workspace_bytes)
+
+    def dims(self):
+        d = LaunchDims()
+        check(self.lib.paella_prefix_attention_dims(self._ref, ctypes.byref(d)), "paella_prefix_attention_dims")
+        return d
+
+    def __call__(self, q, cache, batch, out=None, stream=None, job_id=0, notifier=None):
+        _on_device(q, cache.k, out)
+        batch.check_prefix(cache)
+        qp, qs = _rows(q, self.heads, cache)
+        assert q.shape[0] == batch.tokens, (q.shape[0], batch.tokens)
+        if out is None:
+            out = q.new_empty(q.shape)
+        assert out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()
+        stream = _stream(stream)
+        workspace = self.workspaces(stream, q.device)
+        rc = self._launch(self._ref, cache.ref, batch.ref, qp, qs, out.data_ptr(), None if workspace is None else workspace.data_ptr(), stream, job_id, notifier)
+        if rc:
+            check(rc, "paella_prefix_attention_launch")
+        return out
+
+
+class BeamSelect:
+    """Planned selection: per group of `beams` beams the `count` best continuations over the vocabulary."""
+
+    def __init__(self, groups, beams, vocab, count, dtype=torch.float32):
+        self.lib = _abi.ops()
+        self.plan = BeamSelectPlan()
+        assert dtype in _DTYPES, dtype
+        check(self.lib.paella_beam_select_plan_make(_DTYPES[dtype], groups, beams, vocab, count, ctypes.byref(self.plan)), "paella_beam_select_plan_make")
+        self._ref = ctypes.byref(self.plan)
+        self._launch = self.lib.paella_beam_select_launch
+        self.dtype, self.shape, self.count = dtype, (groups, beams, vocab), count
+        self.workspaces = _Workspaces(self.plan.workspace_bytes)
+
+    def dims(self):
+        d = LaunchDims()
+        check(self.lib.paella_beam_select_dims(self._ref, ctypes.byref(d)), "paella_beam_select_dims")
+        return d
+
+    def __call__(self, logits, scores, finished=None, pad_token=0, stream=None, job_id=0, notifier=None):
+        """logits [groups, beams, vocab] (beams one after the other, rows of any stride), scores float32 [groups, beams], finished uint8 or bool [groups, beams].  Returns scores
+        (float32), parents and tokens (int32), each [groups, count], best first."""
+        _on_device(logits, scores, finished)
+        groups, beams, vocab = self.shape
+        assert logits.dtype == self.dtype and tuple(logits.shape) == self.shape, (logits.dtype, tuple(logits.shape))
+        row = logits.stride(1) if beams > 1 else logits.stride(0) if groups > 1 else vocab
+        assert (vocab == 1 or logits.stride(2) == 1) and (groups == 1 or beams == 1 or logits.stride(0) == beams * row), "rows have to be one stride apart: %s" % (logits.stride(),)
+        if finished is not None:
+            assert finished.dtype in (torch.uint8, torch.bool) and finished.is_contiguous() and finished.numel() == groups * beams
+            finished = finished.data_ptr()
+        out = scores.new_empty((groups, self.count))
+        chosen = torch.empty((2, groups, self.count), dtype=torch.int32, device=scores.device)
+        stream = _stream(stream)
+        workspace = self.workspaces(stream, logits.device)
+        rc = self._launch(self._ref, logits.data_ptr(), row, _floats(scores, groups * beams), finished, pad_token, out.data_ptr(), chosen.data_ptr(),
+                          chosen.data_ptr() + 4 * groups * self.count, workspace.data_ptr(), stream, job_id, notifier)
+        if rc:
+            check(rc, "paella_beam_select_launch")
+        return out, chosen[0], chosen[1]
+
+
+def beam_reorder(cache, parents, past, tables, tables_out, spare, past_out=None, stream=None, job_id=0, notifier=None):
+    """Gives each child beam (parents: int32 [groups, count]) its parent's tokens: rows of tables_out name the parent's full pages and the page of the next token, copied to a
+    spare page (spare: int32, one per child) for every child of a parent but its first.  Returns the children's lengths (past_out).  tables: int32 [groups * beams, max_pages]."""
+    lib = _abi.ops()
+    _on_device(cache.k, parents, past, tables, tables_out, spare, past_out)
+    assert parents.dim() == 2 and tables.dim() == 2
+    groups, count = parents.shape
+    rows, pages = tables.shape
+    assert rows % groups == 0 and spare.numel() == groups * count, (rows, groups, spare.numel())
+    if past_out is None:
+        past_out = past.new_empty(groups * count)
+    desc = BeamReorderDesc(groups, rows // groups, count, pages)
+    rc = lib.paella_beam_reorder_launch(ctypes.byref(desc), cache.ref, _ints(parents, groups, count), _ints(past, rows), _ints(tables, rows, pages),
+                                        _ints(spare, *spare.shape), _ints(tables_out, groups * count, pages), _ints(past_out, groups * count), _stream(stream), job_id,
+                                        notifier)
+    if rc:
+        check(rc, "paella_beam_reorder_launch")
+    return past_out
