@@ -103,7 +103,7 @@ int paella_prefix_attention_launch(const paella_prefix_attention_plan* plan, con
 
 typedef struct paella_beam_select_plan {
     int dtype;                   /* of the logits */
-    int groups, beams, vocab, count;  /* beams <= 32, vocab <= 524288, count <= 64 */
+    int groups, beams, vocab, count;  /* beams <= 32, vocab <= 524288, count <= 64, beams * ceil(vocab / 8192) <= 1024 (PAELLA_ENOSUP beyond) */
     int values, splits;          /* logits per thread; workgroups per beam */
     size_t workspace_bytes;
     paella_launch_dims dims;

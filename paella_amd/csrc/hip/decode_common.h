@@ -46,15 +46,35 @@ template <> __device__ __forceinline__ unsigned pack2<F16>(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, f16x2));
 }
 
+// A value of 16 lanes side by side by the vector unit's own lane moves (an exchange through LDS takes ten times as long), and of all 64.
+template <int CONTROL>
+__device__ __forceinline__ float lane_move(float v) { return as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)as_word(v), CONTROL, 0xF, 0xF, false)); }
+template <int CONTROL>
+__device__ __forceinline__ double lane_move(double v) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, CONTROL, 0xF, 0xF, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), CONTROL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+template <typename V, typename Op>
+__device__ __forceinline__ V row_all(V v, Op op) {
+    v = op(v, lane_move<0xB1>(v));   // lane ^ 1
+    v = op(v, lane_move<0x4E>(v));   // lane ^ 2
+    v = op(v, lane_move<0x141>(v));  // the other half of eight, mirrored
+    return op(v, lane_move<0x140>(v));  // the other half of sixteen, mirrored
+}
+template <typename Op>
+__device__ __forceinline__ float wave_all(float v, Op op) {
+    v = row_all(v, op);
+    const float a = as_float(__builtin_amdgcn_readlane(as_word(v), 0)), b = as_float(__builtin_amdgcn_readlane(as_word(v), 16));
+    const float c = as_float(__builtin_amdgcn_readlane(as_word(v), 32)), d = as_float(__builtin_amdgcn_readlane(as_word(v), 48));
+    return op(op(a, b), op(c, d));
+}
 __device__ __forceinline__ float wave_sum_f(float v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+    return wave_all(v, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ float wave_max_f(float v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-    return v;
+    return wave_all(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 // A descriptor over everything behind `base` (uniform over the wave); offsets are 32-bit, sc1 = 16 writes through / reads past this XCD's caches.

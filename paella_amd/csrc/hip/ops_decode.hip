@@ -197,7 +197,9 @@ __device__ __forceinline__ float key_value(unsigned k) { return as_float(k ^ ((k
 constexpr unsigned kLowestKey = 0x00800000u;  // order_key(-FLT_MAX); -inf lies right below
 __device__ __forceinline__ unsigned long long entry(unsigned key, unsigned index) { return (unsigned long long)key << 32 | (0xFFFFFFFFu - index); }
 
-constexpr int kMostLists = 2048;     // beams * splits
+constexpr int kMostLists = 1024;     // beams * splits
+constexpr int kMostStaged = 1024;    // entries that the merge fetches at once
+constexpr int kCounterStride = 32;   // a cache line each: counts on one line go one after the other, 2048 of 32 groups for 7 us
 constexpr int kWaveCandidates = 128;  // of one wave's logits that go on to the workgroup's ranking
 
 struct SelectArgs {
@@ -208,7 +210,7 @@ struct SelectArgs {
     int pad_token, groups, beams, vocab, count, splits;
     unsigned long long* sums;     // [groups * beams * splits]: maximum and sum of exponentials
     unsigned long long* entries;  // [groups * beams * splits][count], best first
-    unsigned* counters;           // [groups], zero between launches
+    unsigned* counters;           // [groups][kCounterStride], zero between launches
     float* out_scores;
     int *out_parents, *out_tokens;
     uint32_t job_id;
@@ -228,12 +230,12 @@ __device__ __forceinline__ u32x4 load_unaligned(const char* p) {
 }
 
 template <typename T, int VALUES>
-__device__ __forceinline__ void load_logits(const char* row, int first, int vocab, unsigned (&key)[VALUES]) {
+__device__ __forceinline__ void load_logits(const char* row, int first, int vocab, float (&x)[VALUES]) {
     constexpr int VEC = 16 / T::bytes;
 #pragma unroll
     for (int i = 0; i < VALUES / VEC; ++i) {
         const int at = first + (i * 256 + (int)threadIdx.x) * VEC;
-        float f[VEC];
+        float* const f = x + i * VEC;
         if (at + VEC <= vocab) {
             const u32x4 w = load_unaligned(row + (size_t)at * T::bytes);
 #pragma unroll
@@ -256,8 +258,85 @@ __device__ __forceinline__ void load_logits(const char* row, int first, int voca
                 }
             }
         }
+    }
+}
+
+// What at least K of the lanes' keys reach (0 where fewer lanes have one): their K-th largest, bit by bit, to the upper 16 bits -- a few more logits
+// pass than would behind all 32, and it takes half the time.
+__device__ __forceinline__ unsigned kth_of_lanes(unsigned key, int K) {
+    unsigned bound = 0;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) key[i * VEC + e] = order_key(f[e] == f[e] ? f[e] : -INFINITY);
+    for (int bit = 31; bit >= 16; --bit) {
+        const unsigned trial = bound | (1u << bit);
+        if (__popcll(__ballot(key >= trial)) >= K) bound = trial;
+    }
+    return bound;
+}
+
+// c / d for c < 2048 by d's reciprocal: the quotient's distance from a whole number is half of 1 / d at least.
+__device__ __forceinline__ int small_div(int c, float inv) { return (int)(((float)c + 0.5f) * inv); }
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// Calls emit(rank, i) for the K best of n (value, where) pairs in LDS, larger values and then smaller places first; no two places are alike.  Few: each
+// counts those ahead of it.  Many (equal logits by the hundred): one after the other.
+template <typename Emit>
+__device__ __forceinline__ void best_of(const double* value, const unsigned* where, int n, int K, Emit emit) {
+    constexpr int kCounted = 512;
+    __shared__ double step_value[4];
+    __shared__ unsigned step_where[4];
+    __shared__ int step_at[4];
+    auto ahead = [](double v, unsigned f, double w, unsigned g) { return (bool)((int)(v > w) | ((int)(v == w) & (int)(f < g))); };
+    if (n <= kCounted) {
+        for (int c = threadIdx.x; c < n; c += 256) {
+            const double v = value[c];
+            const unsigned f = where[c];
+            int rank = 0;
+#pragma unroll 8
+            for (int o = 0; o < n; ++o) rank += ahead(value[o], where[o], v, f);
+            if (rank < K) emit(rank, c);
+        }
+        return;
+    }
+    double taken = INFINITY;  // the pair taken last
+    unsigned taken_where = 0;
+    for (int rank = 0; rank < K; ++rank) {
+        double v = -INFINITY;
+        unsigned f = 0xFFFFFFFFu;
+        int at = -1;
+        for (int c = threadIdx.x; c < n; c += 256)
+            if (ahead(taken, taken_where, value[c], where[c]) && (at < 0 || ahead(value[c], where[c], v, f))) {
+                v = value[c];
+                f = where[c];
+                at = c;
+            }
+        for (int off = 32; off > 0; off >>= 1) {
+            const double w = __shfl_xor(v, off, 64);
+            const unsigned g = __shfl_xor(f, off, 64);
+            const int other = __shfl_xor(at, off, 64);
+            if (other >= 0 && (at < 0 || ahead(w, g, v, f))) {
+                v = w;
+                f = g;
+                at = other;
+            }
+        }
+        if ((threadIdx.x & 63) == 0) {
+            step_value[threadIdx.x >> 6] = v;
+            step_where[threadIdx.x >> 6] = f;
+            step_at[threadIdx.x >> 6] = at;
+        }
+        __syncthreads();
+        at = -1;
+        for (int w = 0; w < 4; ++w)
+            if (step_at[w] >= 0 && (at < 0 || ahead(step_value[w], step_where[w], v, f))) {
+                v = step_value[w];
+                f = step_where[w];
+                at = step_at[w];
+            }
+        taken = v;
+        taken_where = f;
+        if (threadIdx.x == 0) emit(rank, at);
+        __syncthreads();
     }
 }
 
@@ -266,8 +345,8 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
     hook_entry(a.notifier, a.job_id);
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ float wave_top[4], wave_total[4];
-    __shared__ unsigned found, arrived;
-    __shared__ double row_lse[32];
+    __shared__ unsigned wave_bound[4], found, arrived;
+    __shared__ double row_lse[33], row_score[32];
     constexpr int VEC = 16 / T::bytes;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int row = blockIdx.x / a.splits, split = blockIdx.x - row * a.splits;
@@ -277,99 +356,107 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
     if (!a.finished || !a.finished[row]) {
         unsigned long long* const cand = reinterpret_cast<unsigned long long*>(lds);
         const int first = split * 256 * VALUES;
-        unsigned key[VALUES];
-        load_logits<T, VALUES>(a.logits + (size_t)row * a.row_stride, first, a.vocab, key);
+        float x[VALUES];
+        load_logits<T, VALUES>(a.logits + (size_t)row * a.row_stride, first, a.vocab, x);
         if (threadIdx.x == 0) found = 0;
-        unsigned mine = 0;
+        float mine = -INFINITY;  // (a NaN loses against any number)
 #pragma unroll
-        for (int i = 0; i < VALUES; ++i) mine = max(mine, key[i]);
-        const float top = wave_max_f(key_value(mine));
-        const float base = top == -INFINITY ? 0.f : top;
+        for (int i = 0; i < VALUES; ++i) mine = fmaxf(mine, x[i]);
+        const float top = wave_max_f(mine);
+        // 2^(x log2e - base): what the base lost by its rounding is the same in every term and comes back as one factor
+        const float base = top == -INFINITY ? 0.f : top * kLog2e;
         float sum = 0.f;
-        constexpr float kLog2e = 1.44269504088896340736f;
 #pragma unroll
-        for (int i = 0; i < VALUES; ++i) sum += __builtin_amdgcn_exp2f((key_value(key[i]) - base) * kLog2e);
+        for (int i = 0; i < VALUES; ++i) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], kLog2e, -base));
         sum = wave_sum_f(sum);
+        if (sum < INFINITY) {
+            if (top > -INFINITY) sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(top, kLog2e, -base));
+        } else {  // NaN among the logits, a maximum so large (the type's lowest, where everything is masked) that the base overflows, or an infinity
+            sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < VALUES; ++i) sum += x[i] == x[i] ? __builtin_amdgcn_exp2f((x[i] - top) * kLog2e) : 0.f;
+            sum = wave_sum_f(sum);
+        }
         if (lane == 0) {
             wave_top[wave] = top;
             wave_total[wave] = sum;
         }
-        // A bound that at least K of the wave's logits reach: the K-th largest of the lanes' own maxima, found bit by bit.  Few others reach it.
-        unsigned bound = 0;
-#pragma unroll
-        for (int bit = 31; bit >= 0; --bit) {
-            const unsigned trial = bound | (1u << bit);
-            if (__popcll(__ballot(mine >= trial)) >= K) bound = trial;
-        }
-        bound = max(bound, kLowestKey);
-        int over = 0;
-#pragma unroll
-        for (int i = 0; i < VALUES; ++i) over += __popcll(__ballot(key[i] >= bound));
-        unsigned last = 0xFFFFFFFFu;  // of the logits equal to the bound, the index of the last one taken
-        if (over > kWaveCandidates) {  // equal logits, or the best ones in few lanes: the K-th of all of the wave's logits, ties by index
-            unsigned exact = 0;
-            for (int bit = 31; bit >= 0; --bit) {
-                const unsigned trial = exact | (1u << bit);
-                int n = 0;
-#pragma unroll
-                for (int i = 0; i < VALUES; ++i) n += __popcll(__ballot(key[i] >= trial));
-                if (n >= K) exact = trial;
-            }
-            bound = max(exact, kLowestKey);
-            int larger = 0;
-#pragma unroll
-            for (int i = 0; i < VALUES; ++i) larger += __popcll(__ballot(key[i] > bound));
-            last = 0;
-            for (int bit = 19; bit >= 0; --bit) {  // the largest index with fewer than the wanted number of equals below it
-                const unsigned trial = last | (1u << bit);
-                int n = 0;
-#pragma unroll
-                for (int i = 0; i < VALUES; ++i) {
-                    const unsigned index = first + (i / VEC * 256 + threadIdx.x) * VEC + i % VEC;
-                    n += __popcll(__ballot(key[i] == bound && index < trial));
-                }
-                if (n < K - larger) last = trial;
-            }
-            over = larger;
-#pragma unroll
-            for (int i = 0; i < VALUES; ++i) {
-                const unsigned index = first + (i / VEC * 256 + threadIdx.x) * VEC + i % VEC;
-                over += __popcll(__ballot(key[i] == bound && index <= last));
-            }
-        }
+        // A bound that at least K of the workgroup's logits reach, and few others: what a quarter of K of each wave's lanes reach with their best.
+        unsigned bound = kth_of_lanes(order_key(mine), (K + 3) / 4);
+        if (lane == 0) wave_bound[wave] = bound;
         __syncthreads();
-        unsigned at = 0;
-        if (lane == 0) at = atomicAdd(&found, (unsigned)over);  // (the order of the waves' entries does not matter: they are ranked)
-        at = __builtin_amdgcn_readfirstlane(at);
+        bound = max(min(min(wave_bound[0], wave_bound[1]), min(wave_bound[2], wave_bound[3])), kLowestKey);
+        const float least = key_value(bound);
+        unsigned long long* const own = cand + wave * kWaveCandidates;
+        const int lane_base = first + (int)threadIdx.x * VEC;
+        auto behind = [](int i) { return i / VEC * 256 * VEC + i % VEC; };  // of value i, how far behind the lane's first index
+        int taken = 0;
 #pragma unroll
         for (int i = 0; i < VALUES; ++i) {
-            const unsigned index = first + (i / VEC * 256 + threadIdx.x) * VEC + i % VEC;
-            const bool take = key[i] > bound || (key[i] == bound && index <= last);
-            const unsigned long long who = __ballot(take);
+            const unsigned long long who = __ballot(x[i] >= least);
             if (who) {
-                if (take) cand[at + __popcll(who & ((1ull << lane) - 1))] = entry(key[i], index);
-                at += __popcll(who);
+                const int at = taken + __popcll(who & ((1ull << lane) - 1));
+                if (x[i] >= least && at < kWaveCandidates) own[at] = entry(order_key(x[i]), (unsigned)(lane_base + behind(i)));
+                taken += __popcll(who);
             }
         }
+        if (taken > kWaveCandidates) {  // equal logits, or the best ones in few lanes: the K-th of all of the wave's logits, ties by index
+            unsigned key[VALUES];
+#pragma unroll
+            for (int i = 0; i < VALUES; ++i) key[i] = order_key(x[i] == x[i] ? x[i] : -INFINITY);
+            auto count = [&](auto wanted) {
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < VALUES; ++i) n += __popcll(__ballot(wanted(i)));
+                return n;
+            };
+            bound = 0;
+            for (int bit = 31; bit >= 0; --bit) {
+                const unsigned trial = bound | (1u << bit);
+                if (count([&](int i) { return key[i] >= trial; }) >= K) bound = trial;
+            }
+            bound = max(bound, kLowestKey);
+            const int larger = count([&](int i) { return key[i] > bound; });
+            int last = 0;  // the largest index with fewer than the wanted number of equals below it
+            for (int bit = 19; bit >= 0; --bit) {
+                const int trial = last | (1 << bit);
+                if (count([&](int i) { return key[i] == bound && lane_base < trial - behind(i); }) < K - larger) last = trial;
+            }
+            taken = 0;
+#pragma unroll
+            for (int i = 0; i < VALUES; ++i) {
+                const bool take = key[i] > bound || (key[i] == bound && lane_base <= last - behind(i));
+                const unsigned long long who = __ballot(take);
+                if (take) own[taken + __popcll(who & ((1ull << lane) - 1))] = entry(key[i], (unsigned)(lane_base + behind(i)));
+                taken += __popcll(who);
+            }
+        }
+        // one list of the four waves' (their order does not matter: the entries are ranked)
+        unsigned at = 0;
+        if (lane == 0) at = atomicAdd(&found, (unsigned)taken);
+        at = __builtin_amdgcn_readfirstlane(at);
+        unsigned long long* const all = cand + 4 * kWaveCandidates;
+        for (int c = lane; c < taken; c += 64) all[at + c] = own[c];
         __syncthreads();
         const int n = (int)found;
         unsigned long long* const to = a.entries + (size_t)blockIdx.x * K;
         for (int c = threadIdx.x; c < n; c += 256) {
-            const unsigned long long e = cand[c];
+            const unsigned long long e = all[c];
             int rank = 0;
-            for (int o = 0; o < n; ++o) rank += cand[o] > e;
+#pragma unroll 8
+            for (int o = 0; o < n; ++o) rank += all[o] > e;
             if (rank < K) put64(to + rank, e);
         }
         for (int c = n + threadIdx.x; c < K; c += 256) put64(to + c, 0);
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 255) {
             const float m = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
-            double s = 0.;
+            float s = 0.f;
             if (fabsf(m) < INFINITY) {
 #pragma unroll
                 for (int w = 0; w < 4; ++w)
-                    if (wave_total[w] > 0.f) s += (double)wave_total[w] * (double)__builtin_amdgcn_exp2f((wave_top[w] - m) * kLog2e);
+                    if (wave_total[w] > 0.f) s += wave_total[w] * __builtin_amdgcn_exp2f((wave_top[w] - m) * kLog2e);
             }
-            put64(a.sums + blockIdx.x, (unsigned long long)as_word(m) << 32 | as_word((float)s));
+            put64(a.sums + blockIdx.x, (unsigned long long)as_word(m) << 32 | as_word(s));
         }
     }
 
@@ -377,113 +464,168 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     const int lists = a.beams * a.splits;
-    if (threadIdx.x == 0) arrived = __hip_atomic_fetch_add(a.counters + group, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0) arrived = __hip_atomic_fetch_add(a.counters + group * kCounterStride, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     if (__builtin_amdgcn_readfirstlane(arrived) == (unsigned)lists - 1) {
-        // LDS: each list's best value and flat index w * vocab + t, then the lists taken, then the candidates
-        double* const head = reinterpret_cast<double*>(lds);
-        f32x2* const ms = reinterpret_cast<f32x2*>(head + lists);
-        unsigned* const flat = reinterpret_cast<unsigned*>(ms + lists);
-        int* const taken = reinterpret_cast<int*>(flat + lists + (lists & 1));
-        const int most = min(K, lists);
-        double* const value = reinterpret_cast<double*>(taken + K + (K & 1));
-        unsigned* const where = reinterpret_cast<unsigned*>(value + most * K);
-        const int first_list = group * lists;
-        auto ended = [&](int w) { return a.finished && a.finished[group * a.beams + w]; };
-        for (int l = threadIdx.x; l < lists; l += 256) {
-            const int w = l / a.splits;
-            unsigned long long s = 0, e = 0;
-            if (!ended(w)) {
-                s = get64(a.sums + first_list + l);
-                e = get64(a.entries + (size_t)(first_list + l) * K);
+        const bool whole = lists * K <= kMostStaged;  // every list's entries are fetched at once, else the best ones and then those of the lists that matter
+        const int staged = whole ? lists * K : lists, per = whole ? K : 1;
+        // LDS: (maximum, sum) per list, or what has been found; values and flat indices w * vocab + t of the staged entries
+        double* const value = reinterpret_cast<double*>(lds);
+        unsigned* const where = reinterpret_cast<unsigned*>(value + max(staged, min(lists, K) * K));
+        f32x2* const ms = reinterpret_cast<f32x2*>(lds);
+        const int first_list = group * lists, first_row = group * a.beams;
+        const unsigned long long* const from = a.entries + (size_t)first_list * K;
+        auto ended = [&](int w) { return a.finished && a.finished[first_row + w]; };
+        // All trips to memory that do not wait for one another go out together.
+        constexpr int AHEAD = kMostStaged / 256;
+        const float inv_per = 1.f / (float)per, inv_splits = 1.f / (float)a.splits;
+        auto beam_of = [&](int l) { return small_div(l, inv_splits); };
+        unsigned long long e[AHEAD];
+        const double score = (int)threadIdx.x < a.beams ? (double)a.scores[first_row + threadIdx.x] : 0.;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int c = u * 256 + (int)threadIdx.x;
+            e[u] = 0;
+            if (c < staged) {
+                const int l = small_div(c, inv_per);
+                if (!ended(beam_of(l))) e[u] = get64(from + (size_t)l * K + (c - l * per));
             }
+        }
+        for (int l = threadIdx.x; l < lists; l += 256) {
+            const unsigned long long s = ended(beam_of(l)) ? 0 : get64(a.sums + first_list + l);
             ms[l] = f32x2{as_float((unsigned)(s >> 32)), as_float((unsigned)s)};
-            head[l] = e ? (double)key_value((unsigned)(e >> 32)) : -INFINITY;
-            flat[l] = e ? (unsigned)w * a.vocab + (0xFFFFFFFFu - (unsigned)e) : 0xFFFFFFFFu - (unsigned)l;
         }
         if (threadIdx.x == 0) found = 0;
         __syncthreads();
-        if ((int)threadIdx.x < a.beams) {
-            const int w = threadIdx.x;
+        for (int w = threadIdx.x >> 4; w < (a.beams + 15) / 16 * 16; w += 16) {  // a beam's parts by 16 lanes
+            f32x2 p[4];
             float m = -INFINITY;
-            for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ms[w * a.splits + s].x);
-            double total = 0.;
-            for (int s = 0; s < a.splits; ++s) {
-                const f32x2 p = ms[w * a.splits + s];
-                if (p.y > 0.f) total += (double)p.y * exp((double)p.x - (double)m);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int s = i * 16 + (lane & 15);
+                p[i] = f32x2{-INFINITY, 0.f};
+                if (w < a.beams && s < a.splits) p[i] = ms[w * a.splits + s];
+                m = fmaxf(m, p[i].x);
             }
-            row_lse[w] = m == INFINITY ? INFINITY : (double)m + log(total);
+            m = row_all(m, [](float x, float y) { return fmaxf(x, y); });
+            double total = 0.;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (p[i].y > 0.f) total += (double)p[i].y * (double)__builtin_amdgcn_exp2f((p[i].x - m) * kLog2e);
+            total = row_all(total, [](double x, double y) { return x + y; });
+            if ((lane & 15) == 0 && w < a.beams) {
+                row_lse[w] = total;
+                row_score[w] = (double)m;
+            }
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < a.beams) {
+            const double m = row_score[threadIdx.x];
+            row_lse[threadIdx.x] = m == INFINITY ? INFINITY : m + log(row_lse[threadIdx.x]);
+            row_score[threadIdx.x] = score;
         }
         __syncthreads();
         // in 64 bits: 32 would make equals of neighbours, and the lower index would win
-        auto worth = [&](int w, double logit) {
-            const double v = (double)a.scores[group * a.beams + w] + (logit - row_lse[w]);
-            return v > -INFINITY && v < INFINITY ? v : -INFINITY;
+        auto finite = [](double v) { return v > -INFINITY && v < INFINITY ? v : -INFINITY; };
+        auto worth = [&](unsigned long long e, int w) {
+            return e ? finite(row_score[w] + ((double)key_value((unsigned)(e >> 32)) - row_lse[w])) : -INFINITY;
         };
-        for (int l = threadIdx.x; l < lists; l += 256) {
-            const int w = l / a.splits;
-            if (ended(w)) {
-                if (l == w * a.splits) {
-                    const double v = (double)a.scores[group * a.beams + w];
-                    head[l] = v > -INFINITY && v < INFINITY ? v : -INFINITY;
-                    if (head[l] > -INFINITY) flat[l] = (unsigned)w * a.vocab + (unsigned)a.pad_token;
-                }
-            } else if (head[l] > -INFINITY) {
-                head[l] = worth(w, head[l]);
-            }
-        }
-        __syncthreads();
-        // The K lists with the best heads: no other holds one of the K best.
-        for (int l = threadIdx.x; l < lists; l += 256) {
-            const double v = head[l];
-            const unsigned f = flat[l];
-            int rank = 0;
-            for (int o = 0; o < lists; ++o) rank += head[o] > v || (head[o] == v && flat[o] < f);
-            if (rank < K) taken[rank] = l;
-        }
-        __syncthreads();
-        const double least = lists >= K ? head[taken[K - 1]] : -INFINITY;
-        for (int c = threadIdx.x; c < most * K; c += 256) {
-            const int r = c / K, i = c - r * K, l = taken[r], w = l / a.splits;
-            double v = -INFINITY;
-            unsigned f = 0;
-            if (i == 0) {
-                v = head[l];
-                f = flat[l];
-            } else if (!ended(w)) {
-                const unsigned long long e = get64(a.entries + (size_t)(first_list + l) * K + i);
-                if (e) {
-                    v = worth(w, (double)key_value((unsigned)(e >> 32)));
-                    f = (unsigned)w * a.vocab + (0xFFFFFFFFu - (unsigned)e);
-                }
-            }
+        auto flat = [&](unsigned long long e, int w) { return (unsigned)w * a.vocab + (0xFFFFFFFFu - (unsigned)e); };
+        // Of n entries (up to AHEAD * 256 looked at first, by all threads) those that can be among the K best go to LDS: a bound that K of them reach is the
+        // K-th largest of a wave's lanes' best, rounded down to 32 bits.
+        double least = -INFINITY;
+        auto put = [&](double v, unsigned f) {
             if (v > -INFINITY && v >= least) {
                 const unsigned at = atomicAdd(&found, 1u);
                 value[at] = v;
                 where[at] = f;
             }
-        }
-        __syncthreads();
-        const int n = (int)found;
-        const size_t out = (size_t)group * K;
-        for (int c = threadIdx.x; c < n; c += 256) {
-            const double v = value[c];
-            const unsigned f = where[c];
-            int rank = 0;
-            for (int o = 0; o < n; ++o) rank += value[o] > v || (value[o] == v && where[o] < f);
-            if (rank < K) {
-                const unsigned w = f / (unsigned)a.vocab;
-                store_out(a.out_scores + out + rank, (float)v);
-                __hip_atomic_store(a.out_parents + out + rank, (int)w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(a.out_tokens + out + rank, (int)(f - w * (unsigned)a.vocab), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        };
+        double v[AHEAD];
+        unsigned f[AHEAD];
+        auto filter = [&]() {
+            double best = v[0];
+#pragma unroll
+            for (int u = 1; u < AHEAD; ++u) best = fmax(best, v[u]);
+            float down = (float)best;
+            if ((double)down > best) down = as_float(as_word(down) + (down > 0.f ? -1 : 1));  // (to nearest went up; 0 is exact)
+            const unsigned reached = kth_of_lanes(order_key(down), K);
+            if (lane == 0) wave_top[wave] = reached > kLowestKey ? key_value(reached) : -INFINITY;
+            __syncthreads();
+            least = fmax(least, (double)fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3])));
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) put(v[u], f[u]);
+        };
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            v[u] = -INFINITY;
+            f[u] = 0;
+            const int c = u * 256 + (int)threadIdx.x;
+            if (c < staged) {
+                const int w = beam_of(small_div(c, inv_per));
+                if (!ended(w)) {
+                    v[u] = worth(e[u], w);
+                    f[u] = flat(e[u], w);
+                } else if (c == w * a.splits * per) {
+                    v[u] = finite(row_score[w]);
+                    f[u] = (unsigned)w * a.vocab + (unsigned)a.pad_token;
+                }
             }
         }
+        filter();
+        __syncthreads();
+        int n = (int)found;
+        if (!whole) {  // these were the lists' best: the K best lists hold the K best entries
+            __shared__ unsigned taken_list[64];
+            const int most = min(n, K);
+            best_of(value, where, n, K, [&](int rank, int i) {
+                const unsigned w = where[i] / (unsigned)a.vocab, t = where[i] - w * (unsigned)a.vocab;
+                taken_list[rank] = w * (unsigned)a.splits + (ended(w) ? 0 : t / (256 * VALUES));
+                if (rank == K - 1) row_lse[32] = value[i];
+            });
+            __syncthreads();
+            if (n >= K) least = row_lse[32];  // what the last of them begins with
+            if (threadIdx.x == 0) found = 0;
+            auto fetch = [&](int c, double& v, unsigned& f) {  // the lists' first entries first: they give the better bound
+                v = -INFINITY;
+                f = 0;
+                if (c >= most * K) return;
+                const int i = c / most, l = (int)taken_list[c - i * most], w = beam_of(l);
+                if (!ended(w)) {
+                    const unsigned long long e = get64(from + (size_t)l * K + i);
+                    v = worth(e, w);
+                    f = flat(e, w);
+                } else if (i == 0) {
+                    v = row_score[w];
+                    f = (unsigned)w * a.vocab + (unsigned)a.pad_token;
+                }
+            };
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) fetch(u * 256 + (int)threadIdx.x, v[u], f[u]);
+            filter();
+            for (int c = AHEAD * 256 + (int)threadIdx.x; c < most * K; c += 256) {
+                double v;
+                unsigned f;
+                fetch(c, v, f);
+                put(v, f);
+            }
+            __syncthreads();
+            n = (int)found;
+        }
+        const size_t out = (size_t)group * K;
+        best_of(value, where, n, K, [&](int rank, int i) {
+            if (i < 0) return;
+            const unsigned w = where[i] / (unsigned)a.vocab;
+            store_out(a.out_scores + out + rank, (float)value[i]);
+            __hip_atomic_store(a.out_parents + out + rank, (int)w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(a.out_tokens + out + rank, (int)(where[i] - w * (unsigned)a.vocab), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        });
         for (int c = n + threadIdx.x; c < K; c += 256) {
             store_out(a.out_scores + out + c, -INFINITY);
             __hip_atomic_store(a.out_parents + out + c, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __hip_atomic_store(a.out_tokens + out + c, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        if (threadIdx.x == 0) __hip_atomic_store(a.counters + group, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (threadIdx.x == 0) __hip_atomic_store(a.counters + group * kCounterStride, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     hook_exit(a.notifier, a.job_id);
 }
@@ -561,11 +703,11 @@ int append_check(const paella_kv_append_desc* d, const paella_kv_cache* c, const
     return 0;
 }
 
-// LDS of a selection: the wave's candidates of the pass over the logits, and the merge's lists, in the same place.
+// LDS of a selection: the waves' candidates of the pass over the logits and their common list, and the merge's entries, in the same place.
 unsigned select_lds(const paella_beam_select_plan* p) {
-    const unsigned lists = p->beams * p->splits, most = (unsigned)p->count < lists ? p->count : lists;
-    const unsigned merge = lists * 20 + (lists & 1) * 4 + (p->count + (p->count & 1)) * 4 + most * p->count * 12;
-    const unsigned pass = 4 * kWaveCandidates * 8;
+    const unsigned lists = p->beams * p->splits, taken = ((unsigned)p->count < lists ? p->count : lists) * p->count;
+    const unsigned staged = lists * p->count <= kMostStaged ? lists * p->count : lists;
+    const unsigned merge = (staged > taken ? staged : taken) * 12, pass = 8 * kWaveCandidates * 8;
     return ((merge > pass ? merge : pass) + 15) / 16 * 16;
 }
 
@@ -624,13 +766,13 @@ int paella_beam_select_plan_make(int dtype, int groups, int beams, int vocab, in
     if (beams > 32 || vocab > 524288 || count > 64) return PAELLA_ENOSUP;
     *p = paella_beam_select_plan{};
     p->dtype = dtype; p->groups = groups; p->beams = beams; p->vocab = vocab; p->count = count;
-    // 32 logits per thread where that still gives two workgroups per compute unit, else 8 (up to the 64 lists per beam that the merge takes)
+    // 32 logits per thread where that still gives every compute unit a workgroup, else 8 (up to the 64 lists per beam that the merge takes)
     const int long_splits = (vocab + 8191) / 8192, short_splits = (vocab + 2047) / 2048;
-    p->values = (double)groups * beams * long_splits >= 512 || short_splits > 64 ? 32 : 8;
+    p->values = (double)groups * beams * long_splits >= 256 || short_splits > 64 || beams * short_splits > kMostLists ? 32 : 8;
     p->splits = p->values == 32 ? long_splits : short_splits;
     if (!select_plan_ok(p)) return PAELLA_ENOSUP;
     const size_t lists = (size_t)groups * beams * p->splits;
-    p->workspace_bytes = up256((size_t)groups * 4) + up256(lists * 8) + lists * count * 8;
+    p->workspace_bytes = up256((size_t)groups * 4 * kCounterStride) + up256(lists * 8) + lists * count * 8;
     set_launch_dims(&p->dims, (unsigned)lists, 256, select_lds(p), 64);
     p->flops = 4.0 * groups * beams * vocab;
     p->bytes = (double)groups * beams * vocab * element_bytes(dtype) + groups * (beams * 4.0 + count * 12.0);
@@ -656,7 +798,7 @@ int paella_beam_select_launch(const paella_beam_select_plan* p, const void* logi
     a.logits = (const char*)logits; a.row_stride = row_stride * size; a.scores = scores; a.finished = finished;
     a.pad_token = pad_token; a.groups = p->groups; a.beams = p->beams; a.vocab = p->vocab; a.count = p->count; a.splits = p->splits;
     a.counters = (unsigned*)workspace;
-    a.sums = (unsigned long long*)((char*)workspace + up256((size_t)p->groups * 4));
+    a.sums = (unsigned long long*)((char*)workspace + up256((size_t)p->groups * 4 * kCounterStride));
     a.entries = (unsigned long long*)((char*)a.sums + up256(lists * 8));
     a.out_scores = out_scores; a.out_parents = out_parents; a.out_tokens = out_tokens;
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
