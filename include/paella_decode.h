@@ -12,8 +12,9 @@
  *
  * Device data that the host cannot check is checked where it is used: a page number outside the cache, or a token
  * beyond its row of the table, is never written and takes no part in attention; a negative length counts as 0; no
- * access leaves the tensors whatever the numbers are.  `starts` has to begin with 0 and must not decrease; the outputs
- * of a call that breaks this are undefined, and so is the workspace of an attention call (fill it with zeros again).
+ * access leaves the tensors whatever the numbers are.  `starts` has to begin with 0 and must not decrease, nor grow by more than
+ * max_new from one entry to the next; the outputs of a call that breaks this are undefined, and so is the workspace of an attention
+ * call (fill it with zeros again).
  */
 #ifndef PAELLA_DECODE_H
 #define PAELLA_DECODE_H
@@ -38,8 +39,7 @@ typedef struct paella_kv_cache {
 
 /* The new tokens of a batch.  Row t of queries, keys, values and outputs belongs to sequence b for starts[b] <= t <
  * starts[b + 1] (starts NULL: every sequence has max_new rows); as new token j = t - starts[b] it is the sequence's own
- * token past[b] + j, at position prefix_len + past[b] + j.  Rows behind the last sequence, and rows of a sequence beyond
- * its first max_new, are neither read nor written. */
+ * token past[b] + j, at position prefix_len + past[b] + j.  Rows behind the last sequence are neither read nor written. */
 typedef struct paella_kv_batch {
     int sequences;
     int max_new;                 /* most new tokens of any sequence */
@@ -80,6 +80,7 @@ typedef struct paella_prefix_attention_plan {
     float scale;                 /* of the products of queries and keys; set by the plan to 1 / sqrt(head_dim) where 0 is asked for */
     int prefix_rows, own_rows;   /* query rows (a head of a token each) of a workgroup over the prefix / over a sequence's own tokens */
     int prefix_splits, own_splits;  /* workgroups that share a row's keys, each */
+    int stages;                  /* launches of a call: 2 where the parts of a row's keys are joined by a launch of their own */
     size_t workspace_bytes;      /* 0 where one workgroup does all of a row's keys */
     paella_launch_dims dims;
     double flops;                /* algorithmic, every sequence as long as its table: 4 * head_dim per query head and key */
@@ -91,13 +92,17 @@ typedef struct paella_prefix_attention_plan {
  * gives zeros.  Keys and values in excluded places may hold anything; those of a sequence's later new tokens must be finite.
  * head_dim 64, 128 or 256 (PAELLA_ENOSUP otherwise).  Pure host arithmetic; of the cache and the batch, only the extents are looked at. */
 int paella_prefix_attention_plan_make(const paella_kv_cache* cache, const paella_kv_batch* batch, int heads, float scale, paella_prefix_attention_plan* plan);
-/* Launch shape with the register count and LDS of the kernel that is launched (the plan's own figures without a device). */
-int paella_prefix_attention_dims(const paella_prefix_attention_plan* plan, paella_launch_dims* dims);
+/* Launch shape of a stage with the register count and LDS of the kernel that is launched (the plan's own figures without a device). */
+int paella_prefix_attention_dims(const paella_prefix_attention_plan* plan, int stage, paella_launch_dims* dims);
 /* q: rows of heads * head_dim values, q_stride (a multiple of 8) from one row to the next; out: [tokens][heads][head_dim], not
  * overlapping q.  Cache and batch must have the plan's extents.  workspace: workspace_bytes, zero-filled once before its first use,
- * private to the request (launches that share it must not overlap); NULL where workspace_bytes is 0. */
+ * private to the request (launches that share it must not overlap); NULL where workspace_bytes is 0.  Issues all stages in order, the last
+ * of which reports to `notifier`; PAELLA_ENOSUP for two stages on a queue that keeps no order: there the caller issues them one after
+ * the other with paella_prefix_attention_launch_stage, the second once the first has finished. */
 int paella_prefix_attention_launch(const paella_prefix_attention_plan* plan, const paella_kv_cache* cache, const paella_kv_batch* batch, const void* q,
                                    int64_t q_stride, void* out, void* workspace, void* stream, uint32_t job_id, void* notifier);
+int paella_prefix_attention_launch_stage(const paella_prefix_attention_plan* plan, int stage, const paella_kv_cache* cache, const paella_kv_batch* batch,
+                                         const void* q, int64_t q_stride, void* out, void* workspace, void* stream, uint32_t job_id, void* notifier);
 
 /* ---------------------------------------------------------------- beam search */
 

@@ -23,7 +23,7 @@ class KvAppendDesc(ctypes.Structure):
 
 class PrefixAttentionPlan(ctypes.Structure):
     _fields_ = [(n, c_int) for n in ("dtype", "heads", "kv_heads", "head_dim", "page_size", "sequences", "max_new", "tokens", "max_pages", "prefix_len")] + \
-               [("scale", c_float)] + [(n, c_int) for n in ("prefix_rows", "own_rows", "prefix_splits", "own_splits")] + \
+               [("scale", c_float)] + [(n, c_int) for n in ("prefix_rows", "own_rows", "prefix_splits", "own_splits", "stages")] + \
                [("workspace_bytes", c_size_t), ("dims", LaunchDims), ("flops", c_double), ("bytes", c_double)]
 
 
@@ -43,7 +43,8 @@ DECODE_SYMBOLS = {
     "paella_kv_append_dims": (c_int, [_p(KvAppendDesc), _p(KvCache), _p(KvBatch), _p(LaunchDims)]),
     "paella_kv_append_launch": (c_int, [_p(KvAppendDesc), _p(KvCache), _p(KvBatch)] + [c_void_p] * 7 + _TAIL),
     "paella_prefix_attention_plan_make": (c_int, [_p(KvCache), _p(KvBatch), c_int, c_float, _p(PrefixAttentionPlan)]),
-    "paella_prefix_attention_dims": (c_int, [_p(PrefixAttentionPlan), _p(LaunchDims)]),
+    "paella_prefix_attention_dims": (c_int, [_p(PrefixAttentionPlan), c_int, _p(LaunchDims)]),
+    "paella_prefix_attention_launch_stage": (c_int, [_p(PrefixAttentionPlan), c_int, _p(KvCache), _p(KvBatch), c_void_p, c_i64, c_void_p, c_void_p] + _TAIL),
     "paella_prefix_attention_launch": (c_int, [_p(PrefixAttentionPlan), _p(KvCache), _p(KvBatch), c_void_p, c_i64, c_void_p, c_void_p] + _TAIL),
     "paella_beam_select_plan_make": (c_int, [c_int] * 5 + [_p(BeamSelectPlan)]),
     "paella_beam_select_dims": (c_int, [_p(BeamSelectPlan), _p(LaunchDims)]),

@@ -13,15 +13,19 @@ using namespace paella;
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 AttentionKernel kernel_of(const paella_prefix_attention_plan* p) {
-    const int rp = p->prefix_rows / 16, ro = p->own_rows / 16;
+    const int rp = p->prefix_rows, ro = p->own_rows;
     return p->dtype == PAELLA_F32 ? attention_kernel_f32(p->head_dim, rp, ro)
                                   : p->dtype == PAELLA_BF16 ? attention_kernel_bf16(p->head_dim, rp, ro) : attention_kernel_f16(p->head_dim, rp, ro);
+}
+
+AttentionKernel join_of(const paella_prefix_attention_plan* p) {
+    return p->dtype == PAELLA_F32 ? attention_join_f32(p->head_dim) : p->dtype == PAELLA_BF16 ? attention_join_bf16(p->head_dim) : attention_join_f16(p->head_dim);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Grid {
-    int64_t prefix_tiles, own_tiles, prefix_items, own_items;
+    int64_t prefix_tiles, own_tiles, prefix_items, own_items, all;
 };
 
 Grid grid_of(const paella_prefix_attention_plan* p) {
@@ -31,6 +35,7 @@ Grid grid_of(const paella_prefix_attention_plan* p) {
     g.own_tiles = ceil_div(p->max_new * per_kv, p->own_rows);
     g.prefix_items = g.prefix_tiles * p->kv_heads * p->prefix_splits;
     g.own_items = p->sequences * g.own_tiles * p->kv_heads * p->own_splits;
+    g.all = (ceil_div(g.prefix_items, 8) + ceil_div(g.own_items, 8)) * 8;  // the two kinds alternate by eights
     return g;
 }
 
@@ -46,7 +51,16 @@ bool plan_ok(const paella_prefix_attention_plan* p) {
         return false;
     if (p->own_splits <= 0 || p->own_splits > 64 || p->prefix_splits < 0 || p->prefix_splits > 64 || (p->prefix_splits > 0) != (p->prefix_len > 0)) return false;
     const Grid g = grid_of(p);
-    return (double)g.prefix_items + (double)g.own_items < 1e9;
+    return (double)g.all < 1e9;
+}
+
+// Whether the workgroup that arrives last at a row joins it, or a launch of its own: a joining workgroup makes this many trips to memory one after the other,
+// each above a microsecond; the other launch costs as much as some four.
+int stages_of(const paella_prefix_attention_plan* p) {
+    const int parts = p->prefix_splits + p->own_splits;
+    if (parts == 1) return 1;
+    const int rows = p->prefix_splits && p->prefix_rows > p->own_rows ? p->prefix_rows : p->own_rows;
+    return ceil_div(rows * p->head_dim / 4, 256) * ceil_div(parts, kJoined) <= 4 ? 1 : 2;
 }
 
 size_t workspace_of(const paella_prefix_attention_plan* p) {
@@ -67,12 +81,11 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return PAELLA_ENOSUP;
     if (!extents_ok(p)) return PAELLA_ENOSUP;
     const int64_t per_kv = heads / c->kv_heads, size = element_bytes(c->dtype), row_bytes = c->head_dim * size;
-    // rows of a tile: as many as there are, up to what the registers hold beside a step of keys
-    const int most = row_bytes <= 256 ? 64 : row_bytes <= 512 && c->head_dim <= 128 ? 32 : 16;
-    auto rows = [&](int64_t n) { return n <= 16 || most == 16 ? 16 : n <= 32 || most == 32 ? 32 : 64; };
+    // Rows of a workgroup: where there are few its waves split the keys, else each has rows of its own (see the kernels).
+    auto rows = [&](int64_t n) { return c->head_dim > 128 ? (n <= 16 ? 16 : 64) : n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 || row_bytes > 256 ? 64 : 128; };
     p->own_rows = rows(b->max_new * per_kv);
     p->prefix_rows = p->prefix_len ? rows(b->tokens * per_kv) : p->own_rows;
-    if (p->prefix_rows < p->own_rows) p->prefix_rows = p->own_rows;
+    if (p->own_rows == 64 && p->prefix_rows == 128) p->own_rows = 128;
     // A row's keys are shared by as many workgroups as fill the device twice, each with two steps per wave at least.
     const int step = size == 4 ? 16 : 32;
     auto splits = [&](int64_t others, int64_t keys) {
@@ -87,24 +100,25 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_
     if (!plan_ok(p)) return PAELLA_ENOSUP;
     g = grid_of(p);
     p->workspace_bytes = workspace_of(p);
-    set_launch_dims(&p->dims, (unsigned)(g.prefix_items + g.own_items), 256, 0, 256);
+    p->stages = stages_of(p);
+    set_launch_dims(&p->dims, (unsigned)g.all, 256, 0, 256);
     const double keys = (double)b->max_pages * c->page_size;
     p->flops = 4.0 * c->head_dim * b->tokens * heads * (p->prefix_len + keys);
     p->bytes = 2.0 * (p->prefix_len + b->sequences * keys) * c->kv_heads * row_bytes + 2.0 * b->tokens * heads * row_bytes;
     return 0;
 }
 
-int paella_prefix_attention_dims(const paella_prefix_attention_plan* p, paella_launch_dims* dims) {
-    if (!plan_ok(p) || !dims) return PAELLA_EINVAL;
-    const Grid g = grid_of(p);
-    set_launch_dims(dims, (unsigned)(g.prefix_items + g.own_items), 256, 0, 256);
-    loaded_dims((const void*)kernel_of(p), dims);
+int paella_prefix_attention_dims(const paella_prefix_attention_plan* p, int stage, paella_launch_dims* dims) {
+    if (!plan_ok(p) || !dims || stage < 0 || stage >= stages_of(p)) return PAELLA_EINVAL;
+    if (stage) set_launch_dims(dims, (unsigned)ceil_div((int64_t)p->tokens * p->heads, 1024 / p->head_dim), 256, 0, 64);
+    else set_launch_dims(dims, (unsigned)grid_of(p).all, 256, 0, 256);
+    loaded_dims((const void*)(stage ? join_of(p) : kernel_of(p)), dims);
     return 0;
 }
 
-int paella_prefix_attention_launch(const paella_prefix_attention_plan* p, const paella_kv_cache* c, const paella_kv_batch* b, const void* q, int64_t q_stride,
-                                   void* out, void* workspace, void* stream, uint32_t job_id, void* notifier) {
-    if (!plan_ok(p) || !cache_ok(c) || !batch_ok(b) || !q || !out) return PAELLA_EINVAL;
+int paella_prefix_attention_launch_stage(const paella_prefix_attention_plan* p, int stage, const paella_kv_cache* c, const paella_kv_batch* b, const void* q,
+                                         int64_t q_stride, void* out, void* workspace, void* stream, uint32_t job_id, void* notifier) {
+    if (!plan_ok(p) || !cache_ok(c) || !batch_ok(b) || !q || !out || stage < 0 || stage >= stages_of(p)) return PAELLA_EINVAL;
     if (c->dtype != p->dtype || c->kv_heads != p->kv_heads || c->head_dim != p->head_dim || c->page_size != p->page_size || b->sequences != p->sequences ||
         b->max_new != p->max_new || b->tokens != p->tokens || b->max_pages != p->max_pages || b->prefix_len != p->prefix_len)
         return PAELLA_EINVAL;
@@ -125,14 +139,27 @@ int paella_prefix_attention_launch(const paella_prefix_attention_plan* p, const 
     a.page_blocks_inv = a.page_blocks == 1 ? 0xFFFFFFFFu : (unsigned)(0x100000000ull / a.page_blocks);
     a.scale_log2 = p->scale * 1.44269504088896340736f;
     a.prefix_tiles = (int)g.prefix_tiles; a.prefix_splits = p->prefix_splits; a.own_tiles = (int)g.own_tiles; a.own_splits = p->own_splits;
-    a.prefix_items = (unsigned)g.prefix_items;
+    a.prefix_items = (unsigned)g.prefix_items; a.own_items = (unsigned)g.own_items;
     const size_t parts = (size_t)p->prefix_splits + p->own_splits, rows = (size_t)p->tokens * p->heads;
-    a.counters = need ? (unsigned*)workspace : nullptr;
+    a.counters = need && stages_of(p) == 1 ? (unsigned*)workspace : nullptr;
     a.ml = need ? (f32x2*)((char*)workspace + up256(rows * 4)) : nullptr;
     a.acc = need ? (float*)((char*)a.ml + up256(parts * rows * 8)) : nullptr;
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
-    launch(kernel_of(p), dim3((unsigned)(g.prefix_items + g.own_items)), dim3(256), 0, (hipStream_t)stream, a);
+    const unsigned grid = stage ? (unsigned)ceil_div((int64_t)rows, 1024 / p->head_dim) : (unsigned)g.all;
+    launch(stage ? join_of(p) : kernel_of(p), dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
+}
+
+int paella_prefix_attention_launch(const paella_prefix_attention_plan* p, const paella_kv_cache* c, const paella_kv_batch* b, const void* q, int64_t q_stride,
+                                   void* out, void* workspace, void* stream, uint32_t job_id, void* notifier) {
+    if (!plan_ok(p)) return PAELLA_EINVAL;
+    const int stages = stages_of(p);
+    if (stages > 1) {
+        const DirectQueue* queue = direct_queue_lookup(stream);
+        if (queue && !direct_queue_ordered(queue)) return PAELLA_ENOSUP;
+        if (int rc = paella_prefix_attention_launch_stage(p, 0, c, b, q, q_stride, out, workspace, stream, job_id, nullptr)) return rc;
+    }
+    return paella_prefix_attention_launch_stage(p, stages - 1, c, b, q, q_stride, out, workspace, stream, job_id, notifier);
 }
 
 }  // extern "C"

@@ -3,4 +3,5 @@
 
 namespace paella {
 AttentionKernel attention_kernel_bf16(int dim, int rp, int ro) { return attention_kernel<Bf16>(dim, rp, ro); }
+AttentionKernel attention_join_bf16(int dim) { return attention_join<Bf16>(dim); }
 }  // namespace paella

@@ -4,17 +4,18 @@
 //
 // out = sum_i p_i v_i / sum_i p_i with p_i = exp(scale * q . k_i - m): one pass over the keys with the running maximum m and sum, in 32 bits.
 //
-// Work.  A workgroup takes either a tile of up to 64 query rows (a row: a head of a new token; all heads that share a key head, of all
-// sequences, side by side) over a part of the prefix, or the rows of one sequence over a part of its own tokens; its four waves take every
-// fourth step of 32 (fp32: 16) keys each and put their sums together in LDS.  What the workgroups of a row leave is put together by the one
-// that arrives last at the row (a counter per row), in the order of the parts, so results do not depend on who that is.
+// Work.  A workgroup takes either a tile of query rows (a row: a head of a new token; all heads that share a key head, of all sequences, side by
+// side) over a part of the prefix, or rows of one sequence over a part of its own tokens.  Up to 32 rows: all four waves have them, each takes every fourth
+// step of 32 (fp32: 16) keys, and their sums are put together in LDS.  More: each wave has 16 or 32 rows of its own, and the workgroup
+// brings the keys to LDS for all of them.  What the workgroups of a row leave is put together by the one that arrives last at the row (a
+// counter per row), in the order of the parts, so results do not depend on who that is.
 //
-// Registers instead of LDS.  With v_mfma_*_16x16 and the products turned round (scores^T = K q^T, out^T = V^T p^T), every operand comes
-// straight from memory or from the other product's result: lane l of a wave holds query row l % 16 throughout; lane group l / 16 gets the scores
+// Operands.  With v_mfma_*_16x16 and the products turned round (scores^T = K q^T, out^T = V^T p^T), every operand comes
+// as it lies in the cache or from the other product's result: lane l of a wave holds query row l % 16 throughout; lane group l / 16 gets the scores
 // of exactly the keys whose probabilities it has to supply to the second product (the key that row m of score tile t stands for is
 // m / 4 * TPL + 4 t + m % 4, TPL = 4 * tiles), and of V a lane loads TPL whole keys by 16 bytes, its group's keys by 16 lanes' dimensions: the 16-bit
 // types need one byte permutation per operand register to put a dimension's keys side by side, fp32 none.  The output's dimensions are
-// permuted by the same rule.  K and V are therefore read once per wave, in runs of 64 bytes and of whole keys, and both wait in registers for
+// permuted by the same rule.  Where the waves split the keys, K and V are therefore read once, in runs of 64 bytes and of whole keys, and wait in registers for
 // one step while the other product runs.
 
 #include <hip/hip_runtime.h>
@@ -33,13 +34,15 @@ struct AttentionArgs {
     unsigned page_blocks, page_blocks_inv;  // blocks of 8 tokens in a page, and 2^32 over that, rounded down
     float scale_log2;                       // scale * log2(e): probabilities are powers of two
     int prefix_tiles, prefix_splits, own_tiles, own_splits;
-    unsigned prefix_items;
-    unsigned* counters;  // [tokens * heads], zero between launches
+    unsigned prefix_items, own_items;
+    unsigned* counters;  // [tokens * heads], zero between launches; null where a launch of its own joins
     f32x2* ml;           // [splits][tokens * heads]: running maximum and sum of each part
     float* acc;          // [splits][tokens * heads][head_dim]
     uint32_t job_id;
     Notifier* notifier;
 };
+
+constexpr int kJoined = 8;  // parts of a row that are requested together
 
 template <typename T> struct Mfma;
 template <> struct Mfma<Bf16> {
@@ -62,36 +65,46 @@ struct Keys {
     int table_len;
     const char *k, *v;   // the cache, moved to the key head
     size_t page_bytes;
-    unsigned page_blocks, page_blocks_inv, num_pages;
+    unsigned page_blocks, page_blocks_inv, num_pages;  // a block: 8 keys, which never lie in two pages
+
+    struct Place {
+        unsigned entry, in;  // of the table, and the block's place in the page
+    };
+    // Where block b lies; beyond the table's end in the last entry (the caller's limits mask what is read).
+    __device__ __forceinline__ Place place_of(unsigned b) const {
+        unsigned page = __umulhi(b, page_blocks_inv), in = b - page * page_blocks;
+        if (in >= page_blocks) {
+            ++page;
+            in -= page_blocks;
+        }
+        return {min(page, (unsigned)table_len - 1), in};
+    }
+    __device__ __forceinline__ size_t page_at(int page) const { return ((unsigned)page < num_pages ? (unsigned)page : 0u) * page_bytes; }
 };
 
+// 16 R query rows of a wave: what they have summed so far.  Lane l holds row l % 16 of each 16.
 template <typename T, int D, int R>
-struct AttentionTile {
+struct AttentionRows {
     static constexpr bool F = T::bytes == 4;
     static constexpr int NT = F ? 1 : 2;              // score tiles of 16 keys per step
     static constexpr int TPL = 4 * NT;                // keys of a step that a lane group supplies to the second product
     static constexpr int STEP = 16 * NT;
-    static constexpr int KC = D * T::bytes / 64;      // 16-byte pieces of a key row per lane
-    static constexpr int PER = D / 16 * T::bytes < 16 ? D / 16 : 16 / T::bytes;  // neighbouring dimensions that a lane loads of V
+    static constexpr int ROW = D * T::bytes;          // bytes of a key
+    static constexpr int KC = ROW / 64;               // 16-byte pieces of a key per lane
+    static constexpr int PER = D / 16 * T::bytes < 16 ? D / 16 : 16 / T::bytes;  // neighbouring dimensions that a lane has of V
     static constexpr int GRP = D / 16 / PER;
     static constexpr int VW = PER * T::bytes / 4;     // words of such a piece
-    static constexpr int ROW = D * T::bytes;
 
     f32x4 acc[R][GRP * PER];
-    float m[R], l[R];
+    f32x4 total[R];  // sums of the probabilities; 16-bit types: of the rounded ones, so that what the rounding does to a row's largest weights cancels
+    float m[R];
     u32x4 q[R][KC];
-    u32x4 k[NT][KC];
-    unsigned v[TPL][GRP * VW];
-
-    // page numbers of a lane's blocks of 8 keys in the step whose keys are loaded next, and the blocks' places in them
-    int page_k, page_v;
-    unsigned in_k, in_v;
 
     __device__ __forceinline__ void begin() {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             m[r] = -INFINITY;
-            l[r] = 0.f;
+            total[r] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int d = 0; d < GRP * PER; ++d) acc[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
@@ -102,61 +115,9 @@ struct AttentionTile {
         for (int c = 0; c < KC; ++c) q[r][c] = *reinterpret_cast<const u32x4*>(row + c * 64 + (lane >> 4) * 16);
     }
 
-    // The pages of the step that begins at block b8 (of 8 keys); beyond the table a lane reads the last entry and is masked by the caller's limit.
-    __device__ __forceinline__ void look_up(const Keys& s, unsigned b8, int lane) {
-        constexpr int BLOCK_LANES_K = F ? 8 : 4;  // rows of the score tile that lie in one block
-        const unsigned bk = b8 + (unsigned)(lane & 15) / BLOCK_LANES_K, bv = b8 + (unsigned)(lane >> 4) * TPL / 8;
-        auto split = [&](unsigned b, unsigned& in) {
-            unsigned page = __umulhi(b, s.page_blocks_inv);
-            in = b - page * s.page_blocks;
-            if (in >= s.page_blocks) {
-                ++page;
-                in -= s.page_blocks;
-            }
-            return min(page, (unsigned)s.table_len - 1);
-        };
-        const unsigned ik = split(bk, in_k), iv = split(bv, in_v);
-        page_k = s.table[ik];
-        page_v = s.table[iv];
-    }
-
-    __device__ __forceinline__ void load_k(const Keys& s, int lane) {
-        const unsigned page = (unsigned)page_k < s.num_pages ? page_k : 0;
-        const int mm = lane & 15;
-        const unsigned slot = F ? in_k * 8 + (mm & 7) : in_k * 8 + (mm & 3);
-        const char* p = s.k + page * s.page_bytes + (size_t)slot * ROW + (lane >> 4) * 16;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int c = 0; c < KC; ++c) k[t][c] = *reinterpret_cast<const u32x4*>(p + t * 4 * ROW + c * 64);
-    }
-
-    __device__ __forceinline__ void load_v(const Keys& s, int lane) {
-        const unsigned page = (unsigned)page_v < s.num_pages ? page_v : 0;
-        const unsigned slot = in_v * 8 + (F ? (lane >> 4 & 1) * 4 : 0);
-        const char* p = s.v + page * s.page_bytes + (size_t)slot * ROW + (lane & 15) * PER * T::bytes;
-#pragma unroll
-        for (int u = 0; u < TPL; ++u)
-#pragma unroll
-            for (int g = 0; g < GRP; ++g) {
-                const char* at = p + u * ROW + g * 16 * PER * T::bytes;
-                if constexpr (VW == 4) {
-                    const u32x4 w = *reinterpret_cast<const u32x4*>(at);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[u][g * 4 + e] = w[e];
-                } else {
-                    const u32x2 w = *reinterpret_cast<const u32x2*>(at);
-                    v[u][g * 2] = w.x;
-                    v[u][g * 2 + 1] = w.y;
-                }
-            }
-    }
-
-    // One step over the keys from `first` on, of which row r sees those below limit[r]; `least` and `most` bound the limits of all rows, `absent`: this
-    // lane group's keys are in no page.  next(true) is called once K is no longer needed, next(false) once V is.
-    template <typename Next>
-    __device__ __forceinline__ void step(int first, const bool absent, const int (&limit)[R], int least, int most, float scale, int lane, Next next) {
-        f32x4 x[R][NT];
+    // x = K q^T of a step's keys; k(t, c): the lane's piece c of its key of score tile t
+    template <typename K>
+    __device__ __forceinline__ void scores(f32x4 (&x)[R][NT], K k) const {
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -165,34 +126,32 @@ struct AttentionTile {
         for (int c = 0; c < KC; ++c)
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
+                const u32x4 piece = k(t, c);
                 if constexpr (F) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
-                        for (int r = 0; r < R; ++r) x[r][t] = mfma_f32(as_float(k[t][c][e]), as_float(q[r][c][e]), x[r][t]);
+                        for (int r = 0; r < R; ++r) x[r][t] = mfma_f32(as_float(piece[e]), as_float(q[r][c][e]), x[r][t]);
                 } else {
 #pragma unroll
-                    for (int r = 0; r < R; ++r) x[r][t] = Mfma<T>::go(k[t][c], q[r][c], x[r][t]);
+                    for (int r = 0; r < R; ++r) x[r][t] = Mfma<T>::go(piece, q[r][c], x[r][t]);
                 }
             }
-        next(true);
-        if (first + STEP > least || __any(absent)) {
-            const int mine = first + (lane >> 4) * TPL;
+    }
+
+    // Row r sees the keys below limit[r]; `first`: of the lane group's keys; absent: they are in no page
+    __device__ __forceinline__ static void mask(f32x4 (&x)[R][NT], int first, bool absent, const int (&limit)[R]) {
 #pragma unroll
-            for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (absent || mine + t * 4 + e >= limit[r]) x[r][t][e] = -INFINITY;
-            // what lies in places that no row may see can be anything, and 0 * NaN is NaN
-#pragma unroll
-            for (int u = 0; u < TPL; ++u)
-                if (absent || mine + u >= most) {
-#pragma unroll
-                    for (int w = 0; w < GRP * VW; ++w) v[u][w] = 0;
-                }
-        }
+                for (int e = 0; e < 4; ++e)
+                    if (absent || first + t * 4 + e >= limit[r]) x[r][t][e] = -INFINITY;
+    }
+
+    // Scores to probabilities, as operands of the second product.
+    __device__ __forceinline__ void weigh(const f32x4 (&x)[R][NT], float scale, unsigned (&p)[R][4]) {
         // The running maximum moves only when a score is above it by a factor of 2^8: until then probabilities are at most 256 (their sums stay in
         // 32 bits, and 16-bit ones keep their relative precision), and neither the lanes' exchange nor the rescaling is needed.
         bool grown = false;
@@ -215,12 +174,11 @@ struct AttentionTile {
                 now = fmaxf(now, __shfl_xor(now, 32, 64));
                 const float shrink = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - now);
                 m[r] = now;
-                l[r] *= shrink;
+                total[r] *= shrink;
 #pragma unroll
                 for (int d = 0; d < GRP * PER; ++d) acc[r][d] *= shrink;
             }
         }
-        unsigned p[R][4];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const float base = m[r] == -INFINITY ? 0.f : m[r];
@@ -229,18 +187,23 @@ struct AttentionTile {
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[t * 4 + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r][t][e], scale, -base));
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < TPL; ++e) sum += y[e];
-            l[r] += sum;
             if constexpr (F) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) p[r][e] = as_word(y[e]);
+                for (int e = 0; e < 4; ++e) {
+                    p[r][e] = as_word(y[e]);
+                    total[r][0] += y[e];
+                }
             } else {  // probabilities to the products' type: half a step of relative error each, as much as the values they weigh have
 #pragma unroll
                 for (int e = 0; e < 4; ++e) p[r][e] = pack2<T>(y[2 * e], y[2 * e + 1]);
+                constexpr unsigned one = __is_same(T, Bf16) ? 0x3F803F80u : 0x3C003C00u;
+                total[r] = Mfma<T>::go(u32x4{one, one, one, one}, u32x4{p[r][0], p[r][1], p[r][2], p[r][3]}, total[r]);  // every row of it the same sum
             }
         }
+    }
+
+    // out += V^T p; v: the lane group's keys, PER dimensions of each in every group of 16 PER
+    __device__ __forceinline__ void add_values(const unsigned (&v)[TPL][GRP * VW], const unsigned (&p)[R][4]) {
 #pragma unroll
         for (int d = 0; d < GRP * PER; ++d) {
             if constexpr (F) {
@@ -257,29 +220,277 @@ struct AttentionTile {
                 for (int r = 0; r < R; ++r) acc[r][d] = Mfma<T>::go(a, u32x4{p[r][0], p[r][1], p[r][2], p[r][3]}, acc[r][d]);
             }
         }
+    }
+
+    __device__ __forceinline__ float sum_of(int r) const {
+        float l = total[r][0];
+        if constexpr (F) {  // the lane groups' parts
+            l += __shfl_xor(l, 16, 64);
+            l += __shfl_xor(l, 32, 64);
+        }
+        return l;
+    }
+
+    // Sums to a row of LDS (`to`: of the lane's row in 16 r), dimensions in order.
+    __device__ __forceinline__ void put_sums(int r, float* to, int lane) const {
+#pragma unroll
+        for (int g = 0; g < GRP; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < PER; e += 4) {
+                    const int d = g * PER + e;
+                    *reinterpret_cast<f32x4*>(to + g * 16 * PER + ((lane >> 4) * 4 + i) * PER + e) = f32x4{acc[r][d][i], acc[r][d + 1][i], acc[r][d + 2][i], acc[r][d + 3][i]};
+                }
+    }
+};
+
+// Few rows: a wave has all of the workgroup's rows and every fourth step of its keys, which come straight from memory into registers.
+template <typename T, int D, int R>
+struct NarrowWalk {
+    using Rows = AttentionRows<T, D, R>;
+    static constexpr bool F = Rows::F;
+    static constexpr int ROW = Rows::ROW, TPL = Rows::TPL, STEP = Rows::STEP;
+
+    u32x4 k[Rows::NT][Rows::KC];
+    unsigned v[TPL][Rows::GRP * Rows::VW];
+    int page_k, page_v;   // of the step whose keys are loaded next, for the lane's keys of K and of V
+    unsigned in_k, in_v;  // the blocks' places in the pages
+
+    __device__ __forceinline__ void look_up(const Keys& s, unsigned b8, bool even, int lane) {
+        if (even) {  // a step lies in one page: one look-up for all
+            const Keys::Place at = s.place_of(__builtin_amdgcn_readfirstlane(b8));
+            page_k = page_v = s.table[at.entry];
+            in_k = in_v = at.in;
+        } else {
+            constexpr int BLOCK_LANES_K = F ? 8 : 4;  // rows of the score tile that lie in one block
+            const Keys::Place at_k = s.place_of(b8 + (unsigned)(lane & 15) / BLOCK_LANES_K), at_v = s.place_of(b8 + (unsigned)(lane >> 4) * TPL / 8);
+            page_k = s.table[at_k.entry];
+            page_v = s.table[at_v.entry];
+            in_k = at_k.in;
+            in_v = at_v.in;
+        }
+    }
+
+    __device__ __forceinline__ void load_k(const Keys& s, bool even, int lane) {
+        const int mm = lane & 15;
+        // the key of row mm of score tile 0: mm / 4 * TPL + mm % 4, the blocks before its own among them where one page holds the step
+        const unsigned own = F ? (even ? mm : mm & 7) : (even ? (mm >> 2) * 8 + (mm & 3) : mm & 3);
+        const char* p;
+        if (even) p = s.k + s.page_at(__builtin_amdgcn_readfirstlane(page_k)) + __builtin_amdgcn_readfirstlane(in_k) * 8 * ROW + (own * ROW + (lane >> 4) * 16);
+        else p = s.k + s.page_at(page_k) + (size_t)((in_k * 8 + own) * ROW + (lane >> 4) * 16);
+#pragma unroll
+        for (int t = 0; t < Rows::NT; ++t)
+#pragma unroll
+            for (int c = 0; c < Rows::KC; ++c) k[t][c] = *reinterpret_cast<const u32x4*>(p + t * 4 * ROW + c * 64);
+    }
+
+    __device__ __forceinline__ void load_v(const Keys& s, bool even, int lane) {
+        const unsigned own = F ? (even ? (lane >> 4) * 4 : (lane >> 4 & 1) * 4) : (even ? (lane >> 4) * 8 : 0);
+        const unsigned at = own * ROW + (lane & 15) * Rows::PER * T::bytes;
+        const char* p;
+        if (even) p = s.v + s.page_at(__builtin_amdgcn_readfirstlane(page_v)) + __builtin_amdgcn_readfirstlane(in_v) * 8 * ROW + at;
+        else p = s.v + s.page_at(page_v) + (size_t)(in_v * 8 * ROW + at);
+#pragma unroll
+        for (int u = 0; u < TPL; ++u)
+#pragma unroll
+            for (int g = 0; g < Rows::GRP; ++g) {
+                const char* from = p + u * ROW + g * 16 * Rows::PER * T::bytes;
+                if constexpr (Rows::VW == 4) {
+                    const u32x4 w = *reinterpret_cast<const u32x4*>(from);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[u][g * 4 + e] = w[e];
+                } else {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(from);
+                    v[u][g * 2] = w.x;
+                    v[u][g * 2 + 1] = w.y;
+                }
+            }
+    }
+
+    // One step over the keys from `first` on.  `least` and `most` bound the limits of all rows, absent: this lane group's keys are in no page.
+    // next(true) is called once K is no longer needed, next(false) once V is.
+    template <typename Next>
+    __device__ __forceinline__ void step(Rows& rows, int first, const bool absent, const int (&limit)[R], int least, int most, float scale, int lane, Next next) {
+        f32x4 x[R][Rows::NT];
+        rows.scores(x, [&](int t, int c) { return k[t][c]; });
+        next(true);
+        if (first + STEP > least || __any(absent)) {
+            const int mine = first + (lane >> 4) * TPL;
+            Rows::mask(x, mine, absent, limit);
+            // what lies in places that no row may see can be anything, and 0 * NaN is NaN
+#pragma unroll
+            for (int u = 0; u < TPL; ++u)
+                if (absent || mine + u >= most) {
+#pragma unroll
+                    for (int w = 0; w < Rows::GRP * Rows::VW; ++w) v[u][w] = 0;
+                }
+        }
+        unsigned p[R][4];
+        rows.weigh(x, scale, p);
+        rows.add_values(v, p);
         next(false);
     }
 
-    // Steps `at`, at + 4, ... below `end` (in steps of the table's keys).  Page numbers are asked for a step ahead of the keys.
-    __device__ __forceinline__ void walk(const Keys& s, int at, int end, const int (&limit)[R], int least, int most, float scale, int lane) {
+    // Steps `at`, at + 4, ... below `end`.  Page numbers are asked for a step ahead of the keys.
+    __device__ __forceinline__ void walk(Rows& rows, const Keys& s, int at, int end, const int (&limit)[R], int least, int most, float scale, int lane) {
         if (at >= end) return;
-        look_up(s, (unsigned)at * (STEP / 8), lane);
-        load_k(s, lane);
-        load_v(s, lane);
+        const bool even = s.page_blocks % (STEP / 8) == 0;
+        look_up(s, (unsigned)at * (STEP / 8), even, lane);
+        load_k(s, even, lane);
+        load_v(s, even, lane);
         bool absent = (unsigned)page_v >= s.num_pages;
-        look_up(s, (unsigned)(at + 4) * (STEP / 8), lane);
+        look_up(s, (unsigned)(at + 4) * (STEP / 8), even, lane);
         for (; at + 4 < end; at += 4) {
-            step(at * STEP, absent, limit, least, most, scale, lane, [&](bool k_is_free) {
+            step(rows, at * STEP, absent, limit, least, most, scale, lane, [&](bool k_is_free) {
                 if (k_is_free) {
-                    load_k(s, lane);
+                    load_k(s, even, lane);
                 } else {
-                    load_v(s, lane);
+                    load_v(s, even, lane);
                     absent = (unsigned)page_v >= s.num_pages;
-                    look_up(s, (unsigned)(at + 8) * (STEP / 8), lane);
+                    look_up(s, (unsigned)(at + 8) * (STEP / 8), even, lane);
                 }
             });
         }
-        step(at * STEP, absent, limit, least, most, scale, lane, [](bool) {});
+        step(rows, at * STEP, absent, limit, least, most, scale, lane, [](bool) {});
+    }
+};
+
+// Many rows: each of the four waves has 16 R rows of its own, and all of them walk the same keys, which the workgroup brings to LDS tile by tile: the
+// next tile's loads are under way while the one before is worked on.  16-byte piece c of key i lies at place c ^ turn(i), so that the 16 keys of a score
+// tile are read from different banks.
+template <typename T, int D, int R>
+struct WideWalk {
+    using Rows = AttentionRows<T, D, R>;
+    static constexpr bool F = Rows::F;
+    static constexpr int ROW = Rows::ROW, TPL = Rows::TPL, STEP = Rows::STEP;
+    static constexpr int PIECES = ROW / 16;
+    static constexpr int TILE = 16384 / ROW < 64 ? 16384 / ROW : 64;  // keys
+    static constexpr int PASS = 256 / PIECES, PASSES = TILE / PASS;   // keys that the workgroup's 256 pieces are, and how many such loads of K and of V
+    static constexpr int BUFFER = 2 * TILE * ROW;
+    static constexpr int LDS = 2 * BUFFER + 2 * 16;
+
+    u32x4 k[PASSES], v[PASSES];
+    int page[PASSES];
+    unsigned in[PASSES];
+
+    __device__ __forceinline__ static int turn(int key) {
+        if constexpr (F) return key & 15;
+        else if constexpr (PIECES >= 16) return (key & 3) | (key >> 3 & 3) << 2;
+        else return (key >> 1 & 1) | (key >> 3 & 3) << 1;  // two keys make up the banks
+    }
+
+    __device__ __forceinline__ void look_up(const Keys& s, int first) {
+        const int mine = (int)threadIdx.x / PIECES;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const Keys::Place at = s.place_of((unsigned)(first + i * PASS + mine) / 8);
+            page[i] = s.table[at.entry];
+            in[i] = at.in;
+        }
+    }
+
+    __device__ __forceinline__ void load(const Keys& s) {
+        const int mine = (int)threadIdx.x / PIECES, piece = (int)threadIdx.x % PIECES;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const size_t at = s.page_at(page[i]) + (size_t)((in[i] * 8 + (i * PASS + mine) % 8) * ROW + piece * 16);
+            k[i] = *reinterpret_cast<const u32x4*>(s.k + at);
+            v[i] = *reinterpret_cast<const u32x4*>(s.v + at);
+        }
+    }
+
+    // `first`: the tile's first key, whose keys from `most` on no row sees; bad: bit i where the thread's page of load i is none
+    __device__ __forceinline__ void store(char* buffer, char* absent, int first, int most, unsigned bad) {
+        const int mine = (int)threadIdx.x / PIECES, piece = (int)threadIdx.x % PIECES;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int key = i * PASS + mine;
+            // what lies in places that no row may see can be anything, and 0 * NaN is NaN
+            if (bad >> i & 1 || first + key >= most) v[i] = u32x4{0, 0, 0, 0};
+            char* const to = buffer + key * ROW + (piece ^ turn(key)) * 16;
+            *reinterpret_cast<u32x4*>(to) = k[i];
+            *reinterpret_cast<u32x4*>(to + TILE * ROW) = v[i];
+            if (piece == 0 && key % 8 == 0) absent[key / 8] = (char)(bad >> i & 1);
+        }
+    }
+
+    __device__ __forceinline__ unsigned bad_pages(const Keys& s) const {
+        unsigned bad = 0;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) bad |= (unsigned)((unsigned)page[i] >= s.num_pages) << i;
+        return bad;
+    }
+
+    // Keys `first` (a multiple of STEP) to `end`; `least` and `most` bound the limits of the workgroup's rows, own_most those of the wave's.
+    __device__ __forceinline__ void walk(Rows& rows, const Keys& s, int first, int end, const int (&limit)[R], int least, int most, int own_most, float scale, int lane, char* lds) {
+        if (first >= end) return;
+        char* const absent = lds + 2 * BUFFER;  // [2][16]: per block of 8 keys
+        look_up(s, first);
+        load(s);
+        unsigned bad = bad_pages(s);
+        look_up(s, first + TILE);
+        store(lds, absent, first, most, bad);
+        if (first + TILE < end) {
+            load(s);
+            bad = bad_pages(s);
+            look_up(s, first + 2 * TILE);
+        }
+        __syncthreads();
+        const int group = lane >> 4, mm = lane & 15;
+        int k_at[Rows::KC], v_at[4];
+        {
+            const int key = F ? mm : (mm >> 2) * 8 + (mm & 3);
+#pragma unroll
+            for (int c = 0; c < Rows::KC; ++c) k_at[c] = key * ROW + ((c * 4 + group) ^ turn(key)) * 16;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int from = group * TPL + u, piece = mm * Rows::VW / 4;
+                v_at[u] = TILE * ROW + from * ROW + (piece ^ turn(from)) * 16 + (Rows::VW == 2 ? (mm & 1) * 8 : 0);
+            }
+        }
+        int buffer = 0;
+        for (; first < end; first += TILE, buffer ^= 1) {
+            const char* const from = lds + buffer * BUFFER;
+            const int steps = min(end - first, TILE);
+#pragma unroll
+            for (int sub = 0; sub < TILE / STEP; ++sub) {
+                if (sub * STEP >= steps || first + sub * STEP >= own_most) break;  // uniform over the wave
+                f32x4 x[R][Rows::NT];
+                rows.scores(x, [&](int t, int c) { return *reinterpret_cast<const u32x4*>(from + k_at[c] + sub * STEP * ROW + t * 4 * ROW); });
+                unsigned w[TPL][Rows::GRP * Rows::VW];
+#pragma unroll
+                for (int u = 0; u < TPL; ++u)
+#pragma unroll
+                    for (int g = 0; g < Rows::GRP; ++g) {
+                        // piece g * 16 further on: the turn leaves those bits alone
+                        const char* const at = from + v_at[u & 3] + sub * STEP * ROW + (u >> 2) * 4 * ROW + g * 256;
+                        if constexpr (Rows::VW == 4) {
+                            const u32x4 y = *reinterpret_cast<const u32x4*>(at);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[u][g * 4 + e] = y[e];
+                        } else {
+                            const u32x2 y = *reinterpret_cast<const u32x2*>(at);
+                            w[u][g * 2] = y.x;
+                            w[u][g * 2 + 1] = y.y;
+                        }
+                    }
+                const bool gone = absent[buffer * 16 + sub * STEP / 8 + group * TPL / 8] != 0;
+                if (first + (sub + 1) * STEP > least || __any(gone)) Rows::mask(x, first + sub * STEP + group * TPL, gone, limit);
+                unsigned p[R][4];
+                rows.weigh(x, scale, p);
+                rows.add_values(w, p);
+            }
+            if (first + TILE < end) {
+                store(lds + (buffer ^ 1) * BUFFER, absent + (buffer ^ 1) * 16, first + TILE, most, bad);
+                if (first + 2 * TILE < end) {
+                    load(s);
+                    bad = bad_pages(s);
+                    look_up(s, first + 3 * TILE);
+                }
+                __syncthreads();
+            }
+        }
     }
 };
 
@@ -293,64 +504,83 @@ __device__ __forceinline__ void put_out(__amdgpu_buffer_rsrc_t to, unsigned valu
     }
 }
 
+// A workgroup's form: how many 16-row tiles a wave has, and whether the waves share rows and split the keys, or the other way round.
+template <int TILES, bool WIDE_>
+struct Form {
+    static constexpr int R = TILES;
+    static constexpr bool WIDE = WIDE_;
+    static constexpr int ROWS = 16 * R * (WIDE ? 4 : 1);
+};
+
+template <typename T, int D, typename Fm>
+constexpr int attention_lds() {
+    constexpr int sums = 4 * 16 * Fm::R * (8 + (D + 4) * 4);
+    return Fm::WIDE && WideWalk<T, D, Fm::R>::LDS > sums ? WideWalk<T, D, Fm::R>::LDS : sums;
+}
+
 // A workgroup's part: rows `row_id` (LDS; -1: none) of its tile over steps [begin, end) of `s`, left in slot `part` (or, where there is one, as the output).
-template <typename T, int D, int R>
-__device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, const char* const (&q_row)[R], const int (&limit)[R], int least, int most, int begin,
-                                       int end, int part, const int* row_id, char* lds) {
-    using Tile = AttentionTile<T, D, R>;
+template <typename T, int D, typename Fm>
+__device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, const char* const (&q_row)[Fm::R], const int (&limit)[Fm::R], int least, int most, int own_most,
+                                       int begin, int end, int part, const int* row_id, char* lds) {
+    constexpr int R = Fm::R;
+    using Rows = AttentionRows<T, D, R>;
     constexpr int PITCH = D + 4;  // floats of a row in LDS: lanes of different rows on different banks
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     f32x2* const ml = reinterpret_cast<f32x2*>(lds);                   // [4][16 R]
     float* const sums = reinterpret_cast<float*>(lds + 4 * 16 * R * 8);  // [4][16 R][PITCH]
     {
-        Tile tile;
-        tile.begin();
+        Rows rows;
+        rows.begin();
 #pragma unroll
-        for (int r = 0; r < R; ++r) tile.load_q(r, q_row[r], lane);
-        tile.walk(s, begin + wave, end, limit, least, most, a.scale_log2, lane);
+        for (int r = 0; r < R; ++r) rows.load_q(r, q_row[r], lane);
+        if constexpr (Fm::WIDE) {
+            WideWalk<T, D, R> keys;
+            keys.walk(rows, s, begin * Rows::STEP, end * Rows::STEP, limit, least, most, own_most, a.scale_log2, lane, lds);
+            __syncthreads();  // the sums go where the keys were
+        } else {
+            NarrowWalk<T, D, R> keys;
+            keys.walk(rows, s, begin + wave, end, limit, least, most, a.scale_log2, lane);
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            float l = tile.l[r];
-            l += __shfl_xor(l, 16, 64);
-            l += __shfl_xor(l, 32, 64);
-            if (lane < 16) ml[wave * 16 * R + r * 16 + lane] = f32x2{tile.m[r], l};
-            float* const to = sums + (wave * 16 * R + r * 16 + (lane & 15)) * PITCH;
-#pragma unroll
-            for (int g = 0; g < Tile::GRP; ++g)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < Tile::PER; e += 4) {
-                        const int d = g * Tile::PER + e;
-                        *reinterpret_cast<f32x4*>(to + g * 16 * Tile::PER + ((lane >> 4) * 4 + i) * Tile::PER + e) =
-                            f32x4{tile.acc[r][d][i], tile.acc[r][d + 1][i], tile.acc[r][d + 2][i], tile.acc[r][d + 3][i]};
-                    }
+            const float l = rows.sum_of(r);
+            if (lane < 16) ml[wave * 16 * R + r * 16 + lane] = f32x2{rows.m[r], l};
+            rows.put_sums(r, sums + (wave * 16 * R + r * 16 + (lane & 15)) * PITCH, lane);
         }
     }
     __syncthreads();
-    const size_t rows = (size_t)a.tokens * a.heads;
-    const bool whole = a.counters == nullptr;
-    const __amdgpu_buffer_rsrc_t to = whole ? descriptor(a.out) : descriptor(a.acc + (size_t)part * rows * D);
-    const __amdgpu_buffer_rsrc_t to_ml = descriptor(a.ml + (size_t)part * (whole ? 0 : rows));
-    for (int e = threadIdx.x; e < 16 * R * (D / 4); e += 256) {
+    const size_t all = (size_t)a.tokens * a.heads;
+    const bool whole = a.acc == nullptr;
+    const __amdgpu_buffer_rsrc_t to = whole ? descriptor(a.out) : descriptor(a.acc + (size_t)part * all * D);
+    const __amdgpu_buffer_rsrc_t to_ml = descriptor(a.ml + (size_t)part * (whole ? 0 : all));
+    for (int e = threadIdx.x; e < Fm::ROWS * (D / 4); e += 256) {
         const int row = e / (D / 4), d = (e - row * (D / 4)) * 4;
         const int id = row_id[row];
         if (id < 0) continue;
-        float top = -INFINITY;
-        f32x2 w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            w[i] = ml[i * 16 * R + row];
-            top = fmaxf(top, w[i].x);
-        }
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        float l = 0.f;
-        if (top > -INFINITY) {
+        float top, l;
+        f32x4 sum;
+        if constexpr (Fm::WIDE) {
+            const f32x2 w = ml[row];
+            top = w.x;
+            l = w.y;
+            sum = *reinterpret_cast<const f32x4*>(sums + row * PITCH + d);
+        } else {
+            top = -INFINITY;
+            l = 0.f;
+            sum = f32x4{0.f, 0.f, 0.f, 0.f};
+            f32x2 w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float f = __builtin_amdgcn_exp2f(w[i].x - top);
-                l += w[i].y * f;
-                sum += *reinterpret_cast<const f32x4*>(sums + (i * 16 * R + row) * PITCH + d) * f;
+                w[i] = ml[i * 16 * R + row];
+                top = fmaxf(top, w[i].x);
+            }
+            if (top > -INFINITY) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float f = __builtin_amdgcn_exp2f(w[i].x - top);
+                    l += w[i].y * f;
+                    sum += *reinterpret_cast<const f32x4*>(sums + (i * 16 * R + row) * PITCH + d) * f;
+                }
             }
         }
         if (whole) {
@@ -362,87 +592,107 @@ __device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, co
     }
 }
 
-// Counts the workgroup in at each of its rows and puts together the rows at which it is the last.  (As in the convs' split reductions: parts
-// are written through ahead of the count, and read past this workgroup's caches.)
+// Four outputs of row `id` from d on: the row's parts, in their order, with the running maximum.  (Read past this workgroup's caches.)
 template <typename T, int D>
-__device__ __forceinline__ void join(const AttentionArgs& a, const int* row_id, int rows_here, int* done) {
+__device__ __forceinline__ void join_parts(const AttentionArgs& a, int id, int d) {
+    const int parts = a.prefix_splits + a.own_splits;
+    const size_t rows = (size_t)a.tokens * a.heads;
+    float top = -INFINITY, l = 0.f;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int first = 0; first < parts; first += kJoined) {
+        u32x2 w[kJoined];
+        u32x4 x[kJoined];
+#pragma unroll
+        for (int i = 0; i < kJoined; ++i) {
+            const int part = min(first + i, parts - 1);
+            w[i] = __builtin_amdgcn_raw_buffer_load_b64(descriptor(a.ml + part * rows), id * 8, 0, kThrough);
+            x[i] = __builtin_amdgcn_raw_buffer_load_b128(descriptor(a.acc + part * rows * D), (int)(((unsigned)id * D + d) * 4), 0, kThrough);
+        }
+        float now = top;
+#pragma unroll
+        for (int i = 0; i < kJoined; ++i)
+            if (first + i < parts) now = fmaxf(now, as_float(w[i].x));
+        if (now == -INFINITY) continue;
+        const float shrink = __builtin_amdgcn_exp2f(top - now);
+        sum *= shrink;
+        l *= shrink;
+        top = now;
+#pragma unroll
+        for (int i = 0; i < kJoined; ++i) {
+            if (first + i >= parts) continue;
+            const float f = __builtin_amdgcn_exp2f(as_float(w[i].x) - top);
+            l += as_float(w[i].y) * f;
+            sum += __builtin_bit_cast(f32x4, x[i]) * f;
+        }
+    }
+    put_out<T>(descriptor(a.out), (unsigned)id * D + d, l > 0.f ? sum / l : f32x4{0.f, 0.f, 0.f, 0.f});
+}
+
+// Counts the workgroup in at each of its rows and puts together the rows at which it is the last.  (As in the convs' split reductions: parts
+// are written through ahead of the count.)
+template <typename T, int D, int MOST>
+__device__ __forceinline__ void join_last(const AttentionArgs& a, const int* row_id, int rows_here, int* done) {
     const int lane = threadIdx.x & 63;
     const int parts = a.prefix_splits + a.own_splits;
     __shared__ int count;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x < 64) {
-        const int id = lane < rows_here ? row_id[lane] : -1;
-        bool last = false;
-        if (id >= 0) {
-            last = __hip_atomic_fetch_add(a.counters + id, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)parts - 1;
-            if (last) __hip_atomic_store(a.counters + id, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        int n = 0;
+#pragma unroll
+        for (int first = 0; first < MOST; first += 64) {
+            const int id = first + lane < rows_here ? row_id[first + lane] : -1;
+            bool last = false;
+            if (id >= 0) {
+                last = __hip_atomic_fetch_add(a.counters + id, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)parts - 1;
+                if (last) __hip_atomic_store(a.counters + id, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            const unsigned long long who = __ballot(last);
+            if (last) done[n + __popcll(who & ((1ull << lane) - 1))] = id;
+            n += __popcll(who);
         }
-        const unsigned long long who = __ballot(last);
-        if (last) done[__popcll(who & ((1ull << lane) - 1))] = id;
-        if (lane == 0) count = __popcll(who);
+        if (lane == 0) count = n;
     }
     __syncthreads();
     const int n = count;
-    const size_t rows = (size_t)a.tokens * a.heads;
-    const __amdgpu_buffer_rsrc_t to = descriptor(a.out);
-    for (int e = threadIdx.x; e < n * (D / 4); e += 256) {
-        const int row = e / (D / 4), d = (e - row * (D / 4)) * 4;
-        const int id = done[row];
-        float top = -INFINITY, l = 0.f;
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (int first = 0; first < parts; first += 8) {
-            constexpr int N = 8;  // parts that are requested together
-            u32x2 w[N];
-            u32x4 x[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int part = min(first + i, parts - 1);
-                w[i] = __builtin_amdgcn_raw_buffer_load_b64(descriptor(a.ml + part * rows), id * 8, 0, kThrough);
-                x[i] = __builtin_amdgcn_raw_buffer_load_b128(descriptor(a.acc + part * rows * D), (int)(((unsigned)id * D + d) * 4), 0, kThrough);
-            }
-            float now = top;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (first + i < parts) now = fmaxf(now, as_float(w[i].x));
-            if (now == -INFINITY) continue;
-            const float shrink = __builtin_amdgcn_exp2f(top - now);
-            sum *= shrink;
-            l *= shrink;
-            top = now;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                if (first + i >= parts) continue;
-                const float f = __builtin_amdgcn_exp2f(as_float(w[i].x) - top);
-                l += as_float(w[i].y) * f;
-                sum += __builtin_bit_cast(f32x4, x[i]) * f;
-            }
-        }
-        put_out<T>(to, (unsigned)id * D + d, l > 0.f ? sum / l : f32x4{0.f, 0.f, 0.f, 0.f});
-    }
+    for (int e = threadIdx.x; e < n * (D / 4); e += 256) join_parts<T, D>(a, done[e / (D / 4)], e % (D / 4) * 4);
 }
 
-template <int D, int R>
-constexpr int attention_lds() { return 4 * 16 * R * 8 + 4 * 16 * R * (D + 4) * 4; }
-
-// RP, RO: 16-row tiles of a workgroup over the prefix / over a sequence's own tokens.
-template <typename T, int D, int RP, int RO>
-__global__ __launch_bounds__(256, 1) void prefix_attention_kernel(AttentionArgs a) {
+// All rows' parts by a launch of its own: where a workgroup's rows are many, the one that arrives last would be at it for longer than that takes.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prefix_attention_join_kernel(AttentionArgs a) {
     hook_entry(a.notifier, a.job_id);
-    constexpr int RM = RP > RO ? RP : RO;
-    __shared__ __attribute__((aligned(16))) char lds[attention_lds<D, RM>()];
-    __shared__ int row_id[16 * RM], done[16 * RM];
-    constexpr int STEP = AttentionTile<T, D, 1>::STEP;
-    const int lane = threadIdx.x & 63;
+    const int rows = (a.starts ? min(max(a.starts[a.sequences], 0), a.tokens) : a.tokens) * a.heads;
+    const int row = blockIdx.x * (1024 / D) + (int)threadIdx.x / (D / 4);
+    if (row < rows) join_parts<T, D>(a, row, (int)threadIdx.x % (D / 4) * 4);
+    hook_exit(a.notifier, a.job_id);
+}
+
+// FP, FO: the form of a workgroup over the prefix / over a sequence's own tokens.
+template <typename T, int D, typename FP, typename FO>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(AttentionArgs a) {
+    hook_entry(a.notifier, a.job_id);
+    constexpr int LP = attention_lds<T, D, FP>(), LO = attention_lds<T, D, FO>(), MOST = FP::ROWS > FO::ROWS ? FP::ROWS : FO::ROWS;
+    __shared__ __attribute__((aligned(16))) char lds[LP > LO ? LP : LO];
+    __shared__ int row_id[MOST], done[MOST];
+    constexpr int STEP = AttentionRows<T, D, 1>::STEP;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int head_bytes = D * T::bytes;
     Keys s;
     s.page_bytes = (size_t)a.kv_heads * a.page_size * head_bytes;
     s.page_blocks = a.page_blocks;
     s.page_blocks_inv = a.page_blocks_inv;
     s.num_pages = (unsigned)a.num_pages;
-    unsigned item = blockIdx.x;
-    bool any = false;
-    if (item < a.prefix_items) {
+    // Work over the prefix (bound by the products) and over own tokens (bound by memory) alternate, eight workgroups at a time, one for each XCD, in the
+    // proportion of their numbers, so that compute units have some of either.
+    const unsigned prefix_eights = (a.prefix_items + 7) / 8, eights_of_all = gridDim.x / 8, eight = blockIdx.x / 8;
+    const unsigned before = (unsigned)((unsigned long long)eight * prefix_eights / eights_of_all);
+    const bool over_prefix = (unsigned)((unsigned long long)(eight + 1) * prefix_eights / eights_of_all) > before;
+    unsigned item = (over_prefix ? before : eight - before) * 8 + blockIdx.x % 8;
+    bool any = item < (over_prefix ? a.prefix_items : a.own_items);
+    if (!any) {
+        // the last of an eight that has fewer
+    } else if (over_prefix) {
         // (key head, split) by tile: the tiles of one pair read the same keys, so they follow each other by 8 and share an XCD's cache
         const unsigned pairs = (unsigned)(a.kv_heads * a.prefix_splits), tiles = (unsigned)a.prefix_tiles;
         const unsigned eights = pairs / 8 * 8 * tiles;
@@ -456,22 +706,20 @@ __global__ __launch_bounds__(256, 1) void prefix_attention_kernel(AttentionArgs 
             tile = i / left;
         }
         const int h = (int)(pair / a.prefix_splits), split = (int)(pair % a.prefix_splits);
-        const int group_rows = a.tokens * a.per_kv;
-        const char* q_row[RP];
-        int limit[RP];
+        const int first_row = (int)tile * FP::ROWS, group_rows = a.tokens * a.per_kv;
+        const char* q_row[FP::R];
+        int limit[FP::R];
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
-            const int x = min((int)tile * 16 * RP + r * 16 + (lane & 15), group_rows - 1);
+        for (int r = 0; r < FP::R; ++r) {
+            const int x = min(first_row + (FP::WIDE ? wave * 16 * FP::R : 0) + r * 16 + (lane & 15), group_rows - 1);
             const int t = x / a.per_kv;
             q_row[r] = a.q + t * a.q_stride + (h * a.per_kv + x - t * a.per_kv) * head_bytes;
             limit[r] = a.prefix_len;
         }
-        // rows that belong to no sequence are left out; each of them by a wave of its own where the batch is ragged
-        for (int r = (int)(threadIdx.x >> 6); r < 16 * RP; r += 4) {
-            const int x = (int)tile * 16 * RP + r, t = x / a.per_kv;
-            int seq, j;
-            const bool owned = x < group_rows && row_owner(a.starts, a.sequences, a.max_new, t, lane, &seq, &j);
-            if (lane == 0) row_id[r] = owned ? t * a.heads + h * a.per_kv + x - t * a.per_kv : -1;
+        if ((int)threadIdx.x < FP::ROWS) {  // rows behind the last sequence are left out
+            const int x = first_row + (int)threadIdx.x, t = x / a.per_kv;
+            const int rows = a.starts ? min(a.starts[a.sequences], a.tokens) : a.tokens;
+            row_id[threadIdx.x] = x < group_rows && t < rows ? t * a.heads + h * a.per_kv + x - t * a.per_kv : -1;
         }
         __syncthreads();
         s.table = a.prefix_table;
@@ -481,10 +729,8 @@ __global__ __launch_bounds__(256, 1) void prefix_attention_kernel(AttentionArgs 
         const int steps = (a.prefix_len + STEP - 1) / STEP;
         const int per = (steps + a.prefix_splits - 1) / a.prefix_splits;
         const int begin = min(split * per, steps), end = min(begin + per, steps);
-        attend<T, D, RP>(a, s, q_row, limit, a.prefix_len, a.prefix_len, begin, end, split, row_id, lds);
-        any = true;
+        attend<T, D, FP>(a, s, q_row, limit, a.prefix_len, a.prefix_len, a.prefix_len, begin, end, split, row_id, lds);
     } else {
-        item -= a.prefix_items;
         // the key heads of one sequence side by side: they share the look-ups and, with eight of them, an XCD each
         const int h = (int)(item % a.kv_heads);
         item /= (unsigned)a.kv_heads;
@@ -496,52 +742,66 @@ __global__ __launch_bounds__(256, 1) void prefix_attention_kernel(AttentionArgs 
             first = min(max(__builtin_amdgcn_readfirstlane(a.starts[seq]), 0), a.tokens);
             count = min(min(__builtin_amdgcn_readfirstlane(a.starts[seq + 1]), a.tokens) - first, a.max_new);
         }
-        const int group_rows = max(count, 0) * a.per_kv;
-        any = tile * 16 * RO < group_rows;
+        const int first_row = tile * FO::ROWS, group_rows = max(count, 0) * a.per_kv;
+        any = first_row < group_rows;
         if (any) {
             const int capacity = (int)min((int64_t)a.max_pages * a.page_size, (int64_t)1 << 30);
             const int past = min(max(__builtin_amdgcn_readfirstlane(a.past[seq]), 0), capacity);
-            const char* q_row[RO];
-            int limit[RO];
+            auto limit_of = [&](int row) { return min(past + min(row, group_rows - 1) / a.per_kv + 1, capacity); };
+            const int wave_row = first_row + (FO::WIDE ? wave * 16 * FO::R : 0);
+            const char* q_row[FO::R];
+            int limit[FO::R];
 #pragma unroll
-            for (int r = 0; r < RO; ++r) {
-                const int x = tile * 16 * RO + r * 16 + (lane & 15);
-                const int y = min(x, group_rows - 1), j = y / a.per_kv, t = first + j;
-                const int head = h * a.per_kv + y - j * a.per_kv;
-                q_row[r] = a.q + t * a.q_stride + head * head_bytes;
+            for (int r = 0; r < FO::R; ++r) {
+                const int x = min(wave_row + r * 16 + (lane & 15), group_rows - 1), j = x / a.per_kv;
+                q_row[r] = a.q + (first + j) * a.q_stride + (h * a.per_kv + x - j * a.per_kv) * head_bytes;
                 limit[r] = min(past + j + 1, capacity);
-                if (threadIdx.x < 16) row_id[r * 16 + lane] = x < group_rows ? t * a.heads + head : -1;
+            }
+            if ((int)threadIdx.x < FO::ROWS) {
+                const int x = first_row + (int)threadIdx.x, j = x / a.per_kv;
+                row_id[threadIdx.x] = x < group_rows ? (first + j) * a.heads + h * a.per_kv + x - j * a.per_kv : -1;
             }
             __syncthreads();
             s.table = a.tables + (size_t)seq * a.max_pages;
             s.table_len = a.max_pages;
             s.k = a.k_cache + (size_t)h * a.page_size * head_bytes;
             s.v = a.v_cache + (size_t)h * a.page_size * head_bytes;
-            const int least = min(past + tile * 16 * RO / a.per_kv + 1, capacity);
-            const int most = min(past + min(tile * 16 * RO + 16 * RO - 1, group_rows - 1) / a.per_kv + 1, capacity);
+            const int least = limit_of(wave_row), most = limit_of(first_row + FO::ROWS - 1);
+            const int own_most = FO::WIDE ? limit_of(wave_row + 16 * FO::R - 1) : most;
             const int steps = (most + STEP - 1) / STEP;
             const int per = (steps + a.own_splits - 1) / a.own_splits;
             const int begin = min(split * per, steps), end = min(begin + per, steps);
-            attend<T, D, RO>(a, s, q_row, limit, least, most, begin, end, a.prefix_splits + split, row_id, lds);
+            attend<T, D, FO>(a, s, q_row, limit, least, most, own_most, begin, end, a.prefix_splits + split, row_id, lds);
         }
     }
-    if (any && a.counters) join<T, D>(a, row_id, blockIdx.x < a.prefix_items ? 16 * RP : 16 * RO, done);
+    if (any && a.counters) join_last<T, D, MOST>(a, row_id, over_prefix ? FP::ROWS : FO::ROWS, done);
     hook_exit(a.notifier, a.job_id);
 }
 
 using AttentionKernel = void (*)(AttentionArgs);
 
+// Which forms a type and head size have, by the rows of a workgroup: 16 and 32 (the waves split the keys), 64 and 128 (they split the rows).
 template <typename T, int D>
 AttentionKernel attention_kernel_of(int rp, int ro) {
-    if (rp == 1 && ro == 1) return prefix_attention_kernel<T, D, 1, 1>;
-    if constexpr (D * T::bytes <= 512 && D <= 128) {
-        if (rp == 2 && ro == 1) return prefix_attention_kernel<T, D, 2, 1>;
-        if (rp == 2 && ro == 2) return prefix_attention_kernel<T, D, 2, 2>;
-    }
-    if constexpr (D * T::bytes <= 256) {
-        if (rp == 4 && ro == 1) return prefix_attention_kernel<T, D, 4, 1>;
-        if (rp == 4 && ro == 2) return prefix_attention_kernel<T, D, 4, 2>;
-        if (rp == 4 && ro == 4) return prefix_attention_kernel<T, D, 4, 4>;
+    using N1 = Form<1, false>;
+    using W1 = Form<1, true>;
+    if (rp == 16 && ro == 16) return prefix_attention_kernel<T, D, N1, N1>;
+    if constexpr (D <= 128) {
+        using N2 = Form<2, false>;
+        [[maybe_unused]] typedef Form<2, true> W2;
+        if (rp == 32 && ro == 16) return prefix_attention_kernel<T, D, N2, N1>;
+        if (rp == 32 && ro == 32) return prefix_attention_kernel<T, D, N2, N2>;
+        if (rp == 64 && ro == 16) return prefix_attention_kernel<T, D, W1, N1>;
+        if (rp == 64 && ro == 32) return prefix_attention_kernel<T, D, W1, N2>;
+        if (rp == 64 && ro == 64) return prefix_attention_kernel<T, D, W1, W1>;
+        if constexpr (D * T::bytes <= 256) {  // what the registers hold without a spill
+            if (rp == 128 && ro == 16) return prefix_attention_kernel<T, D, W2, N1>;
+            if (rp == 128 && ro == 32) return prefix_attention_kernel<T, D, W2, N2>;
+            if (rp == 128 && ro == 128) return prefix_attention_kernel<T, D, W2, W2>;
+        }
+    } else {
+        if (rp == 64 && ro == 16) return prefix_attention_kernel<T, D, W1, N1>;
+        if (rp == 64 && ro == 64) return prefix_attention_kernel<T, D, W1, W1>;
     }
     return nullptr;
 }
@@ -551,9 +811,17 @@ AttentionKernel attention_kernel(int dim, int rp, int ro) {
     return dim == 64 ? attention_kernel_of<T, 64>(rp, ro) : dim == 128 ? attention_kernel_of<T, 128>(rp, ro) : dim == 256 ? attention_kernel_of<T, 256>(rp, ro) : nullptr;
 }
 
-// The kernel of a type for a head size and numbers of 16-row tiles; nullptr where there is none.  Defined once per type.
+template <typename T>
+AttentionKernel attention_join(int dim) {
+    return dim == 64 ? prefix_attention_join_kernel<T, 64> : dim == 128 ? prefix_attention_join_kernel<T, 128> : prefix_attention_join_kernel<T, 256>;
+}
+
+// The kernels of a type for a head size and rows per workgroup (nullptr where there is none), and for joining.  Defined once per type.
 AttentionKernel attention_kernel_f32(int dim, int rp, int ro);
 AttentionKernel attention_kernel_bf16(int dim, int rp, int ro);
 AttentionKernel attention_kernel_f16(int dim, int rp, int ro);
+AttentionKernel attention_join_f32(int dim);
+AttentionKernel attention_join_bf16(int dim);
+AttentionKernel attention_join_f16(int dim);
 
 }  // namespace paella

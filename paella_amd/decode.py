@@ -24,31 +24,41 @@ from .ops import _stream, _torch_stream
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
+try:
+    from torch._C import _cuda_getDevice as _current_device
+except ImportError:
+    _current_device = torch.cuda.current_device
+
+
+# As in `ops`, a small call's time is what it costs the calling thread: the checks below look at each tensor once and are kept to under half a microsecond each.
 
 def _on_device(*tensors):
     """Launches go to the current device: every tensor has to live there."""
-    device = torch.cuda.current_device()
+    device = _current_device()
     for t in tensors:
-        assert t is None or (t.is_cuda and t.device.index == device), "tensors of the current device are needed"
+        if t is not None and t.get_device() != device:
+            raise AssertionError("tensors of the current device are needed")
 
 
 def _ints(t, *shape):
-    assert t.dtype == torch.int32 and t.is_contiguous() and tuple(t.shape) == shape, ("contiguous int32 of shape %s" % (shape,), t.dtype, tuple(t.shape))
+    assert t.dtype is torch.int32 and t.shape == shape and t.is_contiguous(), ("contiguous int32 of shape %s" % (shape,), t.dtype, tuple(t.shape))
     return t.data_ptr()
 
 
 def _floats(t, n):
     if t is None:
         return None
-    assert t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n, ("%d contiguous float32" % n, t.dtype, tuple(t.shape))
+    assert t.dtype is torch.float32 and t.numel() == n and t.is_contiguous(), ("%d contiguous float32" % n, t.dtype, tuple(t.shape))
     return t.data_ptr()
 
 
-def _rows(t, heads, cache):
+def _rows(t, tokens, heads, cache):
     """Address and row stride of [tokens, heads, head_dim] whose heads lie side by side."""
-    assert t.dtype == cache.dtype and t.dim() == 3 and t.shape[1:] == (heads, cache.head_dim), (t.dtype, tuple(t.shape))
-    assert t.stride(2) == 1 and (heads == 1 or t.stride(1) == cache.head_dim), "heads have to lie side by side: strides %s" % (t.stride(),)
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else heads * cache.head_dim
+    dim = cache.head_dim
+    row, head, value = t.stride()  # three dimensions
+    assert t.dtype is cache.dtype and t.shape == (tokens, heads, dim), (t.dtype, tuple(t.shape), "wanted", cache.dtype, (tokens, heads, dim))
+    assert value == 1 and (head == dim or heads == 1), "heads have to lie side by side: strides %s" % ((row, head, value),)
+    return t.data_ptr(), row if tokens > 1 else heads * dim
 
 
 class _Workspaces:
@@ -64,10 +74,9 @@ class _Workspaces:
             return None
         if torch.cuda.is_current_stream_capturing():
             return torch.zeros(self.nbytes // 4 + 1, dtype=torch.int32, device=device)
-        key = (device, stream)
-        w = self.of_stream.get(key)
+        w = self.of_stream.get((device.index, stream))
         if w is None:
-            w = self.of_stream[key] = torch.zeros(self.nbytes // 4 + 1, dtype=torch.int32, device=device)
+            w = self.of_stream[device.index, stream] = torch.zeros(self.nbytes // 4 + 1, dtype=torch.int32, device=device)
             if stream != _torch_stream():  # the fill ran on torch's stream
                 torch.cuda.current_stream().synchronize()
         return w
@@ -83,6 +92,7 @@ class KVCache:
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.desc = KvCache(k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], *k.shape)
         self.ref = ctypes.byref(self.desc)
+        self.append_descs = {}  # of the calls so far: a model makes a few kinds
 
     @classmethod
     def empty(cls, num_pages, kv_heads, page_size, head_dim, dtype=torch.float32, device="cuda:0"):
@@ -111,32 +121,29 @@ class KVBatch:
         self.prefix_pages = prefix_table.numel() if prefix_len else 0
         self.ref = ctypes.byref(self.desc)
 
-    def check_prefix(self, cache):
-        assert self.prefix_pages * cache.page_size >= self.prefix_len, "the prefix's table has too few pages"
-
 
 def kv_append(cache, batch, k, v, q=None, q_norm=None, k_norm=None, eps=1e-6, inv_freq=None, interleaved=False, out=None, stream=None, job_id=0, notifier=None):
     """Stores the new tokens' k and v ([tokens, kv_heads, head_dim]) in the cache, k normed per head (k_norm: float32 [head_dim]) and rotated (inv_freq: float32, one
     per rotated pair) on the way; returns q ([tokens, heads, head_dim]) normed and rotated likewise, in `out` where given (which may be q)."""
-    lib = _abi.ops()
     _on_device(cache.k, k, v, q, q_norm, k_norm, inv_freq, out)
-    heads = 0 if q is None else q.shape[1]
-    kp, ks = _rows(k, cache.kv_heads, cache)
-    vp, vs = _rows(v, cache.kv_heads, cache)
-    assert k.shape[0] == v.shape[0] == batch.tokens, (k.shape[0], v.shape[0], batch.tokens)
-    qp = op = None
-    qs = 0
+    tokens, dim = batch.tokens, cache.head_dim
+    kp, ks = _rows(k, tokens, cache.kv_heads, cache)
+    vp, vs = _rows(v, tokens, cache.kv_heads, cache)
+    heads, qs, qp, op = 0, 0, None, None
     if q is not None:
-        qp, qs = _rows(q, heads, cache)
-        assert q.shape[0] == batch.tokens
+        heads = q.shape[1]
+        qp, qs = _rows(q, tokens, heads, cache)
         if out is None:
-            out = q.new_empty(q.shape)
-        assert out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()
+            out = q.new_empty((tokens, heads, dim))
+        else:
+            assert out.shape == (tokens, heads, dim) and out.dtype is q.dtype and out.is_contiguous()
         op = out.data_ptr()
     rotary = 0 if inv_freq is None else 2 * inv_freq.numel()
-    desc = KvAppendDesc(heads, rotary, int(interleaved), eps, qs, ks, vs)
-    rc = lib.paella_kv_append_launch(ctypes.byref(desc), cache.ref, batch.ref, qp, kp, vp, _floats(q_norm, cache.head_dim), _floats(k_norm, cache.head_dim),
-                                     _floats(inv_freq, rotary // 2), op, _stream(stream), job_id, notifier)
+    desc = cache.append_descs.get((heads, rotary, interleaved, eps, qs, ks, vs))
+    if desc is None:
+        desc = cache.append_descs[heads, rotary, interleaved, eps, qs, ks, vs] = ctypes.byref(KvAppendDesc(heads, rotary, int(interleaved), eps, qs, ks, vs))
+    rc = _abi.ops().paella_kv_append_launch(desc, cache.ref, batch.ref, qp, kp, vp, _floats(q_norm, dim), _floats(k_norm, dim), _floats(inv_freq, rotary // 2), op,
+                                            _stream(stream), job_id, notifier)
     if rc:
         check(rc, "paella_kv_append_launch")
     return out
@@ -155,22 +162,27 @@ class PrefixAttention:
         self.heads = heads
         self.workspaces = _Workspaces(self.plan.workspace_bytes)
 
-    def dims(self):
+    def dims(self, stage=0):
         d = LaunchDims()
-        check(self.lib.paella_prefix_attention_dims(self._ref, ctypes.byref(d)), "paella_prefix_attention_dims")
+        check(self.lib.paella_prefix_attention_dims(self._ref, stage, ctypes.byref(d)), "paella_prefix_attention_dims")
         return d
 
-    def __call__(self, q, cache, batch, out=None, stream=None, job_id=0, notifier=None):
+    def __call__(self, q, cache, batch, out=None, stream=None, job_id=0, notifier=None, stage=None):
+        """stage: one of the plan's launches (plan.stages) alone, for queues that keep no order."""
         _on_device(q, cache.k, out)
-        batch.check_prefix(cache)
-        qp, qs = _rows(q, self.heads, cache)
-        assert q.shape[0] == batch.tokens, (q.shape[0], batch.tokens)
+        assert batch.prefix_pages * cache.page_size >= batch.prefix_len, "the prefix's table has too few pages"
+        qp, qs = _rows(q, batch.tokens, self.heads, cache)
         if out is None:
             out = q.new_empty(q.shape)
-        assert out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()
+        else:
+            assert out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous()
         stream = _stream(stream)
         workspace = self.workspaces(stream, q.device)
-        rc = self._launch(self._ref, cache.ref, batch.ref, qp, qs, out.data_ptr(), None if workspace is None else workspace.data_ptr(), stream, job_id, notifier)
+        workspace = None if workspace is None else workspace.data_ptr()
+        if stage is None:
+            rc = self._launch(self._ref, cache.ref, batch.ref, qp, qs, out.data_ptr(), workspace, stream, job_id, notifier)
+        else:
+            rc = self.lib.paella_prefix_attention_launch_stage(self._ref, stage, cache.ref, batch.ref, qp, qs, out.data_ptr(), workspace, stream, job_id, notifier)
         if rc:
             check(rc, "paella_prefix_attention_launch")
         return out
@@ -205,15 +217,15 @@ class BeamSelect:
         if finished is not None:
             assert finished.dtype in (torch.uint8, torch.bool) and finished.is_contiguous() and finished.numel() == groups * beams
             finished = finished.data_ptr()
-        out = scores.new_empty((groups, self.count))
-        chosen = torch.empty((2, groups, self.count), dtype=torch.int32, device=scores.device)
+        shape = (groups, self.count)
+        out, parents, tokens = scores.new_empty(shape), scores.new_empty(shape, dtype=torch.int32), scores.new_empty(shape, dtype=torch.int32)
         stream = _stream(stream)
         workspace = self.workspaces(stream, logits.device)
-        rc = self._launch(self._ref, logits.data_ptr(), row, _floats(scores, groups * beams), finished, pad_token, out.data_ptr(), chosen.data_ptr(),
-                          chosen.data_ptr() + 4 * groups * self.count, workspace.data_ptr(), stream, job_id, notifier)
+        rc = self._launch(self._ref, logits.data_ptr(), row, _floats(scores, groups * beams), finished, pad_token, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+                          workspace.data_ptr(), stream, job_id, notifier)
         if rc:
             check(rc, "paella_beam_select_launch")
-        return out, chosen[0], chosen[1]
+        return out, parents, tokens
 
 
 def beam_reorder(cache, parents, past, tables, tables_out, spare, past_out=None, stream=None, job_id=0, notifier=None):

@@ -155,6 +155,9 @@ ATTEND = [
     (BF16, 8, 8, 64, 64, list(range(0, 200, 5)), 1, None, 1000),  # forty rows per key head
     (F32, 16, 2, 128, 32, [130] * 9, 1, None, 260),
     (BF16, 8, 2, 128, 64, [1500, 700], 1, None, 3000),
+    (BF16, 32, 2, 128, 16, [50, 3, 200, 0] * 3, 1, None, 300),    # 192 rows per key head
+    (F16, 16, 1, 256, 24, [20, 70, 11], 1, None, 130),
+    (F32, 8, 2, 256, 8, [9] * 6, 3, [0, 3, 4, 4, 7, 9, 12], 77),
 ]
 
 
@@ -224,15 +227,16 @@ def test_attention_of_large_scores_and_a_strided_query(cuda):
     within(out, want, ref.attention_bound(want, weight, products, BF16, 170))
 
 
-def test_attention_is_the_same_every_time_in_graphs_on_streams_and_direct_queues(cuda):
+@pytest.mark.parametrize("case,stages", [(3, 1), (16, 2), (17, 2)])
+def test_attention_is_the_same_every_time_in_graphs_on_streams_and_direct_queues(cuda, case, stages):
     """Which workgroup joins a row changes from run to run, the bits do not: eager, replayed (two graphs of one plan side by side, lengths changed between replays), on another
     stream and on a direct-dispatch queue."""
     from paella_amd import decode, ops
-    case = ATTEND[-1]
+    case = ATTEND[case]
     q, k, v, rows, tables, prefix_table, cache, batch = attend_case(case, cuda)
     q = q.to(cuda)
-    attend = decode.PrefixAttention(8, cache, batch)
-    assert attend.plan.workspace_bytes and attend.plan.prefix_splits > 1
+    attend = decode.PrefixAttention(case[1], cache, batch)
+    assert attend.plan.workspace_bytes and attend.plan.stages == stages
     want = attend(q, cache, batch)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -246,7 +250,7 @@ def test_attention_is_the_same_every_time_in_graphs_on_streams_and_direct_queues
         with torch.cuda.graph(graph):
             outs.append(attend(q, cache, batch))
         graphs.append(graph)
-    shorter = batch.past - 100
+    shorter = (batch.past - 100).clamp(min=0)
     longer = batch.past.clone()
     for past in (longer, shorter, longer):
         batch.past.copy_(past)
@@ -261,9 +265,18 @@ def test_attention_is_the_same_every_time_in_graphs_on_streams_and_direct_queues
     with ops.DirectQueue() as queue:
         for _ in range(2):
             out = torch.zeros_like(want)
-            attend(q, cache, batch, out=out, stream=queue.handle)
-            queue.wait()
+            for stage in range(attend.plan.stages):
+                attend(q, cache, batch, out=out, stream=queue.handle, stage=stage)
+                queue.wait()
             assert torch.equal(out, want)
+        if attend.plan.stages > 1:
+            with pytest.raises(RuntimeError, match="-2"):
+                attend(q, cache, batch, out=out, stream=queue.handle)
+    with ops.DirectQueue(ordered=True) as queue:
+        out = torch.zeros_like(want)
+        attend(q, cache, batch, out=out, stream=queue.handle)
+        queue.wait()
+        assert torch.equal(out, want)
 
 
 # ------------------------------------------------------------------ beam search
@@ -496,7 +509,7 @@ def test_a_step_reports_to_its_notifier(cuda):
         assert lib.paella_kv_append_dims(ctypes.byref(KvAppendDesc(8, 0, 0, 1e-6, 1024, 256, 256)), cache.ref, batch.ref, ctypes.byref(append_dims)) == 0
         assert lib.paella_beam_reorder_dims(ctypes.byref(BeamReorderDesc(2, 3, 4, 2)), cache.ref, ctypes.byref(reorder_dims)) == 0
         calls = [(append_dims, lambda i: decode.kv_append(cache, batch, new, new, q=q, job_id=i, notifier=note)),
-                 (attend.dims(), lambda i: attend(q, cache, batch, job_id=i, notifier=note)),
+                 (attend.dims(attend.plan.stages - 1), lambda i: attend(q, cache, batch, job_id=i, notifier=note)),
                  (pick.dims(), lambda i: pick(logits, scores, job_id=i, notifier=note)),
                  (reorder_dims, lambda i: decode.beam_reorder(cache, parents, past, old, out, spare, job_id=i, notifier=note))]
         for i, (dims, call) in enumerate(calls):
