@@ -63,6 +63,16 @@ __device__ __forceinline__ V row_all(V v, Op op) {
     v = op(v, lane_move<0x141>(v));  // the other half of eight, mirrored
     return op(v, lane_move<0x140>(v));  // the other half of sixteen, mirrored
 }
+// The sum over 2^log2 lanes side by side, which is the same for all of the wave.
+__device__ __forceinline__ float lanes_sum(float v, int log2) {
+    if (log2 > 0) v += lane_move<0xB1>(v);
+    if (log2 > 1) v += lane_move<0x4E>(v);
+    if (log2 > 2) v += lane_move<0x141>(v);
+    if (log2 > 3) v += lane_move<0x140>(v);
+    if (log2 > 4) v += __shfl_xor(v, 16, 64);
+    if (log2 > 5) v += __shfl_xor(v, 32, 64);
+    return v;
+}
 template <typename Op>
 __device__ __forceinline__ float wave_all(float v, Op op) {
     v = row_all(v, op);
@@ -77,6 +87,24 @@ __device__ __forceinline__ float wave_max_f(float v) {
     return wave_all(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
+// Division by a number that the host knows: with 2^32 over it, rounded down (all ones for 1), the product's upper half is the quotient or one less.  (A
+// division costs some forty instructions; a workgroup of a small launch spends a microsecond on the half dozen that say what its work is.)
+struct Divisor {
+    unsigned d, inv;
+};
+inline Divisor divisor(unsigned d) { return {d, d <= 1 ? 0xFFFFFFFFu : (unsigned)(0x100000000ull / d)}; }
+struct Quotient {
+    unsigned q, r;
+};
+__device__ __forceinline__ Quotient divide(unsigned n, Divisor by) {
+    unsigned q = __umulhi(n, by.inv), r = n - q * by.d;
+    if (r >= by.d) {
+        ++q;
+        r -= by.d;
+    }
+    return {q, r};
+}
+
 // A descriptor over everything behind `base` (uniform over the wave); offsets are 32-bit, sc1 = 16 writes through / reads past this XCD's caches.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(const void* base) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0xFFFFFFFFu, 0x00027000);
@@ -85,10 +113,11 @@ constexpr int kThrough = 16;
 
 // The sequence of row t and its index j among the sequence's new tokens, found by every wave for itself with one load per 64 sequences;
 // false for rows that belong to none.  t is uniform over the wave.
-__device__ __forceinline__ bool row_owner(const int* __restrict__ starts, int sequences, int max_new, int t, int lane, int* seq, int* j) {
+__device__ __forceinline__ bool row_owner(const int* __restrict__ starts, int sequences, Divisor max_new, int t, int lane, int* seq, int* j) {
     if (!starts) {
-        *seq = t / max_new;
-        *j = t - *seq * max_new;
+        const Quotient at = divide((unsigned)t, max_new);
+        *seq = (int)at.q;
+        *j = (int)at.r;
         return *seq < sequences;
     }
     int b = 0;
@@ -101,7 +130,7 @@ __device__ __forceinline__ bool row_owner(const int* __restrict__ starts, int se
     *seq = b;
     if (b >= sequences) return false;
     *j = t - starts[b];
-    return *j >= 0 && *j < max_new;
+    return *j >= 0 && *j < (int)max_new.d;
 }
 
 // Host side: what every entry point asks of a cache and a batch.  `tables`: the batch's device pointers are needed too.

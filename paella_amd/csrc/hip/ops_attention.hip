@@ -25,7 +25,7 @@ AttentionKernel join_of(const paella_prefix_attention_plan* p) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Grid {
-    int64_t prefix_tiles, own_tiles, prefix_items, own_items, all;
+    int64_t prefix_tiles, own_tiles, prefix_items, own_items, turn, rate, all;
 };
 
 Grid grid_of(const paella_prefix_attention_plan* p) {
@@ -35,7 +35,14 @@ Grid grid_of(const paella_prefix_attention_plan* p) {
     g.own_tiles = ceil_div(p->max_new * per_kv, p->own_rows);
     g.prefix_items = g.prefix_tiles * p->kv_heads * p->prefix_splits;
     g.own_items = p->sequences * g.own_tiles * p->kv_heads * p->own_splits;
-    g.all = (ceil_div(g.prefix_items, 8) + ceil_div(g.own_items, 8)) * 8;  // the two kinds alternate by eights
+    g.turn = g.prefix_items && g.prefix_items + g.own_items > 256 ? 32 : 0;  // (where all start at once, order is nothing)
+    g.rate = 0;
+    if (g.turn) {
+        const int64_t turns = ceil_div(g.prefix_items, g.turn) + ceil_div(g.own_items, g.turn);
+        const int64_t rate = 1024 * ceil_div(g.prefix_items, g.turn) / turns * 3 / 2 + 1;
+        g.rate = rate < 1024 ? rate : 1024;
+    }
+    g.all = g.turn ? (ceil_div(g.prefix_items, g.turn) + ceil_div(g.own_items, g.turn)) * g.turn : g.prefix_items + g.own_items;
     return g;
 }
 
@@ -89,7 +96,7 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_
     // A row's keys are shared by as many workgroups as fill the device twice, each with two steps per wave at least.
     const int step = size == 4 ? 16 : 32;
     auto splits = [&](int64_t others, int64_t keys) {
-        const int64_t want = ceil_div(512, others), least = ceil_div(ceil_div(keys, step), 8);
+        const int64_t want = ceil_div(768, others), least = ceil_div(ceil_div(keys, step), 8);
         const int64_t n = want < least ? want : least;
         return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
     };
@@ -134,12 +141,16 @@ int paella_prefix_attention_launch_stage(const paella_prefix_attention_plan* p, 
     a.starts = b->starts; a.past = b->past; a.tables = b->tables; a.prefix_table = b->prefix_table;
     a.q_stride = q_stride * size;
     a.sequences = b->sequences; a.max_new = b->max_new; a.tokens = b->tokens; a.max_pages = b->max_pages; a.prefix_len = b->prefix_len;
-    a.heads = p->heads; a.kv_heads = p->kv_heads; a.per_kv = p->heads / p->kv_heads; a.page_size = c->page_size; a.num_pages = c->num_pages;
-    a.page_blocks = (unsigned)c->page_size / 8;
-    a.page_blocks_inv = a.page_blocks == 1 ? 0xFFFFFFFFu : (unsigned)(0x100000000ull / a.page_blocks);
+    a.prefix_pages = (int)ceil_div(b->prefix_len, c->page_size);
+    a.heads = p->heads; a.page_size = c->page_size; a.num_pages = c->num_pages;
+    a.kv_heads = divisor((unsigned)p->kv_heads); a.per_kv = divisor((unsigned)(p->heads / p->kv_heads)); a.page_blocks = divisor((unsigned)c->page_size / 8);
     a.scale_log2 = p->scale * 1.44269504088896340736f;
-    a.prefix_tiles = (int)g.prefix_tiles; a.prefix_splits = p->prefix_splits; a.own_tiles = (int)g.own_tiles; a.own_splits = p->own_splits;
-    a.prefix_items = (unsigned)g.prefix_items; a.own_items = (unsigned)g.own_items;
+    const int step = size == 4 ? 16 : 32;  // keys
+    a.eight_tiles = divisor((unsigned)g.prefix_tiles * 8); a.prefix_splits = divisor((unsigned)p->prefix_splits);
+    a.own_tiles = divisor((unsigned)g.own_tiles); a.own_splits = divisor((unsigned)p->own_splits);
+    a.prefix_per = p->prefix_splits ? (int)ceil_div(ceil_div(p->prefix_len, step), p->prefix_splits) : 0;
+    a.prefix_pairs = p->kv_heads * p->prefix_splits;
+    a.prefix_items = (unsigned)g.prefix_items; a.own_items = (unsigned)g.own_items; a.turn = (unsigned)g.turn; a.rate = (unsigned)g.rate;
     const size_t parts = (size_t)p->prefix_splits + p->own_splits, rows = (size_t)p->tokens * p->heads;
     a.counters = need && stages_of(p) == 1 ? (unsigned*)workspace : nullptr;
     a.ml = need ? (f32x2*)((char*)workspace + up256(rows * 4)) : nullptr;

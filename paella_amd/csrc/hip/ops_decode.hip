@@ -22,9 +22,10 @@ struct AppendArgs {
     const float *q_weight, *k_weight, *inv_freq;
     const int *starts, *past, *tables;
     int64_t q_stride, k_stride, v_stride;  // bytes
-    int sequences, max_new, max_pages, prefix_len;
-    int heads, kv_heads, dim, page_size, num_pages, rotary, interleaved, group_log2;  // a head's group of lanes: 2^group_log2 of 8 values each
-    float eps;
+    int sequences, max_pages, prefix_len;
+    Divisor max_new, page_size;
+    int heads, kv_heads, dim, num_pages, rotary, interleaved, group_log2;  // a head's group of lanes: 2^group_log2 of 8 values each
+    float eps, inv_dim;
     uint32_t job_id;
     Notifier* notifier;
 };
@@ -64,6 +65,13 @@ struct Eight {  // eight values of a head as they lie in memory
     }
 };
 
+// 16 bytes from an address on a value's boundary (rows of an odd number of logits begin anywhere, weights may be views).
+__device__ __forceinline__ u32x4 load_unaligned(const char* p) {
+    u32x4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     hook_entry(a.notifier, a.job_id);
@@ -91,9 +99,22 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
             }
         };
         fetch(0);
+        float wq[8], wk[8];  // a lane's values have the same places in every head
+        auto weights = [&](float (&w)[8], const float* from) {
+            const int at = in_head ? li * 8 : 0;
+            const u32x4 a = load_unaligned(reinterpret_cast<const char*>(from + at)), b = load_unaligned(reinterpret_cast<const char*>(from + at + 4));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                w[e] = as_float(a[e]);
+                w[4 + e] = as_float(b[e]);
+            }
+        };
+        if (a.q_weight) weights(wq, a.q_weight);
+        if (a.k_weight) weights(wk, a.k_weight);
         // where the token goes; a place outside the table or the cache is none
         const unsigned own = (unsigned)max(a.past[seq], 0) + (unsigned)j;
-        const unsigned column = own / (unsigned)a.page_size, slot = own - column * (unsigned)a.page_size;
+        const Quotient place = divide(own, a.page_size);
+        const unsigned column = place.q, slot = place.r;
         int page = -1;
         if (column < (unsigned)a.max_pages) page = a.tables[(size_t)seq * a.max_pages + column];
         page = __builtin_amdgcn_readfirstlane(page);  // (descriptors are built from it)
@@ -107,11 +128,20 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
             turn[i] = f32x2{c, s};
         }
         __syncthreads();
-        const size_t page_bytes = (size_t)a.kv_heads * a.page_size * head_bytes;
+        const size_t page_bytes = (size_t)a.kv_heads * a.page_size.d * head_bytes;
         const __amdgpu_buffer_rsrc_t to_q = descriptor(a.q_out + (size_t)t * a.heads * head_bytes);
         const __amdgpu_buffer_rsrc_t to_k = descriptor(a.k_cache + (placed ? page : 0) * page_bytes);
         const __amdgpu_buffer_rsrc_t to_v = descriptor(a.v_cache + (placed ? page : 0) * page_bytes);
-        const int half = a.rotary >> 1;
+        const int half = a.rotary >> 1, d0 = li * 8;  // rotary_dim is a multiple of 16: a lane's values are all in one half, or none is rotated
+        const bool turned = d0 < a.rotary, lower = d0 < half;
+        const int other = ((lane & ~(group - 1)) + (lower ? li + (half >> 3) : li - (half >> 3))) & 63;
+        f32x2 cs[8];  // of a lane's values (interleaved: of its four pairs): the same in every head
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (a.interleaved) cs[e] = turned ? turn[(d0 >> 1) + (e & 3)] : f32x2{1.f, 0.f};
+            else cs[e] = turned ? turn[(lower ? d0 : d0 - half) + e] : f32x2{1.f, 0.f};
+            if (!a.interleaved && lower) cs[e].y = -cs[e].y;
+        }
         for (int first = 0; first < total; first += AHEAD * 4 * per_wave) {
             if (first) fetch(first);
 #pragma unroll
@@ -127,39 +157,31 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) f[e] = 0.f;
                 }
-                const float* weight = is_q ? a.q_weight : a.k_weight;
-                float sum = 0.f;
+                if (a.q_weight || a.k_weight) {
+                    float sum = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum += f[e] * f[e];
-                for (int off = group >> 1; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-                if (weight && live && !is_v) {
-                    const float r = 1.f / sqrtf(sum / (float)a.dim + a.eps);
+                    for (int e = 0; e < 8; ++e) sum += f[e] * f[e];
+                    sum = lanes_sum(sum, a.group_log2);
+                    if (is_q ? a.q_weight != nullptr : !is_v && a.k_weight != nullptr) {
+                        const float r = __builtin_amdgcn_rsqf(sum * a.inv_dim + a.eps);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = f[e] * r * weight[li * 8 + e];
+                        for (int e = 0; e < 8; ++e) f[e] = f[e] * r * (is_q ? wq[e] : wk[e]);
+                    }
                 }
                 if (a.rotary) {
-                    const int d0 = li * 8;  // rotary_dim is a multiple of 16: a lane's values are all in one half, or none is rotated
                     if (a.interleaved) {
-                        if (d0 < a.rotary) {
 #pragma unroll
-                            for (int e = 0; e < 8; e += 2) {
-                                const f32x2 cs = turn[(d0 + e) >> 1];
-                                const float p = f[e], q = f[e + 1];
-                                f[e] = p * cs.x - q * cs.y;
-                                f[e + 1] = q * cs.x + p * cs.y;
-                            }
+                        for (int e = 0; e < 4; ++e) {
+                            const float p = f[2 * e], q = f[2 * e + 1];
+                            f[2 * e] = turned ? p * cs[e].x - q * cs[e].y : p;
+                            f[2 * e + 1] = turned ? q * cs[e].x + p * cs[e].y : q;
                         }
                     } else {
-                        const bool lower = d0 < half;
-                        const int other = (lane & ~(group - 1)) + (lower ? li + (half >> 3) : li - (half >> 3));
+                        float partner[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float partner = __shfl(f[e], other & 63, 64);
-                            if (d0 < a.rotary) {
-                                const f32x2 cs = turn[lower ? d0 + e : d0 - half + e];
-                                f[e] = lower ? f[e] * cs.x - partner * cs.y : f[e] * cs.x + partner * cs.y;
-                            }
-                        }
+                        for (int e = 0; e < 8; ++e) partner[e] = __shfl(f[e], other, 64);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[e] = f[e] * cs[e].x + (turned ? partner[e] * cs[e].y : 0.f);
                     }
                 }
                 if (!live) continue;
@@ -168,7 +190,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
                     x[u].store(to_q, (unsigned)(h * head_bytes + li * 8 * T::bytes));
                 } else if (placed) {
                     const int hk = is_v ? h - a.heads - a.kv_heads : h - a.heads;
-                    const unsigned to = ((unsigned)hk * a.page_size + slot) * head_bytes + li * 8 * T::bytes;
+                    const unsigned to = ((unsigned)hk * a.page_size.d + slot) * head_bytes + li * 8 * T::bytes;
                     if (is_v) {
                         x[u].store(to_v, to);  // as it came
                     } else {
@@ -220,13 +242,6 @@ struct SelectArgs {
 __device__ __forceinline__ void put64(unsigned long long* p, unsigned long long v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ unsigned long long get64(const unsigned long long* p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// 16 bytes from an address on a value's boundary (rows of an odd number of logits begin anywhere).
-__device__ __forceinline__ u32x4 load_unaligned(const char* p) {
-    u32x4 v;
-    __builtin_memcpy(&v, p, 16);
-    return v;
 }
 
 template <typename T, int VALUES>
@@ -751,9 +766,10 @@ int paella_kv_append_launch(const paella_kv_append_desc* d, const paella_kv_cach
     a.q_weight = q_weight; a.k_weight = k_weight; a.inv_freq = inv_freq;
     a.starts = b->starts; a.past = b->past; a.tables = b->tables;
     a.q_stride = d->q_stride * size; a.k_stride = d->k_stride * size; a.v_stride = d->v_stride * size;
-    a.sequences = b->sequences; a.max_new = b->max_new; a.max_pages = b->max_pages; a.prefix_len = b->prefix_len;
-    a.heads = d->heads; a.kv_heads = c->kv_heads; a.dim = c->head_dim; a.page_size = c->page_size; a.num_pages = c->num_pages;
-    a.rotary = d->rotary_dim; a.interleaved = d->interleaved; a.eps = d->eps;
+    a.sequences = b->sequences; a.max_pages = b->max_pages; a.prefix_len = b->prefix_len;
+    a.max_new = divisor((unsigned)b->max_new); a.page_size = divisor((unsigned)c->page_size);
+    a.heads = d->heads; a.kv_heads = c->kv_heads; a.dim = c->head_dim; a.num_pages = c->num_pages;
+    a.rotary = d->rotary_dim; a.interleaved = d->interleaved; a.eps = d->eps; a.inv_dim = 1.f / (float)c->head_dim;
     a.group_log2 = 0;
     while ((8 << a.group_log2) < c->head_dim) ++a.group_log2;
     a.job_id = job_id; a.notifier = (Notifier*)notifier;

@@ -29,12 +29,14 @@ struct AttentionArgs {
     char* out;
     const int *starts, *past, *tables, *prefix_table;
     int64_t q_stride;  // bytes
-    int sequences, max_new, tokens, max_pages, prefix_len;
-    int heads, kv_heads, per_kv, page_size, num_pages;
-    unsigned page_blocks, page_blocks_inv;  // blocks of 8 tokens in a page, and 2^32 over that, rounded down
+    int sequences, max_new, tokens, max_pages, prefix_len, prefix_pages;
+    int heads, page_size, num_pages;
+    Divisor kv_heads, per_kv, page_blocks;  // per_kv: query heads of a key head; page_blocks: blocks of 8 tokens in a page
     float scale_log2;                       // scale * log2(e): probabilities are powers of two
-    int prefix_tiles, prefix_splits, own_tiles, own_splits;
+    Divisor eight_tiles, prefix_splits, own_tiles, own_splits;  // eight_tiles: 8 times the tiles over the prefix
+    int prefix_per, prefix_pairs;                               // steps of a split; key heads by splits
     unsigned prefix_items, own_items;
+    unsigned turn, rate;    // workgroups of one kind in a row (0: all over the prefix, then all over own tokens); 1024ths of the turns that are the prefix's until it is done
     unsigned* counters;  // [tokens * heads], zero between launches; null where a launch of its own joins
     f32x2* ml;           // [splits][tokens * heads]: running maximum and sum of each part
     float* acc;          // [splits][tokens * heads][head_dim]
@@ -65,19 +67,16 @@ struct Keys {
     int table_len;
     const char *k, *v;   // the cache, moved to the key head
     size_t page_bytes;
-    unsigned page_blocks, page_blocks_inv, num_pages;  // a block: 8 keys, which never lie in two pages
+    Divisor page_blocks;  // a block: 8 keys, which never lie in two pages
+    unsigned num_pages;
 
     struct Place {
         unsigned entry, in;  // of the table, and the block's place in the page
     };
     // Where block b lies; beyond the table's end in the last entry (the caller's limits mask what is read).
     __device__ __forceinline__ Place place_of(unsigned b) const {
-        unsigned page = __umulhi(b, page_blocks_inv), in = b - page * page_blocks;
-        if (in >= page_blocks) {
-            ++page;
-            in -= page_blocks;
-        }
-        return {min(page, (unsigned)table_len - 1), in};
+        const Quotient at = divide(b, page_blocks);
+        return {min(at.q, (unsigned)table_len - 1), at.r};
     }
     __device__ __forceinline__ size_t page_at(int page) const { return ((unsigned)page < num_pages ? (unsigned)page : 0u) * page_bytes; }
 };
@@ -335,7 +334,7 @@ struct NarrowWalk {
     // Steps `at`, at + 4, ... below `end`.  Page numbers are asked for a step ahead of the keys.
     __device__ __forceinline__ void walk(Rows& rows, const Keys& s, int at, int end, const int (&limit)[R], int least, int most, float scale, int lane) {
         if (at >= end) return;
-        const bool even = s.page_blocks % (STEP / 8) == 0;
+        const bool even = s.page_blocks.d % (STEP / 8) == 0;
         look_up(s, (unsigned)at * (STEP / 8), even, lane);
         load_k(s, even, lane);
         load_v(s, even, lane);
@@ -367,8 +366,7 @@ struct WideWalk {
     static constexpr int PIECES = ROW / 16;
     static constexpr int TILE = 16384 / ROW < 64 ? 16384 / ROW : 64;  // keys
     static constexpr int PASS = 256 / PIECES, PASSES = TILE / PASS;   // keys that the workgroup's 256 pieces are, and how many such loads of K and of V
-    static constexpr int BUFFER = 2 * TILE * ROW;
-    static constexpr int LDS = 2 * BUFFER + 2 * 16;
+    static constexpr int LDS = 2 * TILE * ROW + 16;
 
     u32x4 k[PASSES], v[PASSES];
     int page[PASSES];
@@ -425,7 +423,7 @@ struct WideWalk {
     // Keys `first` (a multiple of STEP) to `end`; `least` and `most` bound the limits of the workgroup's rows, own_most those of the wave's.
     __device__ __forceinline__ void walk(Rows& rows, const Keys& s, int first, int end, const int (&limit)[R], int least, int most, int own_most, float scale, int lane, char* lds) {
         if (first >= end) return;
-        char* const absent = lds + 2 * BUFFER;  // [2][16]: per block of 8 keys
+        char* const absent = lds + 2 * TILE * ROW;  // per block of 8 keys
         look_up(s, first);
         load(s);
         unsigned bad = bad_pages(s);
@@ -449,9 +447,8 @@ struct WideWalk {
                 v_at[u] = TILE * ROW + from * ROW + (piece ^ turn(from)) * 16 + (Rows::VW == 2 ? (mm & 1) * 8 : 0);
             }
         }
-        int buffer = 0;
-        for (; first < end; first += TILE, buffer ^= 1) {
-            const char* const from = lds + buffer * BUFFER;
+        for (; first < end; first += TILE) {
+            const char* const from = lds;
             const int steps = min(end - first, TILE);
 #pragma unroll
             for (int sub = 0; sub < TILE / STEP; ++sub) {
@@ -475,14 +472,15 @@ struct WideWalk {
                             w[u][g * 2 + 1] = y.y;
                         }
                     }
-                const bool gone = absent[buffer * 16 + sub * STEP / 8 + group * TPL / 8] != 0;
+                const bool gone = absent[sub * STEP / 8 + group * TPL / 8] != 0;
                 if (first + (sub + 1) * STEP > least || __any(gone)) Rows::mask(x, first + sub * STEP + group * TPL, gone, limit);
                 unsigned p[R][4];
                 rows.weigh(x, scale, p);
                 rows.add_values(w, p);
             }
             if (first + TILE < end) {
-                store(lds + (buffer ^ 1) * BUFFER, absent + (buffer ^ 1) * 16, first + TILE, most, bad);
+                __syncthreads();
+                store(lds, absent, first + TILE, most, bad);
                 if (first + 2 * TILE < end) {
                     load(s);
                     bad = bad_pages(s);
@@ -514,7 +512,7 @@ struct Form {
 
 template <typename T, int D, typename Fm>
 constexpr int attention_lds() {
-    constexpr int sums = 4 * 16 * Fm::R * (8 + (D + 4) * 4);
+    constexpr int sums = 4 * 16 * (8 + (D + 4) * 4);
     return Fm::WIDE && WideWalk<T, D, Fm::R>::LDS > sums ? WideWalk<T, D, Fm::R>::LDS : sums;
 }
 
@@ -524,78 +522,78 @@ __device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, co
                                        int begin, int end, int part, const int* row_id, char* lds) {
     constexpr int R = Fm::R;
     using Rows = AttentionRows<T, D, R>;
-    constexpr int PITCH = D + 4;  // floats of a row in LDS: lanes of different rows on different banks
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    f32x2* const ml = reinterpret_cast<f32x2*>(lds);                   // [4][16 R]
-    float* const sums = reinterpret_cast<float*>(lds + 4 * 16 * R * 8);  // [4][16 R][PITCH]
-    {
-        Rows rows;
-        rows.begin();
+    Rows rows;
+    rows.begin();
 #pragma unroll
-        for (int r = 0; r < R; ++r) rows.load_q(r, q_row[r], lane);
-        if constexpr (Fm::WIDE) {
-            WideWalk<T, D, R> keys;
-            keys.walk(rows, s, begin * Rows::STEP, end * Rows::STEP, limit, least, most, own_most, a.scale_log2, lane, lds);
-            __syncthreads();  // the sums go where the keys were
-        } else {
-            NarrowWalk<T, D, R> keys;
-            keys.walk(rows, s, begin + wave, end, limit, least, most, a.scale_log2, lane);
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const float l = rows.sum_of(r);
-            if (lane < 16) ml[wave * 16 * R + r * 16 + lane] = f32x2{rows.m[r], l};
-            rows.put_sums(r, sums + (wave * 16 * R + r * 16 + (lane & 15)) * PITCH, lane);
-        }
+    for (int r = 0; r < R; ++r) rows.load_q(r, q_row[r], lane);
+    if constexpr (Fm::WIDE) {
+        WideWalk<T, D, R> keys;
+        keys.walk(rows, s, begin * Rows::STEP, end * Rows::STEP, limit, least, most, own_most, a.scale_log2, lane, lds);
+    } else {
+        NarrowWalk<T, D, R> keys;
+        keys.walk(rows, s, begin + wave, end, limit, least, most, a.scale_log2, lane);
     }
-    __syncthreads();
+    // Through LDS, so that a row's outputs leave side by side, 16 rows of each wave at a time: the waves' sums of one row where they split the keys
+    constexpr int PITCH = D + 4;  // floats of a row in LDS: lanes of different rows on different banks
+    f32x2* const ml = reinterpret_cast<f32x2*>(lds);                 // [4][16]
+    float* const sums = reinterpret_cast<float*>(lds + 4 * 16 * 8);  // [4][16][PITCH]
     const size_t all = (size_t)a.tokens * a.heads;
     const bool whole = a.acc == nullptr;
     const __amdgpu_buffer_rsrc_t to = whole ? descriptor(a.out) : descriptor(a.acc + (size_t)part * all * D);
     const __amdgpu_buffer_rsrc_t to_ml = descriptor(a.ml + (size_t)part * (whole ? 0 : all));
-    for (int e = threadIdx.x; e < Fm::ROWS * (D / 4); e += 256) {
-        const int row = e / (D / 4), d = (e - row * (D / 4)) * 4;
-        const int id = row_id[row];
-        if (id < 0) continue;
-        float top, l;
-        f32x4 sum;
-        if constexpr (Fm::WIDE) {
-            const f32x2 w = ml[row];
-            top = w.x;
-            l = w.y;
-            sum = *reinterpret_cast<const f32x4*>(sums + row * PITCH + d);
-        } else {
-            top = -INFINITY;
-            l = 0.f;
-            sum = f32x4{0.f, 0.f, 0.f, 0.f};
-            f32x2 w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = ml[i * 16 * R + row];
-                top = fmaxf(top, w[i].x);
-            }
-            if (top > -INFINITY) {
+    for (int r = 0; r < R; ++r) {
+        if (Fm::WIDE || r > 0) __syncthreads();  // the keys, or the rows before, have been read
+        const float own = rows.sum_of(r);
+        if (lane < 16) ml[wave * 16 + lane] = f32x2{rows.m[r], own};
+        rows.put_sums(r, sums + (wave * 16 + (lane & 15)) * PITCH, lane);
+        __syncthreads();
+        for (int e = threadIdx.x; e < (Fm::WIDE ? 64 : 16) * (D / 4); e += 256) {
+            const int row = e / (D / 4), d = (e - row * (D / 4)) * 4;
+            const int id = row_id[Fm::WIDE ? (row >> 4) * 16 * R + r * 16 + (row & 15) : r * 16 + row];
+            if (id < 0) continue;
+            float top, l;
+            f32x4 sum;
+            if constexpr (Fm::WIDE) {
+                const f32x2 w = ml[row];
+                top = w.x;
+                l = w.y;
+                sum = *reinterpret_cast<const f32x4*>(sums + row * PITCH + d);
+            } else {
+                top = -INFINITY;
+                l = 0.f;
+                sum = f32x4{0.f, 0.f, 0.f, 0.f};
+                f32x2 w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float f = __builtin_amdgcn_exp2f(w[i].x - top);
-                    l += w[i].y * f;
-                    sum += *reinterpret_cast<const f32x4*>(sums + (i * 16 * R + row) * PITCH + d) * f;
+                    w[i] = ml[i * 16 + row];
+                    top = fmaxf(top, w[i].x);
+                }
+                if (top > -INFINITY) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float f = __builtin_amdgcn_exp2f(w[i].x - top);
+                        l += w[i].y * f;
+                        sum += *reinterpret_cast<const f32x4*>(sums + (i * 16 + row) * PITCH + d) * f;
+                    }
                 }
             }
-        }
-        if (whole) {
-            put_out<T>(to, (unsigned)id * D + d, l > 0.f ? sum / l : f32x4{0.f, 0.f, 0.f, 0.f});
-        } else {
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), to, (int)(((unsigned)id * D + d) * 4), 0, kThrough);
-            if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{as_word(top), as_word(l)}, to_ml, id * 8, 0, kThrough);
+            if (whole) {
+                put_out<T>(to, (unsigned)id * D + d, l > 0.f ? sum / l : f32x4{0.f, 0.f, 0.f, 0.f});
+            } else {
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), to, (int)(((unsigned)id * D + d) * 4), 0, kThrough);
+                if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{as_word(top), as_word(l)}, to_ml, id * 8, 0, kThrough);
+            }
         }
     }
 }
 
-// Four outputs of row `id` from d on: the row's parts, in their order, with the running maximum.  (Read past this workgroup's caches.)
-template <typename T, int D>
+// Four outputs of row `id` from d on: the row's parts, in their order, with the running maximum.  (CACHE: kThrough where other workgroups of this launch
+// wrote them.)
+template <typename T, int D, int CACHE>
 __device__ __forceinline__ void join_parts(const AttentionArgs& a, int id, int d) {
-    const int parts = a.prefix_splits + a.own_splits;
+    const int parts = (int)(a.prefix_splits.d + a.own_splits.d);
     const size_t rows = (size_t)a.tokens * a.heads;
     float top = -INFINITY, l = 0.f;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
@@ -605,8 +603,8 @@ __device__ __forceinline__ void join_parts(const AttentionArgs& a, int id, int d
 #pragma unroll
         for (int i = 0; i < kJoined; ++i) {
             const int part = min(first + i, parts - 1);
-            w[i] = __builtin_amdgcn_raw_buffer_load_b64(descriptor(a.ml + part * rows), id * 8, 0, kThrough);
-            x[i] = __builtin_amdgcn_raw_buffer_load_b128(descriptor(a.acc + part * rows * D), (int)(((unsigned)id * D + d) * 4), 0, kThrough);
+            w[i] = __builtin_amdgcn_raw_buffer_load_b64(descriptor(a.ml + part * rows), id * 8, 0, CACHE);
+            x[i] = __builtin_amdgcn_raw_buffer_load_b128(descriptor(a.acc + part * rows * D), (int)(((unsigned)id * D + d) * 4), 0, CACHE);
         }
         float now = top;
 #pragma unroll
@@ -633,7 +631,7 @@ __device__ __forceinline__ void join_parts(const AttentionArgs& a, int id, int d
 template <typename T, int D, int MOST>
 __device__ __forceinline__ void join_last(const AttentionArgs& a, const int* row_id, int rows_here, int* done) {
     const int lane = threadIdx.x & 63;
-    const int parts = a.prefix_splits + a.own_splits;
+    const int parts = (int)(a.prefix_splits.d + a.own_splits.d);
     __shared__ int count;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -655,7 +653,7 @@ __device__ __forceinline__ void join_last(const AttentionArgs& a, const int* row
     }
     __syncthreads();
     const int n = count;
-    for (int e = threadIdx.x; e < n * (D / 4); e += 256) join_parts<T, D>(a, done[e / (D / 4)], e % (D / 4) * 4);
+    for (int e = threadIdx.x; e < n * (D / 4); e += 256) join_parts<T, D, kThrough>(a, done[e / (D / 4)], e % (D / 4) * 4);
 }
 
 // All rows' parts by a launch of its own: where a workgroup's rows are many, the one that arrives last would be at it for longer than that takes.
@@ -664,7 +662,7 @@ __global__ __launch_bounds__(256) void prefix_attention_join_kernel(AttentionArg
     hook_entry(a.notifier, a.job_id);
     const int rows = (a.starts ? min(max(a.starts[a.sequences], 0), a.tokens) : a.tokens) * a.heads;
     const int row = blockIdx.x * (1024 / D) + (int)threadIdx.x / (D / 4);
-    if (row < rows) join_parts<T, D>(a, row, (int)threadIdx.x % (D / 4) * 4);
+    if (row < rows) join_parts<T, D, 0>(a, row, (int)threadIdx.x % (D / 4) * 4);
     hook_exit(a.notifier, a.job_id);
 }
 
@@ -679,87 +677,89 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int head_bytes = D * T::bytes;
     Keys s;
-    s.page_bytes = (size_t)a.kv_heads * a.page_size * head_bytes;
+    s.page_bytes = (size_t)a.kv_heads.d * a.page_size * head_bytes;
     s.page_blocks = a.page_blocks;
-    s.page_blocks_inv = a.page_blocks_inv;
     s.num_pages = (unsigned)a.num_pages;
-    // Work over the prefix (bound by the products) and over own tokens (bound by memory) alternate, eight workgroups at a time, one for each XCD, in the
-    // proportion of their numbers, so that compute units have some of either.
-    const unsigned prefix_eights = (a.prefix_items + 7) / 8, eights_of_all = gridDim.x / 8, eight = blockIdx.x / 8;
-    const unsigned before = (unsigned)((unsigned long long)eight * prefix_eights / eights_of_all);
-    const bool over_prefix = (unsigned)((unsigned long long)(eight + 1) * prefix_eights / eights_of_all) > before;
-    unsigned item = (over_prefix ? before : eight - before) * 8 + blockIdx.x % 8;
+    // Work over the prefix (bound by the products) and over own tokens (bound by memory) alternate in the proportion of their numbers, so that compute
+    // units have some of either: `turn` workgroups at a time.  (32: one for each shader engine of each XCD.  Workgroups are handed to the engines in
+    // turn, and one that is full holds the others up: by eights, half of the engines had all of the prefix.)
+    bool over_prefix = blockIdx.x < a.prefix_items;
+    unsigned item = over_prefix ? blockIdx.x : blockIdx.x - a.prefix_items;
+    if (a.turn) {
+        const unsigned prefix_turns = (a.prefix_items + a.turn - 1) / a.turn, turn = blockIdx.x / a.turn;
+        const unsigned before = min(turn * a.rate >> 10, prefix_turns);
+        over_prefix = min((turn + 1) * a.rate >> 10, prefix_turns) > before;
+        item = (over_prefix ? before : turn - before) * a.turn + blockIdx.x % a.turn;
+    }
     bool any = item < (over_prefix ? a.prefix_items : a.own_items);
     if (!any) {
-        // the last of an eight that has fewer
+        // a kind's last turn has fewer
     } else if (over_prefix) {
         // (key head, split) by tile: the tiles of one pair read the same keys, so they follow each other by 8 and share an XCD's cache
-        const unsigned pairs = (unsigned)(a.kv_heads * a.prefix_splits), tiles = (unsigned)a.prefix_tiles;
-        const unsigned eights = pairs / 8 * 8 * tiles;
+        const unsigned eights = (unsigned)a.prefix_pairs / 8 * a.eight_tiles.d, left = (unsigned)a.prefix_pairs % 8;
         unsigned pair, tile;
         if (item < eights) {
-            pair = item / (8 * tiles) * 8 + item % 8;
-            tile = item % (8 * tiles) / 8;
+            const Quotient at = divide(item, a.eight_tiles);
+            pair = at.q * 8 + item % 8;
+            tile = at.r / 8;
         } else {
-            const unsigned left = pairs % 8, i = item - eights;
-            pair = pairs / 8 * 8 + i % left;
-            tile = i / left;
+            tile = (item - eights) / left;
+            pair = (unsigned)a.prefix_pairs / 8 * 8 + (item - eights) - tile * left;
         }
-        const int h = (int)(pair / a.prefix_splits), split = (int)(pair % a.prefix_splits);
-        const int first_row = (int)tile * FP::ROWS, group_rows = a.tokens * a.per_kv;
+        const Quotient who = divide(pair, a.prefix_splits);
+        const int h = (int)who.q, split = (int)who.r, per_kv = (int)a.per_kv.d;
+        const int first_row = (int)tile * FP::ROWS, group_rows = a.tokens * per_kv;
         const char* q_row[FP::R];
         int limit[FP::R];
 #pragma unroll
         for (int r = 0; r < FP::R; ++r) {
             const int x = min(first_row + (FP::WIDE ? wave * 16 * FP::R : 0) + r * 16 + (lane & 15), group_rows - 1);
-            const int t = x / a.per_kv;
-            q_row[r] = a.q + t * a.q_stride + (h * a.per_kv + x - t * a.per_kv) * head_bytes;
+            const Quotient at = divide((unsigned)x, a.per_kv);
+            q_row[r] = a.q + at.q * a.q_stride + (h * per_kv + (int)at.r) * head_bytes;
             limit[r] = a.prefix_len;
         }
         if ((int)threadIdx.x < FP::ROWS) {  // rows behind the last sequence are left out
-            const int x = first_row + (int)threadIdx.x, t = x / a.per_kv;
+            const int x = first_row + (int)threadIdx.x;
+            const Quotient at = divide((unsigned)x, a.per_kv);
             const int rows = a.starts ? min(a.starts[a.sequences], a.tokens) : a.tokens;
-            row_id[threadIdx.x] = x < group_rows && t < rows ? t * a.heads + h * a.per_kv + x - t * a.per_kv : -1;
+            row_id[threadIdx.x] = x < group_rows && (int)at.q < rows ? (int)at.q * a.heads + h * per_kv + (int)at.r : -1;
         }
         __syncthreads();
         s.table = a.prefix_table;
-        s.table_len = (a.prefix_len + a.page_size - 1) / a.page_size;
+        s.table_len = a.prefix_pages;
         s.k = a.k_cache + (size_t)h * a.page_size * head_bytes;
         s.v = a.v_cache + (size_t)h * a.page_size * head_bytes;
         const int steps = (a.prefix_len + STEP - 1) / STEP;
-        const int per = (steps + a.prefix_splits - 1) / a.prefix_splits;
-        const int begin = min(split * per, steps), end = min(begin + per, steps);
+        const int begin = min(split * a.prefix_per, steps), end = min(begin + a.prefix_per, steps);
         attend<T, D, FP>(a, s, q_row, limit, a.prefix_len, a.prefix_len, a.prefix_len, begin, end, split, row_id, lds);
     } else {
         // the key heads of one sequence side by side: they share the look-ups and, with eight of them, an XCD each
-        const int h = (int)(item % a.kv_heads);
-        item /= (unsigned)a.kv_heads;
-        const int split = (int)(item % a.own_splits);
-        item /= (unsigned)a.own_splits;
-        const int tile = (int)(item % a.own_tiles), seq = (int)(item / a.own_tiles);
+        const Quotient by_head = divide(item, a.kv_heads), by_split = divide(by_head.q, a.own_splits), by_tile = divide(by_split.q, a.own_tiles);
+        const int h = (int)by_head.r, split = (int)by_split.r, tile = (int)by_tile.r, seq = (int)by_tile.q, per_kv = (int)a.per_kv.d;
         int first = seq * a.max_new, count = a.max_new;
         if (a.starts) {
             first = min(max(__builtin_amdgcn_readfirstlane(a.starts[seq]), 0), a.tokens);
             count = min(min(__builtin_amdgcn_readfirstlane(a.starts[seq + 1]), a.tokens) - first, a.max_new);
         }
-        const int first_row = tile * FO::ROWS, group_rows = max(count, 0) * a.per_kv;
+        const int first_row = tile * FO::ROWS, group_rows = max(count, 0) * per_kv;
         any = first_row < group_rows;
         if (any) {
             const int capacity = (int)min((int64_t)a.max_pages * a.page_size, (int64_t)1 << 30);
             const int past = min(max(__builtin_amdgcn_readfirstlane(a.past[seq]), 0), capacity);
-            auto limit_of = [&](int row) { return min(past + min(row, group_rows - 1) / a.per_kv + 1, capacity); };
+            auto limit_of = [&](int row) { return min(past + (int)divide((unsigned)min(row, group_rows - 1), a.per_kv).q + 1, capacity); };
             const int wave_row = first_row + (FO::WIDE ? wave * 16 * FO::R : 0);
             const char* q_row[FO::R];
             int limit[FO::R];
 #pragma unroll
             for (int r = 0; r < FO::R; ++r) {
-                const int x = min(wave_row + r * 16 + (lane & 15), group_rows - 1), j = x / a.per_kv;
-                q_row[r] = a.q + (first + j) * a.q_stride + (h * a.per_kv + x - j * a.per_kv) * head_bytes;
-                limit[r] = min(past + j + 1, capacity);
+                const Quotient at = divide((unsigned)min(wave_row + r * 16 + (lane & 15), group_rows - 1), a.per_kv);
+                q_row[r] = a.q + (first + (int)at.q) * a.q_stride + (h * per_kv + (int)at.r) * head_bytes;
+                limit[r] = min(past + (int)at.q + 1, capacity);
             }
             if ((int)threadIdx.x < FO::ROWS) {
-                const int x = first_row + (int)threadIdx.x, j = x / a.per_kv;
-                row_id[threadIdx.x] = x < group_rows ? (first + j) * a.heads + h * a.per_kv + x - j * a.per_kv : -1;
+                const int x = first_row + (int)threadIdx.x;
+                const Quotient at = divide((unsigned)x, a.per_kv);
+                row_id[threadIdx.x] = x < group_rows ? (first + (int)at.q) * a.heads + h * per_kv + (int)at.r : -1;
             }
             __syncthreads();
             s.table = a.tables + (size_t)seq * a.max_pages;
@@ -769,9 +769,9 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(
             const int least = limit_of(wave_row), most = limit_of(first_row + FO::ROWS - 1);
             const int own_most = FO::WIDE ? limit_of(wave_row + 16 * FO::R - 1) : most;
             const int steps = (most + STEP - 1) / STEP;
-            const int per = (steps + a.own_splits - 1) / a.own_splits;
+            const int per = (int)divide((unsigned)steps + a.own_splits.d - 1, a.own_splits).q;
             const int begin = min(split * per, steps), end = min(begin + per, steps);
-            attend<T, D, FO>(a, s, q_row, limit, least, most, own_most, begin, end, a.prefix_splits + split, row_id, lds);
+            attend<T, D, FO>(a, s, q_row, limit, least, most, own_most, begin, end, (int)a.prefix_splits.d + split, row_id, lds);
         }
     }
     if (any && a.counters) join_last<T, D, MOST>(a, row_id, over_prefix ? FP::ROWS : FO::ROWS, done);
