@@ -70,9 +70,11 @@ int stages_of(const paella_prefix_attention_plan* p) {
     return ceil_div(rows * p->head_dim / 4, 256) * ceil_div(parts, kJoined) <= 4 ? 1 : 2;
 }
 
+size_t counter_pitch(const paella_prefix_attention_plan* p) { return up256((size_t)p->tokens * (p->heads / p->kv_heads) * 4) / 4; }
+
 size_t workspace_of(const paella_prefix_attention_plan* p) {
     const size_t parts = (size_t)p->prefix_splits + p->own_splits, rows = (size_t)p->tokens * p->heads;
-    return parts == 1 ? 0 : up256(rows * 4) + up256(parts * rows * 8) + parts * rows * p->head_dim * 4;
+    return parts == 1 ? 0 : p->kv_heads * counter_pitch(p) * 4 + up256(parts * rows * 8) + parts * rows * p->head_dim * 4;
 }
 
 }  // namespace
@@ -117,7 +119,7 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_
 
 int paella_prefix_attention_dims(const paella_prefix_attention_plan* p, int stage, paella_launch_dims* dims) {
     if (!plan_ok(p) || !dims || stage < 0 || stage >= stages_of(p)) return PAELLA_EINVAL;
-    if (stage) set_launch_dims(dims, (unsigned)ceil_div((int64_t)p->tokens * p->heads, 1024 / p->head_dim), 256, 0, 64);
+    if (stage) set_launch_dims(dims, (unsigned)ceil_div((int64_t)p->tokens * p->heads, kJoinRows / p->head_dim), 256, 0, 64);
     else set_launch_dims(dims, (unsigned)grid_of(p).all, 256, 0, 256);
     loaded_dims((const void*)(stage ? join_of(p) : kernel_of(p)), dims);
     return 0;
@@ -153,10 +155,11 @@ int paella_prefix_attention_launch_stage(const paella_prefix_attention_plan* p, 
     a.prefix_items = (unsigned)g.prefix_items; a.own_items = (unsigned)g.own_items; a.turn = (unsigned)g.turn; a.rate = (unsigned)g.rate;
     const size_t parts = (size_t)p->prefix_splits + p->own_splits, rows = (size_t)p->tokens * p->heads;
     a.counters = need && stages_of(p) == 1 ? (unsigned*)workspace : nullptr;
-    a.ml = need ? (f32x2*)((char*)workspace + up256(rows * 4)) : nullptr;
+    a.counter_pitch = (unsigned)counter_pitch(p);
+    a.ml = need ? (f32x2*)((char*)workspace + p->kv_heads * counter_pitch(p) * 4) : nullptr;
     a.acc = need ? (float*)((char*)a.ml + up256(parts * rows * 8)) : nullptr;
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
-    const unsigned grid = stage ? (unsigned)ceil_div((int64_t)rows, 1024 / p->head_dim) : (unsigned)g.all;
+    const unsigned grid = stage ? (unsigned)ceil_div((int64_t)rows, kJoinRows / p->head_dim) : (unsigned)g.all;
     launch(stage ? join_of(p) : kernel_of(p), dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }

@@ -37,14 +37,17 @@ struct AttentionArgs {
     int prefix_per, prefix_pairs;                               // steps of a split; key heads by splits
     unsigned prefix_items, own_items;
     unsigned turn, rate;    // workgroups of one kind in a row (0: all over the prefix, then all over own tokens); 1024ths of the turns that are the prefix's until it is done
-    unsigned* counters;  // [tokens * heads], zero between launches; null where a launch of its own joins
+    unsigned* counters;     // [key heads][rows of one, in whole cache lines], zero between launches; null where a launch of its own joins.  A workgroup's lie side by
+                            // side, and other key heads' on other lines: counts on one line go one after the other
+    unsigned counter_pitch;
     f32x2* ml;           // [splits][tokens * heads]: running maximum and sum of each part
     float* acc;          // [splits][tokens * heads][head_dim]
     uint32_t job_id;
     Notifier* notifier;
 };
 
-constexpr int kJoined = 8;  // parts of a row that are requested together
+constexpr int kJoined = 16;     // parts of a row that the workgroup that joins it requests together
+constexpr int kJoinRows = 256;  // outputs of a workgroup of the joining launch
 
 template <typename T> struct Mfma;
 template <> struct Mfma<Bf16> {
@@ -81,8 +84,9 @@ struct Keys {
     __device__ __forceinline__ size_t page_at(int page) const { return ((unsigned)page < num_pages ? (unsigned)page : 0u) * page_bytes; }
 };
 
-// 16 R query rows of a wave: what they have summed so far.  Lane l holds row l % 16 of each 16.
-template <typename T, int D, int R>
+// 16 R query rows of a wave: what they have summed so far.  Lane l holds row l % 16 of each 16.  STRAIGHT: V comes with its dimensions in order, 16 to a
+// product, else by pieces of PER of them.
+template <typename T, int D, int R, bool STRAIGHT>
 struct AttentionRows {
     static constexpr bool F = T::bytes == 4;
     static constexpr int NT = F ? 1 : 2;              // score tiles of 16 keys per step
@@ -221,6 +225,14 @@ struct AttentionRows {
         }
     }
 
+    // The same from V as the transposing reads of LDS bring it: v[d], dimensions 16 d on of the lane group's keys.
+    __device__ __forceinline__ void add_straight(const u32x4 (&v)[D / 16], const unsigned (&p)[R][4]) {
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+            for (int r = 0; r < R; ++r) acc[r][d] = Mfma<T>::go(v[d], u32x4{p[r][0], p[r][1], p[r][2], p[r][3]}, acc[r][d]);
+    }
+
     __device__ __forceinline__ float sum_of(int r) const {
         float l = total[r][0];
         if constexpr (F) {  // the lane groups' parts
@@ -232,22 +244,27 @@ struct AttentionRows {
 
     // Sums to a row of LDS (`to`: of the lane's row in 16 r), dimensions in order.
     __device__ __forceinline__ void put_sums(int r, float* to, int lane) const {
+        if constexpr (STRAIGHT) {
 #pragma unroll
-        for (int g = 0; g < GRP; ++g)
+            for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4*>(to + d * 16 + (lane >> 4) * 4) = acc[r][d];
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int g = 0; g < GRP; ++g)
 #pragma unroll
-                for (int e = 0; e < PER; e += 4) {
-                    const int d = g * PER + e;
-                    *reinterpret_cast<f32x4*>(to + g * 16 * PER + ((lane >> 4) * 4 + i) * PER + e) = f32x4{acc[r][d][i], acc[r][d + 1][i], acc[r][d + 2][i], acc[r][d + 3][i]};
-                }
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < PER; e += 4) {
+                        const int d = g * PER + e;
+                        *reinterpret_cast<f32x4*>(to + g * 16 * PER + ((lane >> 4) * 4 + i) * PER + e) = f32x4{acc[r][d][i], acc[r][d + 1][i], acc[r][d + 2][i], acc[r][d + 3][i]};
+                    }
+        }
     }
 };
 
 // Few rows: a wave has all of the workgroup's rows and every fourth step of its keys, which come straight from memory into registers.
 template <typename T, int D, int R>
 struct NarrowWalk {
-    using Rows = AttentionRows<T, D, R>;
+    using Rows = AttentionRows<T, D, R, false>;
     static constexpr bool F = Rows::F;
     static constexpr int ROW = Rows::ROW, TPL = Rows::TPL, STEP = Rows::STEP;
 
@@ -357,11 +374,12 @@ struct NarrowWalk {
 
 // Many rows: each of the four waves has 16 R rows of its own, and all of them walk the same keys, which the workgroup brings to LDS tile by tile: the
 // next tile's loads are under way while the one before is worked on.  16-byte piece c of key i lies at place c ^ turn(i), so that the 16 keys of a score
-// tile are read from different banks.
+// tile, and the 8 keys by 32 bytes that half a wave reads of V, come from different banks.  16-bit V comes by transposing reads (of 4 keys by 16 dimensions,
+// per 16 lanes), which leave the vector unit the 32 permutations of a step.
 template <typename T, int D, int R>
 struct WideWalk {
-    using Rows = AttentionRows<T, D, R>;
-    static constexpr bool F = Rows::F;
+    static constexpr bool F = T::bytes == 4;
+    using Rows = AttentionRows<T, D, R, !F>;
     static constexpr int ROW = Rows::ROW, TPL = Rows::TPL, STEP = Rows::STEP;
     static constexpr int PIECES = ROW / 16;
     static constexpr int TILE = 16384 / ROW < 64 ? 16384 / ROW : 64;  // keys
@@ -374,8 +392,8 @@ struct WideWalk {
 
     __device__ __forceinline__ static int turn(int key) {
         if constexpr (F) return key & 15;
-        else if constexpr (PIECES >= 16) return (key & 3) | (key >> 3 & 3) << 2;
-        else return (key >> 1 & 1) | (key >> 3 & 3) << 1;  // two keys make up the banks
+        else if constexpr (PIECES >= 16) return (key >> 4 & 1) | (key & 3) << 1 | (key >> 3 & 1) << 3;
+        else return (key >> 4 & 1) | (key >> 1 & 1) << 1 | (key >> 3 & 1) << 2;  // two keys make up the banks
     }
 
     __device__ __forceinline__ void look_up(const Keys& s, int first) {
@@ -436,15 +454,21 @@ struct WideWalk {
         }
         __syncthreads();
         const int group = lane >> 4, mm = lane & 15;
-        int k_at[Rows::KC], v_at[4];
+        constexpr int V_PLACES = F ? 4 : PIECES < 16 ? PIECES / 2 : 8;
+        int k_at[Rows::KC], v_at[V_PLACES];
         {
             const int key = F ? mm : (mm >> 2) * 8 + (mm & 3);
 #pragma unroll
             for (int c = 0; c < Rows::KC; ++c) k_at[c] = key * ROW + ((c * 4 + group) ^ turn(key)) * 16;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int from = group * TPL + u, piece = mm * Rows::VW / 4;
-                v_at[u] = TILE * ROW + from * ROW + (piece ^ turn(from)) * 16 + (Rows::VW == 2 ? (mm & 1) * 8 : 0);
+            for (int u = 0; u < V_PLACES; ++u) {
+                if constexpr (F) {  // key u of the lane group's, the lane's four dimensions
+                    const int from = group * TPL + u;
+                    v_at[u] = TILE * ROW + from * ROW + (mm ^ turn(from)) * 16;
+                } else {  // key mm / 4 of the lane group's, dimensions 16 u + mm % 4 * 4 on
+                    const int from = group * TPL + (mm >> 2);
+                    v_at[u] = TILE * ROW + from * ROW + ((u * 2 + (mm >> 1 & 1)) ^ turn(from)) * 16 + (mm & 1) * 8;
+                }
             }
         }
         for (; first < end; first += TILE) {
@@ -456,27 +480,34 @@ struct WideWalk {
                 f32x4 x[R][Rows::NT];
                 rows.scores(x, [&](int t, int c) { return *reinterpret_cast<const u32x4*>(from + k_at[c] + sub * STEP * ROW + t * 4 * ROW); });
                 unsigned w[TPL][Rows::GRP * Rows::VW];
+                u32x4 straight[D / 16];
+                // pieces and keys further on whose bits the turn leaves alone are at fixed distances
+                if constexpr (F) {
 #pragma unroll
-                for (int u = 0; u < TPL; ++u)
+                    for (int u = 0; u < TPL; ++u)
 #pragma unroll
-                    for (int g = 0; g < Rows::GRP; ++g) {
-                        // piece g * 16 further on: the turn leaves those bits alone
-                        const char* const at = from + v_at[u & 3] + sub * STEP * ROW + (u >> 2) * 4 * ROW + g * 256;
-                        if constexpr (Rows::VW == 4) {
-                            const u32x4 y = *reinterpret_cast<const u32x4*>(at);
+                        for (int g = 0; g < Rows::GRP; ++g) {
+                            const u32x4 y = *reinterpret_cast<const u32x4*>(from + v_at[u] + sub * STEP * ROW + g * 256);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) w[u][g * 4 + e] = y[e];
-                        } else {
-                            const u32x2 y = *reinterpret_cast<const u32x2*>(at);
-                            w[u][g * 2] = y.x;
-                            w[u][g * 2 + 1] = y.y;
                         }
+                } else {
+                    typedef short s16x4 __attribute__((ext_vector_type(4)));
+                    typedef __attribute__((address_space(3))) s16x4* LdsPointer;
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        const char* const at = from + v_at[d % V_PLACES] + sub * STEP * ROW + d / V_PLACES * 256;
+                        const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPointer)at));
+                        const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPointer)(at + 4 * ROW)));
+                        straight[d] = u32x4{a.x, a.y, b.x, b.y};
                     }
+                }
                 const bool gone = absent[sub * STEP / 8 + group * TPL / 8] != 0;
                 if (first + (sub + 1) * STEP > least || __any(gone)) Rows::mask(x, first + sub * STEP + group * TPL, gone, limit);
                 unsigned p[R][4];
                 rows.weigh(x, scale, p);
-                rows.add_values(w, p);
+                if constexpr (F) rows.add_values(w, p);
+                else rows.add_straight(straight, p);
             }
             if (first + TILE < end) {
                 __syncthreads();
@@ -521,7 +552,7 @@ template <typename T, int D, typename Fm>
 __device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, const char* const (&q_row)[Fm::R], const int (&limit)[Fm::R], int least, int most, int own_most,
                                        int begin, int end, int part, const int* row_id, char* lds) {
     constexpr int R = Fm::R;
-    using Rows = AttentionRows<T, D, R>;
+    using Rows = AttentionRows<T, D, R, Fm::WIDE && T::bytes == 2>;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     Rows rows;
     rows.begin();
@@ -589,49 +620,59 @@ __device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, co
     }
 }
 
-// Four outputs of row `id` from d on: the row's parts, in their order, with the running maximum.  (CACHE: kThrough where other workgroups of this launch
-// wrote them.)
-template <typename T, int D, int CACHE>
-__device__ __forceinline__ void join_parts(const AttentionArgs& a, int id, int d) {
-    const int parts = (int)(a.prefix_splits.d + a.own_splits.d);
-    const size_t rows = (size_t)a.tokens * a.heads;
+// What some parts of a row sum up to, four outputs from d on.
+struct Joined {
     float top = -INFINITY, l = 0.f;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int first = 0; first < parts; first += kJoined) {
-        u32x2 w[kJoined];
-        u32x4 x[kJoined];
-#pragma unroll
-        for (int i = 0; i < kJoined; ++i) {
-            const int part = min(first + i, parts - 1);
-            w[i] = __builtin_amdgcn_raw_buffer_load_b64(descriptor(a.ml + part * rows), id * 8, 0, CACHE);
-            x[i] = __builtin_amdgcn_raw_buffer_load_b128(descriptor(a.acc + part * rows * D), (int)(((unsigned)id * D + d) * 4), 0, CACHE);
-        }
-        float now = top;
-#pragma unroll
-        for (int i = 0; i < kJoined; ++i)
-            if (first + i < parts) now = fmaxf(now, as_float(w[i].x));
-        if (now == -INFINITY) continue;
+    __device__ __forceinline__ void add(float t, float n, f32x4 x) {
+        const float f = __builtin_amdgcn_exp2f(t - top);
+        l += n * f;
+        sum += x * f;
+    }
+    __device__ __forceinline__ bool raise(float now) {  // the running maximum; false while there is nothing
+        if (now == -INFINITY) return false;
         const float shrink = __builtin_amdgcn_exp2f(top - now);
         sum *= shrink;
         l *= shrink;
         top = now;
-#pragma unroll
-        for (int i = 0; i < kJoined; ++i) {
-            if (first + i >= parts) continue;
-            const float f = __builtin_amdgcn_exp2f(as_float(w[i].x) - top);
-            l += as_float(w[i].y) * f;
-            sum += __builtin_bit_cast(f32x4, x[i]) * f;
-        }
+        return true;
     }
-    put_out<T>(descriptor(a.out), (unsigned)id * D + d, l > 0.f ? sum / l : f32x4{0.f, 0.f, 0.f, 0.f});
+    __device__ __forceinline__ f32x4 out() const { return l > 0.f ? sum / l : f32x4{0.f, 0.f, 0.f, 0.f}; }
+};
+
+// Parts first, first + every, ... of row `id`, in their order, N of them requested together.  (CACHE: kThrough where other workgroups of this launch
+// wrote them.)
+template <int D, int N, int CACHE>
+__device__ __forceinline__ Joined join_parts(const AttentionArgs& a, int id, int d, int first, int every) {
+    const int parts = (int)(a.prefix_splits.d + a.own_splits.d);
+    const size_t rows = (size_t)a.tokens * a.heads;
+    Joined all;
+    for (; first < parts; first += N * every) {
+        u32x2 w[N];
+        u32x4 x[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int part = min(first + i * every, parts - 1);
+            w[i] = __builtin_amdgcn_raw_buffer_load_b64(descriptor(a.ml + part * rows), id * 8, 0, CACHE);
+            x[i] = __builtin_amdgcn_raw_buffer_load_b128(descriptor(a.acc + part * rows * D), (int)(((unsigned)id * D + d) * 4), 0, CACHE);
+        }
+        float now = all.top;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (first + i * every < parts) now = fmaxf(now, as_float(w[i].x));
+        if (!all.raise(now)) continue;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (first + i * every < parts) all.add(as_float(w[i].x), as_float(w[i].y), __builtin_bit_cast(f32x4, x[i]));
+    }
+    return all;
 }
 
 // Counts the workgroup in at each of its rows and puts together the rows at which it is the last.  (As in the convs' split reductions: parts
 // are written through ahead of the count.)
 template <typename T, int D, int MOST>
-__device__ __forceinline__ void join_last(const AttentionArgs& a, const int* row_id, int rows_here, int* done) {
-    const int lane = threadIdx.x & 63;
-    const int parts = (int)(a.prefix_splits.d + a.own_splits.d);
+__device__ __forceinline__ void join_last(const AttentionArgs& a, const int* row_id, unsigned first_counter, int rows_here, int* done) {
+    const int lane = threadIdx.x & 63, parts = (int)(a.prefix_splits.d + a.own_splits.d);
     __shared__ int count;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -642,8 +683,9 @@ __device__ __forceinline__ void join_last(const AttentionArgs& a, const int* row
             const int id = first + lane < rows_here ? row_id[first + lane] : -1;
             bool last = false;
             if (id >= 0) {
-                last = __hip_atomic_fetch_add(a.counters + id, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)parts - 1;
-                if (last) __hip_atomic_store(a.counters + id, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                unsigned* const counter = a.counters + first_counter + first + lane;
+                last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)parts - 1;
+                if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             const unsigned long long who = __ballot(last);
             if (last) done[n + __popcll(who & ((1ull << lane) - 1))] = id;
@@ -653,16 +695,40 @@ __device__ __forceinline__ void join_last(const AttentionArgs& a, const int* row
     }
     __syncthreads();
     const int n = count;
-    for (int e = threadIdx.x; e < n * (D / 4); e += 256) join_parts<T, D, kThrough>(a, done[e / (D / 4)], e % (D / 4) * 4);
+    const __amdgpu_buffer_rsrc_t to = descriptor(a.out);
+    for (int e = threadIdx.x; e < n * (D / 4); e += 256) {
+        const int id = done[e / (D / 4)], d = e % (D / 4) * 4;
+        put_out<T>(to, (unsigned)id * D + d, join_parts<D, kJoined, kThrough>(a, id, d, 0, 1).out());
+    }
 }
 
-// All rows' parts by a launch of its own: where a workgroup's rows are many, the one that arrives last would be at it for longer than that takes.
+// All rows' parts by a launch of its own: where a workgroup's rows are many, the one that arrives last would be at it for longer than that takes.  A quarter of
+// a row's parts per group of lanes, all of them requested at once up to 32: 2048 rows of 128 in 34 parts, 36 MB, by whole rows in steps of
+// eight 18 us.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void prefix_attention_join_kernel(AttentionArgs a) {
     hook_entry(a.notifier, a.job_id);
+    constexpr int LANES = D / 4, ROWS = kJoinRows / D;
+    static_assert(ROWS * LANES == 64, "a wave per quarter");
+    __shared__ f32x4 sums[4][ROWS * LANES];
+    __shared__ f32x2 ml[4][ROWS * LANES];
     const int rows = (a.starts ? min(max(a.starts[a.sequences], 0), a.tokens) : a.tokens) * a.heads;
-    const int row = blockIdx.x * (1024 / D) + (int)threadIdx.x / (D / 4);
-    if (row < rows) join_parts<T, D, 0>(a, row, (int)threadIdx.x % (D / 4) * 4);
+    const int at = (int)threadIdx.x % (ROWS * LANES), quarter = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);  // (a wave each: descriptors go by it)
+    const int row = blockIdx.x * ROWS + at / LANES, d = at % LANES * 4;
+    if (row < rows) {
+        const Joined mine = join_parts<D, 8, 0>(a, row, d, quarter, 4);
+        sums[quarter][at] = mine.sum;
+        ml[quarter][at] = f32x2{mine.top, mine.l};
+    }
+    __syncthreads();
+    if (quarter == 0 && row < rows) {
+        Joined all;
+        if (all.raise(fmaxf(fmaxf(ml[0][at].x, ml[1][at].x), fmaxf(ml[2][at].x, ml[3][at].x)))) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) all.add(ml[i][at].x, ml[i][at].y, sums[i][at]);
+        }
+        put_out<T>(descriptor(a.out), (unsigned)row * D + d, all.out());
+    }
     hook_exit(a.notifier, a.job_id);
 }
 
@@ -673,7 +739,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(
     constexpr int LP = attention_lds<T, D, FP>(), LO = attention_lds<T, D, FO>(), MOST = FP::ROWS > FO::ROWS ? FP::ROWS : FO::ROWS;
     __shared__ __attribute__((aligned(16))) char lds[LP > LO ? LP : LO];
     __shared__ int row_id[MOST], done[MOST];
-    constexpr int STEP = AttentionRows<T, D, 1>::STEP;
+    constexpr int STEP = AttentionRows<T, D, 1, false>::STEP;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int head_bytes = D * T::bytes;
     Keys s;
@@ -692,6 +758,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(
         item = (over_prefix ? before : turn - before) * a.turn + blockIdx.x % a.turn;
     }
     bool any = item < (over_prefix ? a.prefix_items : a.own_items);
+    unsigned first_counter = 0;
     if (!any) {
         // a kind's last turn has fewer
     } else if (over_prefix) {
@@ -709,6 +776,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(
         const Quotient who = divide(pair, a.prefix_splits);
         const int h = (int)who.q, split = (int)who.r, per_kv = (int)a.per_kv.d;
         const int first_row = (int)tile * FP::ROWS, group_rows = a.tokens * per_kv;
+        first_counter = (unsigned)h * a.counter_pitch + (unsigned)first_row;
         const char* q_row[FP::R];
         int limit[FP::R];
 #pragma unroll
@@ -743,6 +811,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(
         }
         const int first_row = tile * FO::ROWS, group_rows = max(count, 0) * per_kv;
         any = first_row < group_rows;
+        first_counter = (unsigned)h * a.counter_pitch + (unsigned)(first * per_kv + first_row);
         if (any) {
             const int capacity = (int)min((int64_t)a.max_pages * a.page_size, (int64_t)1 << 30);
             const int past = min(max(__builtin_amdgcn_readfirstlane(a.past[seq]), 0), capacity);
@@ -774,7 +843,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(
             attend<T, D, FO>(a, s, q_row, limit, least, most, own_most, begin, end, (int)a.prefix_splits.d + split, row_id, lds);
         }
     }
-    if (any && a.counters) join_last<T, D, MOST>(a, row_id, over_prefix ? FP::ROWS : FO::ROWS, done);
+    if (any && a.counters) join_last<T, D, MOST>(a, row_id, first_counter, over_prefix ? FP::ROWS : FO::ROWS, done);
     hook_exit(a.notifier, a.job_id);
 }
 

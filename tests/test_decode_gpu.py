@@ -227,7 +227,7 @@ def test_attention_of_large_scores_and_a_strided_query(cuda):
     within(out, want, ref.attention_bound(want, weight, products, BF16, 170))
 
 
-@pytest.mark.parametrize("case,stages", [(3, 1), (16, 2), (17, 2)])
+@pytest.mark.parametrize("case,stages", [(3, 1), (16, 1), (17, 2)])
 def test_attention_is_the_same_every_time_in_graphs_on_streams_and_direct_queues(cuda, case, stages):
     """Which workgroup joins a row changes from run to run, the bits do not: eager, replayed (two graphs of one plan side by side, lengths changed between replays), on another
     stream and on a direct-dispatch queue."""
