@@ -75,7 +75,10 @@ __device__ __forceinline__ u32x4 load_unaligned(const char* p) {
 template <typename T>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     hook_entry(a.notifier, a.job_id);
-    __shared__ f32x2 turn[256];  // (cos, sin) of each pair's angle
+    // (cos, sin) of each pair's angle and the norms' weights, the same for every head.  In LDS rather than in registers: with them there five
+    // workgroups fit a compute unit instead of eight, and the prompts' rate goes by the loads in flight.
+    __shared__ __attribute__((aligned(16))) f32x2 turn[256];
+    __shared__ __attribute__((aligned(16))) float norm[2][512];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int t = blockIdx.x;
     int seq, j;
@@ -99,35 +102,41 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
             }
         };
         fetch(0);
-        float wq[8], wk[8];  // a lane's values have the same places in every head
-        auto weights = [&](float (&w)[8], const float* from) {
-            const int at = in_head ? li * 8 : 0;
-            const u32x4 a = load_unaligned(reinterpret_cast<const char*>(from + at)), b = load_unaligned(reinterpret_cast<const char*>(from + at + 4));
+        // Trips to memory that do not wait for one another go out together: heads, length, weights and frequencies, then the page.
+        const int past = a.past[seq];
+        float wq[2], wk[2], freq = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                w[e] = as_float(a[e]);
-                w[4 + e] = as_float(b[e]);
-            }
-        };
-        if (a.q_weight) weights(wq, a.q_weight);
-        if (a.k_weight) weights(wk, a.k_weight);
+        for (int u = 0; u < 2; ++u) {
+            const int i = u * 256 + (int)threadIdx.x;
+            wq[u] = a.q_weight && i < a.dim ? a.q_weight[i] : 0.f;
+            wk[u] = a.k_weight && i < a.dim ? a.k_weight[i] : 0.f;
+        }
+        if ((int)threadIdx.x < a.rotary / 2) freq = a.inv_freq[threadIdx.x];
         // where the token goes; a place outside the table or the cache is none
-        const unsigned own = (unsigned)max(a.past[seq], 0) + (unsigned)j;
+        const unsigned own = (unsigned)max(past, 0) + (unsigned)j;
         const Quotient place = divide(own, a.page_size);
         const unsigned column = place.q, slot = place.r;
         int page = -1;
         if (column < (unsigned)a.max_pages) page = a.tables[(size_t)seq * a.max_pages + column];
-        page = __builtin_amdgcn_readfirstlane(page);  // (descriptors are built from it)
-        const bool placed = (unsigned)page < (unsigned)a.num_pages;
-        // The angle in revolutions, reduced to half a turn in 64 bits: in 32 bits a position of 100000 would be off by 0.006 radians.  (Each pair once
-        // per token, by one lane; 16 heads' worth of lanes read it from LDS.)
-        for (int i = threadIdx.x; i < a.rotary / 2; i += 256) {
-            const double turns = ((double)a.prefix_len + (double)own) * (double)a.inv_freq[i] * 0.15915494309189533577;
+        // The angle in revolutions, reduced to half a turn in 64 bits: in 32 bits a position of 100000 would be off by 0.006 radians.  Each pair once per
+        // token, by one lane.
+        if ((int)threadIdx.x < a.rotary / 2) {
+            const double turns = ((double)a.prefix_len + (double)own) * (double)freq * 0.15915494309189533577;
             float s, c;
             sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-            turn[i] = f32x2{c, s};
+            turn[threadIdx.x] = f32x2{c, s};
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int i = u * 256 + (int)threadIdx.x;
+            if (i < a.dim) {
+                norm[0][i] = wq[u];
+                norm[1][i] = wk[u];
+            }
         }
         __syncthreads();
+        page = __builtin_amdgcn_readfirstlane(page);  // (descriptors are built from it)
+        const bool placed = (unsigned)page < (unsigned)a.num_pages;
         const size_t page_bytes = (size_t)a.kv_heads * a.page_size.d * head_bytes;
         const __amdgpu_buffer_rsrc_t to_q = descriptor(a.q_out + (size_t)t * a.heads * head_bytes);
         const __amdgpu_buffer_rsrc_t to_k = descriptor(a.k_cache + (placed ? page : 0) * page_bytes);
@@ -135,13 +144,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
         const int half = a.rotary >> 1, d0 = li * 8;  // rotary_dim is a multiple of 16: a lane's values are all in one half, or none is rotated
         const bool turned = d0 < a.rotary, lower = d0 < half;
         const int other = ((lane & ~(group - 1)) + (lower ? li + (half >> 3) : li - (half >> 3))) & 63;
-        f32x2 cs[8];  // of a lane's values (interleaved: of its four pairs): the same in every head
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if (a.interleaved) cs[e] = turned ? turn[(d0 >> 1) + (e & 3)] : f32x2{1.f, 0.f};
-            else cs[e] = turned ? turn[(lower ? d0 : d0 - half) + e] : f32x2{1.f, 0.f};
-            if (!a.interleaved && lower) cs[e].y = -cs[e].y;
-        }
+        const f32x4* const turns = reinterpret_cast<const f32x4*>(turn + (!turned ? 0 : a.interleaved ? d0 >> 1 : lower ? d0 : d0 - half));
         for (int first = 0; first < total; first += AHEAD * 4 * per_wave) {
             if (first) fetch(first);
 #pragma unroll
@@ -164,24 +167,28 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
                     sum = lanes_sum(sum, a.group_log2);
                     if (is_q ? a.q_weight != nullptr : !is_v && a.k_weight != nullptr) {
                         const float r = __builtin_amdgcn_rsqf(sum * a.inv_dim + a.eps);
+                        const f32x4* const w = reinterpret_cast<const f32x4*>(norm[is_q ? 0 : 1] + (in_head ? d0 : 0));
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = f[e] * r * (is_q ? wq[e] : wk[e]);
+                        for (int e = 0; e < 8; ++e) f[e] = f[e] * r * w[e / 4][e % 4];
                     }
                 }
                 if (a.rotary) {
                     if (a.interleaved) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float p = f[2 * e], q = f[2 * e + 1];
-                            f[2 * e] = turned ? p * cs[e].x - q * cs[e].y : p;
-                            f[2 * e + 1] = turned ? q * cs[e].x + p * cs[e].y : q;
+                            const float c = turns[e / 2][e % 2 * 2], s = turns[e / 2][e % 2 * 2 + 1], p = f[2 * e], q = f[2 * e + 1];
+                            f[2 * e] = turned ? p * c - q * s : p;
+                            f[2 * e + 1] = turned ? q * c + p * s : q;
                         }
                     } else {
                         float partner[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) partner[e] = __shfl(f[e], other, 64);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = f[e] * cs[e].x + (turned ? partner[e] * cs[e].y : 0.f);
+                        for (int e = 0; e < 8; ++e) {
+                            const float c = turns[e / 2][e % 2 * 2], s = turns[e / 2][e % 2 * 2 + 1];
+                            if (turned) f[e] = f[e] * c + (lower ? -partner[e] : partner[e]) * s;
+                        }
                     }
                 }
                 if (!live) continue;
