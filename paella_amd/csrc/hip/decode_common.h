@@ -133,7 +133,8 @@ __device__ __forceinline__ bool row_owner(const int* __restrict__ starts, int se
     return *j >= 0 && *j < (int)max_new.d;
 }
 
-// Host side: what every entry point asks of a cache and a batch.  `tables`: the batch's device pointers are needed too.
+// Host side: what every entry point asks of a cache and a batch.
+constexpr double kMostWorkgroups = 16777215.;  // of 256 threads in one launch: the runtime counts threads in 32 bits
 inline int element_bytes(int dtype) { return dtype == PAELLA_F32 ? 4 : 2; }
 
 inline bool cache_extents_ok(const paella_kv_cache* c) {
@@ -146,6 +147,7 @@ inline bool cache_ok(const paella_kv_cache* c) { return cache_extents_ok(c) && c
 inline bool batch_extents_ok(const paella_kv_batch* b) {
     if (!b || b->sequences <= 0 || b->max_new <= 0 || b->tokens <= 0 || b->max_pages <= 0 || b->prefix_len < 0) return false;
     // rows and positions are 32-bit numbers
+    if (b->max_new >= 1 << 30) return false;
     return (double)b->sequences * b->max_new < 2147483648.0 && (double)b->sequences * b->max_pages < 2147483648.0 && b->prefix_len < (1 << 30);
 }
 inline bool batch_ok(const paella_kv_batch* b) {

@@ -58,7 +58,7 @@ bool plan_ok(const paella_prefix_attention_plan* p) {
         return false;
     if (p->own_splits <= 0 || p->own_splits > 64 || p->prefix_splits < 0 || p->prefix_splits > 64 || (p->prefix_splits > 0) != (p->prefix_len > 0)) return false;
     const Grid g = grid_of(p);
-    return (double)g.all < 1e9;
+    return (double)g.all <= kMostWorkgroups;
 }
 
 // Whether the workgroup that arrives last at a row joins it, or a launch of its own: a joining workgroup makes this many trips to memory one after the other,
@@ -95,7 +95,9 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_
     p->own_rows = rows(b->max_new * per_kv);
     p->prefix_rows = p->prefix_len ? rows(b->tokens * per_kv) : p->own_rows;
     if (p->own_rows == 64 && p->prefix_rows == 128) p->own_rows = 128;
-    // A row's keys are shared by as many workgroups as fill the device twice, each with two steps per wave at least.
+    // A row's keys are shared by as many workgroups as give every compute unit three, with two steps per wave at least each.  (32 sequences of up to 5 tokens over
+    // 8190 + 1000 keys, prefix splits 4 / 8 / 11 / 16: 80 / 54 / 51 / 47 us; 64 over 65536 + 4000, 8 / 16 / 24 / 32 and own ones 1, 32 and 2:
+    // 373 / 265 / 252 / 238, 222.)
     const int step = size == 4 ? 16 : 32;
     auto splits = [&](int64_t others, int64_t keys) {
         const int64_t want = ceil_div(768, others), least = ceil_div(ceil_div(keys, step), 8);

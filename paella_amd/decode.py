@@ -30,6 +30,16 @@ except ImportError:
     _current_device = torch.cuda.current_device
 
 
+_lib = None
+
+
+def _library():
+    global _lib
+    if _lib is None:
+        _lib = _abi.ops()
+    return _lib
+
+
 # As in `ops`, a small call's time is what it costs the calling thread: the checks below look at each tensor once and are kept to under half a microsecond each.
 
 def _on_device(*tensors):
@@ -142,7 +152,7 @@ def kv_append(cache, batch, k, v, q=None, q_norm=None, k_norm=None, eps=1e-6, in
     desc = cache.append_descs.get((heads, rotary, interleaved, eps, qs, ks, vs))
     if desc is None:
         desc = cache.append_descs[heads, rotary, interleaved, eps, qs, ks, vs] = ctypes.byref(KvAppendDesc(heads, rotary, int(interleaved), eps, qs, ks, vs))
-    rc = _abi.ops().paella_kv_append_launch(desc, cache.ref, batch.ref, qp, kp, vp, _floats(q_norm, dim), _floats(k_norm, dim), _floats(inv_freq, rotary // 2), op,
+    rc = _library().paella_kv_append_launch(desc, cache.ref, batch.ref, qp, kp, vp, _floats(q_norm, dim), _floats(k_norm, dim), _floats(inv_freq, rotary // 2), op,
                                             _stream(stream), job_id, notifier)
     if rc:
         check(rc, "paella_kv_append_launch")
@@ -231,7 +241,6 @@ class BeamSelect:
 def beam_reorder(cache, parents, past, tables, tables_out, spare, past_out=None, stream=None, job_id=0, notifier=None):
     """Gives each child beam (parents: int32 [groups, count]) its parent's tokens: rows of tables_out name the parent's full pages and the page of the next token, copied to a
     spare page (spare: int32, one per child) for every child of a parent but its first.  Returns the children's lengths (past_out).  tables: int32 [groups * beams, max_pages]."""
-    lib = _abi.ops()
     _on_device(cache.k, parents, past, tables, tables_out, spare, past_out)
     assert parents.dim() == 2 and tables.dim() == 2
     groups, count = parents.shape
@@ -240,7 +249,7 @@ def beam_reorder(cache, parents, past, tables, tables_out, spare, past_out=None,
     if past_out is None:
         past_out = past.new_empty(groups * count)
     desc = BeamReorderDesc(groups, rows // groups, count, pages)
-    rc = lib.paella_beam_reorder_launch(ctypes.byref(desc), cache.ref, _ints(parents, groups, count), _ints(past, rows), _ints(tables, rows, pages),
+    rc = _library().paella_beam_reorder_launch(ctypes.byref(desc), cache.ref, _ints(parents, groups, count), _ints(past, rows), _ints(tables, rows, pages),
                                         _ints(spare, *spare.shape), _ints(tables_out, groups * count, pages), _ints(past_out, groups * count), _stream(stream), job_id,
                                         notifier)
     if rc:

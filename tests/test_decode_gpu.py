@@ -523,3 +523,43 @@ def test_a_step_reports_to_its_notifier(cuda):
             assert int(num[start == 0].sum()) == dims.grid == int(num[start == 1].sum()) and set(job.tolist()) == {11 + i}
     finally:
         lib.paella_ring_destroy(ring)
+
+
+def test_the_front_end_refuses_what_does_not_fit(cuda):
+    """Nothing of these calls is launched: the cache stays as it was."""
+    from paella_amd import decode
+    cache = decode.KVCache.empty(6, 2, 8, 64, BF16)
+    ints = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=cuda)  # noqa: E731
+    past, tables = ints(3), ints(3, 2)
+    batch = decode.KVBatch(past, tables, prefix_table=ints(2), prefix_len=16)
+    k = torch.ones((3, 2, 64), dtype=BF16, device=cuda)
+    q = torch.ones((3, 4, 64), dtype=BF16, device=cuda)
+    attend, pick = decode.PrefixAttention(4, cache, batch), decode.BeamSelect(2, 3, 100, 4)
+    logits, scores = torch.zeros((2, 3, 100), device=cuda), torch.zeros((2, 3), device=cuda)
+    parents, out, spare = ints(1, 3), ints(3, 2), ints(3)
+    wide = torch.ones((3, 4, 128), dtype=BF16, device=cuda)
+    calls = [lambda: decode.KVCache(k, k), lambda: decode.KVCache(cache.k, cache.v.float()), lambda: decode.KVCache(cache.k, cache.v[:5]),
+             lambda: decode.KVBatch(past.long(), tables), lambda: decode.KVBatch(past, tables[:2]), lambda: decode.KVBatch(past, tables.t()), lambda: decode.KVBatch(past.cpu(), tables),
+             lambda: decode.KVBatch(past, tables, tokens=4), lambda: decode.KVBatch(past, tables, starts=ints(4)), lambda: decode.KVBatch(past, tables, starts=ints(3), tokens=3),
+             lambda: decode.KVBatch(past, tables, prefix_len=3), lambda: decode.KVBatch(past, tables, max_new=0),
+             lambda: decode.kv_append(cache, batch, k[:2], k[:2]), lambda: decode.kv_append(cache, batch, k.float(), k), lambda: decode.kv_append(cache, batch, k, k.cpu()),
+             lambda: decode.kv_append(cache, batch, k.transpose(0, 1).contiguous().transpose(0, 1), k), lambda: decode.kv_append(cache, batch, k, k, q=wide),
+             lambda: decode.kv_append(cache, batch, k, k, q=wide[:, :, ::2]), lambda: decode.kv_append(cache, batch, k, k, k_norm=torch.ones(32, device=cuda)),
+             lambda: decode.kv_append(cache, batch, k, k, k_norm=torch.ones(64, device=cuda, dtype=BF16)), lambda: decode.kv_append(cache, batch, k, k, inv_freq=torch.ones(7, device=cuda)),
+             lambda: decode.kv_append(cache, batch, k, k, q=q, out=q[:2]), lambda: decode.kv_append(cache, batch, k, k, inv_freq=torch.ones(40, device=cuda)),
+             lambda: attend(q[:2], cache, batch), lambda: attend(q.float(), cache, batch), lambda: attend(q, cache, batch, out=q), lambda: attend(k, cache, batch),
+             lambda: attend(q, decode.KVCache.empty(6, 2, 16, 64, BF16), batch), lambda: attend(q, cache, decode.KVBatch(past, tables, prefix_table=ints(1), prefix_len=16)),
+             lambda: attend(q, cache, decode.KVBatch(past, tables)), lambda: attend(q, cache, batch, stage=2), lambda: decode.PrefixAttention(3, cache, batch),
+             lambda: decode.PrefixAttention(4, cache, batch, scale=-1.0), lambda: decode.PrefixAttention(4, decode.KVCache.empty(6, 2, 8, 96, BF16), batch),
+             lambda: decode.BeamSelect(1, 33, 10, 1), lambda: decode.BeamSelect(1, 3, 10, 65), lambda: decode.BeamSelect(1, 3, 10, 2, torch.float64),
+             lambda: pick(logits[:, :, :99], scores), lambda: pick(logits.half(), scores), lambda: pick(logits, scores[:, :2]), lambda: pick(logits, scores.double()),
+             lambda: pick(logits.transpose(0, 1).contiguous().transpose(0, 1), scores), lambda: pick(logits, scores, finished=scores), lambda: pick(logits, scores, finished=scores.bool(), pad_token=100),
+             lambda: decode.beam_reorder(cache, parents, past, tables, tables, spare), lambda: decode.beam_reorder(cache, parents, past, tables, out, spare[:2]),
+             lambda: decode.beam_reorder(cache, parents, past, tables, out, spare, past_out=past), lambda: decode.beam_reorder(cache, parents.long(), past, tables, out, spare),
+             lambda: decode.beam_reorder(cache, ints(2, 3), past, tables, out, spare)]
+    for i, call in enumerate(calls):
+        with pytest.raises((AssertionError, RuntimeError)):
+            call()
+            pytest.fail("call %d was taken" % i)
+    torch.cuda.synchronize()
+    assert not cache.k.any() and not cache.v.any() and not out.any()
