@@ -582,7 +582,8 @@ __device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, co
     for (int r = 0; r < R; ++r) {
         if (Fm::WIDE || r > 0) __syncthreads();  // the keys, or the rows before, have been read
         const float own = rows.sum_of(r);
-        if (lane < 16) ml[wave * 16 + lane] = f32x2{rows.m[r], own};
+        // (a NaN among a row's scores is no maximum: an infinite one makes NaN of whatever the sum meets further on)
+        if (lane < 16) ml[wave * 16 + lane] = f32x2{own == own ? rows.m[r] : INFINITY, own};
         rows.put_sums(r, sums + (wave * 16 + (lane & 15)) * PITCH, lane);
         __syncthreads();
         for (int e = threadIdx.x; e < (Fm::WIDE ? 64 : 16) * (D / 4); e += 256) {
@@ -616,7 +617,7 @@ __device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, co
                 }
             }
             if (whole) {
-                put_out<T>(to, (unsigned)id * D + d, l > 0.f ? sum / l : f32x4{0.f, 0.f, 0.f, 0.f});
+                put_out<T>(to, (unsigned)id * D + d, l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : sum / l);
             } else {
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), to, (int)(((unsigned)id * D + d) * 4), 0, kThrough);
                 if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{as_word(top), as_word(l)}, to_ml, id * 8, 0, kThrough);
@@ -642,7 +643,7 @@ struct Joined {
         top = now;
         return true;
     }
-    __device__ __forceinline__ f32x4 out() const { return l > 0.f ? sum / l : f32x4{0.f, 0.f, 0.f, 0.f}; }
+    __device__ __forceinline__ f32x4 out() const { return l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : sum / l; }
 };
 
 // Parts first, first + every, ... of row `id`, in their order, N of them requested together.  (CACHE: kThrough where other workgroups of this launch

@@ -65,8 +65,8 @@ def _floats(t, n):
 def _rows(t, tokens, heads, cache):
     """Address and row stride of [tokens, heads, head_dim] whose heads lie side by side."""
     dim = cache.head_dim
-    row, head, value = t.stride()  # three dimensions
     assert t.dtype is cache.dtype and t.shape == (tokens, heads, dim), (t.dtype, tuple(t.shape), "wanted", cache.dtype, (tokens, heads, dim))
+    row, head, value = t.stride()
     assert value == 1 and (head == dim or heads == 1), "heads have to lie side by side: strides %s" % ((row, head, value),)
     return t.data_ptr(), row if tokens > 1 else heads * dim
 
@@ -112,7 +112,7 @@ class KVCache:
 class KVBatch:
     """The new tokens of a step.  past: int32 [sequences], own tokens in the cache so far; tables: int32 [sequences, max_pages]; prefix_table: int32, the pages of
     the prefix that all sequences share, prefix_len its tokens.  Every sequence has max_new new tokens, or, with starts (int32 [sequences + 1]), rows starts[b] to
-    starts[b + 1] of the `tokens` rows.  The tensors are read at every launch, not here."""
+    starts[b + 1] of the `tokens` rows.  The tensors are read at every launch, not here: change them in place."""
 
     def __init__(self, past, tables, max_new=1, starts=None, tokens=None, prefix_table=None, prefix_len=0):
         assert past.dim() == 1 and tables.dim() == 2 and max_new >= 1

@@ -227,6 +227,32 @@ def test_attention_of_large_scores_and_a_strided_query(cuda):
     within(out, want, ref.attention_bound(want, weight, products, BF16, 170))
 
 
+@pytest.mark.parametrize("case", [0, 4, 14, 17, 19])
+def test_attention_passes_nan_and_infinity_on(cuda, case):
+    """What a row sees of them reaches that row and no other: a query, keys of one sequence, values of another."""
+    from paella_amd import decode
+    case = ATTEND[case]
+    q, k, v, rows, tables, prefix_table, cache, batch = attend_case(case, cuda)
+    attend = decode.PrefixAttention(case[1], cache, batch)
+    want = attend(q.to(cuda), cache, batch)
+    sequences, size = len(case[5]), case[4]
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool)
+    q = q.clone()
+    q[0, 1] = math.nan
+    bad[0, 1] = True
+    last = [t for t, o in enumerate(rows) if o is not None and o[0] == sequences - 1]
+    own = rows[last[0]][1]      # the first new token of the last sequence: all of its rows see it
+    cache.k[int(tables[-1, own // size]), 0, own % size] = math.inf if case[0] != F32 else math.nan
+    bad[last[0]:last[-1] + 1, :case[1] // case[2]] = True   # the heads of key head 0; scores of infinities of both signs, or NaN
+    got = attend(q.to(cuda), cache, batch)
+    torch.cuda.synchronize()
+    owned = torch.tensor([o is not None for o in rows])
+    bad &= owned[:, None]
+    gone = torch.isnan(got.cpu()).any(-1)
+    assert torch.equal(gone[owned], bad[owned])
+    assert torch.equal(got.cpu()[owned][~bad[owned]], want.cpu()[owned][~bad[owned]])
+
+
 @pytest.mark.parametrize("case,stages", [(3, 1), (16, 1), (17, 2)])
 def test_attention_is_the_same_every_time_in_graphs_on_streams_and_direct_queues(cuda, case, stages):
     """Which workgroup joins a row changes from run to run, the bits do not: eager, replayed (two graphs of one plan side by side, lengths changed between replays), on another
