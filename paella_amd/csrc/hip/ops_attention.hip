@@ -2,6 +2,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "prefix_attention.h"
@@ -95,19 +96,22 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_
     p->own_rows = rows(b->max_new * per_kv);
     p->prefix_rows = p->prefix_len ? rows(b->tokens * per_kv) : p->own_rows;
     if (p->own_rows == 64 && p->prefix_rows == 128) p->own_rows = 128;
-    // A row's keys are shared by as many workgroups as give every compute unit three, with two steps per wave at least each.  (32 sequences of up to 5 tokens over
-    // 8190 + 1000 keys, prefix splits 4 / 8 / 11 / 16: 80 / 54 / 51 / 47 us; 64 over 65536 + 4000, 8 / 16 / 24 / 32 and own ones 1, 32 and 2:
-    // 373 / 265 / 252 / 238, 222.)
+    // A row's keys are shared by as many workgroups as fit the device at once: three per compute unit, or two where many rows hold their registers.  A wave has
+    // two steps of keys at least, or one as long as the parts are at most seven.  (32 sequences of up to 5 tokens over 8190 + 1000 keys, the prefix in
+    // 4 / 8 / 11 / 16 parts: 80 / 54 / 51 / 47 us; 64 over 65536 + 4000 in 8 / 16 / 24 / 32, own keys in 1, 32 and 2: 373 / 265 / 252 / 238, 222.  512 against
+    // 768 workgroups for those prefixes, with what joins them: 50 against 55 us and 241 against 257.  One step against two, 4 sequences over 130 + 100 keys in
+    // fp32: 7.8 against 8.9 us.)
     const int step = size == 4 ? 16 : 32;
-    auto splits = [&](int64_t others, int64_t keys) {
-        const int64_t want = ceil_div(768, others), least = ceil_div(ceil_div(keys, step), 8);
+    auto splits = [&](int64_t workgroups, int64_t others, int64_t keys) {
+        const int64_t steps = ceil_div(keys, step), want = ceil_div(workgroups, others), single = ceil_div(steps, 4);
+        const int64_t least = std::max(ceil_div(steps, 8), std::min<int64_t>(single, 7));
         const int64_t n = want < least ? want : least;
         return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
     };
     p->own_splits = 1;
     Grid g = grid_of(p);
-    if (p->prefix_len) p->prefix_splits = splits(g.prefix_tiles * c->kv_heads, p->prefix_len);
-    p->own_splits = splits(b->sequences * g.own_tiles * c->kv_heads, (int64_t)b->max_pages * c->page_size);
+    if (p->prefix_len) p->prefix_splits = splits(p->prefix_rows > 32 ? 512 : 768, g.prefix_tiles * c->kv_heads, p->prefix_len);
+    p->own_splits = splits(768, b->sequences * g.own_tiles * c->kv_heads, (int64_t)b->max_pages * c->page_size);
     if (!plan_ok(p)) return PAELLA_ENOSUP;
     g = grid_of(p);
     p->workspace_bytes = workspace_of(p);
