@@ -377,8 +377,28 @@ struct NarrowWalk {
     }
 };
 
-// Many rows: each of the four waves has 16 R rows of its own, and all of them walk the same keys, which the workgroup brings to LDS tile by tile: the
-// next tile's loads are under way while the one before is worked on.  16-byte piece c of key i lies at place c ^ turn(i), so that the 16 keys of a score
+// Loads of memory into LDS without a register between, in the order of the lanes: 16 bytes (4) of `base` + each lane's offset, from `lds` on.  What has arrived is
+// told by arrived(n): all but the wave's last n loads.  (Written out, because of such a load the compiler waits for all of them ahead of any read of LDS.)
+__device__ __forceinline__ unsigned lds_address(const char* p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
+__device__ __forceinline__ void bring16(const char* base, unsigned offset, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void bring4(const void* base, unsigned offset, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void arrived() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// All waves' accesses to LDS so far are done.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Many rows: each of the four waves has 16 R rows of its own, and all of them walk the same keys, which the workgroup brings to LDS tile by tile, AHEAD tiles ahead
+// of the one that is worked on.  16-byte piece c of key i lies at place c ^ turn(i), so that the 16 keys of a score
 // tile, and the 8 keys by 32 bytes that half a wave reads of V, come from different banks.  16-bit V comes by transposing reads (of 4 keys by 16 dimensions,
 // per 16 lanes), which leave the vector unit the 32 permutations of a step.
 template <typename T, int D, int R>
@@ -387,13 +407,19 @@ struct WideWalk {
     using Rows = AttentionRows<T, D, R, !F>;
     static constexpr int ROW = Rows::ROW, TPL = Rows::TPL, STEP = Rows::STEP;
     static constexpr int PIECES = ROW / 16;
-    static constexpr int TILE = 16384 / ROW < 64 ? 16384 / ROW : 64;  // keys
-    static constexpr int PASS = 256 / PIECES, PASSES = TILE / PASS;   // keys that the workgroup's 256 pieces are, and how many such loads of K and of V
-    static constexpr int LDS = 2 * TILE * ROW + 16;
+    static constexpr int TILE = STEP;
+    static constexpr int KEYS = 1024 / ROW, LOADS = TILE / KEYS / 4;    // keys of a wave's load, which lie in one block, and its loads of a tile's K, and of its V
+    static constexpr int BUFFERS = 4, AHEAD = BUFFERS - 1;
+    static constexpr int BUFFER = 2 * TILE * ROW, PAGES = BUFFERS * BUFFER;
+    static constexpr int LDS = PAGES + 4 * 2 * 64 * 4;
 
-    u32x4 k[PASSES], v[PASSES];
-    int page[PASSES];
-    unsigned in[PASSES];
+    int page;              // lane i: of block `window` + i, and the block's place in it
+    unsigned in;
+    unsigned window;
+    unsigned long long bad;  // bit i: block `window` + i is in no page
+    unsigned long long bad_ahead;  // of the tiles brought and not yet worked on, the next one's blocks in the lowest bits
+    unsigned odd;          // which half of the wave's place in LDS the next window's pages are in
+    unsigned lane_at[LOADS];
 
     __device__ __forceinline__ static int turn(int key) {
         if constexpr (F) return key & 15;
@@ -401,63 +427,68 @@ struct WideWalk {
         else return (key >> 4 & 1) | (key >> 1 & 1) << 1 | (key >> 3 & 1) << 2;  // two keys make up the banks
     }
 
-    __device__ __forceinline__ void look_up(const Keys& s, int first) {
-        const int mine = (int)threadIdx.x / PIECES;
+    __device__ __forceinline__ static int wave_of() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+
+    // The pages of the window behind, through LDS: 64 blocks are 8 tiles or more, so that they are there when they are asked for.
+    __device__ __forceinline__ void look_ahead(const Keys& s, const char* lds, int lane) {
+        bring4(s.table, s.place_of(window + 64 + lane).entry * 4u, lds_address(lds) + PAGES + (wave_of() * 2 + odd) * 256);
+    }
+
+    __device__ __forceinline__ void begin(const Keys& s, int first, const char* lds, int lane) {
+        window = (unsigned)first / 8;
+        const Keys::Place at = s.place_of(window + lane);
+        page = s.table[at.entry];
+        in = at.in;
+        bad = __ballot((unsigned)page >= s.num_pages);
+        bad_ahead = 0;
+        odd = 0;
+        look_ahead(s, lds, lane);
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const Keys::Place at = s.place_of((unsigned)(first + i * PASS + mine) / 8);
-            page[i] = s.table[at.entry];
-            in[i] = at.in;
+        for (int i = 0; i < LOADS; ++i) {
+            const int key = (wave_of() * LOADS + i) * KEYS + lane / PIECES;
+            lane_at[i] = (unsigned)(lane / PIECES * ROW + (lane % PIECES ^ turn(key)) * 16);
         }
     }
 
-    __device__ __forceinline__ void load(const Keys& s) {
-        const int mine = (int)threadIdx.x / PIECES, piece = (int)threadIdx.x % PIECES;
+    // Asks for the tile from key `first` on, which `before` tiles that are not yet worked on precede.
+    __device__ __forceinline__ void bring(const Keys& s, int first, int buffer, int before, const char* lds, int lane) {
+        if ((unsigned)first / 8 == window + 64) {
+            window += 64;
+            page = reinterpret_cast<const int*>(lds + PAGES)[(wave_of() * 2 + odd) * 64 + lane];
+            in = s.place_of(window + lane).in;
+            bad = __ballot((unsigned)page >= s.num_pages);
+            odd ^= 1;
+            look_ahead(s, lds, lane);
+        }
+        const unsigned block = (unsigned)first / 8 - window;
+        bad_ahead |= (bad >> block & ((1ull << TILE / 8) - 1)) << (before * (TILE / 8));
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const size_t at = s.page_at(page[i]) + (size_t)((in[i] * 8 + (i * PASS + mine) % 8) * ROW + piece * 16);
-            k[i] = *reinterpret_cast<const u32x4*>(s.k + at);
-            v[i] = *reinterpret_cast<const u32x4*>(s.v + at);
+        for (int i = 0; i < LOADS; ++i) {
+            const int load = wave_of() * LOADS + i;
+            const int lies = (int)block + load * KEYS / 8;
+            const size_t at = s.page_at(__builtin_amdgcn_readlane(page, lies)) + (size_t)(((unsigned)__builtin_amdgcn_readlane((int)in, lies) * 8 + load * KEYS % 8) * ROW);
+            const unsigned to = lds_address(lds) + buffer * BUFFER + load * 1024;
+            bring16(s.k + at, lane_at[i], to);
+            bring16(s.v + at, lane_at[i], to + TILE * ROW);
         }
     }
 
-    // `first`: the tile's first key, whose keys from `most` on no row sees; bad: bit i where the thread's page of load i is none
-    __device__ __forceinline__ void store(char* buffer, char* absent, int first, int most, unsigned bad) {
-        const int mine = (int)threadIdx.x / PIECES, piece = (int)threadIdx.x % PIECES;
+    // What lies in places of V that no row may see can be anything, and 0 * NaN is NaN.  (Each wave for the keys that it brought.)
+    __device__ __forceinline__ void clear(int first, int most, unsigned gone, char* buffer, int lane) const {
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int key = i * PASS + mine;
-            // what lies in places that no row may see can be anything, and 0 * NaN is NaN
-            if (bad >> i & 1 || first + key >= most) v[i] = u32x4{0, 0, 0, 0};
-            char* const to = buffer + key * ROW + (piece ^ turn(key)) * 16;
-            *reinterpret_cast<u32x4*>(to) = k[i];
-            *reinterpret_cast<u32x4*>(to + TILE * ROW) = v[i];
-            if (piece == 0 && key % 8 == 0) absent[key / 8] = (char)(bad >> i & 1);
+        for (int i = 0; i < LOADS; ++i) {
+            const int load = wave_of() * LOADS + i, key = load * KEYS + lane / PIECES;
+            if (gone >> (key / 8) & 1 || first + key >= most) *reinterpret_cast<u32x4*>(buffer + TILE * ROW + load * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
         }
     }
 
-    __device__ __forceinline__ unsigned bad_pages(const Keys& s) const {
-        unsigned bad = 0;
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) bad |= (unsigned)((unsigned)page[i] >= s.num_pages) << i;
-        return bad;
-    }
-
-    // Keys `first` (a multiple of STEP) to `end`; `least` and `most` bound the limits of the workgroup's rows, own_most those of the wave's.
-    __device__ __forceinline__ void walk(Rows& rows, const Keys& s, int first, int end, const int (&limit)[R], int least, int most, int own_most, float scale, int lane, char* lds) {
+    // Keys `first` (a multiple of STEP) to `end`; `least` and `most` bound the limits of the workgroup's rows.
+    __device__ __forceinline__ void walk(Rows& rows, const Keys& s, int first, int end, const int (&limit)[R], int least, int most, float scale, int lane, char* lds) {
         if (first >= end) return;
-        char* const absent = lds + 2 * TILE * ROW;  // per block of 8 keys
-        look_up(s, first);
-        load(s);
-        unsigned bad = bad_pages(s);
-        look_up(s, first + TILE);
-        store(lds, absent, first, most, bad);
-        if (first + TILE < end) {
-            load(s);
-            bad = bad_pages(s);
-            look_up(s, first + 2 * TILE);
-        }
-        __syncthreads();
+        begin(s, first, lds, lane);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (first + i * TILE < end) bring(s, first + i * TILE, i, i, lds, lane);
         const int group = lane >> 4, mm = lane & 15;
         constexpr int V_PLACES = F ? 4 : PIECES < 16 ? PIECES / 2 : 8;
         int k_at[Rows::KC], v_at[V_PLACES];
@@ -476,54 +507,48 @@ struct WideWalk {
                 }
             }
         }
+        int buffer = 0;
         for (; first < end; first += TILE) {
-            const char* const from = lds;
-            const int steps = min(end - first, TILE);
+            if (first + (AHEAD - 1) * TILE < end) arrived<(AHEAD - 1) * 2 * LOADS>();
+            else arrived<0>();
+            char* const from = lds + buffer * BUFFER;
+            const unsigned gone_blocks = (unsigned)(bad_ahead & ((1ull << TILE / 8) - 1));
+            bad_ahead >>= TILE / 8;
+            if (first + TILE > most || gone_blocks) clear(first, most, gone_blocks, from, lane);
+            lds_barrier();  // the tile is there, and the one before it has been read
+            if (first + AHEAD * TILE < end) bring(s, first + AHEAD * TILE, buffer == 0 ? BUFFERS - 1 : buffer - 1, AHEAD - 1, lds, lane);
+            f32x4 x[R][Rows::NT];
+            rows.scores(x, [&](int t, int c) { return *reinterpret_cast<const u32x4*>(from + k_at[c] + t * 4 * ROW); });
+            unsigned w[TPL][Rows::GRP * Rows::VW];
+            u32x4 straight[D / 16];
+            // pieces and keys further on whose bits the turn leaves alone are at fixed distances
+            if constexpr (F) {
 #pragma unroll
-            for (int sub = 0; sub < TILE / STEP; ++sub) {
-                if (sub * STEP >= steps || first + sub * STEP >= own_most) break;  // uniform over the wave
-                f32x4 x[R][Rows::NT];
-                rows.scores(x, [&](int t, int c) { return *reinterpret_cast<const u32x4*>(from + k_at[c] + sub * STEP * ROW + t * 4 * ROW); });
-                unsigned w[TPL][Rows::GRP * Rows::VW];
-                u32x4 straight[D / 16];
-                // pieces and keys further on whose bits the turn leaves alone are at fixed distances
-                if constexpr (F) {
+                for (int u = 0; u < TPL; ++u)
 #pragma unroll
-                    for (int u = 0; u < TPL; ++u)
+                    for (int g = 0; g < Rows::GRP; ++g) {
+                        const u32x4 y = *reinterpret_cast<const u32x4*>(from + v_at[u] + g * 256);
 #pragma unroll
-                        for (int g = 0; g < Rows::GRP; ++g) {
-                            const u32x4 y = *reinterpret_cast<const u32x4*>(from + v_at[u] + sub * STEP * ROW + g * 256);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) w[u][g * 4 + e] = y[e];
-                        }
-                } else {
-                    typedef short s16x4 __attribute__((ext_vector_type(4)));
-                    typedef __attribute__((address_space(3))) s16x4* LdsPointer;
-#pragma unroll
-                    for (int d = 0; d < D / 16; ++d) {
-                        const char* const at = from + v_at[d % V_PLACES] + sub * STEP * ROW + d / V_PLACES * 256;
-                        const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPointer)at));
-                        const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPointer)(at + 4 * ROW)));
-                        straight[d] = u32x4{a.x, a.y, b.x, b.y};
+                        for (int e = 0; e < 4; ++e) w[u][g * 4 + e] = y[e];
                     }
+            } else {
+                typedef short s16x4 __attribute__((ext_vector_type(4)));
+                typedef __attribute__((address_space(3))) s16x4* LdsPointer;
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    const char* const at = from + v_at[d % V_PLACES] + d / V_PLACES * 256;
+                    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPointer)at));
+                    const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPointer)(at + 4 * ROW)));
+                    straight[d] = u32x4{a.x, a.y, b.x, b.y};
                 }
-                const bool gone = absent[sub * STEP / 8 + group * TPL / 8] != 0;
-                if (first + (sub + 1) * STEP > least || __any(gone)) Rows::mask(x, first + sub * STEP + group * TPL, gone, limit);
-                unsigned p[R][4];
-                rows.weigh(x, scale, p);
-                if constexpr (F) rows.add_values(w, p);
-                else rows.add_straight(straight, p);
             }
-            if (first + TILE < end) {
-                __syncthreads();
-                store(lds, absent, first + TILE, most, bad);
-                if (first + 2 * TILE < end) {
-                    load(s);
-                    bad = bad_pages(s);
-                    look_up(s, first + 3 * TILE);
-                }
-                __syncthreads();
-            }
+            const bool gone = gone_blocks >> (group * TPL / 8) & 1;
+            if (first + STEP > least || gone_blocks) Rows::mask(x, first + group * TPL, gone, limit);
+            unsigned p[R][4];
+            rows.weigh(x, scale, p);
+            if constexpr (F) rows.add_values(w, p);
+            else rows.add_straight(straight, p);
+            buffer = buffer == BUFFERS - 1 ? 0 : buffer + 1;
         }
     }
 };
@@ -554,7 +579,7 @@ constexpr int attention_lds() {
 
 // A workgroup's part: rows `row_id` (LDS; -1: none) of its tile over steps [begin, end) of `s`, left in slot `part` (or, where there is one, as the output).
 template <typename T, int D, typename Fm>
-__device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, const char* const (&q_row)[Fm::R], const int (&limit)[Fm::R], int least, int most, int own_most,
+__device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, const char* const (&q_row)[Fm::R], const int (&limit)[Fm::R], int least, int most,
                                        int begin, int end, int part, const int* row_id, char* lds) {
     constexpr int R = Fm::R;
     using Rows = AttentionRows<T, D, R, Fm::WIDE && T::bytes == 2>;
@@ -565,7 +590,7 @@ __device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, co
     for (int r = 0; r < R; ++r) rows.load_q(r, q_row[r], lane);
     if constexpr (Fm::WIDE) {
         WideWalk<T, D, R> keys;
-        keys.walk(rows, s, begin * Rows::STEP, end * Rows::STEP, limit, least, most, own_most, a.scale_log2, lane, lds);
+        keys.walk(rows, s, begin * Rows::STEP, end * Rows::STEP, limit, least, most, a.scale_log2, lane, lds);
     } else {
         NarrowWalk<T, D, R> keys;
         keys.walk(rows, s, begin + wave, end, limit, least, most, a.scale_log2, lane);
@@ -805,7 +830,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(
         s.v = a.v_cache + (size_t)h * a.page_size * head_bytes;
         const int steps = (a.prefix_len + STEP - 1) / STEP;
         const int begin = min(split * a.prefix_per, steps), end = min(begin + a.prefix_per, steps);
-        attend<T, D, FP>(a, s, q_row, limit, a.prefix_len, a.prefix_len, a.prefix_len, begin, end, split, row_id, lds);
+        attend<T, D, FP>(a, s, q_row, limit, a.prefix_len, a.prefix_len, begin, end, split, row_id, lds);
     } else {
         // the key heads of one sequence side by side: they share the look-ups and, with eight of them, an XCD each
         const Quotient by_head = divide(item, a.kv_heads), by_split = divide(by_head.q, a.own_splits), by_tile = divide(by_split.q, a.own_tiles);
@@ -842,11 +867,10 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(
             s.k = a.k_cache + (size_t)h * a.page_size * head_bytes;
             s.v = a.v_cache + (size_t)h * a.page_size * head_bytes;
             const int least = limit_of(wave_row), most = limit_of(first_row + FO::ROWS - 1);
-            const int own_most = FO::WIDE ? limit_of(wave_row + 16 * FO::R - 1) : most;
             const int steps = (most + STEP - 1) / STEP;
             const int per = (int)divide((unsigned)steps + a.own_splits.d - 1, a.own_splits).q;
             const int begin = min(split * per, steps), end = min(begin + per, steps);
-            attend<T, D, FO>(a, s, q_row, limit, least, most, own_most, begin, end, (int)a.prefix_splits.d + split, row_id, lds);
+            attend<T, D, FO>(a, s, q_row, limit, least, most, begin, end, (int)a.prefix_splits.d + split, row_id, lds);
         }
     }
     if (any && a.counters) join_last<T, D, MOST>(a, row_id, first_counter, over_prefix ? FP::ROWS : FO::ROWS, done);
