@@ -26,7 +26,7 @@ AttentionKernel join_of(const paella_prefix_attention_plan* p) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Grid {
-    int64_t prefix_tiles, own_tiles, prefix_items, own_items, turn, rate, all;
+    int64_t prefix_tiles, own_tiles, prefix_items, all;
 };
 
 Grid grid_of(const paella_prefix_attention_plan* p) {
@@ -35,15 +35,7 @@ Grid grid_of(const paella_prefix_attention_plan* p) {
     g.prefix_tiles = p->prefix_len ? ceil_div(p->tokens * per_kv, p->prefix_rows) : 0;
     g.own_tiles = ceil_div(p->max_new * per_kv, p->own_rows);
     g.prefix_items = g.prefix_tiles * p->kv_heads * p->prefix_splits;
-    g.own_items = p->sequences * g.own_tiles * p->kv_heads * p->own_splits;
-    g.turn = g.prefix_items && g.prefix_items + g.own_items > 256 ? 32 : 0;  // (where all start at once, order is nothing)
-    g.rate = 0;
-    if (g.turn) {
-        const int64_t turns = ceil_div(g.prefix_items, g.turn) + ceil_div(g.own_items, g.turn);
-        const int64_t rate = 1024 * ceil_div(g.prefix_items, g.turn) / turns * 3 / 2 + 1;
-        g.rate = rate < 1024 ? rate : 1024;
-    }
-    g.all = g.turn ? (ceil_div(g.prefix_items, g.turn) + ceil_div(g.own_items, g.turn)) * g.turn : g.prefix_items + g.own_items;
+    g.all = g.prefix_items + p->sequences * g.own_tiles * p->kv_heads * p->own_splits;
     return g;
 }
 
@@ -96,22 +88,29 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_
     p->own_rows = rows(b->max_new * per_kv);
     p->prefix_rows = p->prefix_len ? rows(b->tokens * per_kv) : p->own_rows;
     if (p->own_rows == 64 && p->prefix_rows == 128) p->own_rows = 128;
-    // A row's keys are shared by as many workgroups as fit the device at once: three per compute unit, or two where many rows hold their registers.  A wave has
-    // two steps of keys at least, or one as long as the parts are at most seven.  (32 sequences of up to 5 tokens over 8190 + 1000 keys, the prefix in
-    // 4 / 8 / 11 / 16 parts: 80 / 54 / 51 / 47 us; 64 over 65536 + 4000 in 8 / 16 / 24 / 32, own keys in 1, 32 and 2: 373 / 265 / 252 / 238, 222.  512 against
-    // 768 workgroups for those prefixes, with what joins them: 50 against 55 us and 241 against 257.  One step against two, 4 sequences over 130 + 100 keys in
-    // fp32: 7.8 against 8.9 us.)
+    // A row's keys are shared by so many workgroups that three are there for each compute unit.  A wave has two steps of keys at least, or one as long as the
+    // parts are at most seven (one step against two, 4 sequences over 130 + 100 keys in fp32: 7.8 against 8.9 us).
     const int step = size == 4 ? 16 : 32;
-    auto splits = [&](int64_t workgroups, int64_t others, int64_t keys) {
-        const int64_t steps = ceil_div(keys, step), want = ceil_div(workgroups, others), single = ceil_div(steps, 4);
+    auto splits = [&](int64_t want, int64_t keys) {
+        const int64_t steps = ceil_div(keys, step), single = ceil_div(steps, 4);
         const int64_t least = std::max(ceil_div(steps, 8), std::min<int64_t>(single, 7));
         const int64_t n = want < least ? want : least;
         return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
     };
+    const int64_t own_keys = (int64_t)b->max_pages * c->page_size;
     p->own_splits = 1;
     Grid g = grid_of(p);
-    if (p->prefix_len) p->prefix_splits = splits(p->prefix_rows > 32 ? 512 : 768, g.prefix_tiles * c->kv_heads, p->prefix_len);
-    p->own_splits = splits(768, b->sequences * g.own_tiles * c->kv_heads, (int64_t)b->max_pages * c->page_size);
+    p->own_splits = splits(ceil_div(768, b->sequences * g.own_tiles * c->kv_heads), own_keys);
+    if (p->prefix_len) {
+        // Workgroups over the prefix start first.  Those of many rows are bound by the products, those over own tokens by memory: one of the first to a
+        // compute unit, the second beside it, is best where the own tokens are half as many as the prefix's, by tiles, or more; where they are fewer two; a unit
+        // holds one with heads of 256 anyway.  One more than fits them all costs a whole round.  (bf16, heads of 128, 256 against 512 workgroups:
+        // 64 sequences over 65536 + 4000 / 2000 / 1000 / 500 keys 186 / 129 / 118 / 120 against 216 / 145 / 117 / 105 us, 32 of up to 5 tokens over 8190 + 1000
+        // / 300 39 / 34 against 47 / 38; 528 in place of 504: 39.7 against 37.8; heads of 256 with hardly any own tokens 32 against 39.)
+        const int64_t tiles = g.prefix_tiles * c->kv_heads;
+        const bool beside = c->head_dim > 128 || 2.0 * b->sequences * own_keys >= (double)g.prefix_tiles * b->prefix_len;
+        p->prefix_splits = splits(p->prefix_rows > 32 ? (beside ? 256 : 512) / tiles : ceil_div(768, tiles), b->prefix_len);
+    }
     if (!plan_ok(p)) return PAELLA_ENOSUP;
     g = grid_of(p);
     p->workspace_bytes = workspace_of(p);
@@ -158,7 +157,7 @@ int paella_prefix_attention_launch_stage(const paella_prefix_attention_plan* p, 
     a.own_tiles = divisor((unsigned)g.own_tiles); a.own_splits = divisor((unsigned)p->own_splits);
     a.prefix_per = p->prefix_splits ? (int)ceil_div(ceil_div(p->prefix_len, step), p->prefix_splits) : 0;
     a.prefix_pairs = p->kv_heads * p->prefix_splits;
-    a.prefix_items = (unsigned)g.prefix_items; a.own_items = (unsigned)g.own_items; a.turn = (unsigned)g.turn; a.rate = (unsigned)g.rate;
+    a.prefix_items = (unsigned)g.prefix_items;
     const size_t parts = (size_t)p->prefix_splits + p->own_splits, rows = (size_t)p->tokens * p->heads;
     a.counters = need && stages_of(p) == 1 ? (unsigned*)workspace : nullptr;
     a.counter_pitch = (unsigned)counter_pitch(p);

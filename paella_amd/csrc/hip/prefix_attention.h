@@ -40,8 +40,7 @@ struct AttentionArgs {
     float scale_log2;                       // scale * log2(e): probabilities are powers of two
     Divisor eight_tiles, prefix_splits, own_tiles, own_splits;  // eight_tiles: 8 times the tiles over the prefix
     int prefix_per, prefix_pairs;                               // steps of a split; key heads by splits
-    unsigned prefix_items, own_items;
-    unsigned turn, rate;    // workgroups of one kind in a row (0: all over the prefix, then all over own tokens); 1024ths of the turns that are the prefix's until it is done
+    unsigned prefix_items;
     unsigned* counters;     // [key heads][rows of one, in whole cache lines], zero between launches; null where a launch of its own joins.  A workgroup's lie side by
                             // side, and other key heads' on other lines: counts on one line go one after the other
     unsigned counter_pitch;
@@ -777,22 +776,11 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(
     s.page_bytes = (size_t)a.kv_heads.d * a.page_size * head_bytes;
     s.page_blocks = a.page_blocks;
     s.num_pages = (unsigned)a.num_pages;
-    // Work over the prefix (bound by the products) and over own tokens (bound by memory) alternate in the proportion of their numbers, so that compute
-    // units have some of either: `turn` workgroups at a time.  (32: one for each shader engine of each XCD.  Workgroups are handed to the engines in
-    // turn, and one that is full holds the others up: by eights, half of the engines had all of the prefix.)
-    bool over_prefix = blockIdx.x < a.prefix_items;
-    unsigned item = over_prefix ? blockIdx.x : blockIdx.x - a.prefix_items;
-    if (a.turn) {
-        const unsigned prefix_turns = (a.prefix_items + a.turn - 1) / a.turn, turn = blockIdx.x / a.turn;
-        const unsigned before = min(turn * a.rate >> 10, prefix_turns);
-        over_prefix = min((turn + 1) * a.rate >> 10, prefix_turns) > before;
-        item = (over_prefix ? before : turn - before) * a.turn + blockIdx.x % a.turn;
-    }
-    bool any = item < (over_prefix ? a.prefix_items : a.own_items);
+    const bool over_prefix = blockIdx.x < a.prefix_items;
+    const unsigned item = over_prefix ? blockIdx.x : blockIdx.x - a.prefix_items;
+    bool any = true;
     unsigned first_counter = 0;
-    if (!any) {
-        // a kind's last turn has fewer
-    } else if (over_prefix) {
+    if (over_prefix) {
         // (key head, split) by tile: the tiles of one pair read the same keys, so they follow each other by 8 and share an XCD's cache
         const unsigned eights = (unsigned)a.prefix_pairs / 8 * a.eight_tiles.d, left = (unsigned)a.prefix_pairs % 8;
         unsigned pair, tile;
