@@ -258,33 +258,41 @@ __device__ __forceinline__ unsigned long long get64(const unsigned long long* p)
 template <typename T, int VALUES>
 __device__ __forceinline__ void load_logits(const char* row, int first, int vocab, float (&x)[VALUES]) {
     constexpr int VEC = 16 / T::bytes;
+    if (first + 256 * VALUES <= vocab) {  // all requested ahead of the first use
+        u32x4 w[VALUES / VEC];
 #pragma unroll
-    for (int i = 0; i < VALUES / VEC; ++i) {
-        const int at = first + (i * 256 + (int)threadIdx.x) * VEC;
-        float* const f = x + i * VEC;
-        if (at + VEC <= vocab) {
-            const u32x4 w = load_unaligned(row + (size_t)at * T::bytes);
+        for (int i = 0; i < VALUES / VEC; ++i) w[i] = load_unaligned(row + (unsigned)(first + (i * 256 + (int)threadIdx.x) * VEC) * T::bytes);
+#pragma unroll
+        for (int i = 0; i < VALUES / VEC; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if constexpr (T::bytes == 4) {
-                    f[e] = as_float(w[e]);
+                    x[i * VEC + e] = as_float(w[i][e]);
                 } else {
-                    const f32x2 two = unpack2<T>(w[e]);
-                    f[2 * e] = two.x;
-                    f[2 * e + 1] = two.y;
+                    const f32x2 two = unpack2<T>(w[i][e]);
+                    x[i * VEC + 2 * e] = two.x;
+                    x[i * VEC + 2 * e + 1] = two.y;
                 }
             }
-        } else {
+    } else {  // the row's end: one by one, the last logit in place of what is behind it
+        unsigned w[VALUES];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                f[e] = -INFINITY;
-                if (at + e < vocab) {
-                    if constexpr (T::bytes == 4) f[e] = reinterpret_cast<const float*>(row)[at + e];
-                    else f[e] = unpack2<T>(reinterpret_cast<const unsigned short*>(row)[at + e]).x;
-                }
-            }
+        for (int i = 0; i < VALUES; ++i) {
+            const unsigned at = (unsigned)min(first + (i / VEC * 256 + (int)threadIdx.x) * VEC + i % VEC, vocab - 1);
+            if constexpr (T::bytes == 4) w[i] = *reinterpret_cast<const unsigned*>(row + at * 4);
+            else w[i] = *reinterpret_cast<const unsigned short*>(row + at * 2);
+        }
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) {
+            const float v = T::bytes == 4 ? as_float(w[i]) : unpack2<T>(w[i]).x;
+            x[i] = first + (i / VEC * 256 + (int)threadIdx.x) * VEC + i % VEC < vocab ? v : -INFINITY;
         }
     }
+}
+
+// How many lanes of `who` come before this one.
+__device__ __forceinline__ int lanes_before(unsigned long long who) {
+    return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0));
 }
 
 // What at least K of the lanes' keys reach (0 where fewer lanes have one): their K-th largest, bit by bit, to the upper 16 bits -- a few more logits
@@ -421,7 +429,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
         for (int i = 0; i < VALUES; ++i) {
             const unsigned long long who = __ballot(x[i] >= least);
             if (who) {
-                const int at = taken + __popcll(who & ((1ull << lane) - 1));
+                const int at = taken + lanes_before(who);
                 if (x[i] >= least && at < kWaveCandidates) own[at] = entry(order_key(x[i]), (unsigned)(lane_base + behind(i)));
                 taken += __popcll(who);
             }
@@ -453,7 +461,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
             for (int i = 0; i < VALUES; ++i) {
                 const bool take = key[i] > bound || (key[i] == bound && lane_base <= last - behind(i));
                 const unsigned long long who = __ballot(take);
-                if (take) own[taken + __popcll(who & ((1ull << lane) - 1))] = entry(key[i], (unsigned)(lane_base + behind(i)));
+                if (take) own[taken + lanes_before(who)] = entry(key[i], (unsigned)(lane_base + behind(i)));
                 taken += __popcll(who);
             }
         }
