@@ -3,7 +3,7 @@
  * keys and values (with the norms and the rotation of queries and keys on the way), attention for sequences that share
  * a prefix, and beam search's selection and reordering.  No counterpart in the reference, whose models are CNNs; the
  * entry points follow paella_ops.h (stream or direct-dispatch queue, job_id and notifier hooks, return codes, launch
- * shapes for the scheduler, one launch per call), so a job definition issues them like any other operator.
+ * shapes for the scheduler, one launch per call but for attention plans of two stages), so a job definition issues them like any other operator.
  *
  * The cache of one layer is two tensors [num_pages][kv_heads][page_size][head_dim], keys and values, on 16-byte
  * boundaries.  A sequence's own token i lies in slot i % page_size of page tables[sequence][i / page_size]; the shared

@@ -216,8 +216,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // ------------------------------------------------------------------------------------------ beam selection
 // value(w, t) = scores[w] + x - lse_w: within a beam the order of the logits is the order of the values, so one pass over the logits takes each
 // workgroup's running maximum, its sum of exponentials and its `count` largest logits; the workgroup that arrives last in a group puts the beams'
-// logarithms together and merges the lists.  Few launches and few trips: 4 beams over 32000 fp32 logits take 7.8 us, of which the pass 3 and the merge 5
-// (four trips to memory in a row); 128 rows of 131072 bf16 logits 17.7 us, of which reading 33.5 MB is 5.4, the pass's arithmetic keeps the vector
+// logarithms together and merges the lists.  Few launches and few trips: 4 beams over 32000 fp32 logits take 8.1 us, of which the pass 3 and the merge 5
+// (four trips to memory in a row); 128 rows of 131072 bf16 logits 16.9 us, of which reading 33.5 MB is 5.4, the pass's arithmetic keeps the vector
 // units for about as long, and the merge is the rest.  64 logits per thread instead of 32: 19.9 (its registers leave three workgroups per compute unit).
 //
 // A logit as a number whose order is the logits' (-0 and 0 alike, NaN as -inf), with its index behind it such that the larger of two is the one to

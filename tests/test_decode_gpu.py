@@ -213,6 +213,38 @@ def test_attention(cuda, case, holes):
     within(out, want, bound)
 
 
+LONG_WALKS = [
+    (BF16, 32, 2, 64, 8, [700, 3, 0, 1300], 4, None, 2603),       # 128 rows and one workgroup's each, a page per block of 8 keys
+    (F16, 16, 2, 128, 24, [1100, 40], 9, [0, 9, 15], 1537),
+    (F32, 16, 2, 128, 8, [590, 8], 5, None, 1100),
+    (BF16, 16, 1, 256, 16, [530, 1029], 4, None, 1041),
+]
+
+
+@pytest.mark.parametrize("holes", [False, True], ids=["", "holes"])
+@pytest.mark.parametrize("splits", [(1, 1), (2, 3)], ids=str)
+@pytest.mark.parametrize("case", LONG_WALKS, ids=lambda c: "%s-%dx%dx%d-p%d-%d+%d" % (str(c[0])[6:], c[1], c[2], c[3], c[4], c[8], max(c[5])))
+def test_attention_of_many_rows_over_many_pages_by_one_workgroup(cuda, case, splits, holes):
+    """Walks of many rows over more pages than a workgroup looks up at once, which short inputs get only where the keys are hardly split."""
+    from paella_amd import decode
+    dtype, heads, kv_heads, dim, size, past, new, starts, prefix = case
+    q, k, v, rows, tables, prefix_table, cache, batch = attend_case(case, cuda, holes)
+    attend = decode.PrefixAttention(heads, cache, batch)
+    assert min(attend.plan.prefix_rows, attend.plan.own_rows) > 32 and attend.plan.prefix_splits >= splits[0] and attend.plan.own_splits >= splits[1]
+    attend.plan.prefix_splits, attend.plan.own_splits = splits
+    out = torch.full(q.shape, 7.0, dtype=dtype, device=cuda)
+    for _ in range(2):
+        attend(q.to(cuda), cache, batch, out=out)
+    torch.cuda.synchronize()
+    want, weight, products = ref.attention(q, k, v, rows, tables, prefix_table, prefix, 1 / math.sqrt(dim))
+    bound = ref.attention_bound(want, weight, products, dtype, prefix + max(past) + new)
+    for t, owner in enumerate(rows):
+        if owner is None:
+            want[t] = 7.0    # left as it was
+            bound[t] = 0.0
+    within(out, want, bound)
+
+
 def test_attention_of_large_scores_and_a_strided_query(cuda):
     """Scores of hundreds, all of one sign: the running maximum has to carry them.  q is a view of a packed projection; a scale of its own."""
     from paella_amd import decode
