@@ -54,13 +54,15 @@ bool plan_ok(const paella_prefix_attention_plan* p) {
     return (double)g.all <= kMostWorkgroups;
 }
 
-// Whether the workgroup that arrives last at a row joins it, or a launch of its own: a joining workgroup makes this many trips to memory one after the other,
-// each above a microsecond; the other launch costs as much as some four.
+// Whether the workgroup that arrives last at a row joins it, or a launch of its own does: where its lanes have all of the outputs at once and request all parts
+// together.  (Rows of heads of 128 in 5 parts, twice as many as that, 12.3 us against 10.5 with the other launch, 12 in 21 parts 16.2 against 10.8; 2 sequences of 4
+// rows in 8 parts 9.8 against 10.3.)
 int stages_of(const paella_prefix_attention_plan* p) {
     const int parts = p->prefix_splits + p->own_splits;
     if (parts == 1) return 1;
-    const int rows = p->prefix_splits && p->prefix_rows > p->own_rows ? p->prefix_rows : p->own_rows;
-    return ceil_div(rows * p->head_dim / 4, 256) * ceil_div(parts, kJoined) <= 4 ? 1 : 2;
+    const int64_t per_kv = p->heads / p->kv_heads;
+    const int64_t own = std::min<int64_t>(p->own_rows, p->max_new * per_kv), shared = p->prefix_splits ? std::min<int64_t>(p->prefix_rows, p->tokens * per_kv) : 0;
+    return std::max(own, shared) * p->head_dim / 4 <= 256 && parts <= kJoined ? 1 : 2;
 }
 
 size_t counter_pitch(const paella_prefix_attention_plan* p) { return up256((size_t)p->tokens * (p->heads / p->kv_heads) * 4) / 4; }
@@ -83,33 +85,50 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return PAELLA_ENOSUP;
     if (!extents_ok(p)) return PAELLA_ENOSUP;
     const int64_t per_kv = heads / c->kv_heads, size = element_bytes(c->dtype), row_bytes = c->head_dim * size;
-    // Rows of a workgroup: where there are few its waves split the keys, else each has rows of its own (see the kernels).
-    auto rows = [&](int64_t n) { return c->head_dim > 128 ? (n <= 16 ? 16 : 64) : n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 || row_bytes > 256 ? 64 : 128; };
-    p->own_rows = rows(b->max_new * per_kv);
-    p->prefix_rows = p->prefix_len ? rows(b->tokens * per_kv) : p->own_rows;
-    if (p->own_rows == 64 && p->prefix_rows == 128) p->own_rows = 128;
-    // A row's keys are shared by so many workgroups that three are there for each compute unit.  A wave has two steps of keys at least, or one as long as the
-    // parts are at most seven (one step against two, 4 sequences over 130 + 100 keys in fp32: 7.8 against 8.9 us).
     const int step = size == 4 ? 16 : 32;
-    auto splits = [&](int64_t want, int64_t keys) {
-        const int64_t steps = ceil_div(keys, step), single = ceil_div(steps, 4);
-        const int64_t least = std::max(ceil_div(steps, 8), std::min<int64_t>(single, 7));
-        const int64_t n = want < least ? want : least;
+    // Rows of a workgroup.  Where a key head has few, 16: its waves split the keys.  Else 64 or 128: each wave has rows of its own, the keys are read once
+    // for all of them.  That is no gain up to some number of steps by 16 rows, where latency counts: bf16, 4 key heads of 128, 96 rows each over 1600 keys, 192 over
+    // 1200 / 3000 (1200, 1824 / 4512 steps) 10.9, 12.8 / 17.0 us by 16 rows, 15.4, 14.9 / 17.2 by 128, 8 key heads, 36 rows over 3000 / 8000 (2256 / 6000) 12.9 / 21.2
+    // against 12.3 / 17.0; fp32 96 rows over 1600, 192 over 1200 / 3000 (2400, 3600 / 9024) 16.2, 19.5 / 33.0 against 18.8, 20.8 / 30.0.  Heads of 256 hold few keys'
+    // loads beside 16 rows: 24 rows over 187 keys 16.8 against 13.0.
+    const bool small_heads = c->head_dim <= 128;
+    auto rows = [&](int64_t n) { return n <= 64 || !small_heads || row_bytes > 256 ? 64 : 128; };
+    const int64_t own = b->max_new * per_kv, shared = b->tokens * per_kv;
+    p->own_rows = own <= (small_heads ? 32 : 16) ? 16 : rows(own);
+    p->prefix_rows = p->own_rows;
+    if (p->prefix_len) {
+        const double steps = (double)ceil_div(shared, 16) * c->kv_heads * ceil_div(p->prefix_len, step);
+        const bool few = shared <= 16 || (small_heads && steps <= (size == 4 ? 3072 : 2048));
+        p->prefix_rows = few && p->own_rows == 16 ? 16 : rows(shared);
+    }
+    if (p->own_rows == 64 && p->prefix_rows == 128) p->own_rows = 128;
+    // A row's keys are shared by so many workgroups that three are there for each compute unit, or eight where many sequences' lengths have to even out (64
+    // sequences of up to 4000 tokens in 2 / 3 / 4 parts, beside a prefix, 190 / 186 / 182 us; 32 of 1000 and 5 new in 2 / 3 / 4 / 6 49 / 45 / 44 / 49; but 10 of 1500 in
+    // 7 / 10 15 / 19).  A workgroup of 16 rows has 256 keys at least (28 rows a key head in fp32 over 3000 keys in 12 / 24 parts 18.4 / 23.7 us), one of more eight steps
+    // (96 rows in fp32 over 3000 in 12 / 24 33 / 24), or, of few workgroups, a step for each wave as
+    // long as the parts are at most seven (one step against two, 4 sequences over 130 + 100 keys in fp32: 7.8 against 8.9 us).
+    auto splits = [&](int64_t want, int64_t undivided, int64_t keys, int least) {
+        int64_t n = ceil_div(keys, least);
+        if (undivided < 128) n = std::max(n, std::min<int64_t>(ceil_div(keys, 4 * step), 7));
+        n = std::min(want, n);
         return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
     };
     const int64_t own_keys = (int64_t)b->max_pages * c->page_size;
     p->own_splits = 1;
     Grid g = grid_of(p);
-    p->own_splits = splits(ceil_div(768, b->sequences * g.own_tiles * c->kv_heads), own_keys);
+    const int64_t undivided = b->sequences * g.own_tiles * c->kv_heads;
+    p->own_splits = splits(ceil_div(undivided < 128 ? 768 : 2048, undivided), undivided, own_keys, 256);
     if (p->prefix_len) {
         // Workgroups over the prefix start first.  Those of many rows are bound by the products, those over own tokens by memory: one of the first to a
-        // compute unit, the second beside it, is best where the own tokens are half as many as the prefix's, by tiles, or more; where they are fewer two; a unit
-        // holds one with heads of 256 anyway.  One more than fits them all costs a whole round.  (bf16, heads of 128, 256 against 512 workgroups:
+        // compute unit, the second beside it, is best where the own tokens are half as many as the prefix's, by tiles, or more; where they are fewer, two, if that leaves
+        // each 512 keys (of heads of 128); a unit holds one with heads of 256 anyway.  One more than fits them all costs a whole round.  (bf16, heads of 128, 256 against 512 workgroups:
         // 64 sequences over 65536 + 4000 / 2000 / 1000 / 500 keys 186 / 129 / 118 / 120 against 216 / 145 / 117 / 105 us, 32 of up to 5 tokens over 8190 + 1000
-        // / 300 39 / 34 against 47 / 38; 528 in place of 504: 39.7 against 37.8; heads of 256 with hardly any own tokens 32 against 39.)
+        // / 300 39 / 34 against 47 / 38; 7 over 20000 + 60 25 against 28, heads of 64, 74 over 11439 + 108 28 against 25; 528 in place of 504: 39.7 against 37.8; fp32, 48 over 3000 + 60, 252 in place of 288: 23
+        // against 30; heads of 256 with hardly any own tokens 32 against 39.)
         const int64_t tiles = g.prefix_tiles * c->kv_heads;
-        const bool beside = c->head_dim > 128 || 2.0 * b->sequences * own_keys >= (double)g.prefix_tiles * b->prefix_len;
-        p->prefix_splits = splits(p->prefix_rows > 32 ? (beside ? 256 : 512) / tiles : ceil_div(768, tiles), b->prefix_len);
+        const bool beside = 2.0 * b->sequences * own_keys >= (double)g.prefix_tiles * b->prefix_len;
+        const bool two = c->head_dim <= 128 && !beside && (double)b->prefix_len * tiles >= 2048.0 * c->head_dim;
+        p->prefix_splits = splits(p->prefix_rows > 16 ? (two ? 512 : 256) / tiles : ceil_div(768, tiles), tiles, b->prefix_len, p->prefix_rows > 16 ? 8 * step : 256);
     }
     if (!plan_ok(p)) return PAELLA_ENOSUP;
     g = grid_of(p);

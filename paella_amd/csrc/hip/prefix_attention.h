@@ -5,10 +5,10 @@
 // out = sum_i p_i v_i / sum_i p_i with p_i = exp(scale * q . k_i - m): one pass over the keys with the running maximum m and sum, in 32 bits.
 //
 // Work.  A workgroup takes either a tile of query rows (a row: a head of a new token; all heads that share a key head, of all sequences, side by
-// side) over a part of the prefix, or rows of one sequence over a part of its own tokens.  Up to 32 rows: all four waves have them, each takes every fourth
-// step of 32 (fp32: 16) keys, and their sums are put together in LDS.  More: each wave has 16 or 32 rows of its own, and the workgroup
+// side) over a part of the prefix, or rows of one sequence over a part of its own tokens.  Few rows, or few keys: 16 rows, all four waves have them, each takes every
+// fourth step of 32 (fp32: 16) keys, and their sums are put together in LDS.  Else each wave has 16 or 32 rows of its own, and the workgroup
 // brings the keys to LDS for all of them.  What the workgroups of a row leave is put together by the one that arrives last at the row (a
-// counter per row), in the order of the parts, so results do not depend on who that is.
+// counter per row) or by a launch of its own, in the order of the parts, so results do not depend on who that is.
 //
 // Operands.  With v_mfma_*_16x16 and the products turned round (scores^T = K q^T, out^T = V^T p^T), every operand comes
 // as it lies in the cache or from the other product's result: lane l of a wave holds query row l % 16 throughout; lane group l / 16 gets the scores
@@ -22,7 +22,7 @@
 // fp16.  Own tokens of many sequences: memory, 1.05 GB at 5.6 TB/s (a plain read of this size 6.2).  The prefix of 32 rows and more per
 // key head: the matrix and vector units, which take turns; per 32 x 32 scores 34 matrix instructions of 16 cycles and some 90 vector ones of 4, 16 of
 // them exponentials of 16; 69 GFLOP in 90 us at the 1.9 GHz that the power limit leaves.  Both at once, 64 sequences over 65536 shared and 2000 own keys on average
-// (802 MB, 71 GFLOP): 175 us and the joining launch's 7 when the card is cool, 200 under load without a pause.
+// (802 MB, 71 GFLOP): 162 us and the joining launch's 7 when the card is cool, 195 under load without a pause.
 
 #include <hip/hip_runtime.h>
 
@@ -266,10 +266,10 @@ struct AttentionRows {
     }
 };
 
-// Few rows: a wave has all of the workgroup's rows and every fourth step of its keys, which come straight from memory into registers.
-template <typename T, int D, int R>
+// Few rows: a wave has all 16 of the workgroup's rows and every fourth step of its keys, which come straight from memory into registers.
+template <typename T, int D>
 struct NarrowWalk {
-    using Rows = AttentionRows<T, D, R, false>;
+    using Rows = AttentionRows<T, D, 1, false>;
     static constexpr bool F = Rows::F;
     static constexpr int ROW = Rows::ROW, TPL = Rows::TPL, STEP = Rows::STEP;
 
@@ -332,8 +332,8 @@ struct NarrowWalk {
     // One step over the keys from `first` on.  `least` and `most` bound the limits of all rows, absent: this lane group's keys are in no page.
     // next(true) is called once K is no longer needed, next(false) once V is.
     template <typename Next>
-    __device__ __forceinline__ void step(Rows& rows, int first, const bool absent, const int (&limit)[R], int least, int most, float scale, int lane, Next next) {
-        f32x4 x[R][Rows::NT];
+    __device__ __forceinline__ void step(Rows& rows, int first, const bool absent, const int (&limit)[1], int least, int most, float scale, int lane, Next next) {
+        f32x4 x[1][Rows::NT];
         rows.scores(x, [&](int t, int c) { return k[t][c]; });
         next(true);
         if (first + STEP > least || __any(absent)) {
@@ -347,14 +347,14 @@ struct NarrowWalk {
                     for (int w = 0; w < Rows::GRP * Rows::VW; ++w) v[u][w] = 0;
                 }
         }
-        unsigned p[R][4];
+        unsigned p[1][4];
         rows.weigh(x, scale, p);
         rows.add_values(v, p);
         next(false);
     }
 
     // Steps `at`, at + 4, ... below `end`.  Page numbers are asked for a step ahead of the keys.
-    __device__ __forceinline__ void walk(Rows& rows, const Keys& s, int at, int end, const int (&limit)[R], int least, int most, float scale, int lane) {
+    __device__ __forceinline__ void walk(Rows& rows, const Keys& s, int at, int end, const int (&limit)[1], int least, int most, float scale, int lane) {
         if (at >= end) return;
         const bool even = s.page_blocks.d % (STEP / 8) == 0;
         look_up(s, (unsigned)at * (STEP / 8), even, lane);
@@ -564,7 +564,7 @@ __device__ __forceinline__ void put_out(__amdgpu_buffer_rsrc_t to, unsigned valu
     }
 }
 
-// A workgroup's form: how many 16-row tiles a wave has, and whether the waves share rows and split the keys, or the other way round.
+// A workgroup's form: how many 16-row tiles a wave has, and whether the waves share rows (16) and split the keys, or the other way round.
 template <int TILES, bool WIDE_>
 struct Form {
     static constexpr int R = TILES;
@@ -593,7 +593,7 @@ __device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, co
         WideWalk<T, D, R> keys;
         keys.walk(rows, s, begin * Rows::STEP, end * Rows::STEP, limit, least, most, a.scale_log2, lane, lds);
     } else {
-        NarrowWalk<T, D, R> keys;
+        NarrowWalk<T, D> keys;
         keys.walk(rows, s, begin + wave, end, limit, least, most, a.scale_log2, lane);
     }
     // Through LDS, so that a row's outputs leave side by side, 16 rows of each wave at a time: the waves' sums of one row where they split the keys
@@ -606,7 +606,7 @@ __device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, co
     const __amdgpu_buffer_rsrc_t to_ml = descriptor(a.ml + (size_t)part * (whole ? 0 : all));
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        if (Fm::WIDE || r > 0) __syncthreads();  // the keys, or the rows before, have been read
+        if (Fm::WIDE) __syncthreads();  // the keys, or the rows before, have been read
         const float own = rows.sum_of(r);
         // (a NaN among a row's scores is no maximum: an infinite one makes NaN of whatever the sum meets further on)
         if (lane < 16) ml[wave * 16 + lane] = f32x2{own == own ? rows.m[r] : INFINITY, own};
@@ -614,7 +614,7 @@ __device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, co
         __syncthreads();
         for (int e = threadIdx.x; e < (Fm::WIDE ? 64 : 16) * (D / 4); e += 256) {
             const int row = e / (D / 4), d = (e - row * (D / 4)) * 4;
-            const int id = row_id[Fm::WIDE ? (row >> 4) * 16 * R + r * 16 + (row & 15) : r * 16 + row];
+            const int id = row_id[Fm::WIDE ? (row >> 4) * 16 * R + r * 16 + (row & 15) : row];
             if (id < 0) continue;
             float top, l;
             f32x4 sum;
@@ -869,28 +869,18 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(
 
 using AttentionKernel = void (*)(AttentionArgs);
 
-// Which forms a type and head size have, by the rows of a workgroup: 16 and 32 (the waves split the keys), 64 and 128 (they split the rows).
+// Which forms a type and head size have, by the rows of a workgroup: 16 (the waves split the keys), 64 and 128 (they split the rows).
 template <typename T, int D>
 AttentionKernel attention_kernel_of(int rp, int ro) {
     using N1 = Form<1, false>;
     using W1 = Form<1, true>;
     if (rp == 16 && ro == 16) return prefix_attention_kernel<T, D, N1, N1>;
-    if constexpr (D <= 128) {
-        using N2 = Form<2, false>;
-        [[maybe_unused]] typedef Form<2, true> W2;
-        if (rp == 32 && ro == 16) return prefix_attention_kernel<T, D, N2, N1>;
-        if (rp == 32 && ro == 32) return prefix_attention_kernel<T, D, N2, N2>;
-        if (rp == 64 && ro == 16) return prefix_attention_kernel<T, D, W1, N1>;
-        if (rp == 64 && ro == 32) return prefix_attention_kernel<T, D, W1, N2>;
-        if (rp == 64 && ro == 64) return prefix_attention_kernel<T, D, W1, W1>;
-        if constexpr (D * T::bytes <= 256) {  // what the registers hold without a spill
-            if (rp == 128 && ro == 16) return prefix_attention_kernel<T, D, W2, N1>;
-            if (rp == 128 && ro == 32) return prefix_attention_kernel<T, D, W2, N2>;
-            if (rp == 128 && ro == 128) return prefix_attention_kernel<T, D, W2, W2>;
-        }
-    } else {
-        if (rp == 64 && ro == 16) return prefix_attention_kernel<T, D, W1, N1>;
-        if (rp == 64 && ro == 64) return prefix_attention_kernel<T, D, W1, W1>;
+    if (rp == 64 && ro == 16) return prefix_attention_kernel<T, D, W1, N1>;
+    if (rp == 64 && ro == 64) return prefix_attention_kernel<T, D, W1, W1>;
+    if constexpr (D * T::bytes <= 256) {  // what the registers hold without a spill
+        using W2 = Form<2, true>;
+        if (rp == 128 && ro == 16) return prefix_attention_kernel<T, D, W2, N1>;
+        if (rp == 128 && ro == 128) return prefix_attention_kernel<T, D, W2, W2>;
     }
     return nullptr;
 }

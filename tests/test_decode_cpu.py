@@ -82,15 +82,18 @@ def test_attention_plans(lib):
     rc, p = plan(lib, cache(heads=8, dim=128, size=64, pages=3000), batch(sequences=64, max_pages=63, prefix=65536, prefix_table=AT), 32)
     assert rc == 0 and (p.prefix_rows, p.own_rows, p.stages) == (128, 16, 2) and p.prefix_splits >= 16
     items = [2 * 8 * p.prefix_splits, 64 * 8 * p.own_splits]
-    assert p.dims.grid == sum(-(-n // 32) * 32 for n in items)
+    assert p.dims.grid == sum(items)
     parts, rows = p.prefix_splits + p.own_splits, 64 * 32
     assert p.workspace_bytes == 8 * 1024 + parts * rows * 8 + parts * rows * 128 * 4
     join = _abi.LaunchDims()
     assert lib.paella_prefix_attention_dims(ctypes.byref(p), 1, ctypes.byref(join)) == 0 and join.grid == rows // 2
-    # rows of a key head beyond 16, 32 and 64; head size 256 and wide fp32 heads have fewer forms
-    for dtype, dim, rows, want in [(1, 64, 17, 32), (1, 64, 33, 64), (1, 64, 65, 128), (0, 64, 65, 128), (0, 128, 65, 64), (2, 256, 17, 64), (0, 256, 65, 64), (1, 256, 16, 16)]:
-        p = plan(lib, cache(dtype=dtype, dim=dim, heads=1), batch(sequences=rows, prefix=100, prefix_table=AT), 1)[1]
+    # rows of a key head beyond 16 and 64 over many keys; head size 256 and wide fp32 heads have fewer forms
+    for dtype, dim, rows, prefix, want in [(1, 64, 17, 40000, 64), (1, 64, 65, 40000, 128), (1, 64, 65, 1000, 16), (0, 64, 65, 40000, 128), (0, 128, 65, 40000, 64),
+                                           (0, 128, 32, 1000, 16), (2, 256, 17, 100, 64), (0, 256, 65, 100, 64), (1, 256, 16, 40000, 16)]:
+        p = plan(lib, cache(dtype=dtype, dim=dim, heads=1), batch(sequences=rows, prefix=prefix, prefix_table=AT), 1)[1]
         assert (p.prefix_rows, p.own_rows) == (want, 16), (dtype, dim, rows)
+    for rows, dim, want in [(32, 128, 16), (33, 128, 64), (65, 128, 128), (17, 256, 64)]:   # of one sequence
+        assert plan(lib, cache(dtype=1, dim=dim, heads=1), batch(max_new=rows), 1)[1].own_rows == want
     for n in (1, 16, 33, 70, 500):   # every planned pair of forms has a kernel
         for sequences in (1, 40):
             for dtype in (0, 1, 2):

@@ -158,6 +158,7 @@ ATTEND = [
     (BF16, 32, 2, 128, 16, [50, 3, 200, 0] * 3, 1, None, 300),    # 192 rows per key head
     (F16, 16, 1, 256, 24, [20, 70, 11], 1, None, 130),
     (F32, 8, 2, 256, 8, [9] * 6, 3, [0, 3, 4, 4, 7, 9, 12], 77),
+    (BF16, 32, 2, 128, 16, [50, 3, 200, 0] * 3, 1, None, 4007),   # the same over many keys
 ]
 
 
@@ -213,6 +214,32 @@ def test_attention(cuda, case, holes):
     within(out, want, bound)
 
 
+@pytest.mark.parametrize("form", [(16, 16), (64, 16), (128, 16), (64, 64), (128, 128)], ids=str)
+@pytest.mark.parametrize("case", [0, 1, 2, 4, 7, 8, 9, 12, 14, 15, 17, 18])
+def test_attention_in_every_form(cuda, case, form):
+    """A plan's rows per workgroup are a choice of speed: any form that there is gives the same."""
+    from paella_amd import decode
+    dtype, heads, kv_heads, dim, size, past, new, starts, prefix = ATTEND[case]
+    q, k, v, rows, tables, prefix_table, cache, batch = attend_case(ATTEND[case], cuda, True)
+    attend = decode.PrefixAttention(heads, cache, batch)
+    attend.plan.prefix_rows, attend.plan.own_rows = form
+    if form[0] == 128 and dim * (4 if dtype == F32 else 2) > 256:
+        with pytest.raises(RuntimeError):   # no such kernel
+            attend(q.to(cuda), cache, batch)
+        return
+    out = torch.full(q.shape, 7.0, dtype=dtype, device=cuda)
+    for _ in range(2):
+        attend(q.to(cuda), cache, batch, out=out)
+    torch.cuda.synchronize()
+    want, weight, products = ref.attention(q, k, v, rows, tables, prefix_table, prefix, 1 / math.sqrt(dim))
+    bound = ref.attention_bound(want, weight, products, dtype, prefix + max(past) + new)
+    for t, owner in enumerate(rows):
+        if owner is None:
+            want[t] = 7.0    # left as it was
+            bound[t] = 0.0
+    within(out, want, bound)
+
+
 LONG_WALKS = [
     (BF16, 32, 2, 64, 8, [700, 3, 0, 1300], 4, None, 2603),       # 128 rows and one workgroup's each, a page per block of 8 keys
     (F16, 16, 2, 128, 24, [1100, 40], 9, [0, 9, 15], 1537),
@@ -230,7 +257,7 @@ def test_attention_of_many_rows_over_many_pages_by_one_workgroup(cuda, case, spl
     dtype, heads, kv_heads, dim, size, past, new, starts, prefix = case
     q, k, v, rows, tables, prefix_table, cache, batch = attend_case(case, cuda, holes)
     attend = decode.PrefixAttention(heads, cache, batch)
-    assert min(attend.plan.prefix_rows, attend.plan.own_rows) > 32 and attend.plan.prefix_splits >= splits[0] and attend.plan.own_splits >= splits[1]
+    assert min(attend.plan.prefix_rows, attend.plan.own_rows) > 16 and attend.plan.prefix_splits >= splits[0] and attend.plan.own_splits >= splits[1]
     attend.plan.prefix_splits, attend.plan.own_splits = splits
     out = torch.full(q.shape, 7.0, dtype=dtype, device=cuda)
     for _ in range(2):
@@ -285,7 +312,7 @@ def test_attention_passes_nan_and_infinity_on(cuda, case):
     assert torch.equal(got.cpu()[owned][~bad[owned]], want.cpu()[owned][~bad[owned]])
 
 
-@pytest.mark.parametrize("case,stages", [(3, 1), (16, 1), (17, 2)])
+@pytest.mark.parametrize("case,stages", [(0, 1), (3, 1), (16, 2), (20, 2)])
 def test_attention_is_the_same_every_time_in_graphs_on_streams_and_direct_queues(cuda, case, stages):
     """Which workgroup joins a row changes from run to run, the bits do not: eager, replayed (two graphs of one plan side by side, lengths changed between replays), on another
     stream and on a direct-dispatch queue."""
