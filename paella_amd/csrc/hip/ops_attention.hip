@@ -98,7 +98,7 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_
     p->prefix_rows = p->own_rows;
     if (p->prefix_len) {
         const double steps = (double)ceil_div(shared, 16) * c->kv_heads * ceil_div(p->prefix_len, step);
-        const bool few = shared <= 16 || (small_heads && steps <= (size == 4 ? 3072 : 2048));
+        const bool few = shared <= 16 || (small_heads && steps <= (size == 4 ? 3500 : 2048));
         p->prefix_rows = few && p->own_rows == 16 ? 16 : rows(shared);
     }
     if (p->own_rows == 64 && p->prefix_rows == 128) p->own_rows = 128;
