@@ -216,9 +216,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // ------------------------------------------------------------------------------------------ beam selection
 // value(w, t) = scores[w] + x - lse_w: within a beam the order of the logits is the order of the values, so one pass over the logits takes each
 // workgroup's running maximum, its sum of exponentials and its `count` largest logits; the workgroup that arrives last in a group puts the beams'
-// logarithms together and merges the lists.  Few launches and few trips: 4 beams over 32000 fp32 logits take 8.1 us, of which the pass 3 and the merge 5
-// (four trips to memory in a row); 128 rows of 131072 bf16 logits 16.9 us, of which reading 33.5 MB is 5.4, the pass's arithmetic keeps the vector
-// units for about as long, and the merge is the rest.  64 logits per thread instead of 32: 19.9 (its registers leave three workgroups per compute unit).
+// logarithms together and merges the lists.  Few launches and few trips: 4 beams over 32000 fp32 logits take 7.6 us, of which the pass 3 and the merge 5
+// (four trips to memory in a row); 128 rows of 131072 bf16 logits 15.4 us, of which reading 33.5 MB is 5.4, the pass's arithmetic keeps the vector
+// units for about as long, and the merge is the rest.  (Registers for seven workgroups per compute unit, without the bound six: 16.9; eight, or seven with 32 fp32
+// logits, do not do without scratch memory.)  64 logits per thread instead of 32: 19.9 (its registers leave three workgroups per compute unit).
 //
 // A logit as a number whose order is the logits' (-0 and 0 alike, NaN as -inf), with its index behind it such that the larger of two is the one to
 // take; 0 is no candidate.
@@ -375,7 +376,7 @@ __device__ __forceinline__ void best_of(const double* value, const unsigned* whe
 }
 
 template <typename T, int VALUES>
-__global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
+__global__ __launch_bounds__(256, T::bytes == 4 && VALUES == 32 ? 5 : 7) void beam_select_kernel(SelectArgs a) {
     hook_entry(a.notifier, a.job_id);
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ float wave_top[4], wave_total[4];
