@@ -404,9 +404,10 @@ __global__ __launch_bounds__(256, T::bytes == 4 && VALUES == 32 ? 5 : 7) void be
 #pragma unroll
         for (int i = 0; i < VALUES; ++i) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], kLog2e, -base));
         sum = wave_sum_f(sum);
-        if (sum < INFINITY) {
-            if (top > -INFINITY) sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(top, kLog2e, -base));
-        } else {  // NaN among the logits, a maximum so large (the type's lowest, where everything is masked) that the base overflows, or an infinity
+        if (sum > 0.f && sum < INFINITY) {
+            sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(top, kLog2e, -base));
+        } else {  // NaN among the logits, a maximum so far from 0 that the base overflows (the type's lowest, where everything is masked), or an infinity; NaN where there is no
+                  // number among them, which the sums further on leave out
             sum = 0.f;
 #pragma unroll
             for (int i = 0; i < VALUES; ++i) sum += x[i] == x[i] ? __builtin_amdgcn_exp2f((x[i] - top) * kLog2e) : 0.f;
