@@ -93,7 +93,7 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_
     // loads beside 16 rows: 24 rows over 187 keys 16.8 against 13.0.
     const bool small_heads = c->head_dim <= 128;
     auto rows = [&](int64_t n) { return n <= 64 || !small_heads || row_bytes > 256 ? 64 : 128; };
-    const int64_t own = b->max_new * per_kv, shared = b->tokens * per_kv;
+    const int64_t own = std::min(b->max_new, b->tokens) * per_kv, shared = b->tokens * per_kv;  // no sequence has more than all rows, whatever max_new leaves room for
     p->own_rows = own <= (small_heads ? 32 : 16) ? 16 : rows(own);
     p->prefix_rows = p->own_rows;
     if (p->prefix_len) {

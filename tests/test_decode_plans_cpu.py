@@ -1,0 +1,36 @@
+"""Plans of the decoding step's operators over batches and plans that the ordinary ones do not reach, without a device."""
+import ctypes
+
+import pytest
+
+EINVAL, ENOSUP = -1, -2
+AT = 1 << 20
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from paella_amd import _abi
+    return _abi.ops()
+
+
+def attention_plan(lib, dtype, heads, kv_heads, dim, size, sequences, max_new, tokens, max_pages, prefix):
+    from paella_amd._abi_decode import KvBatch, KvCache, PrefixAttentionPlan
+    p = PrefixAttentionPlan()
+    c = KvCache(AT, AT + (1 << 40), dtype, 1000, kv_heads, size, dim)
+    b = KvBatch(sequences, max_new, tokens, max_pages, prefix, AT, AT, AT, AT if prefix else None)
+    return lib.paella_prefix_attention_plan_make(ctypes.byref(c), ctypes.byref(b), heads, 0.0, ctypes.byref(p)), p
+
+
+def test_a_ragged_batch_with_room_for_more_new_tokens_than_it_has_is_planned(lib):
+    """max_new bounds what a sequence may have: a batch of few rows with a large bound has a kernel like any other."""
+    rc, p = attention_plan(lib, 1, 32, 8, 128, 64, 4, 32, 14, 20, 5000)
+    assert rc == 0 and (p.prefix_rows, p.own_rows) == (64, 64)
+    for dtype in (0, 1, 2):
+        for dim in (64, 128, 256):
+            for per_kv in (1, 4, 8):
+                for sequences in (1, 4):
+                    for max_new in (1, 7, 17, 33, 64, 200):
+                        for tokens in {1, max(1, max_new // 3), max_new, (max_new * sequences + max_new) // 2, max_new * sequences}:
+                            for prefix in (0, 9, 300, 5000):
+                                rc, p = attention_plan(lib, dtype, 2 * per_kv, 2, dim, 16, sequences, max_new, tokens, 20, prefix)
+                                assert rc == 0, (dtype, dim, per_kv, sequences, max_new, tokens, prefix, p.prefix_rows, p.own_rows)
