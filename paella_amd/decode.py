@@ -72,24 +72,48 @@ def _rows(t, tokens, heads, cache):
 
 
 class _Workspaces:
-    """Scratch memory that starts out zeroed, one per stream, so that calls on different streams do not meet in it.  A call under graph capture gets one of
-    its own in the graph's memory: graphs that were captured from one plan may run at once."""
+    """Scratch memory of a plan that starts out zeroed, one per stream, so that calls on different streams do not meet in it.  A call under graph capture gets one of
+    its own in the graph's memory: graphs that were captured from one plan may run at once.  The stages of a call that is issued stage by stage meet in the workspace of
+    their stream; where there is none that both would find, they are refused without one of the caller's."""
 
-    def __init__(self, nbytes):
+    def __init__(self, nbytes, stages=1):
         self.nbytes = nbytes
+        self.stages = stages
         self.of_stream = {}
+        self.begun = set()  # where a first stage has been issued and its second has not
 
-    def __call__(self, stream, device):
+    def new(self, device):
+        return torch.zeros(self.nbytes // 4 + 1, dtype=torch.int32, device=device)
+
+    def given(self, workspace):
+        """Address of a caller's workspace."""
+        assert workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= self.nbytes, "a workspace of %d bytes is needed, from new_workspace()" % self.nbytes
+        _on_device(workspace)
+        return workspace.data_ptr()
+
+    def find(self, stream, device, stage=None):
         if not self.nbytes:
             return None
-        if torch.cuda.is_current_stream_capturing():
-            return torch.zeros(self.nbytes // 4 + 1, dtype=torch.int32, device=device)
+        capturing = torch.cuda.is_current_stream_capturing()
+        if self.stages > 1:
+            if stage is not None and capturing:
+                raise AssertionError("stages of their own under graph capture have to be given one workspace")
+            if ((device.index, stream) in self.begun) != (stage == 1):
+                raise AssertionError("a second stage before its first, or a call between the stages of another, on this stream: give each call a workspace of its own")
+        if capturing:
+            return self.new(device)
         w = self.of_stream.get((device.index, stream))
         if w is None:
-            w = self.of_stream[device.index, stream] = torch.zeros(self.nbytes // 4 + 1, dtype=torch.int32, device=device)
+            w = self.of_stream[device.index, stream] = self.new(device)
             if stream != _torch_stream():  # the fill ran on torch's stream
                 torch.cuda.current_stream().synchronize()
         return w
+
+    def issued(self, stream, device, stage):
+        if stage == 0:
+            self.begun.add((device.index, stream))
+        elif stage == 1:
+            self.begun.discard((device.index, stream))
 
 
 class KVCache:
@@ -170,15 +194,20 @@ class PrefixAttention:
         self._ref = ctypes.byref(self.plan)
         self._launch = self.lib.paella_prefix_attention_launch
         self.heads = heads
-        self.workspaces = _Workspaces(self.plan.workspace_bytes)
+        self.workspaces = _Workspaces(self.plan.workspace_bytes, self.plan.stages)
+
+    def new_workspace(self, device="cuda"):
+        """Scratch memory for one call at a time, zero-filled on the current torch stream; a call leaves it ready for the next."""
+        return self.workspaces.new(device)
 
     def dims(self, stage=0):
         d = LaunchDims()
         check(self.lib.paella_prefix_attention_dims(self._ref, stage, ctypes.byref(d)), "paella_prefix_attention_dims")
         return d
 
-    def __call__(self, q, cache, batch, out=None, stream=None, job_id=0, notifier=None, stage=None):
-        """stage: one of the plan's launches (plan.stages) alone, for queues that keep no order."""
+    def __call__(self, q, cache, batch, out=None, stream=None, job_id=0, notifier=None, stage=None, workspace=None):
+        """stage: one of the plan's launches (plan.stages) alone, for queues that keep no order.  workspace: one of new_workspace() in place of the stream's own.  The stages of a
+        call share it; under graph capture, on different streams, or with other calls of this plan between them they have to be given it."""
         _on_device(q, cache.k, out)
         assert batch.prefix_pages * cache.page_size >= batch.prefix_len, "the prefix's table has too few pages"
         qp, qs = _rows(q, batch.tokens, self.heads, cache)
@@ -187,12 +216,18 @@ class PrefixAttention:
         else:
             assert out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous()
         stream = _stream(stream)
-        workspace = self.workspaces(stream, q.device)
-        workspace = None if workspace is None else workspace.data_ptr()
-        if stage is None:
-            rc = self._launch(self._ref, cache.ref, batch.ref, qp, qs, out.data_ptr(), workspace, stream, job_id, notifier)
+        own = workspace is None
+        if own:
+            workspace = self.workspaces.find(stream, q.device, stage)
+            address = None if workspace is None else workspace.data_ptr()
         else:
-            rc = self.lib.paella_prefix_attention_launch_stage(self._ref, stage, cache.ref, batch.ref, qp, qs, out.data_ptr(), workspace, stream, job_id, notifier)
+            address = self.workspaces.given(workspace)
+        if stage is None:
+            rc = self._launch(self._ref, cache.ref, batch.ref, qp, qs, out.data_ptr(), address, stream, job_id, notifier)
+        else:
+            rc = self.lib.paella_prefix_attention_launch_stage(self._ref, stage, cache.ref, batch.ref, qp, qs, out.data_ptr(), address, stream, job_id, notifier)
+            if own and not rc and self.workspaces.stages > 1:
+                self.workspaces.issued(stream, q.device, stage)
         if rc:
             check(rc, "paella_prefix_attention_launch")
         return out
@@ -230,7 +265,7 @@ class BeamSelect:
         shape = (groups, self.count)
         out, parents, tokens = scores.new_empty(shape), scores.new_empty(shape, dtype=torch.int32), scores.new_empty(shape, dtype=torch.int32)
         stream = _stream(stream)
-        workspace = self.workspaces(stream, logits.device)
+        workspace = self.workspaces.find(stream, logits.device)
         rc = self._launch(self._ref, logits.data_ptr(), row, _floats(scores, groups * beams), finished, pad_token, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
                           workspace.data_ptr(), stream, job_id, notifier)
         if rc:
