@@ -318,6 +318,10 @@ int paella_direct_queue_wait(void* queue);
  * callers must be the same thread.  The set lives until the process ends. */
 int paella_direct_queue_shared(void** queue);
 int paella_direct_queue_destroy(void* queue);
+/* What a handle that a launch function takes for `void* stream` is, as far as the order of what is issued there goes (PAELLA_EINVAL: neither a
+ * stream nor a queue). */
+enum paella_stream_kind { PAELLA_STREAM = 0, PAELLA_STREAM_CAPTURING = 1, PAELLA_QUEUE_UNORDERED = 2, PAELLA_QUEUE_ORDERED = 3 };
+int paella_stream_kind_of(void* stream);
 
 /*
  * Copies `bytes` from src to dst (host memory both) on a helper thread of this library and then calls done(arg) on that

@@ -568,3 +568,14 @@ extern "C" int paella_direct_queue_destroy(void* queue) {
     delete q;
     return 0;
 }
+
+extern "C" int paella_stream_kind_of(void* stream) {
+    if (const DirectQueue* q = paella::direct_queue_lookup(stream)) return q->ordered ? PAELLA_QUEUE_ORDERED : PAELLA_QUEUE_UNORDERED;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (!stream) return PAELLA_STREAM;  // (the default stream is never captured, and asking about it ends a capture elsewhere)
+    if (hipStreamIsCapturing(static_cast<hipStream_t>(stream), &status) != hipSuccess) {
+        (void)hipGetLastError();
+        return PAELLA_EINVAL;
+    }
+    return status == hipStreamCaptureStatusNone ? PAELLA_STREAM : PAELLA_STREAM_CAPTURING;
+}

@@ -20,8 +20,9 @@ import torch
 from . import _abi
 from ._abi import LaunchDims, check
 from ._abi_decode import BeamReorderDesc, BeamSelectPlan, KvAppendDesc, KvBatch, KvCache, PrefixAttentionPlan
-from .ops import _stream, _torch_stream
+from .ops import _stream, _torch_stream, _waits
 
+_STREAM, _STREAM_CAPTURING, _QUEUE_UNORDERED, _QUEUE_ORDERED = range(4)  # enum paella_stream_kind
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 try:
@@ -72,14 +73,16 @@ def _rows(t, tokens, heads, cache):
 
 
 class _Workspaces:
-    """Scratch memory of a plan that starts out zeroed, one per stream, so that calls on different streams do not meet in it.  A call under graph capture gets one of
-    its own in the graph's memory: graphs that were captured from one plan may run at once.  The stages of a call that is issued stage by stage meet in the workspace of
-    their stream; where there is none that both would find, they are refused without one of the caller's."""
+    """Scratch memory of a plan that starts out zeroed, one per stream, so that calls on different streams do not meet in it.  On a queue that keeps no order, a call that
+    finds it in use waits for the queue first.  A call under graph capture gets one of its own in the graph's memory: graphs that were captured from one plan may run at once.
+    The stages of a call that is issued stage by stage meet in the workspace of their stream; where there is none that both would find, they are refused without one of the
+    caller's."""
 
     def __init__(self, nbytes, stages=1):
         self.nbytes = nbytes
         self.stages = stages
         self.of_stream = {}
+        self.used = {}      # on queues: how often the queue had been waited for when the workspace was last given out
         self.begun = set()  # where a first stage has been issued and its second has not
 
     def new(self, device):
@@ -91,7 +94,8 @@ class _Workspaces:
         _on_device(workspace)
         return workspace.data_ptr()
 
-    def find(self, stream, device, stage=None):
+    def find(self, stream, device, stage=None, explicit=False):
+        """The workspace of a call on `stream`, which its caller named (explicit) or not."""
         if not self.nbytes:
             return None
         capturing = torch.cuda.is_current_stream_capturing()
@@ -107,6 +111,10 @@ class _Workspaces:
             w = self.of_stream[device.index, stream] = self.new(device)
             if stream != _torch_stream():  # the fill ran on torch's stream
                 torch.cuda.current_stream().synchronize()
+        if explicit and _library().paella_stream_kind_of(stream) == _QUEUE_UNORDERED:
+            if self.used.get((device.index, stream)) == _waits.get(stream, 0):
+                check(_library().paella_direct_queue_wait(stream), "paella_direct_queue_wait")
+            self.used[device.index, stream] = _waits.get(stream, 0)
         return w
 
     def issued(self, stream, device, stage):
@@ -206,8 +214,9 @@ class PrefixAttention:
         return d
 
     def __call__(self, q, cache, batch, out=None, stream=None, job_id=0, notifier=None, stage=None, workspace=None):
-        """stage: one of the plan's launches (plan.stages) alone, for queues that keep no order.  workspace: one of new_workspace() in place of the stream's own.  The stages of a
-        call share it; under graph capture, on different streams, or with other calls of this plan between them they have to be given it."""
+        """stage: one of the plan's launches (plan.stages) alone, for queues that keep no order.  workspace: one of new_workspace() in place of the stream's own, for calls of one
+        plan that may run at once on such a queue.  The stages of a call share it; under graph capture, on different streams, or with other calls of this plan between them
+        they have to be given it."""
         _on_device(q, cache.k, out)
         assert batch.prefix_pages * cache.page_size >= batch.prefix_len, "the prefix's table has too few pages"
         qp, qs = _rows(q, batch.tokens, self.heads, cache)
@@ -215,10 +224,10 @@ class PrefixAttention:
             out = q.new_empty(q.shape)
         else:
             assert out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous()
-        stream = _stream(stream)
+        explicit, stream = stream is not None, _stream(stream)
         own = workspace is None
         if own:
-            workspace = self.workspaces.find(stream, q.device, stage)
+            workspace = self.workspaces.find(stream, q.device, stage, explicit)
             address = None if workspace is None else workspace.data_ptr()
         else:
             address = self.workspaces.given(workspace)
@@ -251,9 +260,14 @@ class BeamSelect:
         check(self.lib.paella_beam_select_dims(self._ref, ctypes.byref(d)), "paella_beam_select_dims")
         return d
 
-    def __call__(self, logits, scores, finished=None, pad_token=0, stream=None, job_id=0, notifier=None):
+    def new_workspace(self, device="cuda"):
+        """As PrefixAttention.new_workspace."""
+        return self.workspaces.new(device)
+
+    def __call__(self, logits, scores, finished=None, pad_token=0, stream=None, job_id=0, notifier=None, workspace=None):
         """logits [groups, beams, vocab] (beams one after the other, rows of any stride), scores float32 [groups, beams], finished uint8 or bool [groups, beams].  Returns scores
-        (float32), parents and tokens (int32), each [groups, count], best first."""
+        (float32), parents and tokens (int32), each [groups, count], best first.  workspace: one of new_workspace() in place of the stream's own, for calls of one plan that may run
+        at once on a queue that keeps no order."""
         _on_device(logits, scores, finished)
         groups, beams, vocab = self.shape
         assert logits.dtype == self.dtype and tuple(logits.shape) == self.shape, (logits.dtype, tuple(logits.shape))
@@ -264,10 +278,14 @@ class BeamSelect:
             finished = finished.data_ptr()
         shape = (groups, self.count)
         out, parents, tokens = scores.new_empty(shape), scores.new_empty(shape, dtype=torch.int32), scores.new_empty(shape, dtype=torch.int32)
-        stream = _stream(stream)
-        workspace = self.workspaces.find(stream, logits.device)
+        explicit, stream = stream is not None, _stream(stream)
+        if workspace is None:
+            workspace = self.workspaces.find(stream, logits.device, None, explicit)
+            address = workspace.data_ptr()
+        else:
+            address = self.workspaces.given(workspace)
         rc = self._launch(self._ref, logits.data_ptr(), row, _floats(scores, groups * beams), finished, pad_token, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
-                          workspace.data_ptr(), stream, job_id, notifier)
+                          address, stream, job_id, notifier)
         if rc:
             check(rc, "paella_beam_select_launch")
         return out, parents, tokens

@@ -40,6 +40,7 @@ except ImportError:
 
 
 _direct_queues = set()
+_waits = {}  # of a queue's handle: how often it has been waited for
 
 
 def _stream(stream):
@@ -251,11 +252,13 @@ class DirectQueue:
         check(self.lib.paella_direct_queue_create(ctypes.byref(h)), "paella_direct_queue_create")
         self.handle = h.value
         _direct_queues.add(self.handle)
+        _waits[self.handle] = _waits.get(self.handle, 0) + 1  # (a handle may come back)
         if ordered:
             check(self.lib.paella_direct_queue_set_ordered(h, 1), "paella_direct_queue_set_ordered")
 
     def wait(self):
         check(self.lib.paella_direct_queue_wait(ctypes.c_void_p(self.handle)), "paella_direct_queue_wait")
+        _waits[self.handle] += 1
 
     def close(self):
         if self.handle:

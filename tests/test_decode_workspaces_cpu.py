@@ -1,0 +1,67 @@
+"""Which scratch memory a plan's calls get, and what they wait for, with streams and queues that are only numbers and memory of the CPU."""
+import pytest
+import torch
+
+STREAM, CAPTURING, UNORDERED, ORDERED = range(4)
+HOME = 100   # torch's stream
+
+
+class World:
+    """What the front-end asks the library and torch about streams."""
+
+    def __init__(self):
+        self.kinds = {7: UNORDERED, 8: UNORDERED, 9: ORDERED, 20: STREAM, 21: CAPTURING}
+        self.capturing = False
+        self.log = []
+
+    def paella_stream_kind_of(self, stream):
+        return self.kinds.get(stream, STREAM)
+
+    def paella_direct_queue_wait(self, stream):
+        assert self.kinds[stream] in (UNORDERED, ORDERED)
+        self.log.append(("wait", stream))
+        return 0
+
+    def synchronize(self, *device):
+        assert not self.capturing
+        self.log.append(("synchronize",) + device)
+
+
+@pytest.fixture
+def world(monkeypatch):
+    from paella_amd import decode
+    w = World()
+    monkeypatch.setattr(decode, "_library", lambda: w)
+    monkeypatch.setattr(decode, "_torch_stream", lambda: HOME)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: w.capturing)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: w)
+    monkeypatch.setattr(torch.cuda, "synchronize", w.synchronize)
+    return w
+
+
+def spaces(nbytes=64, stages=1):
+    from paella_amd import decode
+    return decode._Workspaces(nbytes, stages)
+
+
+CPU = torch.device("cpu")
+
+
+def test_calls_on_a_queue_without_order_wait_for_one_another(world):
+    from paella_amd import ops
+    own = spaces()
+    first = own.find(7, CPU, None, True)
+    waits = lambda: [e for e in world.log if e[0] == "wait"]  # noqa: E731
+    assert waits() == []                                   # nothing has used it
+    assert own.find(7, CPU, None, True) is first and waits() == [("wait", 7)]
+    assert own.find(7, CPU, None, True) is first and len(waits()) == 2
+    ops._waits[7] = ops._waits.get(7, 0) + 1               # the caller has waited
+    assert own.find(7, CPU, None, True) is first and len(waits()) == 2
+    assert own.find(7, CPU, None, True) is first and len(waits()) == 3
+    assert own.find(8, CPU, None, True) is not first and len(waits()) == 3
+    for stream in (9, 20, HOME):                            # these keep an order themselves
+        for _ in range(2):
+            own.find(stream, CPU, None, True)
+    assert own.find(HOME, CPU) is own.find(HOME, CPU) and len(waits()) == 3
+    assert spaces(0).find(7, CPU, None, True) is None and len(waits()) == 3
+    del ops._waits[7]
