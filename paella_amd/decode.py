@@ -75,8 +75,8 @@ def _rows(t, tokens, heads, cache):
 class _Workspaces:
     """Scratch memory of a plan that starts out zeroed, one per stream, so that calls on different streams do not meet in it.  On a queue that keeps no order, a call that
     finds it in use waits for the queue first.  A call under graph capture gets one of its own in the graph's memory: graphs that were captured from one plan may run at once.
-    The stages of a call that is issued stage by stage meet in the workspace of their stream; where there is none that both would find, they are refused without one of the
-    caller's."""
+    The stages of a call that is issued stage by stage meet in the workspace of their stream.  Where there is none that both would find, or none that a captured call may have,
+    calls are refused without one of the caller's."""
 
     def __init__(self, nbytes, stages=1):
         self.nbytes = nbytes
@@ -99,6 +99,10 @@ class _Workspaces:
         if not self.nbytes:
             return None
         capturing = torch.cuda.is_current_stream_capturing()
+        kind = _library().paella_stream_kind_of(stream) if explicit else _STREAM
+        # a captured workspace is filled on torch's stream; one that eager calls use must not get into a graph
+        if (explicit and stream != _torch_stream()) if capturing else kind == _STREAM_CAPTURING:
+            raise AssertionError("a call captured on another stream than torch's has to be given a workspace")
         if self.stages > 1:
             if stage is not None and capturing:
                 raise AssertionError("stages of their own under graph capture have to be given one workspace")
@@ -111,7 +115,7 @@ class _Workspaces:
             w = self.of_stream[device.index, stream] = self.new(device)
             if stream != _torch_stream():  # the fill ran on torch's stream
                 torch.cuda.current_stream().synchronize()
-        if explicit and _library().paella_stream_kind_of(stream) == _QUEUE_UNORDERED:
+        if kind == _QUEUE_UNORDERED:
             if self.used.get((device.index, stream)) == _waits.get(stream, 0):
                 check(_library().paella_direct_queue_wait(stream), "paella_direct_queue_wait")
             self.used[device.index, stream] = _waits.get(stream, 0)
@@ -193,7 +197,7 @@ def kv_append(cache, batch, k, v, q=None, q_norm=None, k_norm=None, eps=1e-6, in
 
 class PrefixAttention:
     """Planned attention of a batch: every new token over the shared prefix and its own sequence's tokens up to itself.  The plan holds for every cache and batch of these
-    extents (layers, steps); scale: 1 / sqrt(head_dim) unless given."""
+    extents (layers, steps); scale: 1 / sqrt(head_dim) unless given.  A call captured on a stream that is not torch's current one has to be given a workspace."""
 
     def __init__(self, heads, cache, batch, scale=0.0):
         self.lib = _abi.ops()

@@ -65,3 +65,25 @@ def test_calls_on_a_queue_without_order_wait_for_one_another(world):
     assert own.find(HOME, CPU) is own.find(HOME, CPU) and len(waits()) == 3
     assert spaces(0).find(7, CPU, None, True) is None and len(waits()) == 3
     del ops._waits[7]
+
+
+def test_captured_calls_find_no_workspace_that_is_not_the_graphs(world):
+    """The graph's own memory is filled on torch's stream, ahead of what is captured there: a call on another stream of the capture would run beside the fill.  A stream that is
+    captured while torch's is not would put its eager calls' workspace into the graph."""
+    own = spaces()
+    kept = own.find(HOME, CPU)
+    for explicit in (False, True):
+        world.capturing, world.kinds[HOME] = True, CAPTURING
+        held = own.find(HOME, CPU, None, explicit)
+        assert held is not kept and held is not own.find(HOME, CPU, None, explicit)
+        world.capturing, world.kinds[HOME] = False, STREAM
+        assert own.find(HOME, CPU, None, explicit) is kept
+    world.capturing = True
+    for stream in (20, 21, 7, 9):
+        with pytest.raises(AssertionError):
+            own.find(stream, CPU, None, True)
+    assert spaces(0).find(21, CPU, None, True) is None
+    world.capturing = False
+    with pytest.raises(AssertionError):
+        own.find(21, CPU, None, True)
+    assert own.find(20, CPU, None, True) is own.find(20, CPU, None, True)
