@@ -14,13 +14,14 @@ given, arguments that do not fit raise AssertionError here and RuntimeError from
 Lengths and tables are read on the device at every launch, so a captured step may be replayed while they change.
 """
 import ctypes
+import threading
 
 import torch
 
 from . import _abi
 from ._abi import LaunchDims, check
 from ._abi_decode import BeamReorderDesc, BeamSelectPlan, KvAppendDesc, KvBatch, KvCache, PrefixAttentionPlan
-from .ops import _stream, _torch_stream, _waits
+from .ops import _direct_queues, _stream, _torch_stream, _waits
 
 _STREAM, _STREAM_CAPTURING, _QUEUE_UNORDERED, _QUEUE_ORDERED = range(4)  # enum paella_stream_kind
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -72,6 +73,29 @@ def _rows(t, tokens, heads, cache):
     return t.data_ptr(), row if tokens > 1 else heads * dim
 
 
+_parked = []  # (memory, stream, what it is) of dropped plans that calls on streams which torch knows nothing of may still be using
+
+
+_unparking = threading.Lock()
+
+
+def _unpark(stream):
+    """Lets go of parked memory ahead of a call on `stream` that waits for the device anyway."""
+    with _unparking:
+        synchronized = set()
+        for i in reversed(range(len(_parked))):  # (more may be parked at the end meanwhile)
+            memory, where, kind = _parked[i]
+            if kind in (_QUEUE_UNORDERED, _QUEUE_ORDERED):
+                if where == stream:  # only its own thread may wait for a queue
+                    check(_library().paella_direct_queue_wait(stream), "paella_direct_queue_wait")
+                elif where not in _waits or where in _direct_queues:  # (closing a queue waits for it)
+                    continue
+            elif memory.device not in synchronized:
+                torch.cuda.synchronize(memory.device)
+                synchronized.add(memory.device)
+            del _parked[i]
+
+
 class _Workspaces:
     """Scratch memory of a plan that starts out zeroed, one per stream, so that calls on different streams do not meet in it.  On a queue that keeps no order, a call that
     finds it in use waits for the queue first.  A call under graph capture gets one of its own in the graph's memory: graphs that were captured from one plan may run at once.
@@ -82,6 +106,7 @@ class _Workspaces:
         self.nbytes = nbytes
         self.stages = stages
         self.of_stream = {}
+        self.foreign = {}   # what those streams are that torch did not allocate the workspace for
         self.used = {}      # on queues: how often the queue had been waited for when the workspace was last given out
         self.begun = set()  # where a first stage has been issued and its second has not
 
@@ -115,11 +140,17 @@ class _Workspaces:
             w = self.of_stream[device.index, stream] = self.new(device)
             if stream != _torch_stream():  # the fill ran on torch's stream
                 torch.cuda.current_stream().synchronize()
+                self.foreign[device.index, stream] = kind
+                _unpark(stream)
         if kind == _QUEUE_UNORDERED:
             if self.used.get((device.index, stream)) == _waits.get(stream, 0):
                 check(_library().paella_direct_queue_wait(stream), "paella_direct_queue_wait")
             self.used[device.index, stream] = _waits.get(stream, 0)
         return w
+
+    def __del__(self, park=_parked.append):
+        for key, kind in self.foreign.items():
+            park((self.of_stream[key], key[1], kind))
 
     def issued(self, stream, device, stage):
         if stage == 0:

@@ -36,7 +36,8 @@ def world(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: w.capturing)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: w)
     monkeypatch.setattr(torch.cuda, "synchronize", w.synchronize)
-    return w
+    yield w
+    del decode._parked[:]
 
 
 def spaces(nbytes=64, stages=1):
@@ -87,3 +88,31 @@ def test_captured_calls_find_no_workspace_that_is_not_the_graphs(world):
     with pytest.raises(AssertionError):
         own.find(21, CPU, None, True)
     assert own.find(20, CPU, None, True) is own.find(20, CPU, None, True)
+
+
+def test_memory_of_a_dropped_plan_stays_until_its_streams_are_done(world):
+    """torch knows of no use of it but on its own stream, and would give it out again at once."""
+    import gc
+    import weakref
+    from paella_amd import ops
+
+    def used_and_dropped(*streams):
+        own = spaces()
+        refs = [weakref.ref(own.find(s, CPU, None, s != HOME)) for s in streams]
+        del own
+        gc.collect()
+        return refs
+
+    assert used_and_dropped(HOME)[0]() is None             # that one torch knows of
+    stream, = used_and_dropped(20)
+    assert stream() is not None
+    queue, = used_and_dropped(7)                            # (whose first call waits for the device)
+    assert stream() is None and ("synchronize", CPU) in world.log and queue() is not None
+    other, = used_and_dropped(8)
+    assert queue() is not None and other() is not None and ("wait", 7) not in world.log
+    again, = used_and_dropped(7)
+    assert ("wait", 7) in world.log and queue() is None and again() is not None and other() is not None
+    ops._waits[8] = ops._waits.get(8, 0) + 1                # now a queue of ops.DirectQueue that has been closed, and so been waited for
+    used_and_dropped(20)
+    assert other() is None and again() is not None and ("wait", 8) not in world.log
+    del ops._waits[8]
