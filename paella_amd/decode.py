@@ -109,6 +109,7 @@ class _Workspaces:
         self.foreign = {}   # what those streams are that torch did not allocate the workspace for
         self.used = {}      # on queues: how often the queue had been waited for when the workspace was last given out
         self.begun = set()  # where a first stage has been issued and its second has not
+        self.lock = threading.RLock()  # held over a call of two launches: another thread's on the same stream would come between them
 
     def new(self, device):
         return torch.zeros(self.nbytes // 4 + 1, dtype=torch.int32, device=device)
@@ -137,11 +138,15 @@ class _Workspaces:
             return self.new(device)
         w = self.of_stream.get((device.index, stream))
         if w is None:
-            w = self.of_stream[device.index, stream] = self.new(device)
-            if stream != _torch_stream():  # the fill ran on torch's stream
-                torch.cuda.current_stream().synchronize()
-                self.foreign[device.index, stream] = kind
-                _unpark(stream)
+            with self.lock:
+                w = self.of_stream.get((device.index, stream))
+                if w is None:
+                    w = self.new(device)
+                    if stream != _torch_stream():  # the fill ran on torch's stream
+                        torch.cuda.current_stream().synchronize()
+                        self.foreign[device.index, stream] = kind
+                        _unpark(stream)
+                    self.of_stream[device.index, stream] = w
         if kind == _QUEUE_UNORDERED:
             if self.used.get((device.index, stream)) == _waits.get(stream, 0):
                 check(_library().paella_direct_queue_wait(stream), "paella_direct_queue_wait")
@@ -150,7 +155,8 @@ class _Workspaces:
 
     def __del__(self, park=_parked.append):
         for key, kind in self.foreign.items():
-            park((self.of_stream[key], key[1], kind))
+            if key in self.of_stream:
+                park((self.of_stream[key], key[1], kind))
 
     def issued(self, stream, device, stage):
         if stage == 0:
@@ -260,21 +266,22 @@ class PrefixAttention:
         else:
             assert out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous()
         explicit, stream = stream is not None, _stream(stream)
-        own = workspace is None
-        if own:
-            workspace = self.workspaces.find(stream, q.device, stage, explicit)
-            address = None if workspace is None else workspace.data_ptr()
+        if workspace is None:
+            with self.workspaces.lock:
+                workspace = self.workspaces.find(stream, q.device, stage, explicit)
+                rc = self._issue(stage, cache, batch, qp, qs, out, None if workspace is None else workspace.data_ptr(), stream, job_id, notifier)
+                if stage is not None and not rc and self.workspaces.stages > 1:
+                    self.workspaces.issued(stream, q.device, stage)
         else:
-            address = self.workspaces.given(workspace)
-        if stage is None:
-            rc = self._launch(self._ref, cache.ref, batch.ref, qp, qs, out.data_ptr(), address, stream, job_id, notifier)
-        else:
-            rc = self.lib.paella_prefix_attention_launch_stage(self._ref, stage, cache.ref, batch.ref, qp, qs, out.data_ptr(), address, stream, job_id, notifier)
-            if own and not rc and self.workspaces.stages > 1:
-                self.workspaces.issued(stream, q.device, stage)
+            rc = self._issue(stage, cache, batch, qp, qs, out, self.workspaces.given(workspace), stream, job_id, notifier)
         if rc:
             check(rc, "paella_prefix_attention_launch")
         return out
+
+    def _issue(self, stage, cache, batch, qp, qs, out, workspace, stream, job_id, notifier):
+        if stage is None:
+            return self._launch(self._ref, cache.ref, batch.ref, qp, qs, out.data_ptr(), workspace, stream, job_id, notifier)
+        return self.lib.paella_prefix_attention_launch_stage(self._ref, stage, cache.ref, batch.ref, qp, qs, out.data_ptr(), workspace, stream, job_id, notifier)
 
 
 class BeamSelect:
