@@ -232,6 +232,7 @@ constexpr unsigned kLowestKey = 0x00800000u;  // order_key(-FLT_MAX); -inf lies 
 __device__ __forceinline__ unsigned long long entry(unsigned key, unsigned index) { return (unsigned long long)key << 32 | (0xFFFFFFFFu - index); }
 
 constexpr int kMostLists = 1024;     // beams * splits
+constexpr int kMostSplits = 64;      // parts of a beam that the merge adds up
 constexpr int kMostStaged = 1024;    // entries that the merge fetches at once
 constexpr int kCounterStride = 32;   // a cache line each: counts on one line go one after the other, 2048 of 32 groups for 7 us
 constexpr int kWaveCandidates = 128;  // of one wave's logits that go on to the workgroup's ranking
@@ -534,10 +535,10 @@ __global__ __launch_bounds__(256, T::bytes == 4 && VALUES == 32 ? 5 : 7) void be
         if (threadIdx.x == 0) found = 0;
         __syncthreads();
         for (int w = threadIdx.x >> 4; w < (a.beams + 15) / 16 * 16; w += 16) {  // a beam's parts by 16 lanes
-            f32x2 p[4];
+            f32x2 p[kMostSplits / 16];
             float m = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < kMostSplits / 16; ++i) {
                 const int s = i * 16 + (lane & 15);
                 p[i] = f32x2{-INFINITY, 0.f};
                 if (w < a.beams && s < a.splits) p[i] = ms[w * a.splits + s];
@@ -546,7 +547,7 @@ __global__ __launch_bounds__(256, T::bytes == 4 && VALUES == 32 ? 5 : 7) void be
             m = row_all(m, [](float x, float y) { return fmaxf(x, y); });
             double total = 0.;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < kMostSplits / 16; ++i)
                 if (p[i].y > 0.f) total += (double)p[i].y * (double)__builtin_amdgcn_exp2f((p[i].x - m) * kLog2e);
             total = row_all(total, [](double x, double y) { return x + y; });
             if ((lane & 15) == 0 && w < a.beams) {
@@ -752,7 +753,7 @@ bool select_plan_ok(const paella_beam_select_plan* p) {
     if (!p || p->dtype < PAELLA_F32 || p->dtype > PAELLA_F16 || p->groups <= 0 || p->beams <= 0 || p->beams > 32 || p->vocab <= 0 || p->vocab > 524288) return false;
     if (p->count <= 0 || p->count > 64 || (p->values != 8 && p->values != 32)) return false;
     const int splits = (p->vocab + 256 * p->values - 1) / (256 * p->values);
-    return p->splits == splits && p->beams * splits <= kMostLists && (double)p->groups * p->beams * splits <= kMostWorkgroups;
+    return p->splits == splits && splits <= kMostSplits && p->beams * splits <= kMostLists && (double)p->groups * p->beams * splits <= kMostWorkgroups;
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -804,9 +805,9 @@ int paella_beam_select_plan_make(int dtype, int groups, int beams, int vocab, in
     if (beams > 32 || vocab > 524288 || count > 64) return PAELLA_ENOSUP;
     *p = paella_beam_select_plan{};
     p->dtype = dtype; p->groups = groups; p->beams = beams; p->vocab = vocab; p->count = count;
-    // 32 logits per thread where that still gives every compute unit a workgroup, else 8 (up to the 64 lists per beam that the merge takes)
+    // 32 logits per thread where that still gives every compute unit a workgroup, else 8 (up to the lists per beam that the merge takes)
     const int long_splits = (vocab + 8191) / 8192, short_splits = (vocab + 2047) / 2048;
-    p->values = (double)groups * beams * long_splits >= 256 || short_splits > 64 || beams * short_splits > kMostLists ? 32 : 8;
+    p->values = (double)groups * beams * long_splits >= 256 || short_splits > kMostSplits || beams * short_splits > kMostLists ? 32 : 8;
     p->splits = p->values == 32 ? long_splits : short_splits;
     if (!select_plan_ok(p)) return PAELLA_ENOSUP;
     const size_t lists = (size_t)groups * beams * p->splits;

@@ -34,3 +34,17 @@ def test_a_ragged_batch_with_room_for_more_new_tokens_than_it_has_is_planned(lib
                             for prefix in (0, 9, 300, 5000):
                                 rc, p = attention_plan(lib, dtype, 2 * per_kv, 2, dim, 16, sequences, max_new, tokens, 20, prefix)
                                 assert rc == 0, (dtype, dim, per_kv, sequences, max_new, tokens, prefix, p.prefix_rows, p.own_rows)
+
+
+def test_a_selection_of_more_lists_than_the_merge_adds_up_is_refused(lib):
+    """A plan is the caller's memory: one that was not made by the library has to hold to the same bounds, or a beam's normaliser would leave part of the vocabulary out."""
+    from paella_amd import _abi
+    from paella_amd._abi_decode import BeamSelectPlan
+    p, d = BeamSelectPlan(), _abi.LaunchDims()
+    for vocab in (131073, 140000, 524288):
+        assert lib.paella_beam_select_plan_make(0, 1, 1, vocab, 5, ctypes.byref(p)) == 0
+        assert (p.values, p.splits) == (32, -(-vocab // 8192)) and lib.paella_beam_select_dims(ctypes.byref(p), ctypes.byref(d)) == 0
+        p.values, p.splits = 8, -(-vocab // 2048)
+        assert p.splits > 64 and lib.paella_beam_select_dims(ctypes.byref(p), ctypes.byref(d)) == EINVAL
+        assert lib.paella_beam_select_launch(ctypes.byref(p), AT, vocab, AT, None, 0, AT, AT, AT, AT, None, 0, None) == EINVAL
+    assert lib.paella_beam_select_plan_make(0, 1, 1, 131072, 5, ctypes.byref(p)) == 0 and (p.values, p.splits) == (8, 64)
