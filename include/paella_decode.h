@@ -66,7 +66,8 @@ typedef struct paella_kv_append_desc {
  * the angle position * inv_freq[i] (a product taken in 64 bits, so far positions keep their angle), in 32 bits with one rounding
  * at the end.  Queries go to q_out [tokens][heads][head_dim] (which may be q where q_stride is heads * head_dim), keys and, as
  * they are, values to the cache.  q, q_out: NULL where heads is 0; inv_freq: [rotary_dim / 2], NULL where rotary_dim is 0.
- * Two sequences of one call must not share the page that either appends to. */
+ * Two sequences of one call must not share the page that either appends to.  q_out must not overlap k, v or the cache; q, k and v must not lie in places of
+ * the cache that the call writes. */
 int paella_kv_append_dims(const paella_kv_append_desc* desc, const paella_kv_cache* cache, const paella_kv_batch* batch, paella_launch_dims* dims);
 int paella_kv_append_launch(const paella_kv_append_desc* desc, const paella_kv_cache* cache, const paella_kv_batch* batch, const void* q, const void* k,
                             const void* v, const float* q_weight, const float* k_weight, const float* inv_freq, void* q_out, void* stream,
@@ -95,7 +96,7 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* cache, const paella
 /* Launch shape of a stage with the register count and LDS of the kernel that is launched (the plan's own figures without a device). */
 int paella_prefix_attention_dims(const paella_prefix_attention_plan* plan, int stage, paella_launch_dims* dims);
 /* q: rows of heads * head_dim values, q_stride (a multiple of 8) from one row to the next; out: [tokens][heads][head_dim], not
- * overlapping q.  Cache and batch must have the plan's extents.  workspace: workspace_bytes, zero-filled once before its first use,
+ * overlapping q or the cache.  Cache and batch must have the plan's extents.  workspace: workspace_bytes, zero-filled once before its first use,
  * private to the request (launches that share it must not overlap); NULL where workspace_bytes is 0.  Issues all stages in order, the last
  * of which reports to `notifier`; PAELLA_ENOSUP for two stages on a queue that keeps no order: there the caller issues them one after
  * the other with paella_prefix_attention_launch_stage, the second once the first has finished. */
@@ -119,7 +120,8 @@ typedef struct paella_beam_select_plan {
  * log(sum_u exp(x[w][u])); of equals the lower w * vocab + t comes first.  A beam with finished[w] != 0 has one continuation, pad_token, worth
  * scores[w]; its logits are not read.  A NaN logit counts as -inf, a row that holds +inf has no continuations, and what is worth -inf or NaN is no
  * continuation: where fewer than `count` are left, the rest of the outputs are -inf, -1 and -1.  out_scores, out_parents (w), out_tokens (t):
- * [groups][count].  logits: rows of vocab values, row_stride apart; finished (bytes) may be NULL.  workspace as for attention. */
+ * [groups][count], overlapping neither each other nor any input; but out_scores may be scores where count == beams, and may overlap them where groups == 1.
+ * logits: rows of vocab values, row_stride apart; finished (bytes) may be NULL.  workspace as for attention. */
 int paella_beam_select_plan_make(int dtype, int groups, int beams, int vocab, int count, paella_beam_select_plan* plan);
 int paella_beam_select_dims(const paella_beam_select_plan* plan, paella_launch_dims* dims);
 int paella_beam_select_launch(const paella_beam_select_plan* plan, const void* logits, int64_t row_stride, const float* scores, const uint8_t* finished,
@@ -130,7 +132,7 @@ int paella_beam_select_launch(const paella_beam_select_plan* plan, const void* l
  * tables and past: its row g * count + c of tables_out names the parent's full pages (shared, not copied) and then the page of its next
  * token -- for the first child of p the parent's half-filled page itself, for every further one spare[g * count + c], to which that page's tokens are
  * copied; where the parent's pages are all full, the spare page for every child.  Entries behind that page are left as they were; past_out = past[r]. A
- * parent outside 0 .. beams - 1 gives past_out 0 and an untouched row.  tables_out and past_out must not overlap their inputs; the spare pages must be
+ * parent outside 0 .. beams - 1 gives past_out 0 and an untouched row.  tables_out and past_out must overlap neither each other nor any input; the spare pages must be
  * named by no table.  Several layers: one call for each layer's cache with the same tables. */
 typedef struct paella_beam_reorder_desc {
     int groups, beams, count, max_pages;

@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 
 #include "paella_decode.h"
@@ -158,6 +159,19 @@ inline bool batch_ok(const paella_kv_batch* b) {
 inline bool overlap(const void* a, double a_bytes, const void* b, double b_bytes) {
     const double x = (double)(uintptr_t)a, y = (double)(uintptr_t)b;
     return x < y + b_bytes && y < x + a_bytes;
+}
+
+// Of `rows` rows of row_bytes, row_stride bytes (not less) apart: whether any lies over the other memory.
+inline bool rows_overlap(const void* a, int64_t rows, int64_t row_stride, int64_t row_bytes, const void* b, double b_bytes) {
+    const double ahead = (double)(uintptr_t)b - (double)(uintptr_t)a - (double)row_bytes;  // the first row that ends behind b's beginning
+    const double first = ahead < 0 ? 0 : std::floor(ahead / (double)row_stride) + 1;
+    return first < (double)rows && (double)(uintptr_t)a + first * (double)row_stride < (double)(uintptr_t)b + b_bytes;
+}
+
+// Whether outputs lie over the cache.
+inline bool over_cache(const paella_kv_cache* c, const void* out, double bytes) {
+    const double size = (double)c->num_pages * c->kv_heads * c->page_size * c->head_dim * element_bytes(c->dtype);
+    return overlap(c->k, size, out, bytes) || overlap(c->v, size, out, bytes);
 }
 
 inline void set_launch_dims(paella_launch_dims* d, unsigned grid, unsigned block, unsigned lds, unsigned vgprs) {

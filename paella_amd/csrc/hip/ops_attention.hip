@@ -161,6 +161,11 @@ int paella_prefix_attention_launch_stage(const paella_prefix_attention_plan* p, 
     if (overlap(q, ((double)(b->tokens - 1) * q_stride + row) * size, out, (double)b->tokens * row * size)) return PAELLA_EINVAL;
     const size_t need = workspace_of(p);
     if (need && (!workspace || ((uintptr_t)workspace & 15))) return PAELLA_EINVAL;
+    const double out_bytes = (double)b->tokens * row * size;
+    if (over_cache(c, out, out_bytes)) return PAELLA_EINVAL;
+    if (need && (over_cache(c, workspace, (double)need) || overlap(out, out_bytes, workspace, (double)need) ||
+                 rows_overlap(q, b->tokens, q_stride * size, row * size, workspace, (double)need)))
+        return PAELLA_EINVAL;
     const Grid g = grid_of(p);
     AttentionArgs a;
     a.q = (const char*)q; a.k_cache = (const char*)c->k; a.v_cache = (const char*)c->v; a.out = (char*)out;

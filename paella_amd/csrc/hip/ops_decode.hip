@@ -758,6 +758,11 @@ bool select_plan_ok(const paella_beam_select_plan* p) {
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
+size_t select_workspace(const paella_beam_select_plan* p) {
+    const size_t lists = (size_t)p->groups * p->beams * p->splits;
+    return up256((size_t)p->groups * 4 * kCounterStride) + up256(lists * 8) + lists * p->count * 8;
+}
+
 }  // namespace
 
 extern "C" {
@@ -782,6 +787,11 @@ int paella_kv_append_launch(const paella_kv_append_desc* d, const paella_kv_cach
     if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out) & 15) != 0) return PAELLA_EINVAL;
     if (d->heads && overlap(q, (double)(b->tokens - 1) * d->q_stride * size + q_row * size, q_out, (double)b->tokens * q_row * size) &&
         !(q == q_out && d->q_stride == q_row))
+        return PAELLA_EINVAL;
+    // other tokens' workgroups may still read keys and values
+    const double out_bytes = (double)b->tokens * q_row * size;
+    if (d->heads && (rows_overlap(k, b->tokens, d->k_stride * size, kv_row * size, q_out, out_bytes) || over_cache(c, q_out, out_bytes) ||
+                     rows_overlap(v, b->tokens, d->v_stride * size, kv_row * size, q_out, out_bytes)))
         return PAELLA_EINVAL;
     AppendArgs a;
     a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v;
@@ -811,7 +821,7 @@ int paella_beam_select_plan_make(int dtype, int groups, int beams, int vocab, in
     p->splits = p->values == 32 ? long_splits : short_splits;
     if (!select_plan_ok(p)) return PAELLA_ENOSUP;
     const size_t lists = (size_t)groups * beams * p->splits;
-    p->workspace_bytes = up256((size_t)groups * 4 * kCounterStride) + up256(lists * 8) + lists * count * 8;
+    p->workspace_bytes = select_workspace(p);
     set_launch_dims(&p->dims, (unsigned)lists, 256, select_lds(p), 64);
     p->flops = 4.0 * groups * beams * vocab;
     p->bytes = (double)groups * beams * vocab * element_bytes(dtype) + groups * (beams * 4.0 + count * 12.0);
@@ -833,6 +843,17 @@ int paella_beam_select_launch(const paella_beam_select_plan* p, const void* logi
     const int size = element_bytes(p->dtype);
     if (((uintptr_t)logits & (size - 1)) || ((uintptr_t)workspace & 15)) return PAELLA_EINVAL;
     const size_t lists = (size_t)p->groups * p->beams * p->splits;
+    // A group is merged while others are still read.  Its own scores have been by then: they may become the next step's.
+    const int64_t beams = (int64_t)p->groups * p->beams;
+    const double in_bytes = (double)beams * 4, bytes = (double)p->groups * p->count * 4, space = (double)select_workspace(p);
+    const bool in_place = p->groups == 1 || (out_scores == scores && p->count == p->beams);
+    const void* const outs[3] = {out_scores, out_parents, out_tokens};
+    for (int i = 0; i < 3; ++i) {
+        if (rows_overlap(logits, beams, row_stride * size, (int64_t)p->vocab * size, outs[i], bytes) || (finished && overlap(finished, (double)beams, outs[i], bytes)) ||
+            (!(i == 0 && in_place) && overlap(scores, in_bytes, outs[i], bytes)) || overlap(outs[i], bytes, outs[(i + 1) % 3], bytes) || overlap(workspace, space, outs[i], bytes))
+            return PAELLA_EINVAL;
+    }
+    if (rows_overlap(logits, beams, row_stride * size, (int64_t)p->vocab * size, workspace, space) || overlap(scores, in_bytes, workspace, space)) return PAELLA_EINVAL;
     SelectArgs a;
     a.logits = (const char*)logits; a.row_stride = row_stride * size; a.scores = scores; a.finished = finished;
     a.pad_token = pad_token; a.groups = p->groups; a.beams = p->beams; a.vocab = p->vocab; a.count = p->count; a.splits = p->splits;
@@ -868,10 +889,14 @@ int paella_beam_reorder_launch(const paella_beam_reorder_desc* d, const paella_k
                                const int32_t* spare, int32_t* tables_out, int32_t* past_out, void* stream, uint32_t job_id, void* notifier) {
     if (int rc = reorder_check(d, c)) return rc;
     if (!cache_ok(c) || !parents || !past || !tables || !spare || !tables_out || !past_out) return PAELLA_EINVAL;
+    // every output: written by one workgroup while others may still read the inputs
     const double in = (double)d->groups * d->beams * 4, out = (double)d->groups * d->count * 4;
-    if (overlap(tables, in * d->max_pages, tables_out, out * d->max_pages) || overlap(past, in, past_out, out) || overlap(parents, out, past_out, out) ||
-        overlap(spare, out, tables_out, out * d->max_pages))
-        return PAELLA_EINVAL;
+    const struct { const void* at; double bytes; } outs[2] = {{tables_out, out * d->max_pages}, {past_out, out}};
+    for (const auto& o : outs)
+        if (overlap(tables, in * d->max_pages, o.at, o.bytes) || overlap(past, in, o.at, o.bytes) || overlap(parents, out, o.at, o.bytes) ||
+            overlap(spare, out, o.at, o.bytes) || over_cache(c, o.at, o.bytes))
+            return PAELLA_EINVAL;
+    if (overlap(tables_out, out * d->max_pages, past_out, out)) return PAELLA_EINVAL;
     ReorderArgs a;
     a.k_cache = (char*)c->k; a.v_cache = (char*)c->v;
     a.parents = parents; a.past = past; a.tables = tables; a.spare = spare; a.tables_out = tables_out; a.past_out = past_out;
