@@ -208,7 +208,7 @@ class KVBatch:
 def kv_append(cache, batch, k, v, q=None, q_norm=None, k_norm=None, eps=1e-6, inv_freq=None, interleaved=False, out=None, stream=None, job_id=0, notifier=None):
     """Stores the new tokens' k and v ([tokens, kv_heads, head_dim]) in the cache, k normed per head (k_norm: float32 [head_dim]) and rotated (inv_freq: float32, one
     per rotated pair) on the way; returns q ([tokens, heads, head_dim]) normed and rotated likewise, in `out` where given (which may be q)."""
-    _on_device(cache.k, k, v, q, q_norm, k_norm, inv_freq, out)
+    _on_device(cache.k, k, v, q, q_norm, k_norm, inv_freq, out, batch.past)
     tokens, dim = batch.tokens, cache.head_dim
     kp, ks = _rows(k, tokens, cache.kv_heads, cache)
     vp, vs = _rows(v, tokens, cache.kv_heads, cache)
@@ -258,7 +258,7 @@ class PrefixAttention:
         """stage: one of the plan's launches (plan.stages) alone, for queues that keep no order.  workspace: one of new_workspace() in place of the stream's own, for calls of one
         plan that may run at once on such a queue.  The stages of a call share it; under graph capture, on different streams, or with other calls of this plan between them
         they have to be given it."""
-        _on_device(q, cache.k, out)
+        _on_device(q, cache.k, out, batch.past)
         assert batch.prefix_pages * cache.page_size >= batch.prefix_len, "the prefix's table has too few pages"
         qp, qs = _rows(q, batch.tokens, self.heads, cache)
         if out is None:
