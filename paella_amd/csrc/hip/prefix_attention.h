@@ -386,14 +386,17 @@ struct NarrowWalk {
 
 // Loads of memory into LDS without a register between, in the order of the lanes: 16 bytes (4) of `base` + each lane's offset, from `lds` on.  What has arrived is
 // told by arrived(n): all but the wave's last n loads.  (Written out, because ahead of any read of LDS the compiler waits for all of such loads.  The wait states are
-// those between a vector instruction's write of the base and the load.)
+// those between a vector instruction's write of the base and the load.  m0 is named, though reserved, so that the compiler keeps nothing of its own in it across them.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ unsigned lds_address(const char* p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
 __device__ __forceinline__ void bring16(const char* base, unsigned offset, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "m0", "memory");
 }
 __device__ __forceinline__ void bring4(const void* base, unsigned offset, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "m0", "memory");
 }
+#pragma clang diagnostic pop
 template <int N>
 __device__ __forceinline__ void arrived() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
