@@ -741,7 +741,8 @@ int append_check(const paella_kv_append_desc* d, const paella_kv_cache* c, const
     return 0;
 }
 
-// LDS of a selection: the waves' candidates of the pass over the logits and their common list, and the merge's entries, in the same place.
+// LDS of a selection: the waves' candidates of the pass over the logits and their common list, and the merge's entries, in the same place.  At most 48 KiB (64 lists of 64
+// entries), which any launch may have.
 unsigned select_lds(const paella_beam_select_plan* p) {
     const unsigned lists = p->beams * p->splits, taken = ((unsigned)p->count < lists ? p->count : lists) * p->count;
     const unsigned staged = lists * p->count <= kMostStaged ? lists * p->count : lists;
@@ -864,9 +865,6 @@ int paella_beam_select_launch(const paella_beam_select_plan* p, const void* logi
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
     const unsigned lds = select_lds(p);
     const SelectKernel kernel = select_kernel(p->dtype, p->values);
-    if (lds > 65536) {
-        if (hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds)) return (int)e;
-    }
     launch(kernel, dim3((unsigned)lists), dim3(256), lds, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }

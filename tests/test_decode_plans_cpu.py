@@ -48,3 +48,15 @@ def test_a_selection_of_more_lists_than_the_merge_adds_up_is_refused(lib):
         assert p.splits > 64 and lib.paella_beam_select_dims(ctypes.byref(p), ctypes.byref(d)) == EINVAL
         assert lib.paella_beam_select_launch(ctypes.byref(p), AT, vocab, AT, None, 0, AT, AT, AT, AT, None, 0, None) == EINVAL
     assert lib.paella_beam_select_plan_make(0, 1, 1, 131072, 5, ctypes.byref(p)) == 0 and (p.values, p.splits) == (8, 64)
+
+
+def test_no_selection_needs_more_shared_memory_than_any_launch_may_have(lib):
+    from paella_amd._abi_decode import BeamSelectPlan
+    p, most = BeamSelectPlan(), 0
+    for beams in (1, 2, 16, 31, 32):
+        for vocab in (1, 2048, 2049, 50021, 131072, 131073, 262144, 524288):
+            for count in (1, 15, 16, 17, 32, 63, 64):
+                for groups in (1, 300):
+                    if lib.paella_beam_select_plan_make(0, groups, beams, vocab, count, ctypes.byref(p)) == 0:
+                        most = max(most, p.dims.lds_bytes)
+    assert most == 64 * 64 * 12
