@@ -87,10 +87,10 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_
     const int64_t per_kv = heads / c->kv_heads, size = element_bytes(c->dtype), row_bytes = c->head_dim * size;
     const int step = size == 4 ? 16 : 32;
     // Rows of a workgroup.  Where a key head has few, 16: its waves split the keys.  Else 64 or 128: each wave has rows of its own, the keys are read once
-    // for all of them.  That is no gain up to some number of steps by 16 rows, where latency counts: bf16, 4 key heads of 128, 96 rows each over 1600 keys, 192 over
-    // 1200 / 3000 (1200, 1824 / 4512 steps) 10.9, 12.8 / 17.0 us by 16 rows, 15.4, 14.9 / 17.2 by 128, 8 key heads, 36 rows over 3000 / 8000 (2256 / 6000) 12.9 / 21.2
-    // against 12.3 / 17.0; fp32 96 rows over 1600, 192 over 1200 / 3000 (2400, 3600 / 9024) 16.2, 19.5 / 33.0 against 18.8, 20.8 / 30.0.  Heads of 256 hold few keys'
-    // loads beside 16 rows: 24 rows over 187 keys 16.8 against 13.0.
+    // for all of them.  That is no gain up to some number of steps by 16 rows, where latency counts.  fp32, heads of 128, by 16 rows / by 64: 4 key heads, 96 rows each over 1600
+    // keys, 192 over 1200 / 1500 / 2200 / 3000 (2400, 3600 / 4512 / 6624 / 9024 steps) 15.7 / 18.7 us, 19.6 / 20.4, 20.8 / 21.0, 23.2 / 21.7, 32.0 / 23.1; 96 over 3000 (4512)
+    // 21.2 / 20.2.  bf16, by 16 / by 128: 96 over 1600, 192 over 1200 / 2000 / 3000 (1200, 1824 / 3024 / 4512) 10.4 / 15.3, 12.6 / 14.6, 13.7 / 16.2, 16.8 / 16.6, but 8 key
+    // heads, 36 rows over 3000 / 8000 (2256 / 6000) 12.9 / 12.3 and 21.2 / 17.0.  Heads of 256 hold few keys' loads beside 16 rows: 24 rows over 187 keys 16.8 against 13.0.
     const bool small_heads = c->head_dim <= 128;
     auto rows = [&](int64_t n) { return n <= 64 || !small_heads || row_bytes > 256 ? 64 : 128; };
     const int64_t own = std::min(b->max_new, b->tokens) * per_kv, shared = b->tokens * per_kv;  // no sequence has more than all rows, whatever max_new leaves room for
@@ -98,7 +98,7 @@ int paella_prefix_attention_plan_make(const paella_kv_cache* c, const paella_kv_
     p->prefix_rows = p->own_rows;
     if (p->prefix_len) {
         const double steps = (double)ceil_div(shared, 16) * c->kv_heads * ceil_div(p->prefix_len, step);
-        const bool few = shared <= 16 || (small_heads && steps <= (size == 4 ? 3500 : 2048));
+        const bool few = shared <= 16 || (small_heads && steps <= (size == 4 ? 4500 : 2048));
         p->prefix_rows = few && p->own_rows == 16 ? 16 : rows(shared);
     }
     if (p->own_rows == 64 && p->prefix_rows == 128) p->own_rows = 128;

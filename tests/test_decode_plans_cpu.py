@@ -60,3 +60,10 @@ def test_no_selection_needs_more_shared_memory_than_any_launch_may_have(lib):
                     if lib.paella_beam_select_plan_make(0, groups, beams, vocab, count, ctypes.byref(p)) == 0:
                         most = max(most, p.dims.lds_bytes)
     assert most == 64 * 64 * 12
+
+
+@pytest.mark.parametrize("sequences,keys,rows", [(24, 1600, 16), (48, 1200, 16), (48, 2200, 64), (48, 3000, 64), (24, 3000, 64)])
+def test_fp32_rows_by_sixteen_as_long_as_that_is_faster(lib, sequences, keys, rows):
+    """4 key heads of 128 for 16 query heads.  By 16 rows / by 64: 15.7 / 18.7 us, 19.6 / 20.4, then 23.2 / 21.7, 32.0 / 23.1, 21.2 / 20.2."""
+    rc, p = attention_plan(lib, 0, 16, 4, 128, 64, sequences, 1, sequences, 1, keys)
+    assert rc == 0 and (p.prefix_rows, p.own_rows) == (rows, 16)
