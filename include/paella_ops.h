@@ -322,6 +322,9 @@ int paella_direct_queue_destroy(void* queue);
  * stream nor a queue). */
 enum paella_stream_kind { PAELLA_STREAM = 0, PAELLA_STREAM_CAPTURING = 1, PAELLA_QUEUE_UNORDERED = 2, PAELLA_QUEUE_ORDERED = 3 };
 int paella_stream_kind_of(void* stream);
+/* How many of the embedded code objects are loaded for direct dispatch: two with the first queue (the models' operators), the others each with the first of their
+ * kernels that a queue is given. */
+int paella_direct_code_objects(void);
 
 /*
  * Copies `bytes` from src to dst (host memory both) on a helper thread of this library and then calls done(arg) on that

@@ -129,6 +129,7 @@ OPS_SYMBOLS = {
     "paella_direct_queue_shared": (c_int, [ctypes.POINTER(c_void_p)]),
     "paella_direct_queue_destroy": (c_int, [c_void_p]),
     "paella_stream_kind_of": (c_int, [c_void_p]),
+    "paella_direct_code_objects": (c_int, []),
 }
 
 RING_SYMBOLS = {

@@ -55,7 +55,22 @@ struct Runtime {
     hsa_amd_memory_pool_t kernarg_pool{};
     hsa_amd_memory_pool_t device_pool{};  // device memory the host may map (kernel arguments next to the GPU)
     bool have_gpu = false, have_cpu = false, have_pool = false, have_device_pool = false;
-    std::vector<hsa_executable_t> executables;
+};
+
+// The embedded code objects.  What every served model needs is loaded with the runtime, the rest with the first kernel that is in it.
+struct CodeObject {
+    const char *begin, *end, *what;
+    bool at_once;
+    bool loaded = false;
+    hsa_executable_t exe{};
+};
+CodeObject g_objects[] = {  // guarded by g_mutex
+    {paella_hsaco_conv_begin, paella_hsaco_conv_end, "load conv code object", true},
+    {paella_hsaco_misc_begin, paella_hsaco_misc_end, "load misc code object", true},
+    {paella_hsaco_decode_begin, paella_hsaco_decode_end, "load decode code object", false},
+    {paella_hsaco_attention_f32_begin, paella_hsaco_attention_f32_end, "load attention code object (fp32)", false},
+    {paella_hsaco_attention_bf16_begin, paella_hsaco_attention_bf16_end, "load attention code object (bf16)", false},
+    {paella_hsaco_attention_f16_begin, paella_hsaco_attention_f16_end, "load attention code object (fp16)", false},
 };
 
 std::mutex g_mutex;
@@ -121,14 +136,13 @@ hsa_status_t find_device_pool(hsa_amd_memory_pool_t pool, void*) {
     return HSA_STATUS_SUCCESS;
 }
 
-bool load_code_object(const char* begin, const char* end, const char* what) {
+bool load_code_object(CodeObject& o) {
     hsa_code_object_reader_t reader;
-    HSA_TRY(hsa_code_object_reader_create_from_memory(begin, (size_t)(end - begin), &reader), what);
-    hsa_executable_t exe;
-    HSA_TRY(hsa_executable_create_alt(HSA_PROFILE_FULL, HSA_DEFAULT_FLOAT_ROUNDING_MODE_DEFAULT, nullptr, &exe), what);
-    HSA_TRY(hsa_executable_load_agent_code_object(exe, g_rt.gpu, reader, nullptr, nullptr), what);
-    HSA_TRY(hsa_executable_freeze(exe, nullptr), what);
-    g_rt.executables.push_back(exe);
+    HSA_TRY(hsa_code_object_reader_create_from_memory(o.begin, (size_t)(o.end - o.begin), &reader), o.what);
+    HSA_TRY(hsa_executable_create_alt(HSA_PROFILE_FULL, HSA_DEFAULT_FLOAT_ROUNDING_MODE_DEFAULT, nullptr, &o.exe), o.what);
+    HSA_TRY(hsa_executable_load_agent_code_object(o.exe, g_rt.gpu, reader, nullptr, nullptr), o.what);
+    HSA_TRY(hsa_executable_freeze(o.exe, nullptr), o.what);
+    o.loaded = true;
     return true;
 }
 
@@ -151,12 +165,8 @@ bool init_runtime_locked() {
         return false;
     }
     hsa_amd_agent_iterate_memory_pools(g_rt.gpu, find_device_pool, nullptr);
-    if (!load_code_object(paella_hsaco_conv_begin, paella_hsaco_conv_end, "load conv code object")) return false;
-    if (!load_code_object(paella_hsaco_misc_begin, paella_hsaco_misc_end, "load misc code object")) return false;
-    if (!load_code_object(paella_hsaco_decode_begin, paella_hsaco_decode_end, "load decode code object")) return false;
-    if (!load_code_object(paella_hsaco_attention_f32_begin, paella_hsaco_attention_f32_end, "load attention code object (fp32)")) return false;
-    if (!load_code_object(paella_hsaco_attention_bf16_begin, paella_hsaco_attention_bf16_end, "load attention code object (bf16)")) return false;
-    if (!load_code_object(paella_hsaco_attention_f16_begin, paella_hsaco_attention_f16_end, "load attention code object (fp16)")) return false;
+    for (CodeObject& o : g_objects)
+        if (o.at_once && !load_code_object(o)) return false;
     return true;
 }
 
@@ -205,9 +215,16 @@ const DirectKernel* direct_kernel(const void* host_function) {
         std::abort();
     }
     const std::string symbol_name = std::string(name) + ".kd";
-    for (hsa_executable_t exe : g_rt.executables) {
+    for (CodeObject& o : g_objects) {
+        if (!o.loaded) {
+            if (!memmem(o.begin, (size_t)(o.end - o.begin), symbol_name.c_str(), symbol_name.size() + 1)) continue;  // (a name in the object's table of them)
+            if (!load_code_object(o)) {
+                std::fprintf(stderr, "[paella] direct dispatch: %s\n", g_rt.error.c_str());
+                std::abort();
+            }
+        }
         hsa_executable_symbol_t symbol;
-        if (hsa_executable_get_symbol_by_name(exe, symbol_name.c_str(), &g_rt.gpu, &symbol) != HSA_STATUS_SUCCESS) continue;
+        if (hsa_executable_get_symbol_by_name(o.exe, symbol_name.c_str(), &g_rt.gpu, &symbol) != HSA_STATUS_SUCCESS) continue;
         DirectKernel k;
         uint32_t kernarg = 0, lds = 0, priv = 0;
         hsa_executable_symbol_get_info(symbol, HSA_EXECUTABLE_SYMBOL_INFO_KERNEL_OBJECT, &k.object);
@@ -567,6 +584,11 @@ extern "C" int paella_direct_queue_destroy(void* queue) {
     hsa_amd_memory_pool_free(q->kernargs);
     delete q;
     return 0;
+}
+
+extern "C" int paella_direct_code_objects(void) {
+    std::lock_guard<std::mutex> lock(paella::g_mutex);
+    return (int)std::count_if(std::begin(paella::g_objects), std::end(paella::g_objects), [](const paella::CodeObject& o) { return o.loaded; });
 }
 
 extern "C" int paella_stream_kind_of(void* stream) {
