@@ -807,22 +807,22 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_attention_kernel(
         }
         const Quotient who = divide(pair, a.prefix_splits);
         const int h = (int)who.q, split = (int)who.r, per_kv = (int)a.per_kv.d;
-        const int first_row = (int)tile * FP::ROWS, group_rows = a.tokens * per_kv;
+        // rows behind the last sequence are left out (their lanes take the last row's query)
+        const int first_row = (int)tile * FP::ROWS, group_rows = (a.starts ? min(max(a.starts[a.sequences], 0), a.tokens) : a.tokens) * per_kv;
         first_counter = (unsigned)h * a.counter_pitch + (unsigned)first_row;
         const char* q_row[FP::R];
         int limit[FP::R];
 #pragma unroll
         for (int r = 0; r < FP::R; ++r) {
-            const int x = min(first_row + (FP::WIDE ? wave * 16 * FP::R : 0) + r * 16 + (lane & 15), group_rows - 1);
+            const int x = max(min(first_row + (FP::WIDE ? wave * 16 * FP::R : 0) + r * 16 + (lane & 15), group_rows - 1), 0);
             const Quotient at = divide((unsigned)x, a.per_kv);
             q_row[r] = a.q + at.q * a.q_stride + (h * per_kv + (int)at.r) * head_bytes;
             limit[r] = a.prefix_len;
         }
-        if ((int)threadIdx.x < FP::ROWS) {  // rows behind the last sequence are left out
+        if ((int)threadIdx.x < FP::ROWS) {
             const int x = first_row + (int)threadIdx.x;
             const Quotient at = divide((unsigned)x, a.per_kv);
-            const int rows = a.starts ? min(a.starts[a.sequences], a.tokens) : a.tokens;
-            row_id[threadIdx.x] = x < group_rows && (int)at.q < rows ? (int)at.q * a.heads + h * per_kv + (int)at.r : -1;
+            row_id[threadIdx.x] = x < group_rows ? (int)at.q * a.heads + h * per_kv + (int)at.r : -1;
         }
         __syncthreads();
         s.table = a.prefix_table;
