@@ -125,6 +125,8 @@ class _Workspaces:
         if not self.nbytes:
             return None
         capturing = torch.cuda.is_current_stream_capturing()
+        if not (explicit or capturing) and self.stages == 1 and (device.index, stream) in self.of_stream:
+            return self.of_stream[device.index, stream]
         kind = _library().paella_stream_kind_of(stream) if explicit else _STREAM
         # a captured workspace is filled on torch's stream; one that eager calls use must not get into a graph
         if (explicit and stream != _torch_stream()) if capturing else kind == _STREAM_CAPTURING:
@@ -266,14 +268,18 @@ class PrefixAttention:
         else:
             assert out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous()
         explicit, stream = stream is not None, _stream(stream)
-        if workspace is None:
-            with self.workspaces.lock:
-                workspace = self.workspaces.find(stream, q.device, stage, explicit)
-                rc = self._issue(stage, cache, batch, qp, qs, out, None if workspace is None else workspace.data_ptr(), stream, job_id, notifier)
-                if stage is not None and not rc and self.workspaces.stages > 1:
-                    self.workspaces.issued(stream, q.device, stage)
+        spaces = self.workspaces
+        if workspace is not None:
+            rc = self._issue(stage, cache, batch, qp, qs, out, spaces.given(workspace), stream, job_id, notifier)
+        elif spaces.stages == 1:
+            workspace = spaces.find(stream, q.device, stage, explicit)
+            rc = self._issue(stage, cache, batch, qp, qs, out, None if workspace is None else workspace.data_ptr(), stream, job_id, notifier)
         else:
-            rc = self._issue(stage, cache, batch, qp, qs, out, self.workspaces.given(workspace), stream, job_id, notifier)
+            with spaces.lock:
+                workspace = spaces.find(stream, q.device, stage, explicit)
+                rc = self._issue(stage, cache, batch, qp, qs, out, workspace.data_ptr(), stream, job_id, notifier)
+                if stage is not None and not rc:
+                    spaces.issued(stream, q.device, stage)
         if rc:
             check(rc, "paella_prefix_attention_launch")
         return out
