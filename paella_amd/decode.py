@@ -131,13 +131,12 @@ class _Workspaces:
         # a captured workspace is filled on torch's stream; one that eager calls use must not get into a graph
         if (explicit and stream != _torch_stream()) if capturing else kind == _STREAM_CAPTURING:
             raise AssertionError("a call captured on another stream than torch's has to be given a workspace")
-        if self.stages > 1:
-            if stage is not None and capturing:
-                raise AssertionError("stages of their own under graph capture have to be given one workspace")
-            if ((device.index, stream) in self.begun) != (stage == 1):
-                raise AssertionError("a second stage before its first, or a call between the stages of another, on this stream: give each call a workspace of its own")
         if capturing:
+            if self.stages > 1 and stage is not None:
+                raise AssertionError("stages of their own under graph capture have to be given one workspace")
             return self.new(device)
+        if self.stages > 1 and ((device.index, stream) in self.begun) != (stage == 1):
+            raise AssertionError("a second stage before its first, or a call between the stages of another, on this stream: give each call a workspace of its own")
         w = self.of_stream.get((device.index, stream))
         if w is None:
             with self.lock:

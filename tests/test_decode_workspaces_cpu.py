@@ -116,3 +116,23 @@ def test_memory_of_a_dropped_plan_stays_until_its_streams_are_done(world):
     used_and_dropped(20)
     assert other() is None and again() is not None and ("wait", 8) not in world.log
     del ops._waits[8]
+
+
+def test_a_whole_call_is_captured_whatever_the_streams_eager_calls_are_at(world):
+    """It has memory of its own: only eager calls come between the stages of another."""
+    own = spaces(64, 2)
+    kept = own.find(HOME, CPU, 0)
+    own.issued(HOME, CPU, 0)
+    with pytest.raises(AssertionError):
+        own.find(HOME, CPU)
+    world.capturing = True
+    assert own.find(HOME, CPU) is not kept
+    for stage in (0, 1):
+        with pytest.raises(AssertionError):
+            own.find(HOME, CPU, stage)
+    world.capturing = False
+    assert own.find(HOME, CPU, 1) is kept
+    own.issued(HOME, CPU, 1)
+    with pytest.raises(AssertionError):
+        own.find(HOME, CPU, 1)
+    assert own.find(HOME, CPU) is kept
