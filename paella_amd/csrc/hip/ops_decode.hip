@@ -168,7 +168,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
                     for (int e = 0; e < 8; ++e) sum += f[e] * f[e];
                     sum = lanes_sum(sum, a.group_log2);
                     if (is_q ? a.q_weight != nullptr : !is_v && a.k_weight != nullptr) {
-                        const float r = __builtin_amdgcn_rsqf(sum * a.inv_dim + a.eps);
+                        const float r = rsqrtf(sum * a.inv_dim + a.eps);  // (the bare instruction takes subnormal numbers for 0, and eps may be 0)
                         const f32x4* const w = reinterpret_cast<const f32x4*>(norm[is_q ? 0 : 1] + (in_head ? d0 : 0));
 #pragma unroll
                         for (int e = 0; e < 8; ++e) f[e] = f[e] * r * w[e / 4][e % 4];
