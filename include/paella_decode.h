@@ -8,7 +8,7 @@
  * The cache of one layer is two tensors [num_pages][kv_heads][page_size][head_dim], keys and values, on 16-byte
  * boundaries.  A sequence's own token i lies in slot i % page_size of page tables[sequence][i / page_size]; the shared
  * prefix lies the same way in the pages of prefix_table.  All lengths and tables are device data, so a captured graph
- * follows them.  Offsets into the cache are 64-bit.
+ * follows them.  Offsets into the cache are 64-bit; attention sees a sequence's first 2^30 own tokens.
  *
  * Device data that the host cannot check is checked where it is used: a page number outside the cache, or a token
  * beyond its row of the table, is never written and takes no part in attention; a negative length counts as 0; no
@@ -89,8 +89,9 @@ typedef struct paella_prefix_attention_plan {
 } paella_prefix_attention_plan;
 
 /* out[t][h] = sum_i softmax_i(scale * q[t][h] . k_i[h / (heads / kv_heads)]) v_i over the prefix and the own tokens 0 .. past + j of
- * row t.  The prefix is walked once for all rows that share it, tile by tile.  A row whose every key is excluded (pages outside the cache)
- * gives zeros.  Keys and values in excluded places may hold anything; those of a sequence's later new tokens must be finite.
+ * row t.  The prefix is walked once for all rows that share it, tile by tile.  Scores, maxima, sums and outputs are kept in 32 bits; of 16-bit types the weights
+ * softmax_i are rounded to the type ahead of their product with v_i (which takes both in one type) and divided by the sum of the rounded ones, so a result
+ * is off by one more half step of the type than its own rounding.  A row whose every key is excluded (pages outside the cache) gives zeros.  Keys and values in excluded places may hold anything; those of a sequence's later new tokens must be finite.
  * head_dim 64, 128 or 256 (PAELLA_ENOSUP otherwise).  Pure host arithmetic; of the cache and the batch, only the extents are looked at. */
 int paella_prefix_attention_plan_make(const paella_kv_cache* cache, const paella_kv_batch* batch, int heads, float scale, paella_prefix_attention_plan* plan);
 /* Launch shape of a stage with the register count and LDS of the kernel that is launched (the plan's own figures without a device). */
@@ -117,8 +118,9 @@ typedef struct paella_beam_select_plan {
 } paella_beam_select_plan;
 
 /* Per group (request) the `count` best continuations of its beams, best first.  Continuation (w, t) is worth scores[w] + x[w][t] -
- * log(sum_u exp(x[w][u])); of equals the lower w * vocab + t comes first.  A beam with finished[w] != 0 has one continuation, pad_token, worth
- * scores[w]; its logits are not read.  A NaN logit counts as -inf, a row that holds +inf has no continuations, and what is worth -inf or NaN is no
+ * log(sum_u exp(x[w][u])); of equals the lower w * vocab + t comes first.  Worths are added and compared in 64 bits, the exponentials and their sums over up
+ * to 8192 logits are 32-bit: within a beam the order is that of the logits, between beams that of worths whose logarithms carry such sums' roundings.  A beam with finished[w] != 0 has one continuation, pad_token, worth
+ * scores[w]; its logits are not read.  A NaN logit counts as -inf, a row that holds +inf has no continuations, and what is worth an infinity or NaN is no
  * continuation: where fewer than `count` are left, the rest of the outputs are -inf, -1 and -1.  out_scores, out_parents (w), out_tokens (t):
  * [groups][count], overlapping neither each other nor any input; but out_scores may be scores where count == beams, and may overlap them where groups == 1.
  * logits: rows of vocab values, row_stride apart; finished (bytes) may be NULL.  workspace as for attention. */

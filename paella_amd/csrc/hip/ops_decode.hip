@@ -16,8 +16,9 @@ using namespace paella;
 // Per new token: x' = x / sqrt(mean(x^2) + eps) * w for each query and key head, pairs (a, b) turned by the angle p * f_i:
 // (a cos - b sin, b cos + a sin); keys and values to the slot that the page table names.  One pass over the data: a workgroup per token,
 // 16 bytes (8 values of 16 bits; two loads in 32 bits) per lane, a head per group of lanes that lane moves norm and pair up.
-// Bounds: a few tokens the trips to memory in a row (length -> page -> stores), 3.8 us for 4 tokens of 12 heads of 64, 6.7 for 64 of 48 heads of 128 in bf16;
-// prompts memory, 9 k such tokens 39 us, 207 MB at 5.3 TB/s, as fast as a copy.
+// Bounds: a few tokens the trips to memory in a row (length -> page -> stores), 3.8 us for 4 tokens of 12 heads of 64; a batch's step
+// those and a token's 48 heads by one workgroup, on 64 of the 256 compute units, 6.8 us for 64 tokens of heads of 128 in bf16; prompts memory,
+// 9 k such tokens 39 us, 207 MB at 5.3 TB/s, as fast as a copy.
 struct AppendArgs {
     const char *q, *k, *v;
     char *q_out, *k_cache, *v_cache;

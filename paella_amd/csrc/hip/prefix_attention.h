@@ -1,6 +1,6 @@
 #pragma once
 // Attention of a decoding step: every new token over a prefix that all sequences share and over its own sequence's tokens, both in a paged
-// cache.  Included by one translation unit per element type (PAELLA_ATTENTION_TYPE), so that they compile side by side.
+// cache.  Included by one translation unit per element type, so that they compile side by side.
 //
 // out = sum_i p_i v_i / sum_i p_i with p_i = exp(scale * q . k_i - m): one pass over the keys with the running maximum m and sum, in 32 bits.
 //
@@ -18,7 +18,7 @@
 // permuted by the same rule.  Where the waves split the keys, K and V are therefore read once, in runs of 64 bytes and of whole keys, and wait in registers for
 // one step while the other product runs.
 //
-// Bounds.  Few rows: the trips to memory in a row (length, page, keys, parts, count, parts), 7.8 us for 3 rows a head over 333 keys in fp32, 8.3 for 8 over 2011 in
+// Bounds.  Few rows: the trips to memory in a row (length, page, keys, parts, count, parts), 7.7 us for 3 rows a head over 333 keys in fp32, 8.1 for 8 over 2011 in
 // fp16.  Own tokens of many sequences: memory, 1.05 GB at 5.6 TB/s (a plain read of this size 6.2).  The prefix of 32 rows and more per
 // key head: the matrix and vector units, which take turns; per 32 x 32 scores 34 matrix instructions of 16 cycles and some 90 vector ones of 4, 16 of
 // them exponentials of 16; 69 GFLOP in 90 us at the 1.9 GHz that the power limit leaves.  Both at once, 64 sequences over 65536 shared and 2000 own keys on average
@@ -410,7 +410,7 @@ __device__ __forceinline__ void lds_barrier() {
 
 // Many rows: each of the four waves has 16 R rows of its own, and all of them walk the same keys, which the workgroup brings to LDS step by step, AHEAD steps ahead
 // of the one that is worked on, with one barrier a step.  (Through registers, one tile of 64 keys ahead with two barriers: 118 us for 256 rows a key head over
-// 65536 keys, this 100, of which 11 join.  The next step's K to registers ahead of the barrier as well: no change.)  16-byte piece
+// 65536 keys, this 102, of which the launch that joins their 33 parts is 10.  The next step's K to registers ahead of the barrier as well: no change.)  16-byte piece
 // c of key i lies at place c ^ turn(i), so that the 16 keys of a score tile, and the 8 keys by 32 bytes that half a wave reads of V, come from different
 // banks.  16-bit V comes by transposing reads (of 4 keys by 16 dimensions, per 16 lanes), which save the vector unit the 32 permutations of a step.
 template <typename T, int D, int R>
