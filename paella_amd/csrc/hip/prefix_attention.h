@@ -107,17 +107,22 @@ struct AttentionRows {
     // small ones still count (with the maximum at 2^0, keys at e^-16 of the largest came to 0.4 % too little, at e^-17 to 3 %).  2^15 above m (2^16 is infinite) leave all bits to
     // weights down to 2^-25 of the largest, and what is lost below that is at most 2^-36 of it each.  Of these 15, 4 for the maximum's moves cost no time, 2 would: 40.6 us
     // against 39.4 for 32 sequences of up to 5 tokens over 8190 + 1000 keys.  fp32 and bf16 have exponents enough for any.
+    // Where scores are so large that they are in steps of a half and more, m and the exponentials' arguments are off by as much, and 2^8 is what fp16 has room for as well.
     static constexpr float BELOW = __is_same(T, F16) ? 11.f : 0.f, SLACK = __is_same(T, F16) ? 4.f : 8.f;
+    static constexpr float LARGE = 4194304.f;  // 2^22
+    static __device__ __forceinline__ float base_of(float top) { return __is_same(T, F16) && !(fabsf(top) < LARGE) ? top : top - BELOW; }
+    static __device__ __forceinline__ float rise_of(float base) { return base + (__is_same(T, F16) && !(fabsf(base) < LARGE) ? 8.f : BELOW + SLACK); }
 
     f32x4 acc[R][GRP * PER];
     f32x4 total[R];  // sums of the probabilities; 16-bit types: of the rounded ones, so that what the rounding does to a row's largest weights cancels
     float m[R];
+    float rise[R];   // the score above which m moves
     u32x4 q[R][KC];
 
     __device__ __forceinline__ void begin() {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            m[r] = -INFINITY;
+            m[r] = rise[r] = -INFINITY;
             total[r] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int d = 0; d < GRP * PER; ++d) acc[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -177,16 +182,17 @@ struct AttentionRows {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) top[r] = fmaxf(top[r], x[r][t][e]);
             top[r] *= scale;
-            grown |= top[r] > m[r] + (BELOW + SLACK);
+            grown |= top[r] > rise[r];
         }
         if (__any(grown)) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                float now = fmaxf(top[r] - BELOW, m[r]);
+                float now = fmaxf(base_of(top[r]), m[r]);
                 now = fmaxf(now, __shfl_xor(now, 16, 64));
                 now = fmaxf(now, __shfl_xor(now, 32, 64));
                 const float shrink = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - now);
                 m[r] = now;
+                rise[r] = rise_of(now);
                 total[r] *= shrink;
 #pragma unroll
                 for (int d = 0; d < GRP * PER; ++d) acc[r][d] *= shrink;

@@ -58,3 +58,41 @@ def test_attention_beside_one_dominating_key(cuda, dtype, dim, heads, keys, gap,
     err = (out[0].double().cpu() - want).abs()
     assert (err <= bound).all(), "off by %g of its bound, %g of the output" % ((err / bound).max(), (err / want).max())
     assert math.isfinite(float(want.sum())) and want.min() > 0
+
+
+@pytest.mark.parametrize("heads", [1, 40, 70])
+@pytest.mark.parametrize("dtype,dim", [(F16, 64), (F16, 128), (F16, 256), (BF16, 128), (F32, 64)], ids=lambda x: str(x)[6:] if isinstance(x, torch.dtype) else str(x))
+def test_attention_of_scores_of_tens_of_millions(cuda, dtype, dim, heads):
+    """Scores so far from 0 that a step of 32 bits is several units: one key is thousands above the others, and its value is the output; where many are within a few steps of
+    one another their weights are anybody's, but they are weights."""
+    from paella_amd import decode
+    g = torch.Generator()
+    g.manual_seed(dim + heads)
+    size, pages = 64, 40
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    for near in (False, True):
+        for top in (300.0, 600.0, 1000.0, 2000.0):
+            k = torch.zeros((pages * size, dim))
+            if near:
+                k[:, 0] = top
+                k[:, 1] = torch.rand((pages * size,), generator=g) * 40.0
+            else:
+                k[:, 0] = top * (0.25 + 0.5 * torch.rand((pages * size,), generator=g))   # below it in every type
+                one = int(torch.randint(0, pages * size - 40, (1,), generator=g))
+                k[one, 0] = top
+            q = torch.zeros((1, heads, dim))
+            q[..., 0], q[..., 1] = 32768.0, 1.0
+            v = torch.rand((pages * size, dim), generator=g) + 0.5
+            k, v, q = k.to(dtype), v.to(dtype), q.to(dtype)
+            cache = decode.KVCache(*(t.view(pages, 1, size, dim).to(cuda) for t in (k, v)))
+            batch = decode.KVBatch(ints(20), ints(pages - 1).view(1, 1), prefix_table=torch.arange(pages - 1, dtype=torch.int32, device=cuda), prefix_len=(pages - 1) * size)
+            for sign in (1.0, -1.0):
+                if sign < 0 and not near:
+                    continue
+                out = decode.PrefixAttention(heads, cache, batch, scale=1.0)((q * sign).to(cuda), cache, batch)[0].cpu()
+                torch.cuda.synchronize()
+                if near:
+                    assert bool(((out >= v.min() * 0.98) & (out <= v.max() * 1.02)).all()), (top, sign)
+                else:
+                    # the sum and the weight that divides it, and the output: a rounding each
+                    assert ((out.double() - v[one].double()).abs() <= v[one].double() * (HALF_STEP[dtype] * 1.01 + 2.0 ** -22)).all(), top
