@@ -262,8 +262,8 @@ class DirectQueue:
 
     def close(self):
         if self.handle:
-            _direct_queues.discard(self.handle)
             check(self.lib.paella_direct_queue_destroy(ctypes.c_void_p(self.handle)), "paella_direct_queue_destroy")
+            _direct_queues.discard(self.handle)  # (behind the wait for its kernels, which memory of dropped plans goes by)
             self.handle = None
 
     def __enter__(self):

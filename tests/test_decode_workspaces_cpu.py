@@ -136,3 +136,16 @@ def test_a_whole_call_is_captured_whatever_the_streams_eager_calls_are_at(world)
     with pytest.raises(AssertionError):
         own.find(HOME, CPU, 1)
     assert own.find(HOME, CPU) is kept
+
+
+def test_a_queue_counts_as_closed_once_it_has_been_waited_for(world):
+    """Closing waits for the queue's kernels: until then, memory that they may use is not let go of."""
+    import types
+    from paella_amd import ops
+    seen = []
+    queue = ops.DirectQueue.__new__(ops.DirectQueue)
+    queue.handle = 8
+    queue.lib = types.SimpleNamespace(paella_direct_queue_destroy=lambda h: seen.append(8 in ops._direct_queues) or 0)
+    ops._direct_queues.add(8)
+    queue.close()
+    assert seen == [True] and 8 not in ops._direct_queues and queue.handle is None
