@@ -262,8 +262,10 @@ class DirectQueue:
 
     def close(self):
         if self.handle:
-            check(self.lib.paella_direct_queue_destroy(ctypes.c_void_p(self.handle)), "paella_direct_queue_destroy")
-            _direct_queues.discard(self.handle)  # (behind the wait for its kernels, which memory of dropped plans goes by)
+            # Until its kernels are done, memory of dropped plans that goes by this set is kept; once the handle is free it may be another queue's.
+            rc = self.lib.paella_direct_queue_wait(ctypes.c_void_p(self.handle))
+            _direct_queues.discard(self.handle)
+            check(self.lib.paella_direct_queue_destroy(ctypes.c_void_p(self.handle)) or rc, "paella_direct_queue_destroy")
             self.handle = None
 
     def __enter__(self):

@@ -145,7 +145,8 @@ def test_a_queue_counts_as_closed_once_it_has_been_waited_for(world):
     seen = []
     queue = ops.DirectQueue.__new__(ops.DirectQueue)
     queue.handle = 8
-    queue.lib = types.SimpleNamespace(paella_direct_queue_destroy=lambda h: seen.append(8 in ops._direct_queues) or 0)
+    queue.lib = types.SimpleNamespace(paella_direct_queue_wait=lambda h: seen.append(("wait", 8 in ops._direct_queues)) or 0,
+                                      paella_direct_queue_destroy=lambda h: seen.append(("destroy", 8 in ops._direct_queues)) or 0)
     ops._direct_queues.add(8)
     queue.close()
-    assert seen == [True] and 8 not in ops._direct_queues and queue.handle is None
+    assert seen == [("wait", True), ("destroy", False)] and queue.handle is None   # (another thread's new queue may have the handle from then on)
