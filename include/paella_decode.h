@@ -72,6 +72,11 @@ int paella_kv_append_dims(const paella_kv_append_desc* desc, const paella_kv_cac
 int paella_kv_append_launch(const paella_kv_append_desc* desc, const paella_kv_cache* cache, const paella_kv_batch* batch, const void* q, const void* k,
                             const void* v, const float* q_weight, const float* k_weight, const float* inv_freq, void* q_out, void* stream,
                             uint32_t job_id, void* notifier);
+/* The same where positions are not places in the cache, as after an eviction (paella_long_cache.h): new token j of sequence b is at position positions[b] + j (device data, [sequences]; NULL:
+ * prefix_len + past[b] + j).  q_out must not overlap positions. */
+int paella_kv_append_at_launch(const paella_kv_append_desc* desc, const paella_kv_cache* cache, const paella_kv_batch* batch, const int32_t* positions, const void* q,
+                               const void* k, const void* v, const float* q_weight, const float* k_weight, const float* inv_freq, void* q_out, void* stream,
+                               uint32_t job_id, void* notifier);
 
 /* ---------------------------------------------------------------- attention over a shared prefix and each sequence's own tokens */
 

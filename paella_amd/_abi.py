@@ -1,4 +1,4 @@
-"""ctypes declarations for the C-ABI in include/paella_hip.h, paella_ops.h and paella_ring.h (paella_models.h and paella_decode.h: _abi_models, _abi_decode)."""
+"""ctypes declarations for the C-ABI in include/paella_hip.h, paella_ops.h and paella_ring.h (paella_models.h, paella_decode.h and paella_long_cache.h: _abi_models, _abi_decode, _abi_long)."""
 import ctypes
 import os
 
@@ -180,9 +180,10 @@ def load(name):
     elif name == "paella_ops":
         _bind(lib, OPS_SYMBOLS)
         _bind(lib, RING_SYMBOLS)
-        from . import _abi_decode, _abi_models
+        from . import _abi_decode, _abi_long, _abi_models
         _abi_models.bind(lib)
         _abi_decode.bind(lib)
+        _abi_long.bind(lib)
     elif name == "paella_probes":
         _bind(lib, PROBE_SYMBOLS)
     _cache[name] = lib

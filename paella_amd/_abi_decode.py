@@ -42,6 +42,7 @@ _TAIL = [c_void_p, c_u32, c_void_p]  # stream, job_id, notifier
 DECODE_SYMBOLS = {
     "paella_kv_append_dims": (c_int, [_p(KvAppendDesc), _p(KvCache), _p(KvBatch), _p(LaunchDims)]),
     "paella_kv_append_launch": (c_int, [_p(KvAppendDesc), _p(KvCache), _p(KvBatch)] + [c_void_p] * 7 + _TAIL),
+    "paella_kv_append_at_launch": (c_int, [_p(KvAppendDesc), _p(KvCache), _p(KvBatch)] + [c_void_p] * 8 + _TAIL),
     "paella_prefix_attention_plan_make": (c_int, [_p(KvCache), _p(KvBatch), c_int, c_float, _p(PrefixAttentionPlan)]),
     "paella_prefix_attention_dims": (c_int, [_p(PrefixAttentionPlan), c_int, _p(LaunchDims)]),
     "paella_prefix_attention_launch_stage": (c_int, [_p(PrefixAttentionPlan), c_int, _p(KvCache), _p(KvBatch), c_void_p, c_i64, c_void_p, c_void_p] + _TAIL),

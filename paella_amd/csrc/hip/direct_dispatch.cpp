@@ -35,6 +35,14 @@ extern const char paella_hsaco_attention_bf16_begin[];
 extern const char paella_hsaco_attention_bf16_end[];
 extern const char paella_hsaco_attention_f16_begin[];
 extern const char paella_hsaco_attention_f16_end[];
+extern const char paella_hsaco_long_cache_begin[];
+extern const char paella_hsaco_long_cache_end[];
+extern const char paella_hsaco_long_f32_begin[];
+extern const char paella_hsaco_long_f32_end[];
+extern const char paella_hsaco_long_bf16_begin[];
+extern const char paella_hsaco_long_bf16_end[];
+extern const char paella_hsaco_long_f16_begin[];
+extern const char paella_hsaco_long_f16_end[];
 }
 
 namespace paella {
@@ -71,6 +79,10 @@ CodeObject g_objects[] = {  // guarded by g_mutex
     {paella_hsaco_attention_f32_begin, paella_hsaco_attention_f32_end, "load attention code object (fp32)", false},
     {paella_hsaco_attention_bf16_begin, paella_hsaco_attention_bf16_end, "load attention code object (bf16)", false},
     {paella_hsaco_attention_f16_begin, paella_hsaco_attention_f16_end, "load attention code object (fp16)", false},
+    {paella_hsaco_long_cache_begin, paella_hsaco_long_cache_end, "load long cache code object", false},
+    {paella_hsaco_long_f32_begin, paella_hsaco_long_f32_end, "load long cache attention code object (fp32)", false},
+    {paella_hsaco_long_bf16_begin, paella_hsaco_long_bf16_end, "load long cache attention code object (bf16)", false},
+    {paella_hsaco_long_f16_begin, paella_hsaco_long_f16_end, "load long cache attention code object (fp16)", false},
 };
 
 std::mutex g_mutex;

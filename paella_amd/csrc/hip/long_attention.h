@@ -1,0 +1,507 @@
+#pragma once
+// Attention over the pages that were picked for a token, and the attention weight that the tokens of a cache gather.  Included by one translation unit per
+// element type.  Operands of the products as in prefix_attention.h: lane l of a wave holds query row l % 16, lane group l / 16 the scores of TPL keys that follow each other.
+
+#include "long_common.h"
+#include "prefix_attention.h"
+
+namespace paella {
+
+// ------------------------------------------------------------------------------------------ attention over picked pages
+// A workgroup per new token, 16 heads of a key head at most, and part of the list.  It turns its part of the list into places of the cache and the tokens that are seen there, in LDS, and
+// then walks the keys as the decoding step's attention walks a sequence's: each wave every fourth step, keys and values straight from memory into registers.
+struct PageAttentionArgs {
+    AttentionArgs c;
+    const int* pages;  // [tokens][kv_heads][count]
+    int count, per;    // entries of a workgroup
+    Divisor tiles, splits, max_new;
+};
+
+constexpr int kListed = 512;  // entries that a workgroup looks up at a time
+
+template <typename T, int D>
+struct ListWalk : NarrowWalk<T, D> {
+    using Narrow = NarrowWalk<T, D>;
+    using Rows = typename Narrow::Rows;
+    static constexpr bool F = Rows::F;
+    static constexpr int TPL = Rows::TPL, STEP = Rows::STEP;
+
+    int off, seen;            // of the step whose keys are loaded next: the lane group's first key in its page, and how many tokens of the page are seen
+
+    // list: (page, tokens seen), n entries
+    __device__ __forceinline__ void find(const Keys& s, const u32x2* list, int n, unsigned b8, bool even, int lane) {
+        auto at = [&](unsigned block) {
+            const Quotient p = divide(block, s.page_blocks);
+            return Keys::Place{p.q, p.r};
+        };
+        auto get = [&](unsigned entry) { return entry < (unsigned)n ? list[entry] : u32x2{0u, 0u}; };
+        const int group = lane >> 4;
+        if (even) {
+            const Keys::Place p = at(__builtin_amdgcn_readfirstlane(b8));
+            const u32x2 e = get(p.entry);
+            this->page_k = this->page_v = (int)e.x;
+            this->in_k = this->in_v = p.in;
+            seen = (int)e.y;
+            off = (int)p.in * 8 + group * TPL;
+        } else {
+            constexpr int BLOCK_LANES_K = F ? 8 : 4;
+            const Keys::Place k = at(b8 + (unsigned)(lane & 15) / BLOCK_LANES_K), v = at(b8 + (unsigned)group * TPL / 8);
+            const u32x2 ek = get(k.entry), ev = get(v.entry);
+            this->page_k = (int)ek.x;
+            this->page_v = (int)ev.x;
+            this->in_k = k.in;
+            this->in_v = v.in;
+            seen = (int)ev.y;
+            off = (int)v.in * 8 + (F ? (group & 1) * 4 : 0);
+        }
+    }
+
+    template <typename Next>
+    __device__ __forceinline__ void step(Rows& rows, int off, int seen, float scale, Next next) {
+        f32x4 x[1][Rows::NT];
+        rows.scores(x, [&](int t, int c) { return this->k[t][c]; });
+        next(true);
+        if (__any(off + TPL > seen)) {
+            const int limit[1] = {seen};
+            Rows::mask(x, off, false, limit);
+#pragma unroll
+            for (int u = 0; u < TPL; ++u)  // what lies in places that no row may see can be anything
+                if (off + u >= seen) {
+#pragma unroll
+                    for (int w = 0; w < Rows::GRP * Rows::VW; ++w) this->v[u][w] = 0;
+                }
+        }
+        unsigned p[1][4];
+        rows.weigh(x, scale, p);
+        rows.add_values(this->v, p);
+        next(false);
+    }
+
+    // Steps wave, wave + 4, ... of the list's n entries.
+    __device__ __forceinline__ void walk_list(Rows& rows, const Keys& s, const u32x2* list, int n, float scale, int wave, int lane) {
+        const int end = (n * (int)s.page_blocks.d + STEP / 8 - 1) / (STEP / 8);
+        int at = wave;
+        if (at >= end) return;
+        const bool even = s.page_blocks.d % (STEP / 8) == 0;
+        find(s, list, n, (unsigned)at * (STEP / 8), even, lane);
+        this->load_k(s, even, lane);
+        this->load_v(s, even, lane);
+        int here = off, held = seen;
+        find(s, list, n, (unsigned)(at + 4) * (STEP / 8), even, lane);
+        for (; at + 4 < end; at += 4) {
+            step(rows, here, held, scale, [&](bool k_is_free) {
+                if (k_is_free) {
+                    this->load_k(s, even, lane);
+                } else {
+                    this->load_v(s, even, lane);
+                    here = off;
+                    held = seen;
+                    find(s, list, n, (unsigned)(at + 8) * (STEP / 8), even, lane);
+                }
+            });
+        }
+        step(rows, here, held, scale, [](bool) {});
+    }
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void page_attention_kernel(PageAttentionArgs p) {
+    const AttentionArgs& a = p.c;
+    hook_entry(a.notifier, a.job_id);
+    using Fm = Form<1, false>;
+    __shared__ __attribute__((aligned(16))) char lds[attention_lds<T, D, Fm>()];
+    __shared__ u32x2 list[kListed];
+    __shared__ int row_id[16], done[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int head_bytes = D * T::bytes;
+    const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, p.splits), by_tile = divide(by_split.q, p.tiles);
+    const int h = (int)by_head.r, split = (int)by_split.r, tile = (int)by_tile.r, t = (int)by_tile.q, per_kv = (int)a.per_kv.d;
+    int seq, j;
+    if (row_owner(a.starts, a.sequences, p.max_new, t, lane, &seq, &j)) {
+        const int64_t places = (int64_t)a.max_pages * a.page_size;
+        const int visible = (int)min((int64_t)max(__builtin_amdgcn_readfirstlane(a.past[seq]), 0) + j + 1, places);  // own tokens
+        const int* const table = a.tables + (size_t)seq * a.max_pages;
+        const int* const entries = p.pages + ((size_t)t * a.kv_heads.d + h) * p.count;
+        const int first_row = tile * 16;
+        if (threadIdx.x < 16) row_id[threadIdx.x] = first_row + (int)threadIdx.x < per_kv ? t * a.heads + h * per_kv + first_row + (int)threadIdx.x : -1;
+        Keys s;
+        s.page_bytes = (size_t)a.kv_heads.d * a.page_size * head_bytes;
+        s.page_blocks = a.page_blocks;
+        s.num_pages = (unsigned)a.num_pages;
+        s.k = a.k_cache + (size_t)h * a.page_size * head_bytes;
+        s.v = a.v_cache + (size_t)h * a.page_size * head_bytes;
+        AttentionRows<T, D, 1, false> rows;
+        rows.begin();
+        rows.load_q(0, a.q + t * a.q_stride + (size_t)(h * per_kv + min(first_row + (lane & 15), per_kv - 1)) * head_bytes, lane);
+        const int end = min((split + 1) * p.per, p.count);
+        for (int first = split * p.per; first < end; first += kListed) {
+            const int n = min(end - first, kListed);
+            __syncthreads();
+            for (int i = threadIdx.x; i < n; i += 256) {
+                const int e = entries[first + i], o = e - a.prefix_pages;
+                int page = 0, seen = 0;
+                if (e >= 0 && o < 0) {
+                    page = a.prefix_table[e];
+                    seen = a.prefix_len - e * a.page_size;
+                } else if (e >= 0 && o < a.max_pages) {
+                    page = table[o];
+                    seen = visible - o * a.page_size;
+                }
+                if ((unsigned)page >= (unsigned)a.num_pages) seen = 0;
+                list[i] = u32x2{(unsigned)page, (unsigned)max(min(seen, a.page_size), 0)};
+            }
+            __syncthreads();
+            ListWalk<T, D> keys;
+            keys.walk_list(rows, s, list, n, a.scale_log2, __builtin_amdgcn_readfirstlane(wave), lane);
+        }
+        leave<T, D, Fm>(a, rows, split, row_id, lds);
+        if (a.counters) join_last<T, D, 16>(a, row_id, (unsigned)(((size_t)t * p.tiles.d + tile) * a.kv_heads.d + h) * 32, min(per_kv - first_row, 16), done);
+    }
+    hook_exit(a.notifier, a.job_id);
+}
+
+using PageAttentionKernel = void (*)(PageAttentionArgs);
+
+template <typename T>
+PageAttentionKernel page_attention_kernel_of(int dim) {
+    return dim == 64 ? page_attention_kernel<T, 64> : dim == 128 ? page_attention_kernel<T, 128> : dim == 256 ? page_attention_kernel<T, 256> : nullptr;
+}
+
+// ------------------------------------------------------------------------------------------ the weight that tokens gather
+// weights[i] += sum over rows r of exp2(x_ri - m_r) / l_r, x = scale q . k in powers of two.  A first launch leaves each row's maximum and sum over its part of the keys, a second one
+// puts the parts together and adds the rows' weights up, key by key.  A wave has a step's keys in registers and takes the rows through, 16 at a time, from LDS.
+struct WeighArgs {
+    const char *q, *k_cache;
+    float* weights;
+    const int *starts, *past, *tables, *prefix_table;
+    int64_t q_stride;  // bytes
+    int sequences, max_new, tokens, max_pages, prefix_len, prefix_pages, num_pages, page_size, heads;
+    Divisor kv_heads, per_kv, page_blocks, splits, own_splits, chunks;  // chunks: of a sequence's rows
+    float scale_log2;
+    f32x2* ml;         // [splits][tokens * heads]: maximum and sum of each part
+    uint32_t job_id;
+    Notifier* notifier;
+};
+
+// Rows that a workgroup has in LDS: 32 KB of queries.
+template <typename T, int D>
+constexpr int weigh_tiles() { return 32768 / (16 * D * T::bytes) > 8 ? 8 : 32768 / (16 * D * T::bytes); }
+
+// The keys of one key head, step by step: the prefix's pages, then the sequence's own.  Places count along those pages, the prefix's last one to its end.
+template <typename T, int D>
+struct KeyWalk {
+    using Rows = AttentionRows<T, D, 1, false>;
+    static constexpr bool F = Rows::F;
+    static constexpr int ROW = Rows::ROW, TPL = Rows::TPL, STEP = Rows::STEP, NT = Rows::NT, KC = Rows::KC;
+
+    const int *prefix, *own;
+    unsigned prefix_pages, all_pages, num_pages;
+    const char* k;
+    size_t page_bytes;
+    Divisor page_blocks;
+
+    u32x4 keys[NT][KC];
+    int page;      // of the lane's key of K, and of the lane group's scores
+    int page_s;
+    unsigned in;
+
+    __device__ __forceinline__ int page_of(unsigned entry) const {
+        const unsigned e = min(entry, all_pages - 1);
+        return e < prefix_pages ? prefix[e] : own[e - prefix_pages];
+    }
+
+    __device__ __forceinline__ void find(unsigned b8, bool even, int lane) {
+        if (even) {
+            const Quotient at = divide(__builtin_amdgcn_readfirstlane(b8), page_blocks);
+            page = page_s = page_of(at.q);
+            in = at.r;
+        } else {
+            const Quotient k_at = divide(b8 + (unsigned)(lane & 15) / (F ? 8 : 4), page_blocks), s_at = divide(b8 + (unsigned)(lane >> 4) * TPL / 8, page_blocks);
+            page = page_of(k_at.q);
+            page_s = page_of(s_at.q);
+            in = k_at.r;
+        }
+    }
+
+    __device__ __forceinline__ void load(u32x4 (&to)[NT][KC], bool even, int lane) const {
+        const int mm = lane & 15;
+        const unsigned row = F ? (even ? mm : mm & 7) : (even ? (mm >> 2) * 8 + (mm & 3) : mm & 3);
+        const char* p;
+        if (even) {
+            const int at = __builtin_amdgcn_readfirstlane(page);
+            p = k + ((unsigned)at < num_pages ? (unsigned)at : 0u) * page_bytes + __builtin_amdgcn_readfirstlane(in) * 8 * ROW + (row * ROW + (lane >> 4) * 16);
+        } else {
+            p = k + ((unsigned)page < num_pages ? (unsigned)page : 0u) * page_bytes + (size_t)((in * 8 + row) * ROW + (lane >> 4) * 16);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < KC; ++c) to[t][c] = *reinterpret_cast<const u32x4*>(p + t * 4 * ROW + c * 64);
+    }
+
+    // x = K q^T for 16 rows, whose pieces lie in LDS in the order of the lanes
+    __device__ __forceinline__ void scores(f32x4 (&x)[NT], const u32x4* q, int lane) const {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) x[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const u32x4 piece = q[c * 64 + lane];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if constexpr (F) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[t] = mfma_f32(as_float(keys[t][c][e]), as_float(piece[e]), x[t]);
+                } else {
+                    x[t] = Mfma<T>::go(keys[t][c], piece, x[t]);
+                }
+            }
+        }
+    }
+};
+
+template <typename T, int D>
+__device__ __forceinline__ KeyWalk<T, D> key_walk(const WeighArgs& a, int seq, int h) {
+    KeyWalk<T, D> k;
+    k.prefix = a.prefix_table;
+    k.own = a.tables + (size_t)seq * a.max_pages;
+    k.prefix_pages = (unsigned)a.prefix_pages;
+    k.all_pages = (unsigned)(a.prefix_pages + a.max_pages);
+    k.num_pages = (unsigned)a.num_pages;
+    k.page_bytes = (size_t)a.kv_heads.d * a.page_size * D * T::bytes;
+    k.k = a.k_cache + (size_t)h * a.page_size * D * T::bytes;
+    k.page_blocks = a.page_blocks;
+    return k;
+}
+
+// Queries of the rows from `first` on to LDS, piece by piece as the lanes want them; behind the sequence's last row the last one again.
+template <typename T, int D, int TILES>
+__device__ __forceinline__ void stage_queries(const WeighArgs& a, int token, int h, int first, int rows, u32x4* to) {
+    constexpr int KC = D * T::bytes / 64;
+    for (int i = threadIdx.x; i < TILES * KC * 64; i += 256) {
+        const int lane = i & 63, c = i / 64 % KC, tile = i / 64 / KC;
+        if (first + tile * 16 >= rows) break;
+        const Quotient at = divide((unsigned)min(first + tile * 16 + (lane & 15), rows - 1), a.per_kv);
+        to[i] = *reinterpret_cast<const u32x4*>(a.q + (token + (int)at.q) * a.q_stride + (size_t)(h * (int)a.per_kv.d + (int)at.r) * D * T::bytes + c * 64 + (lane >> 4) * 16);
+    }
+}
+
+// Steps over the keys [begin, end) of `walk`, every fourth one for each wave.  each(x, tile): scores of a tile, those of keys that a row does not see
+// -inf; close(first): behind a step's last tile.
+template <typename T, int D, int TILES, typename Each, typename Close>
+__device__ __forceinline__ void walk_keys(const WeighArgs& a, KeyWalk<T, D>& walk, const u32x4* q, int first_row, int rows, int past, int begin, int end, int wave, int lane, Each each,
+                                          Close close) {
+    using Walk = KeyWalk<T, D>;
+    int at = begin + wave;
+    if (at >= end) return;
+    const bool even = a.page_blocks.d % (Walk::STEP / 8) == 0;
+    const int behind = a.prefix_pages * a.page_size;  // the first own token's place
+    const int places = min(a.max_pages * a.page_size, 1 << 30);
+    const int least = behind + min(past + (int)divide((unsigned)first_row, a.per_kv).q + 1, places);  // the first place that some row does not see
+    walk.find((unsigned)at * (Walk::STEP / 8), even, lane);
+    walk.load(walk.keys, even, lane);
+    bool absent = (unsigned)walk.page_s >= walk.num_pages;
+    if (at + 4 < end) walk.find((unsigned)(at + 4) * (Walk::STEP / 8), even, lane);
+    for (; at < end; at += 4) {
+        u32x4 next[Walk::NT][Walk::KC];
+        const bool more = at + 4 < end;
+        if (more) walk.load(next, even, lane);
+        const int first = at * Walk::STEP, mine = first + (lane >> 4) * Walk::TPL;
+        const bool whole = (first + Walk::STEP <= a.prefix_len || (first >= behind && first + Walk::STEP <= least)) && !__any(absent);
+#pragma unroll
+        for (int tile = 0; tile < TILES; ++tile) {
+            if (first_row + tile * 16 >= rows) break;
+            f32x4 x[Walk::NT];
+            walk.scores(x, q + tile * Walk::KC * 64, lane);
+            if (!whole) {
+                const int row = min(first_row + tile * 16 + (lane & 15), rows - 1);
+                const int limit = mine < behind ? a.prefix_len : behind + min(past + (int)divide((unsigned)row, a.per_kv).q + 1, places);
+#pragma unroll
+                for (int t = 0; t < Walk::NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (absent || mine + t * 4 + e >= limit) x[t][e] = -INFINITY;
+            }
+            each(x, tile);
+        }
+        close(first);
+        if (more) {
+#pragma unroll
+            for (int t = 0; t < Walk::NT; ++t)
+#pragma unroll
+                for (int c = 0; c < Walk::KC; ++c) walk.keys[t][c] = next[t][c];
+            absent = (unsigned)walk.page_s >= walk.num_pages;
+            if (at + 8 < end) walk.find((unsigned)(at + 8) * (Walk::STEP / 8), even, lane);
+        }
+    }
+}
+
+template <typename T, int D, int TILES>
+__global__ __launch_bounds__(256) void key_sums_kernel(WeighArgs a) {
+    hook_entry(a.notifier, a.job_id);
+    using Walk = KeyWalk<T, D>;
+    __shared__ u32x4 q[TILES * Walk::KC * 64];
+    __shared__ f32x2 sums[4][TILES * 16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, a.splits), by_chunk = divide(by_split.q, a.chunks);
+    const int h = (int)by_head.r, split = (int)by_split.r, seq = (int)by_chunk.q, first_row = (int)by_chunk.r * TILES * 16;
+    const NewTokens its = new_tokens(a.starts, a.past, seq, a.max_new, a.tokens);
+    const int rows = its.count * (int)a.per_kv.d;
+    if (first_row < rows) {
+        stage_queries<T, D, TILES>(a, its.first, h, first_row, rows, q);
+        float m[TILES], l[TILES];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+        }
+        __syncthreads();
+        const int last_row = min(first_row + TILES * 16, rows) - 1;
+        const int places = min(a.max_pages * a.page_size, 1 << 30), past = min(its.past, places);
+        const int keys = a.prefix_pages * a.page_size + min(past + (int)divide((unsigned)last_row, a.per_kv).q + 1, places);
+        const int steps = (keys + Walk::STEP - 1) / Walk::STEP, per = (int)divide((unsigned)steps + a.splits.d - 1, a.splits).q;
+        const int begin = min(split * per, steps), end = min(begin + per, steps);
+        Walk walk = key_walk<T, D>(a, seq, h);
+        walk_keys<T, D, TILES>(
+            a, walk, q, first_row, rows, past, begin, end, wave, lane,
+            [&](const f32x4 (&x)[Walk::NT], int tile) {
+                float top = x[0][0];
+#pragma unroll
+                for (int t = 0; t < Walk::NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = fmaxf(top, x[t][e]);
+                const float now = fmaxf(m[tile], top * a.scale_log2), base = now == -INFINITY ? 0.f : now;
+                l[tile] *= m[tile] == now ? 1.f : __builtin_amdgcn_exp2f(m[tile] - now);
+                m[tile] = now;
+#pragma unroll
+                for (int t = 0; t < Walk::NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) l[tile] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][e], a.scale_log2, -base));
+            },
+            [](int) {});
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+#pragma unroll
+            for (int off = 16; off < 64; off <<= 1) {
+                const float other = __shfl_xor(m[i], off, 64), more = __shfl_xor(l[i], off, 64), now = fmaxf(m[i], other);
+                l[i] = l[i] * (m[i] == now ? 1.f : __builtin_amdgcn_exp2f(m[i] - now)) + more * (other == now ? 1.f : __builtin_amdgcn_exp2f(other - now));
+                m[i] = now;
+            }
+            if (lane < 16) sums[wave][i * 16 + lane] = f32x2{m[i], l[i]};
+        }
+        __syncthreads();
+        const int row = first_row + (int)threadIdx.x;
+        if ((int)threadIdx.x < TILES * 16 && row < rows) {
+            float top = -INFINITY, total = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = fmaxf(top, sums[w][threadIdx.x].x);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const f32x2 s = sums[w][threadIdx.x];
+                total += s.y * (s.x == top ? 1.f : __builtin_amdgcn_exp2f(s.x - top));
+            }
+            const Quotient at = divide((unsigned)row, a.per_kv);
+            const size_t id = (size_t)split * a.tokens * a.heads + (size_t)(its.first + (int)at.q) * a.heads + h * (int)a.per_kv.d + (int)at.r;
+            put_pair(a.ml + id, top, total);
+        }
+    }
+    hook_exit(a.notifier, a.job_id);
+}
+
+template <typename T, int D, int TILES>
+__global__ __launch_bounds__(256) void key_weights_kernel(WeighArgs a) {
+    hook_entry(a.notifier, a.job_id);
+    using Walk = KeyWalk<T, D>;
+    __shared__ u32x4 q[TILES * Walk::KC * 64];
+    __shared__ f32x2 whole[TILES * 16];  // of each row: maximum and one over the sum
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, a.own_splits);
+    const int h = (int)by_head.r, split = (int)by_split.r, seq = (int)by_split.q;
+    const NewTokens its = new_tokens(a.starts, a.past, seq, a.max_new, a.tokens);
+    const int rows = its.count * (int)a.per_kv.d;
+    if (rows > 0) {
+        const int places = min(a.max_pages * a.page_size, 1 << 30), past = min(its.past, places), held = min(past + its.count, places);
+        const int before = a.prefix_pages * a.page_size / Walk::STEP, steps = (a.prefix_pages * a.page_size + held + Walk::STEP - 1) / Walk::STEP - before;
+        const int per = (int)divide((unsigned)steps + a.own_splits.d - 1, a.own_splits).q;
+        const int begin = before + min(split * per, steps), end = min(begin + per, before + steps);
+        float* const weights = a.weights + ((size_t)seq * a.kv_heads.d + h) * ((size_t)a.max_pages * a.page_size);
+        Walk walk = key_walk<T, D>(a, seq, h);
+        for (int first_row = 0; first_row < rows && begin < end; first_row += TILES * 16) {
+            __syncthreads();
+            stage_queries<T, D, TILES>(a, its.first, h, first_row, rows, q);
+            if ((int)threadIdx.x < TILES * 16) {
+                const int row = first_row + (int)threadIdx.x;
+                float top = -INFINITY, total = 0.f;
+                if (row < rows) {
+                    const Quotient at = divide((unsigned)row, a.per_kv);
+                    const f32x2* from = a.ml + (size_t)(its.first + (int)at.q) * a.heads + h * (int)a.per_kv.d + (int)at.r;
+                    for (unsigned s = 0; s < a.splits.d; ++s, from += (size_t)a.tokens * a.heads) {
+                        const f32x2 part = *from;
+                        const float now = fmaxf(top, part.x);
+                        total = total * (top == now ? 1.f : __builtin_amdgcn_exp2f(top - now)) + part.y * (part.x == now ? 1.f : __builtin_amdgcn_exp2f(part.x - now));
+                        top = now;
+                    }
+                }
+                // a row behind the last one, or one that sees nothing, has no weights
+                whole[threadIdx.x] = total == 0.f ? f32x2{INFINITY, 0.f} : f32x2{top, 1.f / total};
+            }
+            __syncthreads();
+            float w[Walk::TPL];
+#pragma unroll
+            for (int e = 0; e < Walk::TPL; ++e) w[e] = 0.f;
+            walk_keys<T, D, TILES>(
+                a, walk, q, first_row, rows, past, begin, end, wave, lane,
+                [&](const f32x4 (&x)[Walk::NT], int tile) {
+                    const f32x2 row = whole[tile * 16 + (lane & 15)];
+#pragma unroll
+                    for (int t = 0; t < Walk::NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[t * 4 + e] += row.y * __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][e], a.scale_log2, -row.x));
+                },
+                [&](int first) {
+                    float mine = 0.f;
+#pragma unroll
+                    for (int e = 0; e < Walk::TPL; ++e) {
+                        const float sum = row_all(w[e], [](float x, float y) { return x + y; });
+                        if ((lane & 15) == e) mine = sum;
+                        w[e] = 0.f;
+                    }
+                    const int i = first + (lane >> 4) * Walk::TPL + (lane & 15) - a.prefix_pages * a.page_size;
+                    if ((lane & 15) < Walk::TPL && i >= 0 && i < held) {
+                        const float old = first_row || i < past ? __hip_atomic_load(weights + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.f;
+                        store_out(weights + i, old + mine);
+                    }
+                });
+        }
+    }
+    hook_exit(a.notifier, a.job_id);
+}
+
+using WeighKernel = void (*)(WeighArgs);
+
+// few: at most 16 rows a sequence and key head
+template <typename T, int D>
+WeighKernel key_sums_kernel_of(bool few) { return few ? key_sums_kernel<T, D, 1> : key_sums_kernel<T, D, weigh_tiles<T, D>()>; }
+template <typename T, int D>
+WeighKernel key_weights_kernel_of(bool few) { return few ? key_weights_kernel<T, D, 1> : key_weights_kernel<T, D, weigh_tiles<T, D>()>; }
+
+template <typename T>
+WeighKernel key_sums(int dim, bool few) {
+    return dim == 64 ? key_sums_kernel_of<T, 64>(few) : dim == 128 ? key_sums_kernel_of<T, 128>(few) : key_sums_kernel_of<T, 256>(few);
+}
+template <typename T>
+WeighKernel key_weights(int dim, bool few) {
+    return dim == 64 ? key_weights_kernel_of<T, 64>(few) : dim == 128 ? key_weights_kernel_of<T, 128>(few) : key_weights_kernel_of<T, 256>(few);
+}
+
+// Defined once per type.
+PageAttentionKernel page_attention_f32(int dim);
+PageAttentionKernel page_attention_bf16(int dim);
+PageAttentionKernel page_attention_f16(int dim);
+WeighKernel key_sums_f32(int dim, bool few);
+WeighKernel key_sums_bf16(int dim, bool few);
+WeighKernel key_sums_f16(int dim, bool few);
+WeighKernel key_weights_f32(int dim, bool few);
+WeighKernel key_weights_bf16(int dim, bool few);
+WeighKernel key_weights_f16(int dim, bool few);
+
+}  // namespace paella

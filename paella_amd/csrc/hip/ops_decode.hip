@@ -23,7 +23,7 @@ struct AppendArgs {
     const char *q, *k, *v;
     char *q_out, *k_cache, *v_cache;
     const float *q_weight, *k_weight, *inv_freq;
-    const int *starts, *past, *tables;
+    const int *starts, *past, *tables, *positions;
     int64_t q_stride, k_stride, v_stride;  // bytes
     int sequences, max_pages, prefix_len;
     Divisor max_new, page_size;
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
         };
         fetch(0);
         // Trips to memory that do not wait for one another go out together: heads, length, weights and frequencies, then the page.
-        const int past = a.past[seq];
+        const int past = a.past[seq], position = a.positions ? a.positions[seq] : 0;
         float wq[2], wk[2], freq = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
         // The angle in revolutions, reduced to half a turn in 64 bits: in 32 bits a position of 100000 would be off by 0.006 radians.  Each pair once per
         // token, by one lane.
         if ((int)threadIdx.x < a.rotary / 2) {
-            const double turns = ((double)a.prefix_len + (double)own) * (double)freq * 0.15915494309189533577;
+            const double turns = (a.positions ? (double)position + (double)j : (double)a.prefix_len + (double)own) * (double)freq * 0.15915494309189533577;
             float s, c;
             sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
             turn[threadIdx.x] = f32x2{c, s};
@@ -780,6 +780,12 @@ int paella_kv_append_dims(const paella_kv_append_desc* desc, const paella_kv_cac
 int paella_kv_append_launch(const paella_kv_append_desc* d, const paella_kv_cache* c, const paella_kv_batch* b, const void* q, const void* k, const void* v,
                             const float* q_weight, const float* k_weight, const float* inv_freq, void* q_out, void* stream, uint32_t job_id,
                             void* notifier) {
+    return paella_kv_append_at_launch(d, c, b, nullptr, q, k, v, q_weight, k_weight, inv_freq, q_out, stream, job_id, notifier);
+}
+
+int paella_kv_append_at_launch(const paella_kv_append_desc* d, const paella_kv_cache* c, const paella_kv_batch* b, const int32_t* positions, const void* q, const void* k,
+                               const void* v, const float* q_weight, const float* k_weight, const float* inv_freq, void* q_out, void* stream,
+                               uint32_t job_id, void* notifier) {
     if (int rc = append_check(d, c, b)) return rc;
     if (!cache_ok(c) || !batch_ok(b) || !k || !v || (d->heads > 0) != (q != nullptr) || (d->heads > 0) != (q_out != nullptr)) return PAELLA_EINVAL;
     if (d->rotary_dim && !inv_freq) return PAELLA_EINVAL;
@@ -793,13 +799,14 @@ int paella_kv_append_launch(const paella_kv_append_desc* d, const paella_kv_cach
     // other tokens' workgroups may still read keys and values
     const double out_bytes = (double)b->tokens * q_row * size;
     if (d->heads && (rows_overlap(k, b->tokens, d->k_stride * size, kv_row * size, q_out, out_bytes) || over_cache(c, q_out, out_bytes) ||
-                     rows_overlap(v, b->tokens, d->v_stride * size, kv_row * size, q_out, out_bytes)))
+                     rows_overlap(v, b->tokens, d->v_stride * size, kv_row * size, q_out, out_bytes) ||
+                     (positions && overlap(positions, 4.0 * b->sequences, q_out, out_bytes))))
         return PAELLA_EINVAL;
     AppendArgs a;
     a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v;
     a.q_out = (char*)q_out; a.k_cache = (char*)c->k; a.v_cache = (char*)c->v;
     a.q_weight = q_weight; a.k_weight = k_weight; a.inv_freq = inv_freq;
-    a.starts = b->starts; a.past = b->past; a.tables = b->tables;
+    a.starts = b->starts; a.past = b->past; a.tables = b->tables; a.positions = positions;
     a.q_stride = d->q_stride * size; a.k_stride = d->k_stride * size; a.v_stride = d->v_stride * size;
     a.sequences = b->sequences; a.max_pages = b->max_pages; a.prefix_len = b->prefix_len;
     a.max_new = divisor((unsigned)b->max_new); a.page_size = divisor((unsigned)c->page_size);

@@ -1,0 +1,216 @@
+// Attention over picked pages and the attention weight that tokens gather: planning and launch (the kernels: long_attention.h).
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "long_attention.h"
+
+namespace {
+
+using namespace paella;
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+bool scale_ok(float scale) { return scale >= 0.f && scale < INFINITY; }
+bool dim_ok(int dim) { return dim == 64 || dim == 128 || dim == 256; }
+
+// ------------------------------------------------------------------------------------------ attention over picked pages
+
+using PagePlan = paella_page_attention_plan;
+
+PageAttentionKernel kernel_of(const PagePlan* p) {
+    return p->dtype == PAELLA_F32 ? page_attention_f32(p->head_dim) : p->dtype == PAELLA_BF16 ? page_attention_bf16(p->head_dim) : page_attention_f16(p->head_dim);
+}
+AttentionKernel join_of(const PagePlan* p) {
+    return p->dtype == PAELLA_F32 ? attention_join_f32(p->head_dim) : p->dtype == PAELLA_BF16 ? attention_join_bf16(p->head_dim) : attention_join_f16(p->head_dim);
+}
+
+int64_t tiles_of(const PagePlan* p) { return ceil_div(p->heads / p->kv_heads, 16); }
+int64_t grid_of(const PagePlan* p) { return p->tokens * tiles_of(p) * p->kv_heads * p->splits; }
+
+bool plan_ok(const PagePlan* p) {
+    return p && planned_extents_ok(p) && dim_ok(p->head_dim) && p->count > 0 && p->count < 1 << 24 && p->scale > 0.f && scale_ok(p->scale) && p->splits > 0 && p->splits <= 64 &&
+           (double)p->tokens * tiles_of(p) * p->kv_heads * p->splits <= kMostWorkgroups && (double)p->tokens * p->kv_heads * p->count < 2147483648.0;
+}
+
+// As in the decoding step's attention: the workgroup that arrives last joins a row's parts where its lanes have all outputs at once and request all parts together.
+int stages_of(const PagePlan* p) {
+    if (p->splits == 1) return 1;
+    return std::min<int64_t>(16, p->heads / p->kv_heads) * p->head_dim / 4 <= 256 && p->splits <= kJoined ? 1 : 2;
+}
+
+size_t counters_of(const PagePlan* p) { return stages_of(p) == 1 ? up256((size_t)p->tokens * tiles_of(p) * p->kv_heads * 32 * 4) : 0; }
+size_t workspace_of(const PagePlan* p) {
+    const size_t parts = p->splits, rows = (size_t)p->tokens * p->heads;
+    return parts == 1 ? 0 : counters_of(p) + up256(parts * rows * 8) + parts * rows * p->head_dim * 4;
+}
+
+// ------------------------------------------------------------------------------------------ the weight that tokens gather
+
+using WeighPlan = paella_key_weights_plan;
+
+bool few_rows(const WeighPlan* p) { return (int64_t)std::min(p->max_new, p->tokens) * (p->heads / p->kv_heads) <= 16; }
+int chunk_rows(const WeighPlan* p) {
+    if (few_rows(p)) return 16;
+    return 16 * std::min(8, 32768 / (16 * p->head_dim * element_bytes(p->dtype)));
+}
+int64_t chunks_of(const WeighPlan* p) { return ceil_div((int64_t)std::min(p->max_new, p->tokens) * (p->heads / p->kv_heads), chunk_rows(p)); }
+
+WeighKernel kernel_of(const WeighPlan* p, int stage) {
+    const bool few = few_rows(p);
+    const int d = p->head_dim;
+    if (stage) return p->dtype == PAELLA_F32 ? key_weights_f32(d, few) : p->dtype == PAELLA_BF16 ? key_weights_bf16(d, few) : key_weights_f16(d, few);
+    return p->dtype == PAELLA_F32 ? key_sums_f32(d, few) : p->dtype == PAELLA_BF16 ? key_sums_bf16(d, few) : key_sums_f16(d, few);
+}
+
+int64_t grid_of(const WeighPlan* p, int stage) { return stage ? (int64_t)p->sequences * p->kv_heads * p->own_splits : p->sequences * chunks_of(p) * p->kv_heads * p->splits; }
+
+bool plan_ok(const WeighPlan* p) {
+    return p && planned_extents_ok(p) && dim_ok(p->head_dim) && p->scale > 0.f && scale_ok(p->scale) && p->splits > 0 && p->splits <= 64 && p->own_splits > 0 &&
+           (double)p->prefix_len + (double)p->max_pages * p->page_size < 1073741824.0 - 1048576.0 && p->page_size <= 1 << 20 &&
+           (double)p->sequences * chunks_of(p) * p->kv_heads * p->splits <= kMostWorkgroups && (double)p->sequences * p->kv_heads * p->own_splits <= kMostWorkgroups;
+}
+
+size_t workspace_of(const WeighPlan* p) { return (size_t)p->splits * p->tokens * p->heads * 8; }
+
+}  // namespace
+
+extern "C" {
+
+int paella_page_attention_plan_make(const paella_kv_cache* c, const paella_kv_batch* b, int heads, int count, float scale, paella_page_attention_plan* p) {
+    if (!p || !cache_extents_ok(c) || !batch_extents_ok(b) || heads <= 0 || heads % c->kv_heads || count <= 0 || !scale_ok(scale)) return PAELLA_EINVAL;
+    *p = paella_page_attention_plan{};
+    plan_extents(p, c, b, heads);
+    p->count = count;
+    p->scale = scale > 0.f ? scale : 1.f / std::sqrt((float)c->head_dim);
+    p->splits = 1;
+    if (!plan_ok(p)) return PAELLA_ENOSUP;
+    const int64_t undivided = grid_of(p), keys = (int64_t)count * c->page_size;
+    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(undivided < 128 ? 768 : 2048, undivided), ceil_div(keys, 256), (int64_t)count, 64}));
+    if (!plan_ok(p)) return PAELLA_ENOSUP;
+    p->stages = stages_of(p);
+    p->workspace_bytes = workspace_of(p);
+    set_launch_dims(&p->dims, (unsigned)grid_of(p), 256, 0, 256);
+    const double size = element_bytes(c->dtype), rows = (double)p->tokens * p->kv_heads;
+    p->flops = 4.0 * p->head_dim * p->tokens * heads * (double)keys;
+    p->bytes = 2.0 * rows * keys * p->head_dim * size + 2.0 * p->tokens * heads * p->head_dim * size + 4.0 * rows * count;
+    return 0;
+}
+
+int paella_page_attention_dims(const paella_page_attention_plan* p, int stage, paella_launch_dims* dims) {
+    if (!plan_ok(p) || !dims || stage < 0 || stage >= stages_of(p)) return PAELLA_EINVAL;
+    if (stage) set_launch_dims(dims, (unsigned)ceil_div((int64_t)p->tokens * p->heads, kJoinRows / p->head_dim), 256, 0, 64);
+    else set_launch_dims(dims, (unsigned)grid_of(p), 256, 0, 256);
+    loaded_dims(stage ? (const void*)join_of(p) : (const void*)kernel_of(p), dims);
+    return 0;
+}
+
+int paella_page_attention_launch_stage(const paella_page_attention_plan* p, int stage, const paella_kv_cache* c, const paella_kv_batch* b, const void* q, int64_t q_stride,
+                                       const int32_t* pages, void* out, void* workspace, void* stream, uint32_t job_id, void* notifier) {
+    if (!plan_ok(p) || stage < 0 || stage >= stages_of(p) || !planned_for(p, c, b) || !q || !pages || !out || ((uintptr_t)pages & 3)) return PAELLA_EINVAL;
+    const int64_t size = element_bytes(c->dtype), row = (int64_t)p->heads * c->head_dim;
+    if (q_stride < row || q_stride % 8 || (((uintptr_t)q | (uintptr_t)out) & 15)) return PAELLA_EINVAL;
+    const size_t need = workspace_of(p);
+    if (need && (!workspace || ((uintptr_t)workspace & 15))) return PAELLA_EINVAL;
+    const double out_bytes = (double)b->tokens * row * size, list_bytes = 4.0 * p->tokens * p->kv_heads * p->count;
+    const struct { const void* at; double bytes; } outs[2] = {{out, out_bytes}, {workspace, (double)need}};
+    for (const auto& o : outs)
+        if (o.bytes > 0 && (rows_overlap(q, p->tokens, q_stride * size, row * size, o.at, o.bytes) || overlap(pages, list_bytes, o.at, o.bytes) || over_cache(c, o.at, o.bytes) ||
+                            over_batch(b, c->page_size, o.at, o.bytes)))
+            return PAELLA_EINVAL;
+    if (need && overlap(out, out_bytes, workspace, (double)need)) return PAELLA_EINVAL;
+    PageAttentionArgs a{};
+    a.c.q = (const char*)q; a.c.k_cache = (const char*)c->k; a.c.v_cache = (const char*)c->v; a.c.out = (char*)out;
+    a.c.starts = b->starts; a.c.past = b->past; a.c.tables = b->tables; a.c.prefix_table = b->prefix_table;
+    a.c.q_stride = q_stride * size;
+    a.c.sequences = b->sequences; a.c.max_new = b->max_new; a.c.tokens = b->tokens; a.c.max_pages = b->max_pages; a.c.prefix_len = b->prefix_len;
+    a.c.prefix_pages = (int)ceil_div(b->prefix_len, c->page_size);
+    a.c.heads = p->heads; a.c.page_size = c->page_size; a.c.num_pages = c->num_pages;
+    a.c.kv_heads = divisor((unsigned)p->kv_heads); a.c.per_kv = divisor((unsigned)(p->heads / p->kv_heads)); a.c.page_blocks = divisor((unsigned)c->page_size / 8);
+    a.c.scale_log2 = p->scale * 1.44269504088896340736f;
+    a.c.prefix_splits = divisor(0); a.c.own_splits = divisor((unsigned)p->splits);
+    const size_t rows = (size_t)p->tokens * p->heads, counters = counters_of(p);
+    a.c.counters = need && counters ? (unsigned*)workspace : nullptr;
+    a.c.ml = need ? (f32x2*)((char*)workspace + counters) : nullptr;
+    a.c.acc = need ? (float*)((char*)a.c.ml + up256(p->splits * rows * 8)) : nullptr;
+    a.c.job_id = job_id; a.c.notifier = (Notifier*)notifier;
+    a.pages = pages; a.count = p->count; a.per = (int)ceil_div(p->count, p->splits);
+    a.tiles = divisor((unsigned)tiles_of(p)); a.splits = divisor((unsigned)p->splits); a.max_new = divisor((unsigned)p->max_new);
+    if (stage) launch(join_of(p), dim3((unsigned)ceil_div((int64_t)rows, kJoinRows / p->head_dim)), dim3(256), 0, (hipStream_t)stream, a.c);
+    else launch(kernel_of(p), dim3((unsigned)grid_of(p)), dim3(256), 0, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+int paella_page_attention_launch(const paella_page_attention_plan* p, const paella_kv_cache* c, const paella_kv_batch* b, const void* q, int64_t q_stride, const int32_t* pages,
+                                 void* out, void* workspace, void* stream, uint32_t job_id, void* notifier) {
+    if (!plan_ok(p)) return PAELLA_EINVAL;
+    const int stages = stages_of(p);
+    if (stages > 1) {
+        if (keeps_no_order(stream)) return PAELLA_ENOSUP;
+        if (int rc = paella_page_attention_launch_stage(p, 0, c, b, q, q_stride, pages, out, workspace, stream, job_id, nullptr)) return rc;
+    }
+    return paella_page_attention_launch_stage(p, stages - 1, c, b, q, q_stride, pages, out, workspace, stream, job_id, notifier);
+}
+
+int paella_key_weights_plan_make(const paella_kv_cache* c, const paella_kv_batch* b, int heads, float scale, paella_key_weights_plan* p) {
+    if (!p || !cache_extents_ok(c) || !batch_extents_ok(b) || heads <= 0 || heads % c->kv_heads || !scale_ok(scale)) return PAELLA_EINVAL;
+    *p = paella_key_weights_plan{};
+    plan_extents(p, c, b, heads);
+    p->scale = scale > 0.f ? scale : 1.f / std::sqrt((float)c->head_dim);
+    p->splits = p->own_splits = 1;
+    if (!plan_ok(p)) return PAELLA_ENOSUP;
+    const int64_t own = (int64_t)c->page_size * b->max_pages, keys = own + b->prefix_len;
+    const int64_t sums = grid_of(p, 0), weights = grid_of(p, 1);
+    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(2048, sums), ceil_div(keys, 256), 64}));
+    p->own_splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(2048, weights), ceil_div(own, 256)));
+    if (!plan_ok(p)) return PAELLA_ENOSUP;
+    p->stages = 2;
+    p->workspace_bytes = workspace_of(p);
+    set_launch_dims(&p->dims, (unsigned)grid_of(p, 0), 256, 0, 256);
+    const double size = element_bytes(c->dtype);
+    p->flops = 2.0 * p->head_dim * p->tokens * heads * (double)keys;
+    p->bytes = (p->prefix_len + (double)p->sequences * own) * p->kv_heads * p->head_dim * size + (double)p->tokens * heads * p->head_dim * size + 8.0 * p->sequences * own * p->kv_heads;
+    return 0;
+}
+
+int paella_key_weights_dims(const paella_key_weights_plan* p, int stage, paella_launch_dims* dims) {
+    if (!plan_ok(p) || !dims || stage < 0 || stage > 1) return PAELLA_EINVAL;
+    set_launch_dims(dims, (unsigned)grid_of(p, stage), 256, 0, 256);
+    loaded_dims((const void*)kernel_of(p, stage), dims);
+    return 0;
+}
+
+int paella_key_weights_launch_stage(const paella_key_weights_plan* p, int stage, const paella_kv_cache* c, const paella_kv_batch* b, const void* q, int64_t q_stride, float* weights,
+                                    void* workspace, void* stream, uint32_t job_id, void* notifier) {
+    if (!plan_ok(p) || stage < 0 || stage > 1 || !planned_for(p, c, b) || !q || !weights || !workspace || ((uintptr_t)weights & 3) || (((uintptr_t)q | (uintptr_t)workspace) & 15))
+        return PAELLA_EINVAL;
+    const int64_t size = element_bytes(c->dtype), row = (int64_t)p->heads * c->head_dim;
+    if (q_stride < row || q_stride % 8) return PAELLA_EINVAL;
+    const double space = (double)workspace_of(p), weight_bytes = 4.0 * p->sequences * p->kv_heads * p->max_pages * p->page_size;
+    const struct { const void* at; double bytes; } outs[2] = {{weights, weight_bytes}, {workspace, space}};
+    for (const auto& o : outs)
+        if (rows_overlap(q, p->tokens, q_stride * size, row * size, o.at, o.bytes) || over_cache(c, o.at, o.bytes) || over_batch(b, c->page_size, o.at, o.bytes)) return PAELLA_EINVAL;
+    if (overlap(weights, weight_bytes, workspace, space)) return PAELLA_EINVAL;
+    WeighArgs a{};
+    a.q = (const char*)q; a.k_cache = (const char*)c->k; a.weights = weights;
+    a.starts = b->starts; a.past = b->past; a.tables = b->tables; a.prefix_table = b->prefix_table; a.q_stride = q_stride * size;
+    a.sequences = b->sequences; a.max_new = b->max_new; a.tokens = b->tokens; a.max_pages = b->max_pages; a.prefix_len = b->prefix_len;
+    a.prefix_pages = (int)ceil_div(b->prefix_len, c->page_size); a.num_pages = c->num_pages; a.page_size = c->page_size; a.heads = p->heads;
+    a.kv_heads = divisor((unsigned)p->kv_heads); a.per_kv = divisor((unsigned)(p->heads / p->kv_heads)); a.page_blocks = divisor((unsigned)c->page_size / 8);
+    a.splits = divisor((unsigned)p->splits); a.own_splits = divisor((unsigned)p->own_splits); a.chunks = divisor((unsigned)chunks_of(p));
+    a.scale_log2 = p->scale * 1.44269504088896340736f; a.ml = (f32x2*)workspace;
+    a.job_id = job_id; a.notifier = (Notifier*)notifier;
+    launch(kernel_of(p, stage), dim3((unsigned)grid_of(p, stage)), dim3(256), 0, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+int paella_key_weights_launch(const paella_key_weights_plan* p, const paella_kv_cache* c, const paella_kv_batch* b, const void* q, int64_t q_stride, float* weights, void* workspace,
+                              void* stream, uint32_t job_id, void* notifier) {
+    if (!plan_ok(p)) return PAELLA_EINVAL;
+    if (keeps_no_order(stream)) return PAELLA_ENOSUP;
+    if (int rc = paella_key_weights_launch_stage(p, 0, c, b, q, q_stride, weights, workspace, stream, job_id, nullptr)) return rc;
+    return paella_key_weights_launch_stage(p, 1, c, b, q, q_stride, weights, workspace, stream, job_id, notifier);
+}
+
+}  // extern "C"

@@ -595,24 +595,11 @@ constexpr int attention_lds() {
     return Fm::WIDE && WideWalk<T, D, Fm::R>::LDS > sums ? WideWalk<T, D, Fm::R>::LDS : sums;
 }
 
-// A workgroup's part: rows `row_id` (LDS; -1: none) of its tile over steps [begin, end) of `s`, left in slot `part` (or, where there is one, as the output).
+// What the waves have summed for rows `row_id` (LDS; -1: none), to slot `part` (or, where there is one, as the output).
 template <typename T, int D, typename Fm>
-__device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, const char* const (&q_row)[Fm::R], const int (&limit)[Fm::R], int least, int most,
-                                       int begin, int end, int part, const int* row_id, char* lds) {
+__device__ __forceinline__ void leave(const AttentionArgs& a, const AttentionRows<T, D, Fm::R, Fm::WIDE && T::bytes == 2>& rows, int part, const int* row_id, char* lds) {
     constexpr int R = Fm::R;
-    using Rows = AttentionRows<T, D, R, Fm::WIDE && T::bytes == 2>;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    Rows rows;
-    rows.begin();
-#pragma unroll
-    for (int r = 0; r < R; ++r) rows.load_q(r, q_row[r], lane);
-    if constexpr (Fm::WIDE) {
-        WideWalk<T, D, R> keys;
-        keys.walk(rows, s, begin * Rows::STEP, end * Rows::STEP, limit, least, most, a.scale_log2, lane, lds);
-    } else {
-        NarrowWalk<T, D> keys;
-        keys.walk(rows, s, begin + wave, end, limit, least, most, a.scale_log2, lane);
-    }
     // Through LDS, so that a row's outputs leave side by side, 16 rows of each wave at a time: the waves' sums of one row where they split the keys
     constexpr int PITCH = D + 4;  // floats of a row in LDS: lanes of different rows on different banks
     f32x2* const ml = reinterpret_cast<f32x2*>(lds);                 // [4][16]
@@ -667,6 +654,27 @@ __device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, co
             }
         }
     }
+}
+
+// A workgroup's part: the rows of its tile over steps [begin, end) of `s`.
+template <typename T, int D, typename Fm>
+__device__ __forceinline__ void attend(const AttentionArgs& a, const Keys& s, const char* const (&q_row)[Fm::R], const int (&limit)[Fm::R], int least, int most,
+                                       int begin, int end, int part, const int* row_id, char* lds) {
+    constexpr int R = Fm::R;
+    using Rows = AttentionRows<T, D, R, Fm::WIDE && T::bytes == 2>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Rows rows;
+    rows.begin();
+#pragma unroll
+    for (int r = 0; r < R; ++r) rows.load_q(r, q_row[r], lane);
+    if constexpr (Fm::WIDE) {
+        WideWalk<T, D, R> keys;
+        keys.walk(rows, s, begin * Rows::STEP, end * Rows::STEP, limit, least, most, a.scale_log2, lane, lds);
+    } else {
+        NarrowWalk<T, D> keys;
+        keys.walk(rows, s, begin + wave, end, limit, least, most, a.scale_log2, lane);
+    }
+    leave<T, D, Fm>(a, rows, part, row_id, lds);
 }
 
 // What some parts of a row sum up to, four outputs from d on.

@@ -206,10 +206,12 @@ class KVBatch:
         self.ref = ctypes.byref(self.desc)
 
 
-def kv_append(cache, batch, k, v, q=None, q_norm=None, k_norm=None, eps=1e-6, inv_freq=None, interleaved=False, out=None, stream=None, job_id=0, notifier=None):
+def kv_append(cache, batch, k, v, q=None, q_norm=None, k_norm=None, eps=1e-6, inv_freq=None, interleaved=False, out=None, stream=None, job_id=0, notifier=None,
+              positions=None):
     """Stores the new tokens' k and v ([tokens, kv_heads, head_dim]) in the cache, k normed per head (k_norm: float32 [head_dim]) and rotated (inv_freq: float32, one
-    per rotated pair) on the way; returns q ([tokens, heads, head_dim]) normed and rotated likewise, in `out` where given (which may be q)."""
-    _on_device(cache.k, k, v, q, q_norm, k_norm, inv_freq, out, batch.past)
+    per rotated pair) on the way; returns q ([tokens, heads, head_dim]) normed and rotated likewise, in `out` where given (which may be q).  positions: int32 [sequences], of each
+    sequence's first new token, where that is not prefix_len + past (after an eviction)."""
+    _on_device(cache.k, k, v, q, q_norm, k_norm, inv_freq, out, batch.past, positions)
     tokens, dim = batch.tokens, cache.head_dim
     kp, ks = _rows(k, tokens, cache.kv_heads, cache)
     vp, vs = _rows(v, tokens, cache.kv_heads, cache)
@@ -226,8 +228,11 @@ def kv_append(cache, batch, k, v, q=None, q_norm=None, k_norm=None, eps=1e-6, in
     desc = cache.append_descs.get((heads, rotary, interleaved, eps, qs, ks, vs))
     if desc is None:
         desc = cache.append_descs[heads, rotary, interleaved, eps, qs, ks, vs] = ctypes.byref(KvAppendDesc(heads, rotary, int(interleaved), eps, qs, ks, vs))
-    rc = _library().paella_kv_append_launch(desc, cache.ref, batch.ref, qp, kp, vp, _floats(q_norm, dim), _floats(k_norm, dim), _floats(inv_freq, rotary // 2), op,
-                                            _stream(stream), job_id, notifier)
+    args = (qp, kp, vp, _floats(q_norm, dim), _floats(k_norm, dim), _floats(inv_freq, rotary // 2), op, _stream(stream), job_id, notifier)
+    if positions is None:
+        rc = _library().paella_kv_append_launch(desc, cache.ref, batch.ref, *args)
+    else:
+        rc = _library().paella_kv_append_at_launch(desc, cache.ref, batch.ref, _ints(positions, batch.past.shape[0]), *args)
     if rc:
         check(rc, "paella_kv_append_launch")
     return out
