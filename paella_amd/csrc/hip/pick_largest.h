@@ -1,0 +1,245 @@
+#pragma once
+// The largest of many numbers, by one workgroup: which value the last one taken has, and the taken ones in the order of their places.
+
+#include "decode_common.h"
+
+namespace paella {
+
+// Which of n places the threads of WAVES waves have: those of a wave lie side by side, so that what is taken comes out in order.  KEYS: places of a thread at most, whose values may
+// then lie in registers, or 0 for any number.
+template <int WAVES, int KEYS>
+struct Span {
+    unsigned begin, end;
+    __device__ __forceinline__ explicit Span(unsigned n) {
+        const unsigned wave = (unsigned)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), per = (n + WAVES * 64 - 1) / (WAVES * 64) * 64;
+        begin = min(wave * per, n);
+        end = min(begin + per, n);
+    }
+    // each(u, i, is, value): place i, the thread's u-th, is there (whole waves come along behind the last one), and what get(u, i) has for it.  Where that reads memory, several are read ahead.
+    template <typename Get, typename Each>
+    __device__ __forceinline__ void visit(Get get, Each each) const {
+        const unsigned lane = threadIdx.x & 63;
+        if constexpr (KEYS > 0) {
+#pragma unroll
+            for (int u = 0; u < KEYS; ++u)
+                if (begin + u * 64 < end) each(u, begin + u * 64 + lane, begin + u * 64 + lane < end, get(u, begin + u * 64 + lane));
+        } else {
+            constexpr int AHEAD = 8;
+            for (unsigned first = begin; first < end; first += AHEAD * 64) {
+                decltype(get(0, 0u)) value[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) value[u] = get(0, min(first + u * 64 + lane, end - 1));
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u)
+                    if (first + u * 64 < end) each(0, first + u * 64 + lane, first + u * 64 + lane < end, value[u]);
+            }
+        }
+    }
+    // Registers' first values, from memory.
+    template <typename Value, typename Load>
+    __device__ __forceinline__ void hold(Value (&held)[KEYS ? KEYS : 1], Load load) const {
+        if constexpr (KEYS > 0) {
+            const unsigned lane = threadIdx.x & 63;
+#pragma unroll
+            for (int u = 0; u < KEYS; ++u)
+                if (begin + u * 64 < end) held[u] = load(min(begin + u * 64 + lane, end - 1));
+        }
+    }
+};
+
+constexpr unsigned kRanked = 256;  // candidates that are ranked against each other: one of each thread, and the ranking no longer than another histogram
+
+template <int WAVES>
+struct PickSpace {
+    unsigned bins[256];
+    unsigned long long list[kRanked];
+    unsigned long long low[WAVES], high[WAVES], bound;
+    unsigned count[3][WAVES];
+    unsigned digit, size, left, found;
+};
+
+// Numbers as ones whose order is theirs, above 0, -0 and 0 alike; NaN as `nan`.
+__device__ __forceinline__ unsigned number_key(float v, unsigned nan) {
+    const unsigned b = as_word(v + 0.f);
+    return v != v ? nan : b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ float key_number(unsigned k) { return as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
+__device__ __forceinline__ unsigned long long number_key(double v, unsigned long long nan) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, v + 0.0);
+    return v != v ? nan : b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
+}
+
+__device__ __forceinline__ unsigned long long shuffle_xor64(unsigned long long b, int mask) {
+    const unsigned lo = (unsigned)__shfl_xor((int)(unsigned)b, mask, 64), hi = (unsigned)__shfl_xor((int)(unsigned)(b >> 32), mask, 64);
+    return (unsigned long long)hi << 32 | lo;
+}
+
+// The least and largest of the keys that are not 0, and how many there are, over all threads.
+template <typename Key>
+struct Range {
+    Key least = ~(Key)0, most = 0;
+    unsigned some = 0;
+    __device__ __forceinline__ void add(Key k) {
+        if (k) {
+            least = min(least, k);
+            ++some;
+        }
+        most = max(most, k);
+    }
+    template <int WAVES>
+    __device__ __forceinline__ void join(PickSpace<WAVES>& s) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        for (int off = 32; off; off >>= 1) {
+            if constexpr (sizeof(Key) == 8) {
+                least = min(least, (Key)shuffle_xor64(least, off));
+                most = max(most, (Key)shuffle_xor64(most, off));
+            } else {
+                least = min(least, (Key)__shfl_xor((int)least, off, 64));
+                most = max(most, (Key)__shfl_xor((int)most, off, 64));
+            }
+            some += __shfl_xor((int)some, off, 64);
+        }
+        __syncthreads();
+        if (lane == 0) {
+            s.low[wave] = least;
+            s.high[wave] = most;
+            s.count[0][wave] = some;
+        }
+        __syncthreads();
+        some = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            least = min(least, (Key)s.low[w]);
+            most = max(most, (Key)s.high[w]);
+            some += s.count[0][w];
+        }
+    }
+};
+
+// What is taken: keys above `bound`, and the first `left` of those equal to it (all of them where left is ~0).
+template <typename Key>
+struct Bound {
+    Key bound;
+    unsigned left;
+};
+
+// Of the keys get(u, i) (0 is none), `range` of which is known: the `want` largest.  Digit by digit from the highest one in which the keys differ, by a histogram of the
+// keys that agree with the bound so far, until they are so few that each is ranked against all others.  Called by all threads.
+template <int WAVES, int KEYS, typename Key, typename Get>
+__device__ __forceinline__ Bound<Key> find_bound(const Span<WAVES, KEYS>& span, const Range<Key>& range, unsigned want, PickSpace<WAVES>& s, Get get) {
+    if (range.some <= want) return {1, ~0u};
+    const int lane = threadIdx.x & 63;
+    const int differ = range.least == range.most ? 0 : 64 - __clzll((unsigned long long)(range.least ^ range.most));  // bits; those above are the same in all keys
+    if (!differ) return {range.most, want};
+    int shift = max(differ - 8, 0);
+    Key known = shift + 8 < (int)sizeof(Key) * 8 ? (Key)(~(Key)0 << (shift + 8)) : (Key)0;  // the bits that the bound has so far
+    Key bound = range.most & known;
+    unsigned left = want, size = range.some;
+    while (size > kRanked) {
+        __syncthreads();
+        if (threadIdx.x < 256) s.bins[threadIdx.x] = 0;
+        __syncthreads();
+        span.visit(get, [&](int, unsigned, bool is, Key k) {
+            if (is && k && (k & known) == bound) atomicAdd(&s.bins[(unsigned)(k >> shift) & 255u], 1u);
+        });
+        __syncthreads();
+        if (threadIdx.x < 64) {  // four digits a lane, the highest first
+            unsigned c[4], sum = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                c[e] = s.bins[255 - (lane * 4 + e)];
+                sum += c[e];
+            }
+            unsigned upto = sum;
+            for (int off = 1; off < 64; off <<= 1) {
+                const unsigned other = __shfl_up((int)upto, off, 64);
+                if (lane >= off) upto += other;
+            }
+            unsigned before = upto - sum;
+            if (before < left && left <= upto) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (before < left && left <= before + c[e]) {
+                        s.digit = 255 - (lane * 4 + e);
+                        s.left = left - before;
+                        s.size = c[e];
+                    }
+                    before += c[e];
+                }
+            }
+        }
+        __syncthreads();
+        bound |= (Key)s.digit << shift;
+        left = s.left;
+        size = s.size;
+        known |= (Key)255 << shift;
+        if (size == left) return {bound, ~0u};  // all that begin so
+        if (shift == 0) return {bound, left};
+        shift = max(shift - 8, 0);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) s.found = 0;
+    __syncthreads();
+    span.visit(get, [&](int, unsigned, bool is, Key k) {
+        if (is && k && (k & known) == bound) s.list[atomicAdd(&s.found, 1u)] = k;
+    });
+    __syncthreads();
+    if (threadIdx.x < size) {
+        const Key mine = (Key)s.list[threadIdx.x];
+        unsigned above = 0, equal = 0;
+#pragma unroll 8
+        for (unsigned o = 0; o < size; ++o) {
+            const Key other = (Key)s.list[o];
+            above += other > mine;
+            equal += other == mine;
+        }
+        if (above < left && left <= above + equal) {  // the same for all that are equal
+            s.bound = mine;
+            s.left = above + equal == left ? ~0u : left - above;
+        }
+    }
+    __syncthreads();
+    return {(Key)s.bound, s.left};
+}
+
+// take(place, i) for what is taken, in order; returns how many.
+template <int WAVES, int KEYS, typename Key, typename Get, typename Take>
+__device__ __forceinline__ unsigned emit_taken(const Span<WAVES, KEYS>& span, Bound<Key> b, PickSpace<WAVES>& s, Get get, Take take) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    unsigned above = 0, equal = 0;
+    span.visit(get, [&](int, unsigned, bool is, Key k) {
+        if (!is) k = 0;
+        above += __popcll(__ballot(b.left == ~0u ? k >= b.bound : k > b.bound));
+        equal += __popcll(__ballot(b.left != ~0u && k == b.bound));
+    });
+    __syncthreads();
+    if (lane == 0) {
+        s.count[1][wave] = above;
+        s.count[2][wave] = equal;
+    }
+    __syncthreads();
+    unsigned place = 0, ties = 0, all = 0, ties_all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const unsigned here = b.left == ~0u ? 0u : min(s.count[2][w], b.left - min(b.left, ties_all));
+        if (w < wave) {
+            place += s.count[1][w] + here;
+            ties += s.count[2][w];
+        }
+        all += s.count[1][w] + here;
+        ties_all += s.count[2][w];
+    }
+    const unsigned long long before = (1ull << lane) - 1;
+    span.visit(get, [&](int, unsigned i, bool is, Key k) {
+        if (!is) k = 0;
+        const unsigned long long tied = __ballot(b.left != ~0u && k == b.bound);
+        const bool mine = b.left == ~0u ? k >= b.bound : k > b.bound || (k == b.bound && ties + __popcll(tied & before) < b.left);
+        const unsigned long long who = __ballot(mine);
+        if (mine) take(place + __popcll(who & before), i);
+        place += __popcll(who);
+        ties += __popcll(tied);
+    });
+    return all;
+}
+
+}  // namespace paella

@@ -113,6 +113,8 @@ PICK = [
     (F16, 2, 2, 256, 16, [5000, 100], 1, None, 0, 400, 2, 2),                 # more than there are
     (BF16, 4, 4, 64, 8, [20000], 2, None, 0, 300, 1, 1),                      # as many heads as key heads; thousands of pages
     (F32, 2, 1, 256, 8, [600], 1, None, 9, 1, 0, 1),
+    (F16, 3, 1, 64, 8, [40000, 100], 1, None, 0, 200, 4, 4),                  # more pages than one form's registers hold, and than another's
+    (BF16, 2, 1, 64, 8, [150000], 1, None, 5, 77, 1, 2),
 ]
 
 
@@ -169,6 +171,27 @@ def test_selection_decided_in_the_last_digits(cuda):
     got = select(q.to(cuda), bounds.to(cuda), cache, batch)
     same(got, long_ref.pick(c.host, q, bounds, 20, 0, 1))
     assert set(got.flatten().tolist()) == {e for e in range(99) if (e * 37) % 99 >= 80} | {99}
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=lambda d: str(d)[6:])
+def test_selection_by_subnormal_bounds_and_by_the_largest(cuda, dtype):
+    """Products of the type's least numbers count, and sums beyond 32 bits are compared like any."""
+    from paella_amd import long_cache
+    c = Case(2, dtype, 1, 64, 8, [1600], 1)
+    cache, batch = c.to(cuda)
+    info = torch.finfo(dtype)
+    large = math.sqrt(info.max) if dtype == F16 else 2.0 ** 120
+    least = info.smallest_normal / 2 ** (4 if dtype == BF16 else 6)
+    ones = (1.0 + torch.rand((c.total, 1, 2, 64), generator=c.gen)).float()
+    for q, bounds in (((torch.rand((1, 3, 64), generator=c.gen) * large).to(dtype), (ones * least).to(dtype)),
+                      ((torch.rand((1, 3, 64), generator=c.gen) * info.max * 0.5).to(dtype), (ones * large).to(dtype)),
+                      ((torch.rand((1, 3, 64), generator=c.gen) * least).to(dtype), (ones * least).to(dtype))):
+        bounds = bounds.sort(2).values
+        mixed = bounds.clone()
+        mixed[::2] *= -1
+        for b in (bounds, mixed.sort(2).values):
+            select = long_cache.PageSelect(3, cache, batch, 30)
+            same(select(q.to(cuda), b.to(cuda), cache, batch), long_ref.pick(c.host, q, b, 30, 0, 1))
 
 
 # ------------------------------------------------------------------ attention over picked pages
@@ -333,6 +356,8 @@ EVICT = [
     (F16, 2, 8, 8, [5000], 1, 0, 1),
     (BF16, 2, 96, 128, [2000], 1500, 100, 300),
     (F32, 1, 64, 8, [40], 1000, 3, 3),                  # longer than any
+    (F16, 1, 8, 8, [9000, 3000], 2100, 4, 8),           # longer than one form's registers hold, and than another's
+    (BF16, 1, 8, 8, [20000], 1900, 0, 100),
 ]
 
 
