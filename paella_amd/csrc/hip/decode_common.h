@@ -57,6 +57,12 @@ __device__ __forceinline__ double lane_move(double v) {
     const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), CONTROL, 0xF, 0xF, false);
     return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
+template <int CONTROL>
+__device__ __forceinline__ unsigned lane_move(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, 0xF, 0xF, false); }
+template <int CONTROL>
+__device__ __forceinline__ unsigned long long lane_move(unsigned long long v) {
+    return (unsigned long long)lane_move<CONTROL>((unsigned)(v >> 32)) << 32 | lane_move<CONTROL>((unsigned)v);
+}
 template <typename V, typename Op>
 __device__ __forceinline__ V row_all(V v, Op op) {
     v = op(v, lane_move<0xB1>(v));   // lane ^ 1

@@ -116,50 +116,37 @@ __global__ __launch_bounds__(256) void page_bounds_kernel(BoundsArgs a) {
 // ------------------------------------------------------------------------------------------ selection of pages
 // worth(e) = max over the key head's query heads of sum_d max(q_d low_d, q_d high_d) = q+ . high + q- . low, q+ and q- the values above and below 0.  Which of two neighbours is taken is decided by their last
 // digits, in 64 bits; but nearly all pages are far from the border.  So the matrix units take the worths in 32 bits, at the rate that memory delivers the bounds, together with how far each can
-// be off: of a sum of 2 D products by 4 D * 2^-24 of the sum of their magnitudes, |q| . max(|low|, |high|).  Pages that are further from the border than
+// be off: of a sum of 2 D products, half of them 0, by (2 D + 8) * 2^-24 of the sum of their magnitudes, q+ . |high| - q- . |low|.  Pages that are further from the border than
 // that are decided; the few others, if they are not all taken or none of them, get their worths in 64 bits.  (All of them in 64 bits by the vector unit: 58 us for 32 rows of 1024 pages of 8 heads of 128 in bf16, 100 MB.)
 struct SelectArgs {
     const char *q, *bounds;
     const int *starts, *past, *tables, *prefix_table;
-    f32x2* entries;    // [tokens][kv_heads][pitch]
+    unsigned* entries;           // [tokens][kv_heads][pitch]
+    float* errors;               // [tokens][kv_heads][4 * splits]: how far the worths can be off, over (2 D + 8) * 2^-24
+    unsigned long long* worths;  // [tokens][kv_heads][pitch]
     int* pages;
     int64_t q_stride;  // bytes
     int sequences, tokens, max_pages, prefix_pages, num_pages, heads, first, last, count, dim, dtype;
     unsigned pitch;
-    Divisor max_new, kv_heads, splits, page_size;
+    Divisor max_new, kv_heads, per_kv, splits, tiles, page_size;  // tiles: of a sequence's new tokens
     uint32_t job_id;
     Notifier* notifier;
 };
 
-// What a page's entry holds beside its worth: how far that can be off, over 4 D * 2^-24, +inf where it is no number or may be infinite; or
-constexpr float kNoPage = -1.f, kForced = -2.f;
+// A page's entry: its worth as a number whose order is the worths', or
+constexpr unsigned kNoPage = 0, kUnknown = 1, kForced = ~0u;  // (unknown: it is no number, or may be infinite)
 
 __device__ __forceinline__ int page_along(const SelectArgs& a, int seq, unsigned e) {
     return e < (unsigned)a.prefix_pages ? a.prefix_table[e] : a.tables[(size_t)seq * a.max_pages + (e - a.prefix_pages)];
 }
 
-template <typename T> __device__ __forceinline__ u32x4 sign_mask(u32x4 q) {
-    u32x4 m;
+// Values below 0, and magnitudes, of 16 bytes.
+template <typename T> __device__ __forceinline__ u32x4 below_zero(u32x4 q) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) m[e] = T::bytes == 4 ? (unsigned)((int)q[e] >> 31) : (q[e] >> 15 & 0x00010001u) * 0xFFFFu;
-    return m;
+    for (int e = 0; e < 4; ++e) q[e] &= T::bytes == 4 ? (unsigned)((int)q[e] >> 31) : (q[e] >> 15 & 0x00010001u) * 0xFFFFu;
+    return q;
 }
 template <typename T> __device__ __forceinline__ u32x4 magnitude(u32x4 v) { return v & (T::bytes == 4 ? 0x7FFFFFFFu : 0x7FFF7FFFu); }
-template <typename T> __device__ __forceinline__ u32x4 larger_magnitude(u32x4 v, u32x4 w) {  // (magnitudes compare as whole numbers do, a NaN above all)
-    v = magnitude<T>(v);
-    w = magnitude<T>(w);
-    u32x4 m;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if constexpr (T::bytes == 4) {
-            m[e] = max(v[e], w[e]);
-        } else {
-            typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-            m[e] = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, v[e]), __builtin_bit_cast(u16x2, w[e])));
-        }
-    }
-    return m;
-}
 
 // x += v w^T of 16 rows each, 16 bytes of a row per lane
 template <typename T>
@@ -173,199 +160,257 @@ __device__ __forceinline__ f32x4 multiply(u32x4 v, u32x4 w, f32x4 x) {
     }
 }
 
-constexpr int kScreened = 32;  // pages of a wave's turn
+constexpr int kScreened = 16;  // pages of a wave's turn
 
-// Turns first, first + step, ... of a row's pages: put(page, entry).
-template <typename T, int D, typename Put>
-__device__ __forceinline__ void screen_pages(const SelectArgs& a, int t, int seq, int h, unsigned pages, unsigned first, unsigned step, Put put) {
-    constexpr int ROW = D * T::bytes, KC = ROW / 64, U = kScreened / 16;
-    const int lane = threadIdx.x & 63, mm = lane & 15, group = lane >> 4;
-    const int heads = a.heads / (int)a.kv_heads.d;
-    for (unsigned turn = first; turn * kScreened < pages; turn += step) {
-        int page[U];
-        const char* from[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            page[u] = page_along(a, seq, min(turn * kScreened + u * 16 + mm, pages - 1));
-            from[u] = a.bounds + ((size_t)((unsigned)page[u] < (unsigned)a.num_pages ? page[u] : 0) * a.kv_heads.d + h) * 2 * ROW + group * 16;
-        }
-        f32x4 worth[U], error[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            worth[u] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            error[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        for (int g = 0; g < heads; g += 16) {
-            const char* const row = a.q + t * a.q_stride + (size_t)(h * heads + min(g + mm, heads - 1)) * ROW + group * 16;
-            f32x4 x[U], y[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) x[u] = y[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+// New tokens of a sequence whose heads for one key head make up a tile of 16 rows: the bounds are read once for all of them.
+__host__ __device__ constexpr int tokens_of_tile(int heads) { return heads >= 16 ? 1 : 16 / heads; }
+
+// A turn's bounds go to registers while the ones before are worked on, and the numbers of the pages behind them.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void page_screen_kernel(SelectArgs a) {
+    hook_entry(a.notifier, a.job_id);
+    constexpr int ROW = D * T::bytes, KC = ROW / 64;
+    const int lane = threadIdx.x & 63, mm = lane & 15, group = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, a.splits), by_tile = divide(by_split.q, a.tiles);
+    const int h = (int)by_head.r, seq = (int)by_tile.q, heads = (int)a.per_kv.d, each = tokens_of_tile(heads), j0 = (int)by_tile.r * each;
+    const NewTokens its = new_tokens(a.starts, a.past, seq, (int)a.max_new.d, a.tokens);
+    const int n = min(its.count - j0, each);  // tokens here
+    auto pages_of = [&](int j) { return (unsigned)a.prefix_pages + (unsigned)own_pages(its.past, j0 + j, a.page_size, a.max_pages); };
+    const unsigned pages = n > 0 ? pages_of(n - 1) : 0u, step = a.splits.d * 4;
+    unsigned turn = by_split.r * 4 + wave;
+    float worst = 0.f;
+    if (turn * kScreened < pages) {
+        const Quotient row = divide((unsigned)min(mm, n * heads - 1), a.per_kv);  // the lane's token and head
+        auto number_of = [&](unsigned turn) { return page_along(a, seq, min(turn * kScreened + mm, pages - 1)); };
+        auto load = [&](int page, u32x4 (&low)[KC], u32x4 (&high)[KC]) {
+            const char* const from = a.bounds + ((size_t)((unsigned)page < (unsigned)a.num_pages ? page : 0) * a.kv_heads.d + h) * 2 * ROW + group * 16;
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
-                const u32x4 q = *reinterpret_cast<const u32x4*>(row + c * 64), below = sign_mask<T>(q);
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const u32x4 low = *reinterpret_cast<const u32x4*>(from[u] + c * 64), high = *reinterpret_cast<const u32x4*>(from[u] + ROW + c * 64);
-                    x[u] = multiply<T>(high, q & ~below, x[u]);
-                    x[u] = multiply<T>(low, q & below, x[u]);
-                    y[u] = multiply<T>(larger_magnitude<T>(low, high), magnitude<T>(q), y[u]);
-                }
+                low[c] = *reinterpret_cast<const u32x4*>(from + c * 64);
+                high[c] = *reinterpret_cast<const u32x4*>(from + ROW + c * 64);
             }
+        };
+        u32x4 low[KC], high[KC], above[KC], below[KC];  // of the queries: values above 0 and below it
+        auto query = [&](int g) {
+            const int head = heads > 16 ? min(g + mm, heads - 1) : (int)row.r;
+            const char* const from = a.q + (size_t)(its.first + j0 + (heads > 16 ? 0 : (int)row.q)) * a.q_stride + (size_t)(h * heads + head) * ROW + group * 16;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int c = 0; c < KC; ++c) {
+                const u32x4 q = *reinterpret_cast<const u32x4*>(from + c * 64);
+                below[c] = below_zero<T>(q);
+                above[c] = q ^ below[c];
+            }
+        };
+        int page = number_of(turn);
+        query(0);
+        load(page, low, high);
+        int page_ahead = number_of(turn + step);
+        const bool one_group = n * heads <= 4;  // the first lane group has all rows
+        for (; turn * kScreened < pages; turn += step) {
+            // Lane mm has page mm, register e of lane group g row 4 g + e.
+            f32x4 worth = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, error = {0.f, 0.f, 0.f, 0.f};
+            const bool more = (turn + step) * kScreened < pages;
+            u32x4 next_low[KC], next_high[KC];
+            if (KC <= 8 && more) load(page_ahead, next_low, next_high);
+            for (int g = 0; g < heads; g += 16) {  // more than once where a token has more heads than a tile rows
+                if (heads > 16) query(g);
+                f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x, z = x;
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    x = multiply<T>(above[c], high[c], x);
+                    x = multiply<T>(below[c], low[c], x);
+                    y = multiply<T>(above[c], magnitude<T>(high[c]), y);
+                    z = multiply<T>(below[c], magnitude<T>(low[c]), z);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    worth[u][e] = fmaxf(worth[u][e], x[u][e]);
-                    error[u][e] = fmaxf(error[u][e], y[u][e] < 1e38f ? y[u][e] : INFINITY);  // (below it no sum on the way was infinite either)
+                    const float off = y[e] - z[e];
+                    worth[e] = fmaxf(worth[e], x[e]);
+                    error[e] = fmaxf(error[e], off < 1e38f ? off : INFINITY);  // (below it no sum on the way was infinite either)
+                    if (off < 1e38f) worst = fmaxf(worst, off);
                 }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            f32x2 mine = {0.f, 0.f};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {  // over the heads; lane mm = e has that of page 4 group + e
-                const float w = row_all(worth[u][e], [](float p, float q) { return fmaxf(p, q); }), r = row_all(error[u][e], [](float p, float q) { return fmaxf(p, q); });
-                if (mm == e) mine = f32x2{w, r};
             }
-            const unsigned e = turn * kScreened + u * 16 + group * 4 + mm;
-            const int at = __shfl(page[u], group * 4 + (mm & 3), 64);
-            if (e < (unsigned)a.first || e + a.last >= pages) mine.y = kForced;
-            if ((unsigned)at >= (unsigned)a.num_pages) mine.y = kNoPage;
-            if (mm < 4 && e < pages) put(e, mine);
+            const unsigned e = turn * kScreened + mm;
+            for (int j = 0; j < n; ++j) {
+                f32x2 mine = {-INFINITY, 0.f};  // worth, and how far it can be off
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // the token's rows
+                    const int r = group * 4 + i;
+                    const bool ours = heads > 16 || (r >= j * heads && r < (j + 1) * heads);
+                    mine.x = fmaxf(mine.x, ours ? worth[i] : -INFINITY);
+                    mine.y = fmaxf(mine.y, ours ? error[i] : 0.f);
+                }
+                if (!one_group) {
+#pragma unroll
+                    for (int off = 16; off < 64; off <<= 1) {
+                        mine.x = fmaxf(mine.x, __shfl_xor(mine.x, off, 64));
+                        mine.y = fmaxf(mine.y, __shfl_xor(mine.y, off, 64));
+                    }
+                }
+                const unsigned seen = pages_of(j);
+                unsigned key = mine.y < INFINITY ? number_key(mine.x, kUnknown) : kUnknown;
+                if (e < (unsigned)a.first || e + a.last >= seen) key = kForced;
+                if ((unsigned)page >= (unsigned)a.num_pages) key = kNoPage;
+                const size_t at = (size_t)(its.first + j0 + j) * a.kv_heads.d + h;
+                if (group == 0 && e < seen) __hip_atomic_store(a.entries + at * a.pitch + e, key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            if (more) {
+                page = page_ahead;
+                if constexpr (KC <= 8) {
+#pragma unroll
+                    for (int c = 0; c < KC; ++c) {
+                        low[c] = next_low[c];
+                        high[c] = next_high[c];
+                    }
+                } else {
+                    load(page, low, high);
+                }
+                page_ahead = number_of(turn + 2 * step);
+            }
         }
     }
+    worst = wave_max_f(worst);  // of all rows of the tile
+    if (lane < n) store_out(a.errors + ((size_t)(its.first + j0 + lane) * a.kv_heads.d + h) * step + by_split.r * 4 + wave, worst);
+    hook_exit(a.notifier, a.job_id);
 }
 
-__device__ __forceinline__ double value_at(const char* p, int i, int dtype) {
-    if (dtype == PAELLA_F32) return (double)reinterpret_cast<const float*>(p)[i];
-    const unsigned w = reinterpret_cast<const unsigned short*>(p)[i];
-    return (double)(dtype == PAELLA_BF16 ? unpack2<Bf16>(w).x : unpack2<F16>(w).x);
-}
-
-// A page's worth in 64 bits, by a whole wave.
-__device__ __forceinline__ unsigned long long exact_worth(const SelectArgs& a, int t, int seq, int h, unsigned e) {
-    const int lane = threadIdx.x & 63, heads = a.heads / (int)a.kv_heads.d, row = a.dim * (a.dtype == PAELLA_F32 ? 4 : 2);
+// A page's worth in 64 bits, by a whole wave: 16 bytes of a row per lane, the bounds and four heads' queries requested together.
+template <typename T>
+__device__ __forceinline__ unsigned long long exact_worth_of(const SelectArgs& a, int t, int seq, int h, unsigned e) {
+    constexpr int G = 4, V = 16 / T::bytes;
+    const int lane = threadIdx.x & 63, heads = (int)a.per_kv.d, row = a.dim * T::bytes;
+    const int at = min(lane * 16, row - 16);
+    const char* const q = a.q + t * a.q_stride + (size_t)h * heads * row + at;
     const int page = page_along(a, seq, e);  // (in the cache: others are not asked for)
-    const char* const low = a.bounds + ((size_t)page * a.kv_heads.d + h) * 2 * row;
-    const char* const q = a.q + t * a.q_stride + (size_t)h * heads * row;
+    const char* const from = a.bounds + ((size_t)page * a.kv_heads.d + h) * 2 * row + at;
+    const u32x4 low = *reinterpret_cast<const u32x4*>(from), high = *reinterpret_cast<const u32x4*>(from + row);
     unsigned long long best = 0;
-    for (int g = 0; g < heads; ++g) {
-        double sum = 0.0;
-        for (int d = lane; d < a.dim; d += 64) {
-            const double x = value_at(q + (size_t)g * row, d, a.dtype), u = x * value_at(low, d, a.dtype), v = x * value_at(low + row, d, a.dtype);
-            sum += u > v || u != u ? u : v;
+    for (int g = 0; g < heads; g += G) {
+        u32x4 x[G];
+        double sum[G];
+#pragma unroll
+        for (int i = 0; i < G; ++i) x[i] = *reinterpret_cast<const u32x4*>(q + (size_t)min(g + i, heads - 1) * row);
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            sum[i] = 0.0;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                auto value = [&](u32x4 w) {
+                    if constexpr (T::bytes == 4) return (double)as_float(w[v]);
+                    else return (double)(v & 1 ? unpack2<T>(w[v / 2]).y : unpack2<T>(w[v / 2]).x);
+                };
+                const double l = value(x[i]) * value(low), r = value(x[i]) * value(high);
+                sum[i] += l > r || l != l ? l : r;
+            }
+            sum[i] = lane * 16 < row ? sum[i] : 0.0;
+            sum[i] = row_all(sum[i], Sum());
+#pragma unroll
+            for (int off = 16; off < 64; off <<= 1) {
+                const unsigned long long b = __builtin_bit_cast(unsigned long long, sum[i]);
+                sum[i] += __builtin_bit_cast(double, (unsigned long long)(unsigned)__shfl_xor((int)(unsigned)(b >> 32), off, 64) << 32 | (unsigned)__shfl_xor((int)(unsigned)b, off, 64));
+            }
+            best = max(best, number_key(sum[i], number_key((double)INFINITY, 0ull)));  // a worth that is no number counts as the largest
         }
-        for (int off = 32; off; off >>= 1) sum += __builtin_bit_cast(double, shuffle_xor64(__builtin_bit_cast(unsigned long long, sum), off));
-        best = max(best, number_key(sum, number_key((double)INFINITY, 0ull)));  // a worth that is no number counts as the largest
     }
     return best;
+}
+__device__ __forceinline__ unsigned long long exact_worth(const SelectArgs& a, int t, int seq, int h, unsigned e) {
+    return a.dtype == PAELLA_F32 ? exact_worth_of<F32>(a, t, seq, h, e) : a.dtype == PAELLA_BF16 ? exact_worth_of<Bf16>(a, t, seq, h, e) : exact_worth_of<F16>(a, t, seq, h, e);
 }
 
 __device__ __forceinline__ void put_int(int* p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-constexpr unsigned kOpen = 512;  // pages whose worths in 64 bits are taken at a time
+constexpr unsigned kOpen = 256;  // pages whose worths in 64 bits are ranked against each other
 
 template <int WAVES>
 struct PageSpace {
     PickSpace<WAVES> pick;
-    unsigned forced[WAVES], unknown[WAVES];
+    unsigned forced[WAVES], unknown[WAVES], inside[WAVES], open[WAVES];
     float error[WAVES];
-    unsigned inside[WAVES], open[WAVES];
     unsigned list[kOpen];
     unsigned long long worth[kOpen];
 };
 
-// The row's pages by their entries, load(i).  KEYS as in Span; where it is 0, keys take the entries' places, keep(i, key).
-template <int WAVES, int KEYS, typename Load, typename Keep>
-__device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, int h, unsigned pages, int* to, PageSpace<WAVES>& s, Load load, Keep keep) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// The row's pages by their entries.  KEYS as in Span.
+template <int WAVES, int KEYS>
+__device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, int h, unsigned pages, const unsigned* entries, const float* errors, unsigned long long* worths, int* to,
+                                           PageSpace<WAVES>& s) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const Span<WAVES, KEYS> span(pages);
-    unsigned long long held[KEYS ? KEYS : 1];  // entries, and then keys
+    unsigned held[KEYS ? KEYS : 1];
+    auto load = [&](unsigned i) { return entries[i]; };
     span.hold(held, load);
     auto get = [&](int u, unsigned i) { return KEYS ? held[u] : load(i); };
-    auto entry_of = [](bool is, unsigned long long v) { return is ? __builtin_bit_cast(f32x2, v) : f32x2{0.f, kNoPage}; };
-    auto known = [](f32x2 e) { return e.y >= 0.f && e.y < INFINITY; };
+    auto known = [](unsigned k) { return k > kUnknown && k < kForced ? k : 0u; };
     Range<unsigned> range;
     unsigned forced = 0, unknown = 0;
-    float error = 0.f;
-    span.visit(get, [&](int, unsigned, bool is, unsigned long long v) {
-        const f32x2 e = entry_of(is, v);
-        forced += __popcll(__ballot(e.y == kForced));
-        unknown += __popcll(__ballot(e.y == INFINITY));
-        range.add(known(e) ? number_key(e.x, 1u) : 0u);
-        if (known(e)) error = fmaxf(error, e.y);
+    span.visit(get, [&](int, unsigned, bool is, unsigned k) {
+        forced += is && k == kForced;
+        unknown += is && k == kUnknown;
+        range.add(is ? known(k) : 0u);
     });
+    float error = 0.f;
+    for (unsigned i = threadIdx.x; i < 4 * a.splits.d; i += WAVES * 64) error = fmaxf(error, errors[i]);
     error = wave_max_f(error);
+    forced = wave_all(forced, Sum());
+    unknown = wave_all(unknown, Sum());
     if (lane == 0) {
         s.forced[wave] = forced;
         s.unknown[wave] = unknown;
         s.error[wave] = error;
     }
     range.join(s.pick);
-    forced = unknown = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        forced += s.forced[w];
-        unknown += s.unknown[w];
-        error = fmaxf(error, s.error[w]);
-    }
+    error = waves_all(s.error, Most());
+    forced = uniform(waves_all(s.forced, Sum()));
+    unknown = uniform(waves_all(s.unknown, Sum()));
     const unsigned want = (unsigned)a.count - min(forced, (unsigned)a.count);
-    // Pages worth more than `in` are taken, those worth less than `out` are not, those between are open.
-    float in = -INFINITY, out = -INFINITY;
-    const bool all = range.some + unknown <= want;
-    if (!all && want) {
-        const float off = 2.f * (error * (float)(4 * a.dim) * 0x1p-24f + 0x1p-110f);  // (products below the least number of 32 bits are lost, too)
-        in = INFINITY;
+    // Pages whose entries are above `in` are taken, those below `out` are not, those between are open, and those that nothing is known of as well.
+    unsigned in = kForced - 1, out = kForced;
+    bool any_unknown = false;
+    if (range.some + unknown <= want) {
+        in = kNoPage;
+    } else if (want) {
+        any_unknown = unknown > 0;
+        out = 0;
         if (range.some >= want) {
-            const float border = key_number(range.some == want ? range.least
-                                                               : find_bound<WAVES, KEYS, unsigned>(span, range, want, s.pick, [&](int u, unsigned i) {
-                                                                     const f32x2 e = entry_of(true, get(u, i));
-                                                                     return known(e) ? number_key(e.x, 1u) : 0u;
-                                                                 }).bound);
-            out = border - off;
-            if (!unknown) in = border + off;  // (a page that nothing is known of may be worth more)
+            const float border = key_number(range.some == want ? range.least : find_bound<WAVES, KEYS, unsigned>(span, range, want, s.pick, [&](int u, unsigned i) { return known(get(u, i)); }).bound);
+            const float off = 2.f * (error * (float)(2 * a.dim + 8) * 0x1p-24f + 0x1p-110f);  // (products below the least number of 32 bits are lost, too)
+            out = number_key(border - off, 1u);
+            if (!unknown) in = number_key(border + off, 1u);  // (a page that nothing is known of may be worth more)
         }
+        out = max(out, kUnknown + 1);
     }
-    auto is_in = [&](f32x2 e) { return e.y == kForced || (all && e.y >= 0.f) || (known(e) && want && e.x > in); };
-    auto is_open = [&](f32x2 e) { return !all && want && (e.y == INFINITY || (known(e) && e.x >= out && e.x <= in)); };
+    auto is_in = [&](unsigned k) { return k > in; };
+    auto is_open = [&](unsigned k) { return (k >= out && k <= in) || (any_unknown && k == kUnknown); };
     unsigned inside = 0, open = 0;
-    span.visit(get, [&](int, unsigned, bool is, unsigned long long v) {
-        const f32x2 e = entry_of(is, v);
-        inside += __popcll(__ballot(is_in(e)));
-        open += __popcll(__ballot(is_open(e)));
+    span.visit(get, [&](int, unsigned, bool is, unsigned k) {
+        inside += is && is_in(k);
+        open += is && is_open(k);
     });
+    inside = wave_all(inside, Sum());
+    open = wave_all(open, Sum());
     if (lane == 0) {
         s.inside[wave] = inside;
         s.open[wave] = open;
     }
     __syncthreads();
-    inside = open = 0;
-    unsigned ahead = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        if (w < wave) ahead += s.open[w];
-        inside += s.inside[w];
-        open += s.open[w];
-    }
-    const bool decided = inside + open <= (unsigned)a.count;  // all that are open are taken
-    auto set = [&](int u, unsigned i, bool is, unsigned long long k) {
-        if constexpr (KEYS > 0) held[u] = k;
-        else if (is) keep(i, k);
-    };
-    // Keys: all ones for what is taken, 0 for what is not, and for what is open 1 until its worth in 64 bits is there (whose key is above that and below all ones).
-    constexpr unsigned long long kIn = ~0ull, kWaiting = 1;
-    span.visit(get, [&](int u, unsigned i, bool is, unsigned long long v) {
-        const f32x2 e = entry_of(is, v);
-        set(u, i, is, is_in(e) || (decided && is_open(e)) ? kIn : is_open(e) ? kWaiting : 0ull);
-    });
-    Bound<unsigned long long> bound = {1, ~0u};
-    if (!decided) {
-        for (unsigned first = 0; first < open; first += kOpen) {  // the waves share them
+    inside = uniform(waves_all(s.inside, Sum()));
+    open = uniform(waves_all(s.open, Sum()));
+    auto take = [&](unsigned place, unsigned i) { put_int(to + place, (int)i); };
+    auto none = [](auto) { return false; };
+    unsigned taken;
+    if (inside + open <= (unsigned)a.count) {
+        taken = emit(span, s.pick, get, [&](unsigned k) { return is_in(k) || is_open(k); }, none, 0u, take);
+    } else {
+        // The open pages, in order, a list at a time, whose worths the waves share out.
+        unsigned ahead = 0;
+        for (int w = 0; w < wave; ++w) ahead += s.open[w];
+        for (unsigned first = 0; first < open; first += kOpen) {
             const unsigned n = min(open - first, kOpen);
-            auto each_open = [&](auto&& then) {
-                unsigned slot = ahead - first;  // (those of other turns are far above n)
-                span.visit(get, [&](int u, unsigned i, bool is, unsigned long long v) {
-                    const bool mine = is && v && v != kIn;
+            auto each_open = [&](auto then) {
+                unsigned slot = ahead - first;  // (those of other lists are far above n)
+                span.visit(get, [&](int u, unsigned i, bool is, unsigned k) {
+                    const bool mine = is && is_open(k);
                     const unsigned long long who = __ballot(mine);
                     const unsigned at = slot + (unsigned)__popcll(who & ((1ull << lane) - 1));
                     if (mine && at < n) then(u, i, at);
@@ -374,36 +419,40 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
             };
             each_open([&](int, unsigned i, unsigned at) { s.list[at] = i; });
             __syncthreads();
-            for (unsigned k = (unsigned)__builtin_amdgcn_readfirstlane(wave); k < n; k += WAVES) {
-                const unsigned long long worth = exact_worth(a, t, seq, h, (unsigned)__builtin_amdgcn_readfirstlane((int)s.list[k]));
+            for (unsigned k = wave; k < n; k += WAVES) {
+                const unsigned long long worth = exact_worth(a, t, seq, h, uniform(s.list[k]));
                 if (lane == 0) s.worth[k] = worth;
             }
             __syncthreads();
-            each_open([&](int u, unsigned i, unsigned at) { set(u, i, true, s.worth[at]); });
-            __syncthreads();
+            if (open <= kOpen && KEYS > 0) {  // all of them: each is ranked against the others
+                for (unsigned k = threadIdx.x; k < n; k += WAVES * 64) {
+                    const unsigned long long mine = s.worth[k];
+                    unsigned before = 0;
+                    for (unsigned o = 0; o < n; ++o) before += s.worth[o] > mine || (s.worth[o] == mine && o < k);
+                    s.list[k] = before < (unsigned)a.count - inside ? kForced : kNoPage;
+                }
+                __syncthreads();
+                each_open([&](int u, unsigned, unsigned at) { held[u] = s.list[at]; });
+            } else {
+                for (unsigned k = threadIdx.x; k < n; k += WAVES * 64) worths[s.list[k]] = s.worth[k];
+                __syncthreads();
+            }
         }
-        Range<unsigned long long> keys;
-        span.visit(get, [&](int, unsigned, bool is, unsigned long long v) { keys.add(is ? v : 0ull); });
-        keys.join(s.pick);
-        bound = find_bound<WAVES, KEYS, unsigned long long>(span, keys, (unsigned)a.count, s.pick, get);
+        if (open <= kOpen && KEYS > 0) {
+            taken = emit(span, s.pick, get, is_in, none, 0u, take);
+        } else {  // the worths are in memory, in the pages' places
+            const Span<WAVES, 0> all(pages);
+            auto key = [&](int, unsigned i) {
+                const unsigned k = entries[i];
+                return is_in(k) ? ~0ull : is_open(k) ? worths[i] : 0ull;
+            };
+            Range<unsigned long long> keys;
+            all.visit(key, [&](int, unsigned, bool is, unsigned long long k) { keys.add(is ? k : 0ull); });
+            keys.join(s.pick);
+            taken = emit_taken<WAVES, 0, unsigned long long>(all, find_bound<WAVES, 0, unsigned long long>(all, keys, (unsigned)a.count, s.pick, key), s.pick, key, take);
+        }
     }
-    const unsigned taken = emit_taken<WAVES, KEYS, unsigned long long>(span, bound, s.pick, get, [&](unsigned place, unsigned i) { put_int(to + place, (int)i); });
     for (unsigned i = taken + threadIdx.x; i < (unsigned)a.count; i += WAVES * 64) put_int(to + i, -1);
-}
-
-template <typename T, int D>
-__global__ __launch_bounds__(256) void page_screen_kernel(SelectArgs a) {
-    hook_entry(a.notifier, a.job_id);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, a.splits);
-    const int t = (int)by_split.q, h = (int)by_head.r;
-    int seq, j;
-    if (row_owner(a.starts, a.sequences, a.max_new, t, lane, &seq, &j)) {
-        const unsigned pages = (unsigned)a.prefix_pages + (unsigned)own_pages(__builtin_amdgcn_readfirstlane(a.past[seq]), j, a.page_size, a.max_pages);
-        f32x2* const entries = a.entries + ((size_t)t * a.kv_heads.d + h) * a.pitch;
-        screen_pages<T, D>(a, t, seq, h, pages, by_split.r * 4 + wave, a.splits.d * 4, [&](unsigned e, f32x2 x) { put_pair(entries + e, x.x, x.y); });
-    }
-    hook_exit(a.notifier, a.job_id);
 }
 
 template <int WAVES, int KEYS>
@@ -416,9 +465,8 @@ __global__ __launch_bounds__(WAVES * 64) void page_pick_kernel(SelectArgs a) {
     int seq, j;
     if (row_owner(a.starts, a.sequences, a.max_new, t, lane, &seq, &j)) {
         const unsigned pages = (unsigned)a.prefix_pages + (unsigned)own_pages(__builtin_amdgcn_readfirstlane(a.past[seq]), j, a.page_size, a.max_pages);
-        unsigned long long* const entries = reinterpret_cast<unsigned long long*>(a.entries) + (size_t)blockIdx.x * a.pitch;
-        pick_pages<WAVES, KEYS>(
-            a, t, seq, h, pages, a.pages + (size_t)blockIdx.x * a.count, space, [&](unsigned i) { return entries[i]; }, [&](unsigned i, unsigned long long k) { entries[i] = k; });
+        const size_t row = blockIdx.x;
+        pick_pages<WAVES, KEYS>(a, t, seq, h, pages, a.entries + row * a.pitch, a.errors + row * 4 * a.splits.d, a.worths + row * a.pitch, a.pages + row * a.count, space);
     }
     hook_exit(a.notifier, a.job_id);
 }
@@ -469,13 +517,13 @@ __global__ __launch_bounds__(WAVES * 64) void evict_pick_kernel(EvictArgs a) {
 }
 
 // Tokens move to lower places, in order: a workgroup takes some bytes of every key, or of every value, of a sequence's key head through, a run of tokens at a time, all of which it has read
-// before it writes the first.  What later runs read lies behind everything that earlier ones wrote, and no two workgroups touch the same bytes, so nothing waits for another workgroup, and a
-// run's reads go out ahead of the writes of the one before it.
-constexpr int kMoveAhead = 4;   // tokens of a lane in a run
+// before it writes the first.  What later runs read lies behind everything that earlier ones wrote, and no two workgroups touch the same bytes, so nothing waits for another workgroup.
 
 // 16 bytes that go through to memory.  (The wait states are those between a store and the next write of its registers.)
 __device__ __forceinline__ void put16(char* p, u32x4 v) { asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(p), "v"(v) : "memory"); }
 
+// AHEAD: tokens of a lane in a run.
+template <int AHEAD>
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
     hook_entry(a.notifier, a.job_id);
     const Quotient by_slice = divide(blockIdx.x, a.slices), by_head = divide(by_slice.q, a.kv_heads);
@@ -506,44 +554,46 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
             const unsigned lanes_log2 = a.slice_log2 - 4, tokens = 256u >> lanes_log2;  // side by side
             const unsigned piece = ((slice < half ? slice : slice - half) << a.slice_log2) + (threadIdx.x & ((1u << lanes_log2) - 1)) * 16;
             const unsigned mine = threadIdx.x >> lanes_log2;
-            // a token's bytes, or nullptr where it is in no page
-            auto at = [&](unsigned token) -> char* {
-                const Quotient p = divide(token, a.pages);
-                const int page = p.q < (unsigned)a.max_pages ? table[p.q] : -1;
-                return (unsigned)page < (unsigned)a.num_pages ? cache + (((size_t)page * a.kv_heads.d + h) * a.page_size + p.r) * a.row_bytes + piece : nullptr;
-            };
-            u32x4 x[kMoveAhead];
-            char* to[kMoveAhead];
-            auto read = [&](unsigned first) {
+            const bool in = piece < (unsigned)a.row_bytes;
+            const unsigned run = tokens * AHEAD;
+            int from[AHEAD];  // of the next run, known ahead
+            auto look = [&](unsigned first) {
 #pragma unroll
-                for (int u = 0; u < kMoveAhead; ++u) {
+                for (int u = 0; u < AHEAD; ++u) {
                     const unsigned i = first + u * tokens + mine;
-                    const int from = i < keep && piece < (unsigned)a.row_bytes ? kept[i] : -1;
-                    const char* whence = nullptr;
-                    to[u] = nullptr;
-                    if (from >= 0 && (unsigned)from != i) {
-                        whence = at((unsigned)from);
-                        to[u] = at(i);
-                    }
-                    if (!whence) to[u] = nullptr;
-                    if (to[u]) x[u] = *reinterpret_cast<const u32x4*>(whence);
+                    from[u] = kept[min(i, keep - 1)];
+                    if (!in || i >= keep || (unsigned)from[u] == i) from[u] = -1;
                 }
             };
-            read(0);
-            for (unsigned first = 0; first < keep; first += tokens * kMoveAhead) {
-                u32x4 y[kMoveAhead];
-                char* p[kMoveAhead];
+            look(0);
+            for (unsigned first = 0; first < keep; first += run) {
+                int page[AHEAD], page_to[AHEAD];
+                unsigned slot[AHEAD], slot_to[AHEAD];
 #pragma unroll
-                for (int u = 0; u < kMoveAhead; ++u) {
-                    y[u] = x[u];
-                    p[u] = to[u];
+                for (int u = 0; u < AHEAD; ++u) {  // (a token that does not move: the first one's page, which is there)
+                    const Quotient p = divide(from[u] < 0 ? 0u : (unsigned)from[u], a.pages), q = divide(from[u] < 0 ? 0u : first + u * tokens + mine, a.pages);
+                    page[u] = table[min(p.q, (unsigned)a.max_pages - 1)];
+                    page_to[u] = table[min(q.q, (unsigned)a.max_pages - 1)];
+                    slot[u] = p.r;
+                    slot_to[u] = q.r;
+                    if (from[u] < 0 || p.q >= (unsigned)a.max_pages || q.q >= (unsigned)a.max_pages) page_to[u] = -1;
                 }
+                u32x4 x[AHEAD];
+                char* to[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    to[u] = nullptr;
+                    if ((unsigned)page[u] < (unsigned)a.num_pages && (unsigned)page_to[u] < (unsigned)a.num_pages) {
+                        to[u] = cache + (((size_t)page_to[u] * a.kv_heads.d + h) * a.page_size + slot_to[u]) * a.row_bytes + piece;
+                        x[u] = *reinterpret_cast<const u32x4*>(cache + (((size_t)page[u] * a.kv_heads.d + h) * a.page_size + slot[u]) * a.row_bytes + piece);
+                    }
+                }
+                if (first + run < keep) look(first + run);
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads();
-                if (first + tokens * kMoveAhead < keep) read(first + tokens * kMoveAhead);
 #pragma unroll
-                for (int u = 0; u < kMoveAhead; ++u)
-                    if (p[u]) put16(p[u], y[u]);
+                for (int u = 0; u < AHEAD; ++u)
+                    if (to[u]) put16(to[u], x[u]);
             }
         }
     } else if (slice == a.slices.d - 1 && h == 0 && threadIdx.x == 0) {
@@ -590,6 +640,7 @@ struct PickForm {
 };
 PickForm<SelectKernel> page_pick(int64_t n) {
     if (n <= 1024) return {page_pick_kernel<4, 4>, 256};
+    if (n <= 2048) return {page_pick_kernel<4, 8>, 256};
     if (n <= 4096) return {page_pick_kernel<16, 4>, 1024};
     if (n <= 16384) return {page_pick_kernel<16, 16>, 1024};
     return {page_pick_kernel<16, 0>, 1024};
@@ -602,29 +653,39 @@ PickForm<EvictKernel> evict_pick(int64_t n) {
     return {evict_pick_kernel<16, 0>, 1024};
 }
 
+int64_t select_tiles(const paella_page_select_plan* p) { return ceil_div(std::min(p->max_new, p->tokens), tokens_of_tile(p->heads / p->kv_heads)); }
+int64_t screen_grid(const paella_page_select_plan* p) { return p->sequences * select_tiles(p) * p->kv_heads * p->splits; }
 int64_t select_pages(const paella_page_select_plan* p) { return ceil_div(p->prefix_len, p->page_size) + p->max_pages; }
 
 bool select_plan_ok(const paella_page_select_plan* p) {
     if (!p || !planned_extents_ok(p) || p->count <= 0 || p->first < 0 || p->last < 1 || (int64_t)p->first + p->last > p->count || p->splits <= 0) return false;
     if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256) return false;
     const double rows = (double)p->tokens * p->kv_heads;
-    return rows * p->splits <= kMostWorkgroups && rows * p->count < 2147483648.0 && select_pages(p) < (1 << 30);
+    return rows <= kMostWorkgroups / 4 && (double)p->sequences * select_tiles(p) * p->kv_heads * p->splits <= kMostWorkgroups && rows * p->count < 2147483648.0 && select_pages(p) < (1 << 30);
 }
 
 size_t select_pitch(const paella_page_select_plan* p) { return (size_t)(select_pages(p) + 15) / 16 * 16; }
-size_t select_workspace(const paella_page_select_plan* p) { return (size_t)p->tokens * p->kv_heads * select_pitch(p) * 8; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+size_t select_errors(const paella_page_select_plan* p) { return up256((size_t)p->tokens * p->kv_heads * p->splits * 16); }
+size_t select_entries(const paella_page_select_plan* p) { return up256((size_t)p->tokens * p->kv_heads * select_pitch(p) * 4); }
+size_t select_workspace(const paella_page_select_plan* p) { return select_errors(p) + 3 * select_entries(p); }  // errors, entries, worths in 64 bits
 
-// Bytes of a row that a workgroup moves.
-int evict_slice_log2(const paella_kv_cache* c) {
-    (void)c;
-    return 6;
+// Bytes of a row that a workgroup moves: 128, which memory likes best, where that still makes two workgroups for each compute unit, else 64, or 32 where even those leave half of the device
+// idle.  (bf16 heads of 128, 4096 tokens kept: 24 sequences of 8 heads by 128 / 64 bytes 192 / 247 us, 4 sequences 89 / 53; fp32 heads of 64, 1000 tokens of 2 heads by 64 / 32 bytes 10 / XX.)
+int evict_slice_log2(int sequences, const paella_kv_cache* c) {
+    const int64_t heads = (int64_t)sequences * c->kv_heads, row = (int64_t)c->head_dim * element_bytes(c->dtype);
+    return 2 * heads * ceil_div(row, 128) >= 512 ? 7 : 2 * heads * ceil_div(row, 64) >= 128 ? 6 : 5;
 }
-int64_t evict_slices(const paella_kv_cache* c) { return 2 * ceil_div((int64_t)c->head_dim * element_bytes(c->dtype), 1 << evict_slice_log2(c)) + 1; }
+int64_t evict_slices(int sequences, const paella_kv_cache* c) {
+    return 2 * ceil_div((int64_t)c->head_dim * element_bytes(c->dtype), 1 << evict_slice_log2(sequences, c)) + 1;
+}
+using MoveKernel = void (*)(EvictArgs);
+MoveKernel move_kernel(int slice_log2) { return slice_log2 == 7 ? evict_move_kernel<8> : evict_move_kernel<16>; }
 
 int evict_check(const paella_kv_evict_desc* d, const paella_kv_cache* c) {
     if (!d || !cache_extents_ok(c) || d->sequences <= 0 || d->max_pages <= 0 || d->keep <= 0 || d->first < 0 || d->recent < 0 || (int64_t)d->first + d->recent > d->keep) return PAELLA_EINVAL;
     const double heads = (double)d->sequences * c->kv_heads;
-    if ((double)d->max_pages * c->page_size >= 1073741824.0 || heads * evict_slices(c) > kMostWorkgroups || (double)d->sequences * d->max_pages >= 2147483648.0) return PAELLA_ENOSUP;
+    if ((double)d->max_pages * c->page_size >= 1073741824.0 || heads * evict_slices(d->sequences, c) > kMostWorkgroups || (double)d->sequences * d->max_pages >= 2147483648.0) return PAELLA_ENOSUP;
     return 0;
 }
 
@@ -665,11 +726,13 @@ int paella_page_select_plan_make(const paella_kv_cache* c, const paella_kv_batch
     p->count = count; p->first = first; p->last = last;
     const int64_t pages = select_pages(p), rows = (int64_t)p->tokens * p->kv_heads;
     // enough workgroups to fill the device, none without a turn for each wave
-    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(2048, rows), ceil_div(pages, 4 * kScreened)));
+    p->splits = 1;
+    if (!select_plan_ok(p)) return PAELLA_ENOSUP;
+    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(1024, screen_grid(p)), ceil_div(pages, 4 * kScreened)));
     if (!select_plan_ok(p)) return PAELLA_ENOSUP;
     p->stages = 2;
     p->workspace_bytes = select_workspace(p);
-    set_launch_dims(&p->dims, (unsigned)(rows * p->splits), 256, 0, 128);
+    set_launch_dims(&p->dims, (unsigned)screen_grid(p), 256, 0, 128);
     const double size = element_bytes(c->dtype);
     p->flops = 4.0 * p->tokens * p->heads * pages * p->head_dim;
     p->bytes = 2.0 * (pages - p->max_pages + (double)p->sequences * p->max_pages) * p->kv_heads * p->head_dim * size + (double)p->tokens * p->heads * p->head_dim * size + 4.0 * rows * count;
@@ -680,7 +743,7 @@ int paella_page_select_dims(const paella_page_select_plan* p, int stage, paella_
     if (!select_plan_ok(p) || !dims || stage < 0 || stage > 1) return PAELLA_EINVAL;
     const auto pick = page_pick(select_pages(p));
     if (stage) set_launch_dims(dims, (unsigned)(p->tokens * p->kv_heads), pick.threads, 0, 64);
-    else set_launch_dims(dims, (unsigned)(p->tokens * p->kv_heads * p->splits), 256, 0, 128);
+    else set_launch_dims(dims, (unsigned)screen_grid(p), 256, 0, 128);
     loaded_dims(stage ? (const void*)pick.kernel : (const void*)screen_kernel(p), dims);
     return 0;
 }
@@ -699,14 +762,15 @@ int paella_page_select_launch_stage(const paella_page_select_plan* p, int stage,
     SelectArgs a;
     a.q = (const char*)q; a.bounds = (const char*)bounds;
     a.starts = b->starts; a.past = b->past; a.tables = b->tables; a.prefix_table = b->prefix_table;
-    a.entries = (f32x2*)workspace; a.pages = pages; a.q_stride = q_stride * size;
+    a.errors = (float*)workspace; a.entries = (unsigned*)((char*)workspace + select_errors(p)); a.worths = (unsigned long long*)((char*)a.entries + select_entries(p)); a.pages = pages; a.q_stride = q_stride * size;
     a.sequences = b->sequences; a.tokens = b->tokens; a.max_pages = b->max_pages; a.prefix_pages = (int)ceil_div(b->prefix_len, c->page_size); a.num_pages = c->num_pages;
     a.heads = p->heads; a.first = p->first; a.last = p->last; a.count = p->count; a.dim = p->head_dim; a.dtype = p->dtype; a.pitch = (unsigned)select_pitch(p);
-    a.max_new = divisor((unsigned)b->max_new); a.kv_heads = divisor((unsigned)p->kv_heads); a.splits = divisor((unsigned)p->splits); a.page_size = divisor((unsigned)c->page_size);
+    a.max_new = divisor((unsigned)b->max_new); a.kv_heads = divisor((unsigned)p->kv_heads); a.per_kv = divisor((unsigned)(p->heads / p->kv_heads)); a.splits = divisor((unsigned)p->splits);
+    a.tiles = divisor((unsigned)select_tiles(p)); a.page_size = divisor((unsigned)c->page_size);
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
     const unsigned rows = (unsigned)(p->tokens * p->kv_heads);
     if (stage == 0) {
-        launch(screen_kernel(p), dim3(rows * (unsigned)p->splits), dim3(256), 0, (hipStream_t)stream, a);
+        launch(screen_kernel(p), dim3((unsigned)screen_grid(p)), dim3(256), 0, (hipStream_t)stream, a);
     } else {
         const auto pick = page_pick(select_pages(p));
         launch(pick.kernel, dim3(rows), dim3(pick.threads), 0, (hipStream_t)stream, a);
@@ -725,10 +789,10 @@ int paella_page_select_launch(const paella_page_select_plan* p, const paella_kv_
 int paella_kv_evict_dims(const paella_kv_evict_desc* d, const paella_kv_cache* c, int stage, paella_launch_dims* dims) {
     if (int rc = evict_check(d, c)) return rc;
     if (!dims || stage < 0 || stage > 1) return PAELLA_EINVAL;
-    if (stage) set_launch_dims(dims, (unsigned)(d->sequences * c->kv_heads * evict_slices(c)), 256, 0, 64);
+    if (stage) set_launch_dims(dims, (unsigned)(d->sequences * c->kv_heads * evict_slices(d->sequences, c)), 256, 0, 64);
     const auto pick = evict_pick((int64_t)d->max_pages * c->page_size);
     if (!stage) set_launch_dims(dims, (unsigned)(d->sequences * c->kv_heads), pick.threads, 0, 64);
-    loaded_dims(stage ? (const void*)evict_move_kernel : (const void*)pick.kernel, dims);
+    loaded_dims(stage ? (const void*)move_kernel(evict_slice_log2(d->sequences, c)) : (const void*)pick.kernel, dims);
     return 0;
 }
 
@@ -749,12 +813,12 @@ int paella_kv_evict_launch_stage(const paella_kv_evict_desc* d, int stage, const
     a.k_cache = (char*)c->k; a.v_cache = (char*)c->v; a.weights = weights; a.past = past; a.tables = tables; a.kept = kept; a.past_out = past_out;
     a.sequences = d->sequences; a.max_pages = d->max_pages; a.num_pages = c->num_pages; a.page_size = c->page_size; a.row_bytes = c->head_dim * element_bytes(c->dtype);
     a.keep = d->keep; a.first = d->first; a.recent = d->recent; a.places = (unsigned)(d->max_pages * c->page_size);
-    a.kv_heads = divisor((unsigned)c->kv_heads); a.slices = divisor((unsigned)evict_slices(c)); a.pages = divisor((unsigned)c->page_size);
+    a.kv_heads = divisor((unsigned)c->kv_heads); a.slices = divisor((unsigned)evict_slices(d->sequences, c)); a.pages = divisor((unsigned)c->page_size);
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
-    a.slice_log2 = (unsigned)evict_slice_log2(c);
+    a.slice_log2 = (unsigned)evict_slice_log2(d->sequences, c);
     const auto pick = evict_pick((int64_t)a.places);
     if (stage == 0) launch(pick.kernel, dim3((unsigned)(d->sequences * c->kv_heads)), dim3(pick.threads), 0, (hipStream_t)stream, a);
-    else launch(evict_move_kernel, dim3((unsigned)(d->sequences * c->kv_heads * evict_slices(c))), dim3(256), 0, (hipStream_t)stream, a);
+    else launch(move_kernel((int)a.slice_log2), dim3((unsigned)(d->sequences * c->kv_heads * evict_slices(d->sequences, c))), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 

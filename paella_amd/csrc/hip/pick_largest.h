@@ -47,11 +47,12 @@ struct Span {
     }
 };
 
-constexpr unsigned kRanked = 256;  // candidates that are ranked against each other: one of each thread, and the ranking no longer than another histogram
+constexpr unsigned kRanked = 128;  // candidates that are ranked against each other: that takes no longer than another histogram
+constexpr int kDigit = 10;         // bits of a digit: of thousands of keys, few are left behind the first histogram
 
 template <int WAVES>
 struct PickSpace {
-    unsigned bins[256];
+    __attribute__((aligned(16))) unsigned bins[1 << kDigit];
     unsigned long long list[kRanked];
     unsigned long long low[WAVES], high[WAVES], bound;
     unsigned count[3][WAVES];
@@ -69,9 +70,46 @@ __device__ __forceinline__ unsigned long long number_key(double v, unsigned long
     return v != v ? nan : b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
 }
 
-__device__ __forceinline__ unsigned long long shuffle_xor64(unsigned long long b, int mask) {
-    const unsigned lo = (unsigned)__shfl_xor((int)(unsigned)b, mask, 64), hi = (unsigned)__shfl_xor((int)(unsigned)(b >> 32), mask, 64);
-    return (unsigned long long)hi << 32 | lo;
+// op of all lanes' whole numbers, the same for the whole wave.
+template <typename Op>
+__device__ __forceinline__ unsigned wave_all(unsigned v, Op op) {
+    v = row_all(v, op);
+    return op(op((unsigned)__builtin_amdgcn_readlane((int)v, 0), (unsigned)__builtin_amdgcn_readlane((int)v, 16)),
+              op((unsigned)__builtin_amdgcn_readlane((int)v, 32), (unsigned)__builtin_amdgcn_readlane((int)v, 48)));
+}
+template <typename Op>
+__device__ __forceinline__ unsigned long long wave_all(unsigned long long v, Op op) {
+    v = row_all(v, op);
+    auto at = [&](int lane) {
+        return (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), lane) << 32 | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, lane);
+    };
+    return op(op(at(0), at(16)), op(at(32), at(48)));
+}
+struct Least {
+    template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return min(a, b); }
+};
+struct Most {
+    template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return max(a, b); }
+};
+struct Sum {
+    template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
+};
+// Of the waves' values in LDS.
+template <int WAVES, typename V, typename Op>
+__device__ __forceinline__ V waves_all(const V (&of)[WAVES], Op op) {
+    if constexpr (WAVES == 16) {
+        return row_all(of[threadIdx.x & 15], op);
+    } else {
+        V v = of[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v = op(v, of[w]);
+        return v;
+    }
+}
+template <typename V> __device__ __forceinline__ V uniform(V v) { return v; }
+template <> __device__ __forceinline__ unsigned uniform(unsigned v) { return (unsigned)__builtin_amdgcn_readfirstlane((int)v); }
+template <> __device__ __forceinline__ unsigned long long uniform(unsigned long long v) {
+    return (unsigned long long)uniform((unsigned)(v >> 32)) << 32 | uniform((unsigned)v);
 }
 
 // The least and largest of the keys that are not 0, and how many there are, over all threads.
@@ -89,16 +127,9 @@ struct Range {
     template <int WAVES>
     __device__ __forceinline__ void join(PickSpace<WAVES>& s) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        for (int off = 32; off; off >>= 1) {
-            if constexpr (sizeof(Key) == 8) {
-                least = min(least, (Key)shuffle_xor64(least, off));
-                most = max(most, (Key)shuffle_xor64(most, off));
-            } else {
-                least = min(least, (Key)__shfl_xor((int)least, off, 64));
-                most = max(most, (Key)__shfl_xor((int)most, off, 64));
-            }
-            some += __shfl_xor((int)some, off, 64);
-        }
+        least = wave_all(least, Least());
+        most = wave_all(most, Most());
+        some = wave_all(some, Sum());
         __syncthreads();
         if (lane == 0) {
             s.low[wave] = least;
@@ -106,13 +137,9 @@ struct Range {
             s.count[0][wave] = some;
         }
         __syncthreads();
-        some = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            least = min(least, (Key)s.low[w]);
-            most = max(most, (Key)s.high[w]);
-            some += s.count[0][w];
-        }
+        least = (Key)uniform(waves_all(s.low, Least()));
+        most = (Key)uniform(waves_all(s.high, Most()));
+        some = uniform(waves_all(s.count[0], Sum()));
     }
 };
 
@@ -131,24 +158,27 @@ __device__ __forceinline__ Bound<Key> find_bound(const Span<WAVES, KEYS>& span, 
     const int lane = threadIdx.x & 63;
     const int differ = range.least == range.most ? 0 : 64 - __clzll((unsigned long long)(range.least ^ range.most));  // bits; those above are the same in all keys
     if (!differ) return {range.most, want};
-    int shift = max(differ - 8, 0);
-    Key known = shift + 8 < (int)sizeof(Key) * 8 ? (Key)(~(Key)0 << (shift + 8)) : (Key)0;  // the bits that the bound has so far
+    int shift = max(differ - kDigit, 0);
+    Key known = shift + kDigit < (int)sizeof(Key) * 8 ? (Key)(~(Key)0 << (shift + kDigit)) : (Key)0;  // the bits that the bound has so far
     Key bound = range.most & known;
     unsigned left = want, size = range.some;
     while (size > kRanked) {
         __syncthreads();
-        if (threadIdx.x < 256) s.bins[threadIdx.x] = 0;
+        for (unsigned b = threadIdx.x; b < 1u << kDigit; b += WAVES * 64) s.bins[b] = 0;
         __syncthreads();
         span.visit(get, [&](int, unsigned, bool is, Key k) {
-            if (is && k && (k & known) == bound) atomicAdd(&s.bins[(unsigned)(k >> shift) & 255u], 1u);
+            if (is && k && (k & known) == bound) atomicAdd(&s.bins[(unsigned)(k >> shift) & ((1u << kDigit) - 1)], 1u);
         });
         __syncthreads();
-        if (threadIdx.x < 64) {  // four digits a lane, the highest first
-            unsigned c[4], sum = 0;
+        if (threadIdx.x < 64) {  // some digits a lane, the highest first
+            constexpr int EACH = (1 << kDigit) / 64;
+            const u32x4* const mine = reinterpret_cast<const u32x4*>(s.bins) + (63 - lane) * (EACH / 4);
+            u32x4 c[EACH / 4];
+            unsigned sum = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                c[e] = s.bins[255 - (lane * 4 + e)];
-                sum += c[e];
+            for (int e = 0; e < EACH / 4; ++e) {
+                c[e] = mine[e];
+                sum += c[e].x + c[e].y + c[e].z + c[e].w;
             }
             unsigned upto = sum;
             for (int off = 1; off < 64; off <<= 1) {
@@ -158,13 +188,14 @@ __device__ __forceinline__ Bound<Key> find_bound(const Span<WAVES, KEYS>& span, 
             unsigned before = upto - sum;
             if (before < left && left <= upto) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (before < left && left <= before + c[e]) {
-                        s.digit = 255 - (lane * 4 + e);
+                for (int e = EACH - 1; e >= 0; --e) {
+                    const unsigned here = c[e / 4][e % 4];
+                    if (before < left && left <= before + here) {
+                        s.digit = (63 - lane) * EACH + e;
                         s.left = left - before;
-                        s.size = c[e];
+                        s.size = here;
                     }
-                    before += c[e];
+                    before += here;
                 }
             }
         }
@@ -172,10 +203,10 @@ __device__ __forceinline__ Bound<Key> find_bound(const Span<WAVES, KEYS>& span, 
         bound |= (Key)s.digit << shift;
         left = s.left;
         size = s.size;
-        known |= (Key)255 << shift;
+        known |= (Key)((1u << kDigit) - 1) << shift;
         if (size == left) return {bound, ~0u};  // all that begin so
         if (shift == 0) return {bound, left};
-        shift = max(shift - 8, 0);
+        shift = max(shift - kDigit, 0);
     }
     __syncthreads();
     if (threadIdx.x == 0) s.found = 0;
@@ -202,26 +233,27 @@ __device__ __forceinline__ Bound<Key> find_bound(const Span<WAVES, KEYS>& span, 
     return {(Key)s.bound, s.left};
 }
 
-// take(place, i) for what is taken, in order; returns how many.
-template <int WAVES, int KEYS, typename Key, typename Get, typename Take>
-__device__ __forceinline__ unsigned emit_taken(const Span<WAVES, KEYS>& span, Bound<Key> b, PickSpace<WAVES>& s, Get get, Take take) {
+// take(place, i) for every place whose value above(value), and for the first `left` of those whose value is tied(value), in order; returns how many.
+template <int WAVES, int KEYS, typename Get, typename Above, typename Tied, typename Take>
+__device__ __forceinline__ unsigned emit(const Span<WAVES, KEYS>& span, PickSpace<WAVES>& s, Get get, Above above, Tied tied, unsigned left, Take take) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    unsigned above = 0, equal = 0;
-    span.visit(get, [&](int, unsigned, bool is, Key k) {
-        if (!is) k = 0;
-        above += __popcll(__ballot(b.left == ~0u ? k >= b.bound : k > b.bound));
-        equal += __popcll(__ballot(b.left != ~0u && k == b.bound));
+    unsigned more = 0, equal = 0;
+    span.visit(get, [&](int, unsigned, bool is, auto k) {
+        more += is && above(k);
+        if (left) equal += is && tied(k);
     });
+    more = wave_all(more, Sum());
+    if (left) equal = wave_all(equal, Sum());
     __syncthreads();
     if (lane == 0) {
-        s.count[1][wave] = above;
+        s.count[1][wave] = more;
         s.count[2][wave] = equal;
     }
     __syncthreads();
     unsigned place = 0, ties = 0, all = 0, ties_all = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-        const unsigned here = b.left == ~0u ? 0u : min(s.count[2][w], b.left - min(b.left, ties_all));
+        const unsigned here = min(s.count[2][w], left - min(left, ties_all));
         if (w < wave) {
             place += s.count[1][w] + here;
             ties += s.count[2][w];
@@ -229,17 +261,29 @@ __device__ __forceinline__ unsigned emit_taken(const Span<WAVES, KEYS>& span, Bo
         all += s.count[1][w] + here;
         ties_all += s.count[2][w];
     }
+    place = uniform(place);
+    ties = uniform(ties);
     const unsigned long long before = (1ull << lane) - 1;
-    span.visit(get, [&](int, unsigned i, bool is, Key k) {
-        if (!is) k = 0;
-        const unsigned long long tied = __ballot(b.left != ~0u && k == b.bound);
-        const bool mine = b.left == ~0u ? k >= b.bound : k > b.bound || (k == b.bound && ties + __popcll(tied & before) < b.left);
+    span.visit(get, [&](int, unsigned i, bool is, auto k) {
+        bool mine = is && above(k);
+        if (left) {
+            const unsigned long long who = __ballot(is && tied(k));
+            mine |= is && tied(k) && ties + (unsigned)__popcll(who & before) < left;
+            ties += (unsigned)__popcll(who);
+        }
         const unsigned long long who = __ballot(mine);
-        if (mine) take(place + __popcll(who & before), i);
-        place += __popcll(who);
-        ties += __popcll(tied);
+        if (who) {
+            if (mine) take(place + (unsigned)__popcll(who & before), i);
+            place += (unsigned)__popcll(who);
+        }
     });
-    return all;
+    return uniform(all);
+}
+
+template <int WAVES, int KEYS, typename Key, typename Get, typename Take>
+__device__ __forceinline__ unsigned emit_taken(const Span<WAVES, KEYS>& span, Bound<Key> b, PickSpace<WAVES>& s, Get get, Take take) {
+    const Key from = b.left == ~0u ? b.bound : b.bound + 1;  // (no bound of which only some are taken is all ones)
+    return emit(span, s, get, [&](Key k) { return k >= from; }, [&](Key k) { return k == b.bound; }, b.left == ~0u ? 0u : b.left, take);
 }
 
 }  // namespace paella
