@@ -118,9 +118,12 @@ __global__ __launch_bounds__(256) void page_bounds_kernel(BoundsArgs a) {
 // digits, in 64 bits; but nearly all pages are far from the border.  So the matrix units take the worths in 32 bits, at the rate that memory delivers the bounds, together with how far each can
 // be off: of a sum of 2 D products, half of them 0, by (2 D + 8) * 2^-24 of the sum of their magnitudes, q+ . |high| - q- . |low|.  Pages that are further from the border than
 // that are decided; the few others, if they are not all taken or none of them, get their worths in 64 bits.  (All of them in 64 bits by the vector unit: 58 us for 32 rows of 1024 pages of 8 heads of 128 in bf16, 100 MB.)
+constexpr int kCounterStride = 32;  // a cache line each
+
 struct SelectArgs {
     const char *q, *bounds;
     const int *starts, *past, *tables, *prefix_table;
+    unsigned* counters;          // [tokens][kv_heads][kCounterStride], zero between launches
     unsigned* entries;           // [tokens][kv_heads][pitch]
     float* errors;               // [tokens][kv_heads][4 * splits]: how far the worths can be off, over (2 D + 8) * 2^-24
     unsigned long long* worths;  // [tokens][kv_heads][pitch]
@@ -165,19 +168,35 @@ constexpr int kScreened = 16;  // pages of a wave's turn
 // New tokens of a sequence whose heads for one key head make up a tile of 16 rows: the bounds are read once for all of them.
 __host__ __device__ constexpr int tokens_of_tile(int heads) { return heads >= 16 ? 1 : 16 / heads; }
 
+// What a workgroup of the screen works on: the tile's tokens from j0 on, for one key head, and its part of their pages.
+struct Screened {
+    int h, seq, j0, n, split;
+    NewTokens its;
+    __device__ __forceinline__ explicit Screened(const SelectArgs& a) {
+        const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, a.splits), by_tile = divide(by_split.q, a.tiles);
+        const int each = tokens_of_tile((int)a.per_kv.d);
+        h = (int)by_head.r;
+        split = (int)by_split.r;
+        seq = (int)by_tile.q;
+        j0 = (int)by_tile.r * each;
+        its = new_tokens(a.starts, a.past, seq, (int)a.max_new.d, a.tokens);
+        n = min(its.count - j0, each);
+    }
+    __device__ __forceinline__ unsigned pages(const SelectArgs& a, int j) const {
+        return (unsigned)a.prefix_pages + (unsigned)own_pages(its.past, j0 + j, a.page_size, a.max_pages);
+    }
+};
+
 // A turn's bounds go to registers while the ones before are worked on, and the numbers of the pages behind them.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void page_screen_kernel(SelectArgs a) {
-    hook_entry(a.notifier, a.job_id);
+__device__ __forceinline__ void screen_pages(const SelectArgs& a, const Screened& w) {
     constexpr int ROW = D * T::bytes, KC = ROW / 64;
     const int lane = threadIdx.x & 63, mm = lane & 15, group = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, a.splits), by_tile = divide(by_split.q, a.tiles);
-    const int h = (int)by_head.r, seq = (int)by_tile.q, heads = (int)a.per_kv.d, each = tokens_of_tile(heads), j0 = (int)by_tile.r * each;
-    const NewTokens its = new_tokens(a.starts, a.past, seq, (int)a.max_new.d, a.tokens);
-    const int n = min(its.count - j0, each);  // tokens here
-    auto pages_of = [&](int j) { return (unsigned)a.prefix_pages + (unsigned)own_pages(its.past, j0 + j, a.page_size, a.max_pages); };
+    const int h = w.h, seq = w.seq, heads = (int)a.per_kv.d, j0 = w.j0, n = w.n;
+    const NewTokens& its = w.its;
+    auto pages_of = [&](int j) { return w.pages(a, j); };
     const unsigned pages = n > 0 ? pages_of(n - 1) : 0u, step = a.splits.d * 4;
-    unsigned turn = by_split.r * 4 + wave;
+    unsigned turn = (unsigned)w.split * 4 + wave;
     float worst = 0.f;
     if (turn * kScreened < pages) {
         const Quotient row = divide((unsigned)min(mm, n * heads - 1), a.per_kv);  // the lane's token and head
@@ -270,8 +289,7 @@ __global__ __launch_bounds__(256) void page_screen_kernel(SelectArgs a) {
         }
     }
     worst = wave_max_f(worst);  // of all rows of the tile
-    if (lane < n) store_out(a.errors + ((size_t)(its.first + j0 + lane) * a.kv_heads.d + h) * step + by_split.r * 4 + wave, worst);
-    hook_exit(a.notifier, a.job_id);
+    if (lane < n) store_out(a.errors + ((size_t)(its.first + j0 + lane) * a.kv_heads.d + h) * step + (unsigned)w.split * 4 + wave, worst);
 }
 
 // A page's worth in 64 bits, by a whole wave: 16 bytes of a row per lane, the bounds and four heads' queries requested together.
@@ -331,14 +349,18 @@ struct PageSpace {
     unsigned long long worth[kOpen];
 };
 
-// The row's pages by their entries.  KEYS as in Span.
-template <int WAVES, int KEYS>
-__device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, int h, unsigned pages, const unsigned* entries, const float* errors, unsigned long long* worths, int* to,
-                                           PageSpace<WAVES>& s) {
+// The row's pages by their entries, which read(address) reads, as it does the errors.  KEYS as in Span.
+template <int WAVES, int KEYS, typename Read>
+__device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, int h, unsigned pages, PageSpace<WAVES>& s, Read read) {
+    const size_t row = (size_t)t * a.kv_heads.d + h;
+    const unsigned* const entries = a.entries + row * a.pitch;
+    const float* const errors = a.errors + row * 4 * a.splits.d;
+    unsigned long long* const worths = a.worths + row * a.pitch;
+    int* const to = a.pages + row * a.count;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const Span<WAVES, KEYS> span(pages);
     unsigned held[KEYS ? KEYS : 1];
-    auto load = [&](unsigned i) { return entries[i]; };
+    auto load = [&](unsigned i) { return read(entries + i); };
     span.hold(held, load);
     auto get = [&](int u, unsigned i) { return KEYS ? held[u] : load(i); };
     auto known = [](unsigned k) { return k > kUnknown && k < kForced ? k : 0u; };
@@ -350,7 +372,7 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
         range.add(is ? known(k) : 0u);
     });
     float error = 0.f;
-    for (unsigned i = threadIdx.x; i < 4 * a.splits.d; i += WAVES * 64) error = fmaxf(error, errors[i]);
+    for (unsigned i = threadIdx.x; i < 4 * a.splits.d; i += WAVES * 64) error = fmaxf(error, read(errors + i));
     error = wave_max_f(error);
     forced = wave_all(forced, Sum());
     unknown = wave_all(unknown, Sum());
@@ -443,7 +465,7 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
         } else {  // the worths are in memory, in the pages' places
             const Span<WAVES, 0> all(pages);
             auto key = [&](int, unsigned i) {
-                const unsigned k = entries[i];
+                const unsigned k = load(i);
                 return is_in(k) ? ~0ull : is_open(k) ? worths[i] : 0ull;
             };
             Range<unsigned long long> keys;
@@ -453,6 +475,13 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
         }
     }
     for (unsigned i = taken + threadIdx.x; i < (unsigned)a.count; i += WAVES * 64) put_int(to + i, -1);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void page_screen_kernel(SelectArgs a) {
+    hook_entry(a.notifier, a.job_id);
+    screen_pages<T, D>(a, Screened(a));
+    hook_exit(a.notifier, a.job_id);
 }
 
 template <int WAVES, int KEYS>
@@ -465,8 +494,42 @@ __global__ __launch_bounds__(WAVES * 64) void page_pick_kernel(SelectArgs a) {
     int seq, j;
     if (row_owner(a.starts, a.sequences, a.max_new, t, lane, &seq, &j)) {
         const unsigned pages = (unsigned)a.prefix_pages + (unsigned)own_pages(__builtin_amdgcn_readfirstlane(a.past[seq]), j, a.page_size, a.max_pages);
-        const size_t row = blockIdx.x;
-        pick_pages<WAVES, KEYS>(a, t, seq, h, pages, a.entries + row * a.pitch, a.errors + row * 4 * a.splits.d, a.worths + row * a.pitch, a.pages + row * a.count, space);
+        pick_pages<WAVES, KEYS>(a, t, seq, h, pages, space, [](auto* p) { return *p; });
+    }
+    hook_exit(a.notifier, a.job_id);
+}
+
+// One launch for both: the workgroup that arrives last at a row picks its pages, while others are still screening.  (Entries are written through ahead of the count, and read past this XCD's
+// caches.)
+constexpr int kSelectKeys = 8;  // of a thread: up to 2048 pages
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void page_select_kernel(SelectArgs a) {
+    hook_entry(a.notifier, a.job_id);
+    __shared__ PageSpace<4> space;
+    __shared__ unsigned arrived;
+    const Screened w(a);
+    if (w.n > 0) {
+        screen_pages<T, D>(a, w);
+        if (a.splits.d > 1) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                unsigned* const counter = a.counters + ((size_t)(w.its.first + w.j0) * a.kv_heads.d + w.h) * kCounterStride;
+                arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (arrived == a.splits.d - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        __syncthreads();
+        if (a.splits.d == 1 || arrived == a.splits.d - 1) {
+            for (int j = 0; j < w.n; ++j) {
+                if (j) __syncthreads();
+                pick_pages<4, kSelectKeys>(a, w.its.first + w.j0 + j, w.seq, w.h, w.pages(a, j), space,
+                                           [](auto* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
+            }
+        }
     }
     hook_exit(a.notifier, a.job_id);
 }
@@ -627,9 +690,15 @@ int bounds_check(const paella_kv_cache* c, const paella_kv_batch* b) {
 
 using SelectKernel = void (*)(SelectArgs);
 template <typename T>
-SelectKernel screen_kernel_of(int dim) { return dim == 64 ? page_screen_kernel<T, 64> : dim == 128 ? page_screen_kernel<T, 128> : page_screen_kernel<T, 256>; }
-SelectKernel screen_kernel(const paella_page_select_plan* p) {
-    return p->dtype == PAELLA_F32 ? screen_kernel_of<F32>(p->head_dim) : p->dtype == PAELLA_BF16 ? screen_kernel_of<Bf16>(p->head_dim) : screen_kernel_of<F16>(p->head_dim);
+SelectKernel screen_kernel_of(int dim, bool whole) {
+    if (whole) return dim == 64 ? page_select_kernel<T, 64> : dim == 128 ? page_select_kernel<T, 128> : page_select_kernel<T, 256>;
+    return dim == 64 ? page_screen_kernel<T, 64> : dim == 128 ? page_screen_kernel<T, 128> : page_screen_kernel<T, 256>;
+}
+// whole: the kernel that does both stages in one launch
+SelectKernel screen_kernel(const paella_page_select_plan* p, bool whole) {
+    return p->dtype == PAELLA_F32    ? screen_kernel_of<F32>(p->head_dim, whole)
+           : p->dtype == PAELLA_BF16 ? screen_kernel_of<Bf16>(p->head_dim, whole)
+                                     : screen_kernel_of<F16>(p->head_dim, whole);
 }
 
 // A kernel of one of these forms, by how many there are to pick from at most: with their keys in registers, or, beyond what the registers of 16 waves hold, read again for every pass.
@@ -665,10 +734,18 @@ bool select_plan_ok(const paella_page_select_plan* p) {
 }
 
 size_t select_pitch(const paella_page_select_plan* p) { return (size_t)(select_pages(p) + 15) / 16 * 16; }
+// One launch where four waves hold a row's pages in registers, a tile is one token's (a workgroup that picked for several would take as much longer), and the workgroups are at most one to a
+// compute unit; of more, those that pick are in the way of those that still screen.  (3 fp32 rows of 57 pages of 2 heads of 64 in one launch / two 9.4 / 10.5 us, 32 bf16 rows of 1025 pages of 8 heads
+// of 128, 1024 workgroups, 45.2 / 41.3.)
+int select_stages(const paella_page_select_plan* p) {
+    const bool one = std::min(p->max_new, p->tokens) == 1 || tokens_of_tile(p->heads / p->kv_heads) == 1;
+    return one && screen_grid(p) <= 256 && select_pages(p) <= 256 * kSelectKeys ? 1 : 2;
+}
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+size_t select_counters(const paella_page_select_plan* p) { return select_stages(p) == 1 ? (size_t)p->tokens * p->kv_heads * kCounterStride * 4 : 0; }
 size_t select_errors(const paella_page_select_plan* p) { return up256((size_t)p->tokens * p->kv_heads * p->splits * 16); }
 size_t select_entries(const paella_page_select_plan* p) { return up256((size_t)p->tokens * p->kv_heads * select_pitch(p) * 4); }
-size_t select_workspace(const paella_page_select_plan* p) { return select_errors(p) + 3 * select_entries(p); }  // errors, entries, worths in 64 bits
+size_t select_workspace(const paella_page_select_plan* p) { return select_counters(p) + select_errors(p) + 3 * select_entries(p); }  // (worths of 64 bits: twice the entries)
 
 // Bytes of a row that a workgroup moves: 128, which memory likes best, where that still makes two workgroups for each compute unit, else 64, or 32 where even those leave half of the device
 // idle.  (bf16 heads of 128, 4096 tokens kept: 24 sequences of 8 heads by 128 / 64 bytes 192 / 247 us, 4 sequences 89 / 53; fp32 heads of 64, 1000 tokens of 2 heads by 64 / 32 bytes 10 / XX.)
@@ -730,7 +807,7 @@ int paella_page_select_plan_make(const paella_kv_cache* c, const paella_kv_batch
     if (!select_plan_ok(p)) return PAELLA_ENOSUP;
     p->splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(1024, screen_grid(p)), ceil_div(pages, 4 * kScreened)));
     if (!select_plan_ok(p)) return PAELLA_ENOSUP;
-    p->stages = 2;
+    p->stages = select_stages(p);
     p->workspace_bytes = select_workspace(p);
     set_launch_dims(&p->dims, (unsigned)screen_grid(p), 256, 0, 128);
     const double size = element_bytes(c->dtype);
@@ -740,17 +817,17 @@ int paella_page_select_plan_make(const paella_kv_cache* c, const paella_kv_batch
 }
 
 int paella_page_select_dims(const paella_page_select_plan* p, int stage, paella_launch_dims* dims) {
-    if (!select_plan_ok(p) || !dims || stage < 0 || stage > 1) return PAELLA_EINVAL;
+    if (!select_plan_ok(p) || !dims || stage < 0 || stage >= select_stages(p)) return PAELLA_EINVAL;
     const auto pick = page_pick(select_pages(p));
     if (stage) set_launch_dims(dims, (unsigned)(p->tokens * p->kv_heads), pick.threads, 0, 64);
     else set_launch_dims(dims, (unsigned)screen_grid(p), 256, 0, 128);
-    loaded_dims(stage ? (const void*)pick.kernel : (const void*)screen_kernel(p), dims);
+    loaded_dims(stage ? (const void*)pick.kernel : (const void*)screen_kernel(p, select_stages(p) == 1), dims);
     return 0;
 }
 
 int paella_page_select_launch_stage(const paella_page_select_plan* p, int stage, const paella_kv_cache* c, const paella_kv_batch* b, const void* q, int64_t q_stride,
                                     const void* bounds, int32_t* pages, void* workspace, void* stream, uint32_t job_id, void* notifier) {
-    if (!select_plan_ok(p) || stage < 0 || stage > 1 || !planned_for(p, c, b) || !q || !bounds || !pages || !workspace) return PAELLA_EINVAL;
+    if (!select_plan_ok(p) || stage < 0 || stage >= select_stages(p) || !planned_for(p, c, b) || !q || !bounds || !pages || !workspace) return PAELLA_EINVAL;
     const int64_t size = element_bytes(c->dtype), row = (int64_t)p->heads * p->head_dim;
     if (q_stride < row || q_stride % 8 || (((uintptr_t)q | (uintptr_t)bounds | (uintptr_t)workspace) & 15) || ((uintptr_t)pages & 3)) return PAELLA_EINVAL;
     const double out_bytes = 4.0 * p->tokens * p->kv_heads * p->count, space = (double)select_workspace(p);
@@ -762,7 +839,7 @@ int paella_page_select_launch_stage(const paella_page_select_plan* p, int stage,
     SelectArgs a;
     a.q = (const char*)q; a.bounds = (const char*)bounds;
     a.starts = b->starts; a.past = b->past; a.tables = b->tables; a.prefix_table = b->prefix_table;
-    a.errors = (float*)workspace; a.entries = (unsigned*)((char*)workspace + select_errors(p)); a.worths = (unsigned long long*)((char*)a.entries + select_entries(p)); a.pages = pages; a.q_stride = q_stride * size;
+    a.counters = (unsigned*)workspace; a.errors = (float*)((char*)workspace + select_counters(p)); a.entries = (unsigned*)((char*)a.errors + select_errors(p)); a.worths = (unsigned long long*)((char*)a.entries + select_entries(p)); a.pages = pages; a.q_stride = q_stride * size;
     a.sequences = b->sequences; a.tokens = b->tokens; a.max_pages = b->max_pages; a.prefix_pages = (int)ceil_div(b->prefix_len, c->page_size); a.num_pages = c->num_pages;
     a.heads = p->heads; a.first = p->first; a.last = p->last; a.count = p->count; a.dim = p->head_dim; a.dtype = p->dtype; a.pitch = (unsigned)select_pitch(p);
     a.max_new = divisor((unsigned)b->max_new); a.kv_heads = divisor((unsigned)p->kv_heads); a.per_kv = divisor((unsigned)(p->heads / p->kv_heads)); a.splits = divisor((unsigned)p->splits);
@@ -770,7 +847,7 @@ int paella_page_select_launch_stage(const paella_page_select_plan* p, int stage,
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
     const unsigned rows = (unsigned)(p->tokens * p->kv_heads);
     if (stage == 0) {
-        launch(screen_kernel(p), dim3((unsigned)screen_grid(p)), dim3(256), 0, (hipStream_t)stream, a);
+        launch(screen_kernel(p, select_stages(p) == 1), dim3((unsigned)screen_grid(p)), dim3(256), 0, (hipStream_t)stream, a);
     } else {
         const auto pick = page_pick(select_pages(p));
         launch(pick.kernel, dim3(rows), dim3(pick.threads), 0, (hipStream_t)stream, a);
@@ -781,9 +858,12 @@ int paella_page_select_launch_stage(const paella_page_select_plan* p, int stage,
 int paella_page_select_launch(const paella_page_select_plan* p, const paella_kv_cache* c, const paella_kv_batch* b, const void* q, int64_t q_stride, const void* bounds,
                               int32_t* pages, void* workspace, void* stream, uint32_t job_id, void* notifier) {
     if (!select_plan_ok(p)) return PAELLA_EINVAL;
-    if (keeps_no_order(stream)) return PAELLA_ENOSUP;
-    if (int rc = paella_page_select_launch_stage(p, 0, c, b, q, q_stride, bounds, pages, workspace, stream, job_id, nullptr)) return rc;
-    return paella_page_select_launch_stage(p, 1, c, b, q, q_stride, bounds, pages, workspace, stream, job_id, notifier);
+    const int stages = select_stages(p);
+    if (stages > 1) {
+        if (keeps_no_order(stream)) return PAELLA_ENOSUP;
+        if (int rc = paella_page_select_launch_stage(p, 0, c, b, q, q_stride, bounds, pages, workspace, stream, job_id, nullptr)) return rc;
+    }
+    return paella_page_select_launch_stage(p, stages - 1, c, b, q, q_stride, bounds, pages, workspace, stream, job_id, notifier);
 }
 
 int paella_kv_evict_dims(const paella_kv_evict_desc* d, const paella_kv_cache* c, int stage, paella_launch_dims* dims) {

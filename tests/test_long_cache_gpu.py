@@ -115,6 +115,9 @@ PICK = [
     (F32, 2, 1, 256, 8, [600], 1, None, 9, 1, 0, 1),
     (F16, 3, 1, 64, 8, [40000, 100], 1, None, 0, 200, 4, 4),                  # more pages than one form's registers hold, and than another's
     (BF16, 2, 1, 64, 8, [150000], 1, None, 5, 77, 1, 2),
+    (BF16, 4, 1, 128, 16, [16000, 9000], 1, None, 0, 50, 0, 1),               # one launch, a row's pages shared out
+    (F32, 32, 2, 64, 8, [4000], 3, None, 0, 20, 0, 2),
+    (F16, 8, 8, 64, 16, [1000] * 40, 1, None, 300, 30, 1, 1),                 # many rows
 ]
 
 
