@@ -169,7 +169,8 @@ PageAttentionKernel page_attention_kernel_of(int dim) {
 
 // ------------------------------------------------------------------------------------------ the weight that tokens gather
 // weights[i] += sum over rows r of exp2(x_ri - m_r) / l_r, x = scale q . k in powers of two.  A first launch leaves each row's maximum and sum over its part of the keys, a second one
-// puts the parts together and adds the rows' weights up, key by key.  A wave has a step's keys in registers and takes the rows through, 16 at a time, from LDS.
+// puts the parts together and adds the rows' weights up, key by key.  A wave has a step's keys in registers and takes the rows through, 16 at a time, from LDS.  Where a key head has 16 rows at most, as
+// in a step of single tokens, memory bounds both: the first launch leaves the scores, too, a sixteenth of what the keys are, and the second reads those instead of the keys.
 struct WeighArgs {
     const char *q, *k_cache;
     float* weights;
@@ -179,9 +180,13 @@ struct WeighArgs {
     Divisor kv_heads, per_kv, page_blocks, splits, own_splits, chunks;  // chunks: of a sequence's rows
     float scale_log2;
     f32x2* ml;         // [splits][tokens * heads]: maximum and sum of each part
+    float* scores;     // q . k: [sequences][kv_heads][score_rows][max_pages * page_size], -inf where a row does not see the token
+    int score_rows;
     uint32_t job_id;
     Notifier* notifier;
 };
+
+constexpr float kRise = 8.f;  // how far scores may be above the running maximum before it moves
 
 // Rows that a workgroup has in LDS: 32 KB of queries.
 template <typename T, int D>
@@ -201,42 +206,42 @@ struct KeyWalk {
     Divisor page_blocks;
 
     u32x4 keys[NT][KC];
-    int page;      // of the lane's key of K, and of the lane group's scores
-    int page_s;
-    unsigned in;
 
-    __device__ __forceinline__ int page_of(unsigned entry) const {
-        const unsigned e = min(entry, all_pages - 1);
-        return e < prefix_pages ? prefix[e] : own[e - prefix_pages];
+    // Where the blocks of a wave's steps lie, some steps ahead: lane i has block i % BLOCKS of step i / BLOCKS.  A request that follows keys' requests is answered after them: looked up
+    // step by step, pages would have each step's keys wait for those of the one before.
+    static constexpr int BLOCKS = STEP / 8, STEPS = 64 / BLOCKS;
+    int page, page_behind;        // of this window, and of the next
+    unsigned in, in_behind;       // the blocks' places in the pages
+    int left;                     // steps of the window that have not been asked for
+
+    __device__ __forceinline__ void look(int step, int lane, int* page, unsigned* in) const {
+        const Quotient at = divide((unsigned)(step + lane / BLOCKS * 4) * BLOCKS + lane % BLOCKS, page_blocks);
+        const unsigned e = min(at.q, all_pages - 1);
+        *page = *(e < prefix_pages ? prefix + e : own + (e - prefix_pages));  // (one load: two that meet are waited for)
+        *in = at.r;
     }
-
-    __device__ __forceinline__ void find(unsigned b8, bool even, int lane) {
-        if (even) {
-            const Quotient at = divide(__builtin_amdgcn_readfirstlane(b8), page_blocks);
-            page = page_s = page_of(at.q);
-            in = at.r;
-        } else {
-            const Quotient k_at = divide(b8 + (unsigned)(lane & 15) / (F ? 8 : 4), page_blocks), s_at = divide(b8 + (unsigned)(lane >> 4) * TPL / 8, page_blocks);
-            page = page_of(k_at.q);
-            page_s = page_of(s_at.q);
-            in = k_at.r;
-        }
+    __device__ __forceinline__ void begin(int step, int lane) {
+        look(step, lane, &page, &in);
+        look(step + STEPS * 4, lane, &page_behind, &in_behind);
+        left = STEPS;
     }
-
-    __device__ __forceinline__ void load(u32x4 (&to)[NT][KC], bool even, int lane) const {
-        const int mm = lane & 15;
-        const unsigned row = F ? (even ? mm : mm & 7) : (even ? (mm >> 2) * 8 + (mm & 3) : mm & 3);
-        const char* p;
-        if (even) {
-            const int at = __builtin_amdgcn_readfirstlane(page);
-            p = k + ((unsigned)at < num_pages ? (unsigned)at : 0u) * page_bytes + __builtin_amdgcn_readfirstlane(in) * 8 * ROW + (row * ROW + (lane >> 4) * 16);
-        } else {
-            p = k + ((unsigned)page < num_pages ? (unsigned)page : 0u) * page_bytes + (size_t)((in * 8 + row) * ROW + (lane >> 4) * 16);
+    // Asks for the keys of `step`, the steps in turn; gone: the lane group's lie in no page.
+    __device__ __forceinline__ void request(u32x4 (&to)[NT][KC], bool& gone, int step, int lane) {
+        if (left == 0) {
+            page = page_behind;
+            in = in_behind;
+            look(step + STEPS * 4, lane, &page_behind, &in_behind);
+            left = STEPS;
         }
+        const int mm = lane & 15, first = (STEPS - left) * BLOCKS, mine = first + mm / (F ? 8 : 4);
+        --left;
+        gone = (unsigned)__shfl(page, first + (lane >> 4) * TPL / 8, 64) >= num_pages;
+        const unsigned p = (unsigned)__shfl(page, mine, 64), row = (unsigned)__shfl((int)in, mine, 64) * 8 + (F ? mm & 7 : mm & 3);
+        const char* const from = k + (p < num_pages ? p : 0u) * page_bytes + (size_t)(row * ROW + (lane >> 4) * 16);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int c = 0; c < KC; ++c) to[t][c] = *reinterpret_cast<const u32x4*>(p + t * 4 * ROW + c * 64);
+            for (int c = 0; c < KC; ++c) to[t][c] = *reinterpret_cast<const u32x4*>(from + t * 4 * ROW + c * 64);
     }
 
     // x = K q^T for 16 rows, whose pieces lie in LDS in the order of the lanes
@@ -285,26 +290,18 @@ __device__ __forceinline__ void stage_queries(const WeighArgs& a, int token, int
     }
 }
 
-// Steps over the keys [begin, end) of `walk`, every fourth one for each wave.  each(x, tile): scores of a tile, those of keys that a row does not see
-// -inf; close(first): behind a step's last tile.
-template <typename T, int D, int TILES, typename Each, typename Close>
-__device__ __forceinline__ void walk_keys(const WeighArgs& a, KeyWalk<T, D>& walk, const u32x4* q, int first_row, int rows, int past, int begin, int end, int wave, int lane, Each each,
-                                          Close close) {
+// Steps over the keys [begin, end) of `walk`, every fourth one for each wave.  each(x, tile, first): scores of a tile for the step's keys, those of keys that a row does not see
+// -inf; close(first): behind a step's last tile; open(): ahead of a step's requests.
+template <typename T, int D, int TILES, typename Open, typename Each, typename Close>
+__device__ __forceinline__ void walk_keys(const WeighArgs& a, KeyWalk<T, D>& walk, const u32x4* q, int first_row, int rows, int past, int begin, int end, int wave, int lane, Open open,
+                                          Each each, Close close) {
     using Walk = KeyWalk<T, D>;
     int at = begin + wave;
     if (at >= end) return;
-    const bool even = a.page_blocks.d % (Walk::STEP / 8) == 0;
     const int behind = a.prefix_pages * a.page_size;  // the first own token's place
     const int places = min(a.max_pages * a.page_size, 1 << 30);
     const int least = behind + min(past + (int)divide((unsigned)first_row, a.per_kv).q + 1, places);  // the first place that some row does not see
-    walk.find((unsigned)at * (Walk::STEP / 8), even, lane);
-    walk.load(walk.keys, even, lane);
-    bool absent = (unsigned)walk.page_s >= walk.num_pages;
-    if (at + 4 < end) walk.find((unsigned)(at + 4) * (Walk::STEP / 8), even, lane);
-    for (; at < end; at += 4) {
-        u32x4 next[Walk::NT][Walk::KC];
-        const bool more = at + 4 < end;
-        if (more) walk.load(next, even, lane);
+    auto work = [&](bool absent) {
         const int first = at * Walk::STEP, mine = first + (lane >> 4) * Walk::TPL;
         const bool whole = (first + Walk::STEP <= a.prefix_len || (first >= behind && first + Walk::STEP <= least)) && !__any(absent);
 #pragma unroll
@@ -321,18 +318,32 @@ __device__ __forceinline__ void walk_keys(const WeighArgs& a, KeyWalk<T, D>& wal
                     for (int e = 0; e < 4; ++e)
                         if (absent || mine + t * 4 + e >= limit) x[t][e] = -INFINITY;
             }
-            each(x, tile);
+            each(x, tile, first);
         }
         close(first);
-        if (more) {
+    };
+    using Held = u32x4[Walk::NT][Walk::KC];
+    auto move = [](Held& to, const Held& from) {
 #pragma unroll
-            for (int t = 0; t < Walk::NT; ++t)
+        for (int t = 0; t < Walk::NT; ++t)
 #pragma unroll
-                for (int c = 0; c < Walk::KC; ++c) walk.keys[t][c] = next[t][c];
-            absent = (unsigned)walk.page_s >= walk.num_pages;
-            if (at + 8 < end) walk.find((unsigned)(at + 8) * (Walk::STEP / 8), even, lane);
-        }
+            for (int c = 0; c < Walk::KC; ++c) to[t][c] = from[t][c];
+    };
+    // A step's keys are requested one step ahead.  Not under a condition: a request that may not have been made turns every wait for older ones into one for all.  (Two steps ahead: no faster, 180 us
+    // for 32 sequences of up to 16384 tokens of 8 heads of 128 in bf16 in 16 parts either way.)
+    Held next;
+    bool absent, absent_next;
+    walk.begin(at, lane);
+    walk.request(walk.keys, absent, at, lane);
+    for (; at + 4 < end; at += 4) {
+        open();
+        walk.request(next, absent_next, at + 4, lane);
+        work(absent);
+        move(walk.keys, next);
+        absent = absent_next;
     }
+    open();
+    work(absent);
 }
 
 template <typename T, int D, int TILES>
@@ -341,6 +352,7 @@ __global__ __launch_bounds__(256) void key_sums_kernel(WeighArgs a) {
     using Walk = KeyWalk<T, D>;
     __shared__ u32x4 q[TILES * Walk::KC * 64];
     __shared__ f32x2 sums[4][TILES * 16];
+    __shared__ __attribute__((aligned(16))) float stored[TILES == 1 ? 4 * 16 * Walk::STEP : 4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, a.splits), by_chunk = divide(by_split.q, a.chunks);
     const int h = (int)by_head.r, split = (int)by_split.r, seq = (int)by_chunk.q, first_row = (int)by_chunk.r * TILES * 16;
@@ -361,23 +373,52 @@ __global__ __launch_bounds__(256) void key_sums_kernel(WeighArgs a) {
         const int steps = (keys + Walk::STEP - 1) / Walk::STEP, per = (int)divide((unsigned)steps + a.splits.d - 1, a.splits).q;
         const int begin = min(split * per, steps), end = min(begin + per, steps);
         Walk walk = key_walk<T, D>(a, seq, h);
+        const int behind = a.prefix_pages * a.page_size, places_all = a.max_pages * a.page_size;
+        const __amdgpu_buffer_rsrc_t to_scores = descriptor(TILES == 1 ? a.scores + ((size_t)seq * a.kv_heads.d + h) * a.score_rows * (size_t)places_all : nullptr);
+        // Scores leave through LDS, so that whole lines do, 16 bytes of a row's per lane, and a step late, ahead of the requests of the next: a wait for keys waits for the stores ahead of them as well.
+        float* const mine = stored + (TILES == 1 ? wave * (16 * Walk::STEP) : 0);
+        int waiting = -1;
+        auto put_scores = [&]() {
+            if constexpr (TILES == 1) {
+                constexpr int PIECES = Walk::STEP / 4;
+                if (waiting < 0) return;
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+                for (int u = 0; u < 16 * PIECES / 64; ++u) {
+                    const int i = u * 64 + lane, row = i / PIECES, at = waiting + i % PIECES * 4 - behind;
+                    if (row < rows && at >= 0 && at < places_all)
+                        __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u32x4*>(mine + i * 4), to_scores, (row * places_all + at) * 4, 0, kThrough);
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
+        };
         walk_keys<T, D, TILES>(
-            a, walk, q, first_row, rows, past, begin, end, wave, lane,
-            [&](const f32x4 (&x)[Walk::NT], int tile) {
+            a, walk, q, first_row, rows, past, begin, end, wave, lane, put_scores,
+            [&](const f32x4 (&x)[Walk::NT], int tile, int first) {
                 float top = x[0][0];
 #pragma unroll
                 for (int t = 0; t < Walk::NT; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) top = fmaxf(top, x[t][e]);
-                const float now = fmaxf(m[tile], top * a.scale_log2), base = now == -INFINITY ? 0.f : now;
-                l[tile] *= m[tile] == now ? 1.f : __builtin_amdgcn_exp2f(m[tile] - now);
-                m[tile] = now;
+                top *= a.scale_log2;
+                if (__any(top > m[tile] + kRise)) {  // (until then the exponentials have room above 1)
+                    const float now = fmaxf(m[tile], top);
+                    l[tile] *= m[tile] == now ? 1.f : __builtin_amdgcn_exp2f(m[tile] - now);
+                    m[tile] = now;
+                }
+                const float base = m[tile] == -INFINITY ? 0.f : m[tile];
 #pragma unroll
                 for (int t = 0; t < Walk::NT; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) l[tile] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][e], a.scale_log2, -base));
+                if constexpr (TILES == 1) {
+#pragma unroll
+                    for (int t = 0; t < Walk::NT; ++t) *reinterpret_cast<f32x4*>(mine + (lane & 15) * Walk::STEP + (lane >> 4) * Walk::TPL + t * 4) = x[t];
+                    waiting = first;
+                }
             },
             [](int) {});
+        put_scores();
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
 #pragma unroll
@@ -407,6 +448,70 @@ __global__ __launch_bounds__(256) void key_sums_kernel(WeighArgs a) {
     hook_exit(a.notifier, a.job_id);
 }
 
+// Of each of ROWS rows from `first` on: maximum and one over the sum, the parts put together in their order.  Behind the last row, and where a row sees nothing, what gives no weights.
+template <int ROWS>
+__device__ __forceinline__ void join_rows(const WeighArgs& a, int token, int h, int first, int rows, f32x2* whole) {
+    constexpr int AHEAD = 8;
+    if ((int)threadIdx.x < ROWS) {
+        const int row = first + (int)threadIdx.x;
+        float top = -INFINITY, total = 0.f;
+        if (row < rows) {
+            const Quotient at = divide((unsigned)row, a.per_kv);
+            const size_t all = (size_t)a.tokens * a.heads;
+            const f32x2* const from = a.ml + (size_t)(token + (int)at.q) * a.heads + h * (int)a.per_kv.d + (int)at.r;
+            for (unsigned s = 0; s < a.splits.d; s += AHEAD) {
+                f32x2 part[AHEAD];
+                float now = top;
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) part[u] = from[min(s + u, a.splits.d - 1) * all];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) now = fmaxf(now, part[u].x);
+                total *= top == now ? 1.f : __builtin_amdgcn_exp2f(top - now);
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u)
+                    if (s + u < a.splits.d) total += part[u].y * (part[u].x == now ? 1.f : __builtin_amdgcn_exp2f(part[u].x - now));
+                top = now;
+            }
+        }
+        whole[threadIdx.x] = total == 0.f ? f32x2{INFINITY, 0.f} : f32x2{top, 1.f / total};
+    }
+}
+
+// From stored scores: four tokens a thread.
+static __global__ __launch_bounds__(256) void stored_weights_kernel(WeighArgs a) {
+    hook_entry(a.notifier, a.job_id);
+    __shared__ f32x2 whole[16];
+    const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, a.own_splits);
+    const int h = (int)by_head.r, split = (int)by_split.r, seq = (int)by_split.q;
+    const NewTokens its = new_tokens(a.starts, a.past, seq, a.max_new, a.tokens);
+    const int rows = its.count * (int)a.per_kv.d, places = a.max_pages * a.page_size, past = min(its.past, places), held = min(past + its.count, places);
+    const int per = (int)divide((unsigned)held + a.own_splits.d - 1, a.own_splits).q, begin = min(split * ((per + 3) / 4 * 4), held), end = min(begin + (per + 3) / 4 * 4, held);
+    if (rows > 0 && begin < end) {
+        join_rows<16>(a, its.first, h, 0, rows, whole);
+        __syncthreads();
+        const size_t head = (size_t)seq * a.kv_heads.d + h;
+        const float* const scores = a.scores + head * a.score_rows * (size_t)places;
+        float* const weights = a.weights + head * (size_t)places;
+        const __amdgpu_buffer_rsrc_t to = descriptor(weights);
+        for (int i = begin + (int)threadIdx.x * 4; i < end; i += 1024) {  // (places are a multiple of eight: four of them are there)
+            const f32x4 old = *reinterpret_cast<const f32x4*>(weights + i);
+            f32x4 w = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(scores + (size_t)r * places + i);
+                const f32x2 row = whole[r];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] += row.y * __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale_log2, -row.x));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                w[e] = i + e >= held ? old[e] : i + e >= past ? w[e] : old[e] + w[e];
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, w), to, i * 4, 0, kThrough);
+        }
+    }
+    hook_exit(a.notifier, a.job_id);
+}
+
 template <typename T, int D, int TILES>
 __global__ __launch_bounds__(256) void key_weights_kernel(WeighArgs a) {
     hook_entry(a.notifier, a.job_id);
@@ -428,29 +533,14 @@ __global__ __launch_bounds__(256) void key_weights_kernel(WeighArgs a) {
         for (int first_row = 0; first_row < rows && begin < end; first_row += TILES * 16) {
             __syncthreads();
             stage_queries<T, D, TILES>(a, its.first, h, first_row, rows, q);
-            if ((int)threadIdx.x < TILES * 16) {
-                const int row = first_row + (int)threadIdx.x;
-                float top = -INFINITY, total = 0.f;
-                if (row < rows) {
-                    const Quotient at = divide((unsigned)row, a.per_kv);
-                    const f32x2* from = a.ml + (size_t)(its.first + (int)at.q) * a.heads + h * (int)a.per_kv.d + (int)at.r;
-                    for (unsigned s = 0; s < a.splits.d; ++s, from += (size_t)a.tokens * a.heads) {
-                        const f32x2 part = *from;
-                        const float now = fmaxf(top, part.x);
-                        total = total * (top == now ? 1.f : __builtin_amdgcn_exp2f(top - now)) + part.y * (part.x == now ? 1.f : __builtin_amdgcn_exp2f(part.x - now));
-                        top = now;
-                    }
-                }
-                // a row behind the last one, or one that sees nothing, has no weights
-                whole[threadIdx.x] = total == 0.f ? f32x2{INFINITY, 0.f} : f32x2{top, 1.f / total};
-            }
+            join_rows<TILES * 16>(a, its.first, h, first_row, rows, whole);
             __syncthreads();
             float w[Walk::TPL];
 #pragma unroll
             for (int e = 0; e < Walk::TPL; ++e) w[e] = 0.f;
             walk_keys<T, D, TILES>(
-                a, walk, q, first_row, rows, past, begin, end, wave, lane,
-                [&](const f32x4 (&x)[Walk::NT], int tile) {
+                a, walk, q, first_row, rows, past, begin, end, wave, lane, [] {},
+                [&](const f32x4 (&x)[Walk::NT], int tile, int) {
                     const f32x2 row = whole[tile * 16 + (lane & 15)];
 #pragma unroll
                     for (int t = 0; t < Walk::NT; ++t)
@@ -481,16 +571,14 @@ using WeighKernel = void (*)(WeighArgs);
 // few: at most 16 rows a sequence and key head
 template <typename T, int D>
 WeighKernel key_sums_kernel_of(bool few) { return few ? key_sums_kernel<T, D, 1> : key_sums_kernel<T, D, weigh_tiles<T, D>()>; }
-template <typename T, int D>
-WeighKernel key_weights_kernel_of(bool few) { return few ? key_weights_kernel<T, D, 1> : key_weights_kernel<T, D, weigh_tiles<T, D>()>; }
-
 template <typename T>
 WeighKernel key_sums(int dim, bool few) {
     return dim == 64 ? key_sums_kernel_of<T, 64>(few) : dim == 128 ? key_sums_kernel_of<T, 128>(few) : key_sums_kernel_of<T, 256>(few);
 }
 template <typename T>
 WeighKernel key_weights(int dim, bool few) {
-    return dim == 64 ? key_weights_kernel_of<T, 64>(few) : dim == 128 ? key_weights_kernel_of<T, 128>(few) : key_weights_kernel_of<T, 256>(few);
+    if (few) return stored_weights_kernel;
+    return dim == 64 ? key_weights_kernel<T, 64, weigh_tiles<T, 64>()> : dim == 128 ? key_weights_kernel<T, 128, weigh_tiles<T, 128>()> : key_weights_kernel<T, 256, weigh_tiles<T, 256>()>;
 }
 
 // Defined once per type.

@@ -50,7 +50,11 @@ size_t workspace_of(const PagePlan* p) {
 
 using WeighPlan = paella_key_weights_plan;
 
-bool few_rows(const WeighPlan* p) { return (int64_t)std::min(p->max_new, p->tokens) * (p->heads / p->kv_heads) <= 16; }
+// Scores are stored by 32-bit offsets.
+bool few_rows(const WeighPlan* p) {
+    const int64_t rows = (int64_t)std::min(p->max_new, p->tokens) * (p->heads / p->kv_heads);
+    return rows <= 16 && (double)rows * p->max_pages * p->page_size < 1073741824.0 / 2;
+}
 int chunk_rows(const WeighPlan* p) {
     if (few_rows(p)) return 16;
     return 16 * std::min(8, 32768 / (16 * p->head_dim * element_bytes(p->dtype)));
@@ -72,7 +76,9 @@ bool plan_ok(const WeighPlan* p) {
            (double)p->sequences * chunks_of(p) * p->kv_heads * p->splits <= kMostWorkgroups && (double)p->sequences * p->kv_heads * p->own_splits <= kMostWorkgroups;
 }
 
-size_t workspace_of(const WeighPlan* p) { return (size_t)p->splits * p->tokens * p->heads * 8; }
+size_t parts_of(const WeighPlan* p) { return up256((size_t)p->splits * p->tokens * p->heads * 8); }
+int score_rows(const WeighPlan* p) { return few_rows(p) ? std::min(p->max_new, p->tokens) * (p->heads / p->kv_heads) : 0; }
+size_t workspace_of(const WeighPlan* p) { return parts_of(p) + (size_t)p->sequences * p->kv_heads * score_rows(p) * p->max_pages * p->page_size * 4; }
 
 }  // namespace
 
@@ -162,8 +168,12 @@ int paella_key_weights_plan_make(const paella_kv_cache* c, const paella_kv_batch
     if (!plan_ok(p)) return PAELLA_ENOSUP;
     const int64_t own = (int64_t)c->page_size * b->max_pages, keys = own + b->prefix_len;
     const int64_t sums = grid_of(p, 0), weights = grid_of(p, 1);
-    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(2048, sums), ceil_div(keys, 256), 64}));
-    p->own_splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(2048, weights), ceil_div(own, 256)));
+    // Few rows: memory bounds it, and parts are as many as even out the sequences' lengths (32 sequences of 8192 to 16384 tokens of 8 heads of 128 in bf16 in 4 / 8 / 16 / 32 parts 204 / 187 / 180 / 173 us).
+    // Many rows: as many workgroups as the device holds at once, two to a compute unit in the first stage (4 sequences, 128 rows over 17000 keys of 8 heads, in 12 / 16 / 24 parts 41 / 34 / 52 us) and three
+    // in the second.
+    const bool few = few_rows(p);
+    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(few ? 8192 : 512, sums), ceil_div(keys, 256), 64}));
+    p->own_splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(few ? 2048 : 768, weights), ceil_div(own, few ? 1024 : 256)));
     if (!plan_ok(p)) return PAELLA_ENOSUP;
     p->stages = 2;
     p->workspace_bytes = workspace_of(p);
@@ -183,7 +193,7 @@ int paella_key_weights_dims(const paella_key_weights_plan* p, int stage, paella_
 
 int paella_key_weights_launch_stage(const paella_key_weights_plan* p, int stage, const paella_kv_cache* c, const paella_kv_batch* b, const void* q, int64_t q_stride, float* weights,
                                     void* workspace, void* stream, uint32_t job_id, void* notifier) {
-    if (!plan_ok(p) || stage < 0 || stage > 1 || !planned_for(p, c, b) || !q || !weights || !workspace || ((uintptr_t)weights & 3) || (((uintptr_t)q | (uintptr_t)workspace) & 15))
+    if (!plan_ok(p) || stage < 0 || stage > 1 || !planned_for(p, c, b) || !q || !weights || !workspace || (((uintptr_t)q | (uintptr_t)weights | (uintptr_t)workspace) & 15))
         return PAELLA_EINVAL;
     const int64_t size = element_bytes(c->dtype), row = (int64_t)p->heads * c->head_dim;
     if (q_stride < row || q_stride % 8) return PAELLA_EINVAL;
@@ -200,6 +210,7 @@ int paella_key_weights_launch_stage(const paella_key_weights_plan* p, int stage,
     a.kv_heads = divisor((unsigned)p->kv_heads); a.per_kv = divisor((unsigned)(p->heads / p->kv_heads)); a.page_blocks = divisor((unsigned)c->page_size / 8);
     a.splits = divisor((unsigned)p->splits); a.own_splits = divisor((unsigned)p->own_splits); a.chunks = divisor((unsigned)chunks_of(p));
     a.scale_log2 = p->scale * 1.44269504088896340736f; a.ml = (f32x2*)workspace;
+    a.scores = (float*)((char*)workspace + parts_of(p)); a.score_rows = score_rows(p);
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
     launch(kernel_of(p, stage), dim3((unsigned)grid_of(p, stage)), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();

@@ -140,7 +140,7 @@ struct SelectArgs {
 constexpr unsigned kNoPage = 0, kUnknown = 1, kForced = ~0u;  // (unknown: it is no number, or may be infinite)
 
 __device__ __forceinline__ int page_along(const SelectArgs& a, int seq, unsigned e) {
-    return e < (unsigned)a.prefix_pages ? a.prefix_table[e] : a.tables[(size_t)seq * a.max_pages + (e - a.prefix_pages)];
+    return *(e < (unsigned)a.prefix_pages ? a.prefix_table + e : a.tables + (size_t)seq * a.max_pages + (e - a.prefix_pages));  // (one load: two that meet are waited for)
 }
 
 // Values below 0, and magnitudes, of 16 bytes.
@@ -200,7 +200,18 @@ __device__ __forceinline__ void screen_pages(const SelectArgs& a, const Screened
     float worst = 0.f;
     if (turn * kScreened < pages) {
         const Quotient row = divide((unsigned)min(mm, n * heads - 1), a.per_kv);  // the lane's token and head
-        auto number_of = [&](unsigned turn) { return page_along(a, seq, min(turn * kScreened + mm, pages - 1)); };
+        // Numbers of the pages of four turns, 16 each, and of the four behind.  (A request that follows others is answered after them: looked up turn by turn, pages would have each turn's bounds wait for
+        // those of the one before.)
+        auto look = [&](unsigned turn) { return page_along(a, seq, min((turn + group * step) * kScreened + mm, pages - 1)); };
+        int numbers = look(turn), numbers_behind = look(turn + 4 * step), left = 4;
+        auto next_page = [&](unsigned turn) {  // of the turns one after the other
+            if (left == 0) {
+                numbers = numbers_behind;
+                numbers_behind = look(turn + 4 * step);
+                left = 4;
+            }
+            return __shfl(numbers, (4 - left--) * 16 + mm, 64);
+        };
         auto load = [&](int page, u32x4 (&low)[KC], u32x4 (&high)[KC]) {
             const char* const from = a.bounds + ((size_t)((unsigned)page < (unsigned)a.num_pages ? page : 0) * a.kv_heads.d + h) * 2 * ROW + group * 16;
 #pragma unroll
@@ -220,17 +231,13 @@ __device__ __forceinline__ void screen_pages(const SelectArgs& a, const Screened
                 above[c] = q ^ below[c];
             }
         };
-        int page = number_of(turn);
-        query(0);
+        int page = next_page(turn);
         load(page, low, high);
-        int page_ahead = number_of(turn + step);
+        query(0);
         const bool one_group = n * heads <= 4;  // the first lane group has all rows
-        for (; turn * kScreened < pages; turn += step) {
+        auto work = [&]() {
             // Lane mm has page mm, register e of lane group g row 4 g + e.
             f32x4 worth = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, error = {0.f, 0.f, 0.f, 0.f};
-            const bool more = (turn + step) * kScreened < pages;
-            u32x4 next_low[KC], next_high[KC];
-            if (KC <= 8 && more) load(page_ahead, next_low, next_high);
             for (int g = 0; g < heads; g += 16) {  // more than once where a token has more heads than a tile rows
                 if (heads > 16) query(g);
                 f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x, z = x;
@@ -273,20 +280,26 @@ __device__ __forceinline__ void screen_pages(const SelectArgs& a, const Screened
                 const size_t at = (size_t)(its.first + j0 + j) * a.kv_heads.d + h;
                 if (group == 0 && e < seen) __hip_atomic_store(a.entries + at * a.pitch + e, key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
-            if (more) {
-                page = page_ahead;
-                if constexpr (KC <= 8) {
+        };
+        // (The next turn's bounds are requested whatever comes, or not at all: a request that may not have been made turns every wait for older ones into one for all.)
+        for (; (turn + step) * kScreened < pages; turn += step) {
+            const int page_next = next_page(turn + step);
+            if constexpr (KC <= 8) {
+                u32x4 next_low[KC], next_high[KC];
+                load(page_next, next_low, next_high);
+                work();
 #pragma unroll
-                    for (int c = 0; c < KC; ++c) {
-                        low[c] = next_low[c];
-                        high[c] = next_high[c];
-                    }
-                } else {
-                    load(page, low, high);
+                for (int c = 0; c < KC; ++c) {
+                    low[c] = next_low[c];
+                    high[c] = next_high[c];
                 }
-                page_ahead = number_of(turn + 2 * step);
+            } else {
+                work();
+                load(page_next, low, high);
             }
+            page = page_next;
         }
+        work();
     }
     worst = wave_max_f(worst);  // of all rows of the tile
     if (lane < n) store_out(a.errors + ((size_t)(its.first + j0 + lane) * a.kv_heads.d + h) * step + (unsigned)w.split * 4 + wave, worst);
@@ -802,10 +815,11 @@ int paella_page_select_plan_make(const paella_kv_cache* c, const paella_kv_batch
     plan_extents(p, c, b, heads);
     p->count = count; p->first = first; p->last = last;
     const int64_t pages = select_pages(p), rows = (int64_t)p->tokens * p->kv_heads;
-    // enough workgroups to fill the device, none without a turn for each wave
+    // as many workgroups as the device holds at once, two to a compute unit, or none without a turn for each wave (32 rows of 1025 pages of 8 heads of 128 in bf16 by 512 / 1024 / 2048 workgroups 21.9 /
+    // 22.8 / 26.1 us, 4 of 15626 of 8 heads of 64 13.2 / 12.0 / 12.7)
     p->splits = 1;
     if (!select_plan_ok(p)) return PAELLA_ENOSUP;
-    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(1024, screen_grid(p)), ceil_div(pages, 4 * kScreened)));
+    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, screen_grid(p)), ceil_div(pages, 4 * kScreened)));
     if (!select_plan_ok(p)) return PAELLA_ENOSUP;
     p->stages = select_stages(p);
     p->workspace_bytes = select_workspace(p);
