@@ -48,6 +48,10 @@ __device__ __forceinline__ void widen(u32x4 w, float (&low)[16 / T::bytes], floa
     }
 }
 
+// Of numbers: by comparison, since the library's minimum makes every operand canonical first.
+__device__ __forceinline__ float lesser(float v, float w) { return v < w ? v : w; }
+__device__ __forceinline__ float greater(float v, float w) { return v > w ? v : w; }
+
 template <typename T>
 __device__ __forceinline__ u32x4 packed(const float (&x)[16 / T::bytes]) {  // values of the type, so nothing is rounded
     u32x4 w;
@@ -59,8 +63,35 @@ __device__ __forceinline__ u32x4 packed(const float (&x)[16 / T::bytes]) {  // v
     return w;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void page_bounds_kernel(BoundsArgs a) {
+// Least and largest of the lanes that are multiples of 2^log2 apart, by the vector unit's own lane moves (some meet more than once).
+template <int V>
+__device__ __forceinline__ void lanes_apart(float (&low)[V], float (&high)[V], int log2) {
+    auto meet = [&](auto other) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            low[e] = lesser(other(low[e]), low[e]);
+            high[e] = greater(other(high[e]), high[e]);
+        }
+    };
+    if (log2 <= 0) meet([](float v) { return lane_move<0xB1>(v); });   // lane ^ 1
+    if (log2 <= 1) meet([](float v) { return lane_move<0x4E>(v); });   // lane ^ 2
+    if (log2 <= 2) meet([](float v) { return lane_move<0x124>(v); });  // a quarter of a turn of sixteen, and half of one
+    if (log2 <= 3) meet([](float v) { return lane_move<0x128>(v); });
+    auto swapped = [&](auto swap) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const auto l = swap(as_word(low[e])), h = swap(as_word(high[e]));
+            low[e] = lesser(as_float(l[0]), as_float(l[1]));
+            high[e] = greater(as_float(h[0]), as_float(h[1]));
+        }
+    };
+    if (log2 <= 4) swapped([](unsigned v) { return __builtin_amdgcn_permlane16_swap(v, v, false, false); });  // even and odd sixteens
+    if (log2 <= 5) swapped([](unsigned v) { return __builtin_amdgcn_permlane32_swap(v, v, false, false); });  // both halves
+}
+
+// AHEAD: requests of a lane that go out together.
+template <typename T, int AHEAD>
+__global__ __launch_bounds__(256, AHEAD == 4 ? 8 : 1) void page_bounds_kernel(BoundsArgs a) {
     hook_entry(a.notifier, a.job_id);
     constexpr int V = 16 / T::bytes;
     const int lane = threadIdx.x & 63;
@@ -87,7 +118,6 @@ __global__ __launch_bounds__(256) void page_bounds_kernel(BoundsArgs a) {
                     low[e] = INFINITY;
                     high[e] = -INFINITY;
                 }
-                constexpr int AHEAD = 8;
                 for (int key = lane >> a.group_log2; key < held; key += AHEAD * each) {
                     u32x4 w[AHEAD];
 #pragma unroll
@@ -96,13 +126,7 @@ __global__ __launch_bounds__(256) void page_bounds_kernel(BoundsArgs a) {
 #pragma unroll
                     for (int u = 0; u < AHEAD; ++u) widen<T>(w[u], low, high);
                 }
-                for (int off = group; off < 64; off <<= 1) {
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        low[e] = fminf(low[e], __shfl_xor(low[e], off, 64));
-                        high[e] = fmaxf(high[e], __shfl_xor(high[e], off, 64));
-                    }
-                }
+                lanes_apart<V>(low, high, a.group_log2);
                 if (lane < group && in) {
                     __builtin_amdgcn_raw_buffer_store_b128(packed<T>(low), to, piece * 16, 0, kThrough);
                     __builtin_amdgcn_raw_buffer_store_b128(packed<T>(high), to, a.row_bytes + piece * 16, 0, kThrough);
@@ -598,19 +622,27 @@ __global__ __launch_bounds__(WAVES * 64) void evict_pick_kernel(EvictArgs a) {
 // 16 bytes that go through to memory.  (The wait states are those between a store and the next write of its registers.)
 __device__ __forceinline__ void put16(char* p, u32x4 v) { asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(p), "v"(v) : "memory"); }
 
-// AHEAD: tokens of a lane in a run.
-template <int AHEAD>
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
     hook_entry(a.notifier, a.job_id);
+    constexpr int AHEAD = 8;  // tokens of a lane in a run
     const Quotient by_slice = divide(blockIdx.x, a.slices), by_head = divide(by_slice.q, a.kv_heads);
     const unsigned slice = by_slice.r, h = by_head.r, seq = by_head.q, keep = (unsigned)a.keep;
     const int* const kept = a.kept + (size_t)by_slice.q * a.keep;
     const int* const table = a.tables + (size_t)seq * a.max_pages;
     const unsigned half = (a.slices.d - 1) / 2;  // slices of the keys, of the values, and one for the weights
-    if (kept[keep - 1] >= 0) {                   // else all of the sequence stays
+    // What leads the list with its own places stays where it is: a place's distance from its token's does not shrink along the list, so 256 samples tell where to begin, but for a sample's distance.
+    __shared__ unsigned alike[4];
+    const unsigned apart = (keep + 255) / 256, sample = threadIdx.x * apart;
+    const bool stays = sample < keep && (unsigned)kept[sample] == sample;
+    const int last = kept[keep - 1];
+    const unsigned long long who = __ballot(stays);
+    if ((threadIdx.x & 63) == 0) alike[threadIdx.x >> 6] = (unsigned)__popcll(who);
+    __syncthreads();
+    const unsigned lead = alike[0] + alike[1] + alike[2] + alike[3], begin = lead ? (lead - 1) * apart : 0u;
+    if (last >= 0) {  // else all of the sequence stays
         if (slice == a.slices.d - 1) {
             float* const w = a.weights + (size_t)by_slice.q * a.places;
-            for (unsigned first = 0; first < keep; first += 1024) {
+            for (unsigned first = begin; first < keep; first += 1024) {
                 float x[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
@@ -632,7 +664,9 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
             const unsigned mine = threadIdx.x >> lanes_log2;
             const bool in = piece < (unsigned)a.row_bytes;
             const unsigned run = tokens * AHEAD;
-            int from[AHEAD];  // of the next run, known ahead
+            // A run's pages are looked up while the one ahead of it is read, and its tokens a run earlier still: then only keys and values, and the stores behind them, are waited for.
+            int from[AHEAD], page[AHEAD], page_to[AHEAD];
+            unsigned slot[AHEAD], slot_to[AHEAD];
             auto look = [&](unsigned first) {
 #pragma unroll
                 for (int u = 0; u < AHEAD; ++u) {
@@ -641,30 +675,32 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
                     if (!in || i >= keep || (unsigned)from[u] == i) from[u] = -1;
                 }
             };
-            look(0);
-            for (unsigned first = 0; first < keep; first += run) {
-                int page[AHEAD], page_to[AHEAD];
-                unsigned slot[AHEAD], slot_to[AHEAD];
+            auto resolve = [&](unsigned first) {
 #pragma unroll
                 for (int u = 0; u < AHEAD; ++u) {  // (a token that does not move: the first one's page, which is there)
                     const Quotient p = divide(from[u] < 0 ? 0u : (unsigned)from[u], a.pages), q = divide(from[u] < 0 ? 0u : first + u * tokens + mine, a.pages);
                     page[u] = table[min(p.q, (unsigned)a.max_pages - 1)];
                     page_to[u] = table[min(q.q, (unsigned)a.max_pages - 1)];
-                    slot[u] = p.r;
+                    slot[u] = from[u] < 0 || p.q >= (unsigned)a.max_pages || q.q >= (unsigned)a.max_pages ? ~0u : p.r;
                     slot_to[u] = q.r;
-                    if (from[u] < 0 || p.q >= (unsigned)a.max_pages || q.q >= (unsigned)a.max_pages) page_to[u] = -1;
                 }
+            };
+            look(begin);
+            resolve(begin);
+            look(begin + run);
+            for (unsigned first = begin; first < keep; first += run) {
                 u32x4 x[AHEAD];
                 char* to[AHEAD];
 #pragma unroll
                 for (int u = 0; u < AHEAD; ++u) {
                     to[u] = nullptr;
-                    if ((unsigned)page[u] < (unsigned)a.num_pages && (unsigned)page_to[u] < (unsigned)a.num_pages) {
+                    if (slot[u] != ~0u && (unsigned)page[u] < (unsigned)a.num_pages && (unsigned)page_to[u] < (unsigned)a.num_pages) {
                         to[u] = cache + (((size_t)page_to[u] * a.kv_heads.d + h) * a.page_size + slot_to[u]) * a.row_bytes + piece;
                         x[u] = *reinterpret_cast<const u32x4*>(cache + (((size_t)page[u] * a.kv_heads.d + h) * a.page_size + slot[u]) * a.row_bytes + piece);
                     }
                 }
-                if (first + run < keep) look(first + run);
+                resolve(first + run);
+                look(first + 2 * run);
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads();
 #pragma unroll
@@ -681,9 +717,18 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
 // ------------------------------------------------------------------------------------------ host
 
 using BoundsKernel = void (*)(BoundsArgs);
-BoundsKernel bounds_kernel(int dtype) {
-    return dtype == PAELLA_F32 ? page_bounds_kernel<F32> : dtype == PAELLA_BF16 ? page_bounds_kernel<Bf16> : page_bounds_kernel<F16>;
+template <int AHEAD>
+BoundsKernel bounds_kernel_of(int dtype) {
+    return dtype == PAELLA_F32 ? page_bounds_kernel<F32, AHEAD> : dtype == PAELLA_BF16 ? page_bounds_kernel<Bf16, AHEAD> : page_bounds_kernel<F16, AHEAD>;
 }
+// 2^n lanes side by side have a key's 16-byte pieces.
+int bounds_group_log2(const paella_kv_cache* c) {
+    int n = 0;
+    while ((16 << n) < c->head_dim * element_bytes(c->dtype) && n < 6) ++n;
+    return n;
+}
+// A page's keys in one go of four requests a lane where they fit that: with half the registers twice as many waves are there.
+BoundsKernel bounds_kernel(const paella_kv_cache* c) { return c->page_size <= 4 * (64 >> bounds_group_log2(c)) ? bounds_kernel_of<4>(c->dtype) : bounds_kernel_of<8>(c->dtype); }
 
 struct BoundsGrid {
     int64_t touched, items;
@@ -760,18 +805,15 @@ size_t select_errors(const paella_page_select_plan* p) { return up256((size_t)p-
 size_t select_entries(const paella_page_select_plan* p) { return up256((size_t)p->tokens * p->kv_heads * select_pitch(p) * 4); }
 size_t select_workspace(const paella_page_select_plan* p) { return select_counters(p) + select_errors(p) + 3 * select_entries(p); }  // (worths of 64 bits: twice the entries)
 
-// Bytes of a row that a workgroup moves: 128, which memory likes best, where that still makes two workgroups for each compute unit, else 64, or 32 where even those leave half of the device
-// idle.  (bf16 heads of 128, 4096 tokens kept: 24 sequences of 8 heads by 128 / 64 bytes 192 / 247 us, 4 sequences 89 / 53; fp32 heads of 64, 1000 tokens of 2 heads by 64 / 32 bytes 10 / XX.)
+// Bytes of a row that a workgroup moves: 128, which memory likes best, where that still makes a workgroup for each compute unit, else 64, or 32 where even those leave half of the device idle.  (bf16
+// heads of 128, 4096 tokens kept of 8 heads: 24 sequences by 128 / 64 bytes 193 / 247 us, 8 91 / 94, 4 57 / 48; one by 64 / 32 40 / 26.)
 int evict_slice_log2(int sequences, const paella_kv_cache* c) {
     const int64_t heads = (int64_t)sequences * c->kv_heads, row = (int64_t)c->head_dim * element_bytes(c->dtype);
-    return 2 * heads * ceil_div(row, 128) >= 512 ? 7 : 2 * heads * ceil_div(row, 64) >= 128 ? 6 : 5;
+    return 2 * heads * ceil_div(row, 128) >= 256 ? 7 : 2 * heads * ceil_div(row, 64) >= 128 ? 6 : 5;
 }
 int64_t evict_slices(int sequences, const paella_kv_cache* c) {
     return 2 * ceil_div((int64_t)c->head_dim * element_bytes(c->dtype), 1 << evict_slice_log2(sequences, c)) + 1;
 }
-using MoveKernel = void (*)(EvictArgs);
-MoveKernel move_kernel(int slice_log2) { return slice_log2 == 7 ? evict_move_kernel<8> : evict_move_kernel<16>; }
-
 int evict_check(const paella_kv_evict_desc* d, const paella_kv_cache* c) {
     if (!d || !cache_extents_ok(c) || d->sequences <= 0 || d->max_pages <= 0 || d->keep <= 0 || d->first < 0 || d->recent < 0 || (int64_t)d->first + d->recent > d->keep) return PAELLA_EINVAL;
     const double heads = (double)d->sequences * c->kv_heads;
@@ -787,7 +829,7 @@ int paella_page_bounds_dims(const paella_kv_cache* c, const paella_kv_batch* b, 
     if (int rc = bounds_check(c, b)) return rc;
     if (!dims) return PAELLA_EINVAL;
     set_launch_dims(dims, bounds_grid(c, b).grid(), 256, 0, 64);
-    loaded_dims((const void*)bounds_kernel(c->dtype), dims);
+    loaded_dims((const void*)bounds_kernel(c), dims);
     return 0;
 }
 
@@ -801,11 +843,10 @@ int paella_page_bounds_launch(const paella_kv_cache* c, const paella_kv_batch* b
     a.k_cache = (const char*)c->k; a.bounds = (char*)bounds;
     a.starts = b->starts; a.past = b->past; a.tables = b->tables;
     a.sequences = b->sequences; a.max_new = b->max_new; a.tokens = b->tokens; a.max_pages = b->max_pages; a.num_pages = c->num_pages; a.page_size = c->page_size;
-    a.row_bytes = c->head_dim * element_bytes(c->dtype); a.pieces = a.row_bytes / 16; a.group_log2 = 0;
-    while ((1 << a.group_log2) < a.pieces && a.group_log2 < 6) ++a.group_log2;
+    a.row_bytes = c->head_dim * element_bytes(c->dtype); a.pieces = a.row_bytes / 16; a.group_log2 = bounds_group_log2(c);
     a.kv_heads = divisor((unsigned)c->kv_heads); a.touched = divisor((unsigned)g.touched); a.items = (unsigned)g.items;
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
-    launch(bounds_kernel(c->dtype), dim3(g.grid()), dim3(256), 0, (hipStream_t)stream, a);
+    launch(bounds_kernel(c), dim3(g.grid()), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 
@@ -886,7 +927,7 @@ int paella_kv_evict_dims(const paella_kv_evict_desc* d, const paella_kv_cache* c
     if (stage) set_launch_dims(dims, (unsigned)(d->sequences * c->kv_heads * evict_slices(d->sequences, c)), 256, 0, 64);
     const auto pick = evict_pick((int64_t)d->max_pages * c->page_size);
     if (!stage) set_launch_dims(dims, (unsigned)(d->sequences * c->kv_heads), pick.threads, 0, 64);
-    loaded_dims(stage ? (const void*)move_kernel(evict_slice_log2(d->sequences, c)) : (const void*)pick.kernel, dims);
+    loaded_dims(stage ? (const void*)evict_move_kernel : (const void*)pick.kernel, dims);
     return 0;
 }
 
@@ -912,7 +953,7 @@ int paella_kv_evict_launch_stage(const paella_kv_evict_desc* d, int stage, const
     a.slice_log2 = (unsigned)evict_slice_log2(d->sequences, c);
     const auto pick = evict_pick((int64_t)a.places);
     if (stage == 0) launch(pick.kernel, dim3((unsigned)(d->sequences * c->kv_heads)), dim3(pick.threads), 0, (hipStream_t)stream, a);
-    else launch(move_kernel((int)a.slice_log2), dim3((unsigned)(d->sequences * c->kv_heads * evict_slices(d->sequences, c))), dim3(256), 0, (hipStream_t)stream, a);
+    else launch(evict_move_kernel, dim3((unsigned)(d->sequences * c->kv_heads * evict_slices(d->sequences, c))), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 
