@@ -56,17 +56,18 @@ struct ListWalk : NarrowWalk<T, D> {
         }
     }
 
+    // One step, whose places are (here, held).  next(true) is called once K is no longer needed, next(false) once V is.
     template <typename Next>
-    __device__ __forceinline__ void step(Rows& rows, int off, int seen, float scale, Next next) {
+    __device__ __forceinline__ void step(Rows& rows, int here, int held, float scale, Next next) {
         f32x4 x[1][Rows::NT];
         rows.scores(x, [&](int t, int c) { return this->k[t][c]; });
         next(true);
-        if (__any(off + TPL > seen)) {
-            const int limit[1] = {seen};
-            Rows::mask(x, off, false, limit);
+        if (__any(here + TPL > held)) {
+            const int limit[1] = {held};
+            Rows::mask(x, here, false, limit);
 #pragma unroll
             for (int u = 0; u < TPL; ++u)  // what lies in places that no row may see can be anything
-                if (off + u >= seen) {
+                if (here + u >= held) {
 #pragma unroll
                     for (int w = 0; w < Rows::GRP * Rows::VW; ++w) this->v[u][w] = 0;
                 }
@@ -76,33 +77,35 @@ struct ListWalk : NarrowWalk<T, D> {
         rows.add_values(this->v, p);
         next(false);
     }
-
-    // Steps wave, wave + 4, ... of the list's n entries.
-    __device__ __forceinline__ void walk_list(Rows& rows, const Keys& s, const u32x2* list, int n, float scale, int wave, int lane) {
-        const int end = (n * (int)s.page_blocks.d + STEP / 8 - 1) / (STEP / 8);
-        int at = wave;
-        if (at >= end) return;
-        const bool even = s.page_blocks.d % (STEP / 8) == 0;
-        find(s, list, n, (unsigned)at * (STEP / 8), even, lane);
-        this->load_k(s, even, lane);
-        this->load_v(s, even, lane);
-        int here = off, held = seen;
-        find(s, list, n, (unsigned)(at + 4) * (STEP / 8), even, lane);
-        for (; at + 4 < end; at += 4) {
-            step(rows, here, held, scale, [&](bool k_is_free) {
-                if (k_is_free) {
-                    this->load_k(s, even, lane);
-                } else {
-                    this->load_v(s, even, lane);
-                    here = off;
-                    held = seen;
-                    find(s, list, n, (unsigned)(at + 8) * (STEP / 8), even, lane);
-                }
-            });
-        }
-        step(rows, here, held, scale, [](bool) {});
-    }
 };
+
+// Steps wave, wave + 4, ... of the list's n entries, the next one's keys and values in flight while one is worked on.  Nothing is requested under a condition within the loop, and nothing that is not
+// there: a request that may not have been made turns every wait for older ones into one for all, and the workgroup waits for all of them in the end.
+template <typename T, int D>
+__device__ __forceinline__ void walk_list(AttentionRows<T, D, 1, false>& rows, const Keys& s, const u32x2* list, int n, float scale, int wave, int lane) {
+    using Walk = ListWalk<T, D>;
+    constexpr int BLOCKS = Walk::STEP / 8;
+    const int steps = (n * (int)s.page_blocks.d + BLOCKS - 1) / BLOCKS;
+    if (wave >= steps) return;
+    const bool even = s.page_blocks.d % BLOCKS == 0;
+    Walk walk;
+    walk.find(s, list, n, (unsigned)wave * BLOCKS, even, lane);
+    walk.load_k(s, even, lane);
+    walk.load_v(s, even, lane);
+    int at = wave;
+    for (; at + 4 < steps; at += 4) {
+        const int here = walk.off, held = walk.seen;
+        walk.step(rows, here, held, scale, [&](bool k_is_free) {
+            if (k_is_free) {
+                walk.find(s, list, n, (unsigned)(at + 4) * BLOCKS, even, lane);
+                walk.load_k(s, even, lane);
+            } else {
+                walk.load_v(s, even, lane);
+            }
+        });
+    }
+    walk.step(rows, walk.off, walk.seen, scale, [](bool) {});
+}
 
 template <typename T, int D>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void page_attention_kernel(PageAttentionArgs p) {
@@ -151,8 +154,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void page_attention_kernel(Pa
                 list[i] = u32x2{(unsigned)page, (unsigned)max(min(seen, a.page_size), 0)};
             }
             __syncthreads();
-            ListWalk<T, D> keys;
-            keys.walk_list(rows, s, list, n, a.scale_log2, __builtin_amdgcn_readfirstlane(wave), lane);
+            walk_list<T, D>(rows, s, list, n, a.scale_log2, __builtin_amdgcn_readfirstlane(wave), lane);
         }
         leave<T, D, Fm>(a, rows, split, row_id, lds);
         if (a.counters) join_last<T, D, 16>(a, row_id, (unsigned)(((size_t)t * p.tiles.d + tile) * a.kv_heads.d + h) * 32, min(per_kv - first_row, 16), done);
@@ -477,41 +479,6 @@ __device__ __forceinline__ void join_rows(const WeighArgs& a, int token, int h, 
     }
 }
 
-// From stored scores: four tokens a thread.
-static __global__ __launch_bounds__(256) void stored_weights_kernel(WeighArgs a) {
-    hook_entry(a.notifier, a.job_id);
-    __shared__ f32x2 whole[16];
-    const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, a.own_splits);
-    const int h = (int)by_head.r, split = (int)by_split.r, seq = (int)by_split.q;
-    const NewTokens its = new_tokens(a.starts, a.past, seq, a.max_new, a.tokens);
-    const int rows = its.count * (int)a.per_kv.d, places = a.max_pages * a.page_size, past = min(its.past, places), held = min(past + its.count, places);
-    const int per = (int)divide((unsigned)held + a.own_splits.d - 1, a.own_splits).q, begin = min(split * ((per + 3) / 4 * 4), held), end = min(begin + (per + 3) / 4 * 4, held);
-    if (rows > 0 && begin < end) {
-        join_rows<16>(a, its.first, h, 0, rows, whole);
-        __syncthreads();
-        const size_t head = (size_t)seq * a.kv_heads.d + h;
-        const float* const scores = a.scores + head * a.score_rows * (size_t)places;
-        float* const weights = a.weights + head * (size_t)places;
-        const __amdgpu_buffer_rsrc_t to = descriptor(weights);
-        for (int i = begin + (int)threadIdx.x * 4; i < end; i += 1024) {  // (places are a multiple of eight: four of them are there)
-            const f32x4 old = *reinterpret_cast<const f32x4*>(weights + i);
-            f32x4 w = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-            for (int r = 0; r < rows; ++r) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(scores + (size_t)r * places + i);
-                const f32x2 row = whole[r];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] += row.y * __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale_log2, -row.x));
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                w[e] = i + e >= held ? old[e] : i + e >= past ? w[e] : old[e] + w[e];
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, w), to, i * 4, 0, kThrough);
-        }
-    }
-    hook_exit(a.notifier, a.job_id);
-}
-
 template <typename T, int D, int TILES>
 __global__ __launch_bounds__(256) void key_weights_kernel(WeighArgs a) {
     hook_entry(a.notifier, a.job_id);
@@ -568,6 +535,8 @@ __global__ __launch_bounds__(256) void key_weights_kernel(WeighArgs a) {
 
 using WeighKernel = void (*)(WeighArgs);
 
+WeighKernel stored_weights();  // from stored scores, of every type
+
 // few: at most 16 rows a sequence and key head
 template <typename T, int D>
 WeighKernel key_sums_kernel_of(bool few) { return few ? key_sums_kernel<T, D, 1> : key_sums_kernel<T, D, weigh_tiles<T, D>()>; }
@@ -577,7 +546,7 @@ WeighKernel key_sums(int dim, bool few) {
 }
 template <typename T>
 WeighKernel key_weights(int dim, bool few) {
-    if (few) return stored_weights_kernel;
+    if (few) return stored_weights();
     return dim == 64 ? key_weights_kernel<T, 64, weigh_tiles<T, 64>()> : dim == 128 ? key_weights_kernel<T, 128, weigh_tiles<T, 128>()> : key_weights_kernel<T, 256, weigh_tiles<T, 256>()>;
 }
 

@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "long_attention.h"
 #include "long_common.h"
 #include "pick_largest.h"
 #include "prefix_attention.h"
@@ -821,7 +822,47 @@ int evict_check(const paella_kv_evict_desc* d, const paella_kv_cache* c) {
     return 0;
 }
 
+// ------------------------------------------------------------------------------------------ the weights of stored scores (long_attention.h)
+// Four tokens a thread.
+__global__ __launch_bounds__(256) void stored_weights_kernel(WeighArgs a) {
+    hook_entry(a.notifier, a.job_id);
+    __shared__ f32x2 whole[16];
+    const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, a.own_splits);
+    const int h = (int)by_head.r, split = (int)by_split.r, seq = (int)by_split.q;
+    const NewTokens its = new_tokens(a.starts, a.past, seq, a.max_new, a.tokens);
+    const int rows = its.count * (int)a.per_kv.d, places = a.max_pages * a.page_size, past = min(its.past, places), held = min(past + its.count, places);
+    const int per = (int)divide((unsigned)held + a.own_splits.d - 1, a.own_splits).q, begin = min(split * ((per + 3) / 4 * 4), held), end = min(begin + (per + 3) / 4 * 4, held);
+    if (rows > 0 && begin < end) {
+        join_rows<16>(a, its.first, h, 0, rows, whole);
+        __syncthreads();
+        const size_t head = (size_t)seq * a.kv_heads.d + h;
+        const float* const scores = a.scores + head * a.score_rows * (size_t)places;
+        float* const weights = a.weights + head * (size_t)places;
+        const __amdgpu_buffer_rsrc_t to = descriptor(weights);
+        for (int i = begin + (int)threadIdx.x * 4; i < end; i += 1024) {  // (places are a multiple of eight: four of them are there)
+            const f32x4 old = *reinterpret_cast<const f32x4*>(weights + i);
+            f32x4 w = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(scores + (size_t)r * places + i);
+                const f32x2 row = whole[r];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] += row.y * __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale_log2, -row.x));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                w[e] = i + e >= held ? old[e] : i + e >= past ? w[e] : old[e] + w[e];
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, w), to, (int)((unsigned)i * 4), 0, kThrough);
+        }
+    }
+    hook_exit(a.notifier, a.job_id);
+}
+
 }  // namespace
+
+namespace paella {
+WeighKernel stored_weights() { return stored_weights_kernel; }
+}  // namespace paella
 
 extern "C" {
 
