@@ -159,10 +159,10 @@ def test_calls_captured_on_a_side_stream_need_a_workspace(cuda, name):
     use = Use(name, cuda)
     assert use.spaces
     want, space, s = use.eager(), use.plan.new_workspace(), use.fresh()
-    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    home, side, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()   # (one after the other: two of torch's streams)
+    assert home.cuda_stream != side.cuda_stream
     torch.cuda.synchronize()
-    with torch.cuda.graph(graph):
-        home = torch.cuda.current_stream()
+    with torch.cuda.graph(graph, stream=home):
         use.begin(s)
         side.wait_stream(home)
         with pytest.raises(AssertionError):
