@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void page_attention_kernel(Pa
             const int n = min(end - first, kListed);
             __syncthreads();
             for (int i = threadIdx.x; i < n; i += 256) {
-                const int e = entries[first + i], o = e - a.prefix_pages;
+                const int e = entries[first + i], o = e < 0 ? e : e - a.prefix_pages;
                 int page = 0, seen = 0;
                 if (e >= 0 && o < 0) {
                     page = a.prefix_table[e];

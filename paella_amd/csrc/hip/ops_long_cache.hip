@@ -399,21 +399,20 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
     const Span<WAVES, KEYS> span(pages);
     unsigned held[KEYS ? KEYS : 1];
     auto load = [&](unsigned i) { return read(entries + i); };
-    span.hold(held, load);
+    unsigned each = threadIdx.x;  // (the last error again behind it)
+    float error = read(errors + min(each, 4 * a.splits.d - 1));
+    span.hold(held, load, [](unsigned k) { return k; });
     auto get = [&](int u, unsigned i) { return KEYS ? held[u] : load(i); };
-    auto known = [](unsigned k) { return k > kUnknown && k < kForced ? k : 0u; };
+    auto known = [](unsigned k) { return k - (kUnknown + 1) < kForced - (kUnknown + 1) ? k : 0u; };
     Range<unsigned> range;
     unsigned forced = 0, unknown = 0;
-    span.visit(get, [&](int, unsigned, bool is, unsigned k) {
-        forced += is && k == kForced;
-        unknown += is && k == kUnknown;
-        range.add(is ? known(k) : 0u);
+    span.visit(get, [&](int, unsigned, unsigned k) {
+        forced += wave_count(k == kForced);
+        unknown += wave_count(k == kUnknown);
+        range.add(known(k));
     });
-    float error = 0.f;
-    for (unsigned i = threadIdx.x; i < 4 * a.splits.d; i += WAVES * 64) error = fmaxf(error, read(errors + i));
+    while ((each += WAVES * 64) < 4 * a.splits.d) error = fmaxf(error, read(errors + each));
     error = wave_max_f(error);
-    forced = wave_all(forced, Sum());
-    unknown = wave_all(unknown, Sum());
     if (lane == 0) {
         s.forced[wave] = forced;
         s.unknown[wave] = unknown;
@@ -440,22 +439,21 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
         }
         out = max(out, kUnknown + 1);
     }
+    const unsigned width = in >= out ? in - out + 1 : 0;
     auto is_in = [&](unsigned k) { return k > in; };
-    auto is_open = [&](unsigned k) { return (k >= out && k <= in) || (any_unknown && k == kUnknown); };
+    auto is_open = [&](unsigned k) { return k - out < width || (any_unknown && k == kUnknown); };
     unsigned inside = 0, open = 0;
-    span.visit(get, [&](int, unsigned, bool is, unsigned k) {
-        inside += is && is_in(k);
-        open += is && is_open(k);
+    span.visit(get, [&](int, unsigned, unsigned k) {
+        inside += wave_count(is_in(k));
+        open += wave_count(is_open(k));
     });
-    inside = wave_all(inside, Sum());
-    open = wave_all(open, Sum());
     if (lane == 0) {
         s.inside[wave] = inside;
         s.open[wave] = open;
     }
     __syncthreads();
+    const unsigned open_ahead = ahead_of(s.open, wave, &open);
     inside = uniform(waves_all(s.inside, Sum()));
-    open = uniform(waves_all(s.open, Sum()));
     auto take = [&](unsigned place, unsigned i) { put_int(to + place, (int)i); };
     auto none = [](auto) { return false; };
     unsigned taken;
@@ -463,14 +461,12 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
         taken = emit(span, s.pick, get, [&](unsigned k) { return is_in(k) || is_open(k); }, none, 0u, take);
     } else {
         // The open pages, in order, a list at a time, whose worths the waves share out.
-        unsigned ahead = 0;
-        for (int w = 0; w < wave; ++w) ahead += s.open[w];
         for (unsigned first = 0; first < open; first += kOpen) {
             const unsigned n = min(open - first, kOpen);
             auto each_open = [&](auto then) {
-                unsigned slot = ahead - first;  // (those of other lists are far above n)
-                span.visit(get, [&](int u, unsigned i, bool is, unsigned k) {
-                    const bool mine = is && is_open(k);
+                unsigned slot = open_ahead - first;  // (those of other lists are far above n)
+                span.visit(get, [&](int u, unsigned i, unsigned k) {
+                    const bool mine = is_open(k);
                     const unsigned long long who = __ballot(mine);
                     const unsigned at = slot + (unsigned)__popcll(who & ((1ull << lane) - 1));
                     if (mine && at < n) then(u, i, at);
@@ -507,7 +503,7 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
                 return is_in(k) ? ~0ull : is_open(k) ? worths[i] : 0ull;
             };
             Range<unsigned long long> keys;
-            all.visit(key, [&](int, unsigned, bool is, unsigned long long k) { keys.add(is ? k : 0ull); });
+            all.visit(key, [&](int, unsigned, unsigned long long k) { keys.add(k); });
             keys.join(s.pick);
             taken = emit_taken<WAVES, 0, unsigned long long>(all, find_bound<WAVES, 0, unsigned long long>(all, keys, (unsigned)a.count, s.pick, key), s.pick, key, take);
         }
@@ -552,7 +548,7 @@ __global__ __launch_bounds__(256) void page_select_kernel(SelectArgs a) {
         if (a.splits.d > 1) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (threadIdx.x == 0) {
+            if (threadIdx.x == 0) {  // (a tile is one token's)
                 unsigned* const counter = a.counters + ((size_t)(w.its.first + w.j0) * a.kv_heads.d + w.h) * kCounterStride;
                 arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 if (arrived == a.splits.d - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -562,11 +558,7 @@ __global__ __launch_bounds__(256) void page_select_kernel(SelectArgs a) {
         }
         __syncthreads();
         if (a.splits.d == 1 || arrived == a.splits.d - 1) {
-            for (int j = 0; j < w.n; ++j) {
-                if (j) __syncthreads();
-                pick_pages<4, kSelectKeys>(a, w.its.first + w.j0 + j, w.seq, w.h, w.pages(a, j), space,
-                                           [](auto* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
-            }
+            pick_pages<4, kSelectKeys>(a, w.its.first + w.j0, w.seq, w.h, w.pages(a, 0), space, [](auto* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
         }
     }
     hook_exit(a.notifier, a.job_id);
@@ -604,11 +596,12 @@ __global__ __launch_bounds__(WAVES * 64) void evict_pick_kernel(EvictArgs a) {
             const float* const w = a.weights + (size_t)blockIdx.x * a.places + first;
             const Span<WAVES, KEYS> span(middle);
             unsigned held[KEYS ? KEYS : 1];
-            auto load = [&](unsigned i) { return number_key(w[i], 1u); };
-            span.hold(held, load);
-            auto get = [&](int u, unsigned i) { return KEYS ? held[u] : load(i); };
+            auto load = [&](unsigned i) { return as_word(w[i]); };
+            auto key = [](unsigned bits) { return number_key(as_float(bits), 1u); };
+            span.hold(held, load, key);
+            auto get = [&](int u, unsigned i) { return KEYS ? held[u] : key(load(i)); };
             Range<unsigned> range;
-            span.visit(get, [&](int, unsigned, bool is, unsigned k) { range.add(is ? k : 0u); });
+            span.visit(get, [&](int, unsigned, unsigned k) { range.add(k); });
             range.join(space);
             const Bound<unsigned> bound = find_bound<WAVES, KEYS, unsigned>(span, range, want, space, get);
             emit_taken<WAVES, KEYS, unsigned>(span, bound, space, get, [&](unsigned place, unsigned i) { put_int(to + first + place, (int)(first + i)); });
@@ -793,12 +786,12 @@ bool select_plan_ok(const paella_page_select_plan* p) {
 }
 
 size_t select_pitch(const paella_page_select_plan* p) { return (size_t)(select_pages(p) + 15) / 16 * 16; }
-// One launch where four waves hold a row's pages in registers, a tile is one token's (a workgroup that picked for several would take as much longer), and the workgroups are at most one to a
+// One launch where four waves hold a row's pages in registers, a tile is one token's (a workgroup that picked for several would take as much longer), and the workgroups are at most two to a
 // compute unit; of more, those that pick are in the way of those that still screen.  (3 fp32 rows of 57 pages of 2 heads of 64 in one launch / two 9.4 / 10.5 us, 32 bf16 rows of 1025 pages of 8 heads
-// of 128, 1024 workgroups, 45.2 / 41.3.)
+// of 128, 512 workgroups, 30.9 / 33.6; by 1024 45.2 / 41.3.)
 int select_stages(const paella_page_select_plan* p) {
     const bool one = std::min(p->max_new, p->tokens) == 1 || tokens_of_tile(p->heads / p->kv_heads) == 1;
-    return one && screen_grid(p) <= 256 && select_pages(p) <= 256 * kSelectKeys ? 1 : 2;
+    return one && screen_grid(p) <= 512 && select_pages(p) <= 256 * kSelectKeys ? 1 : 2;
 }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 size_t select_counters(const paella_page_select_plan* p) { return select_stages(p) == 1 ? (size_t)p->tokens * p->kv_heads * kCounterStride * 4 : 0; }

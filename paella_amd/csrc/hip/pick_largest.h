@@ -15,14 +15,14 @@ struct Span {
         begin = min(wave * per, n);
         end = min(begin + per, n);
     }
-    // each(u, i, is, value): place i, the thread's u-th, is there (whole waves come along behind the last one), and what get(u, i) has for it.  Where that reads memory, several are read ahead.
+    // each(u, i, value) for place i, the thread's u-th, and what get(u, i) has for it: 0 behind the last one, where whole waves come along.  Where that reads memory, several are read ahead.
     template <typename Get, typename Each>
     __device__ __forceinline__ void visit(Get get, Each each) const {
         const unsigned lane = threadIdx.x & 63;
         if constexpr (KEYS > 0) {
 #pragma unroll
             for (int u = 0; u < KEYS; ++u)
-                if (begin + u * 64 < end) each(u, begin + u * 64 + lane, begin + u * 64 + lane < end, get(u, begin + u * 64 + lane));
+                if (begin + u * 64 < end) each(u, begin + u * 64 + lane, get(u, begin + u * 64 + lane));
         } else {
             constexpr int AHEAD = 8;
             for (unsigned first = begin; first < end; first += AHEAD * 64) {
@@ -31,18 +31,21 @@ struct Span {
                 for (int u = 0; u < AHEAD; ++u) value[u] = get(0, min(first + u * 64 + lane, end - 1));
 #pragma unroll
                 for (int u = 0; u < AHEAD; ++u)
-                    if (first + u * 64 < end) each(0, first + u * 64 + lane, first + u * 64 + lane < end, value[u]);
+                    if (first + u * 64 < end) each(0, first + u * 64 + lane, first + u * 64 + lane < end ? value[u] : 0);
             }
         }
     }
-    // Registers' first values, from memory.
-    template <typename Value, typename Load>
-    __device__ __forceinline__ void hold(Value (&held)[KEYS ? KEYS : 1], Load load) const {
+    // Registers' first values: key(load(i)), all requested before the first is looked at.
+    template <typename Value, typename Load, typename Key>
+    __device__ __forceinline__ void hold(Value (&held)[KEYS ? KEYS : 1], Load load, Key key) const {
         if constexpr (KEYS > 0) {
             const unsigned lane = threadIdx.x & 63;
 #pragma unroll
             for (int u = 0; u < KEYS; ++u)
                 if (begin + u * 64 < end) held[u] = load(min(begin + u * 64 + lane, end - 1));
+#pragma unroll
+            for (int u = 0; u < KEYS; ++u)
+                if (begin + u * 64 < end) held[u] = begin + u * 64 + lane < end ? key(held[u]) : 0;
         }
     }
 };
@@ -69,6 +72,9 @@ __device__ __forceinline__ unsigned long long number_key(double v, unsigned long
     const unsigned long long b = __builtin_bit_cast(unsigned long long, v + 0.0);
     return v != v ? nan : b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
 }
+
+// How many lanes say so: counted by the scalar unit.
+__device__ __forceinline__ unsigned wave_count(bool b) { return (unsigned)__popcll(__ballot(b)); }
 
 // op of all lanes' whole numbers, the same for the whole wave.
 template <typename Op>
@@ -115,21 +121,18 @@ template <> __device__ __forceinline__ unsigned long long uniform(unsigned long 
 // The least and largest of the keys that are not 0, and how many there are, over all threads.
 template <typename Key>
 struct Range {
-    Key least = ~(Key)0, most = 0;
-    unsigned some = 0;
-    __device__ __forceinline__ void add(Key k) {
-        if (k) {
-            least = min(least, k);
-            ++some;
-        }
+    Key least = ~(Key)0, most = 0;  // (the least one less, until they are joined)
+    unsigned some = 0;  // of the wave, until they are joined
+    __device__ __forceinline__ void add(Key k) {  // by whole waves
+        least = min(least, (Key)(k - 1));  // (none is the largest)
         most = max(most, k);
+        some += wave_count(k != 0);
     }
     template <int WAVES>
     __device__ __forceinline__ void join(PickSpace<WAVES>& s) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         least = wave_all(least, Least());
         most = wave_all(most, Most());
-        some = wave_all(some, Sum());
         __syncthreads();
         if (lane == 0) {
             s.low[wave] = least;
@@ -137,7 +140,7 @@ struct Range {
             s.count[0][wave] = some;
         }
         __syncthreads();
-        least = (Key)uniform(waves_all(s.low, Least()));
+        least = (Key)uniform(waves_all(s.low, Least())) + 1;
         most = (Key)uniform(waves_all(s.high, Most()));
         some = uniform(waves_all(s.count[0], Sum()));
     }
@@ -166,8 +169,8 @@ __device__ __forceinline__ Bound<Key> find_bound(const Span<WAVES, KEYS>& span, 
         __syncthreads();
         for (unsigned b = threadIdx.x; b < 1u << kDigit; b += WAVES * 64) s.bins[b] = 0;
         __syncthreads();
-        span.visit(get, [&](int, unsigned, bool is, Key k) {
-            if (is && k && (k & known) == bound) atomicAdd(&s.bins[(unsigned)(k >> shift) & ((1u << kDigit) - 1)], 1u);
+        span.visit(get, [&](int, unsigned, Key k) {
+            if (k && (k & known) == bound) atomicAdd(&s.bins[(unsigned)(k >> shift) & ((1u << kDigit) - 1)], 1u);
         });
         __syncthreads();
         if (threadIdx.x < 64) {  // some digits a lane, the highest first
@@ -211,8 +214,8 @@ __device__ __forceinline__ Bound<Key> find_bound(const Span<WAVES, KEYS>& span, 
     __syncthreads();
     if (threadIdx.x == 0) s.found = 0;
     __syncthreads();
-    span.visit(get, [&](int, unsigned, bool is, Key k) {
-        if (is && k && (k & known) == bound) s.list[atomicAdd(&s.found, 1u)] = k;
+    span.visit(get, [&](int, unsigned, Key k) {
+        if (k && (k & known) == bound) s.list[atomicAdd(&s.found, 1u)] = k;
     });
     __syncthreads();
     if (threadIdx.x < size) {
@@ -233,42 +236,51 @@ __device__ __forceinline__ Bound<Key> find_bound(const Span<WAVES, KEYS>& span, 
     return {(Key)s.bound, s.left};
 }
 
+// Sum of the waves' numbers in LDS ahead of this wave's, and of all.
+template <int WAVES>
+__device__ __forceinline__ unsigned ahead_of(const unsigned (&of)[WAVES], int wave, unsigned* all) {
+    unsigned ahead = 0, sum = 0;
+    if constexpr (WAVES == 16) {
+        const unsigned v = of[threadIdx.x & 15];
+        sum = row_all(v, Sum());
+        ahead = row_all((int)(threadIdx.x & 15) < wave ? v : 0u, Sum());
+    } else {
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            ahead += w < wave ? of[w] : 0;
+            sum += of[w];
+        }
+    }
+    *all = uniform(sum);
+    return uniform(ahead);
+}
+
 // take(place, i) for every place whose value above(value), and for the first `left` of those whose value is tied(value), in order; returns how many.
 template <int WAVES, int KEYS, typename Get, typename Above, typename Tied, typename Take>
 __device__ __forceinline__ unsigned emit(const Span<WAVES, KEYS>& span, PickSpace<WAVES>& s, Get get, Above above, Tied tied, unsigned left, Take take) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     unsigned more = 0, equal = 0;
-    span.visit(get, [&](int, unsigned, bool is, auto k) {
-        more += is && above(k);
-        if (left) equal += is && tied(k);
+    span.visit(get, [&](int, unsigned, auto k) {
+        more += wave_count(above(k));
+        if (left) equal += wave_count(tied(k));
     });
-    more = wave_all(more, Sum());
-    if (left) equal = wave_all(equal, Sum());
     __syncthreads();
     if (lane == 0) {
         s.count[1][wave] = more;
         s.count[2][wave] = equal;
     }
     __syncthreads();
-    unsigned place = 0, ties = 0, all = 0, ties_all = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        const unsigned here = min(s.count[2][w], left - min(left, ties_all));
-        if (w < wave) {
-            place += s.count[1][w] + here;
-            ties += s.count[2][w];
-        }
-        all += s.count[1][w] + here;
-        ties_all += s.count[2][w];
-    }
-    place = uniform(place);
-    ties = uniform(ties);
+    unsigned all, ties_all = 0, ties = 0;
+    unsigned place = ahead_of(s.count[1], wave, &all);
+    if (left) ties = ahead_of(s.count[2], wave, &ties_all);
+    place += min(ties, left);
+    all += min(ties_all, left);
     const unsigned long long before = (1ull << lane) - 1;
-    span.visit(get, [&](int, unsigned i, bool is, auto k) {
-        bool mine = is && above(k);
+    span.visit(get, [&](int, unsigned i, auto k) {
+        bool mine = above(k);
         if (left) {
-            const unsigned long long who = __ballot(is && tied(k));
-            mine |= is && tied(k) && ties + (unsigned)__popcll(who & before) < left;
+            const unsigned long long who = __ballot(tied(k));
+            mine |= tied(k) && ties + (unsigned)__popcll(who & before) < left;
             ties += (unsigned)__popcll(who);
         }
         const unsigned long long who = __ballot(mine);
@@ -277,7 +289,7 @@ __device__ __forceinline__ unsigned emit(const Span<WAVES, KEYS>& span, PickSpac
             place += (unsigned)__popcll(who);
         }
     });
-    return uniform(all);
+    return all;
 }
 
 template <int WAVES, int KEYS, typename Key, typename Get, typename Take>

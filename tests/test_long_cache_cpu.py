@@ -110,10 +110,11 @@ def test_plans_refuse(lib, make):
 
 def test_what_plans_plan(lib):
     from paella_amd import _abi
-    # few rows of few pages: one launch; more workgroups than the device has units, or more pages than it holds: two
+    # few rows of few pages: one launch; more workgroups than two to a compute unit, or more pages than four waves hold: two
     assert select_plan(lib, cache(), batch())[1].stages == 1
     rc, p = select_plan(lib, cache(heads=8, dim=128, size=64, pages=9000), batch(sequences=32, max_pages=1025), 32, 64, 1, 2)
-    assert rc == 0 and p.stages == 2 and p.workspace_bytes >= 3 * 32 * 8 * 1025 * 4
+    assert rc == 0 and p.stages == 1 and p.workspace_bytes >= 3 * 32 * 8 * 1025 * 4
+    assert select_plan(lib, cache(heads=8, dim=128, size=64, pages=9000), batch(sequences=80, max_pages=1025), 32, 64, 1, 2)[1].stages == 2
     assert select_plan(lib, cache(pages=9000), batch(sequences=1, max_pages=5000))[1].stages == 2
     # lists that fill the device are not shared out; one of many pages is, and a wide one's parts are joined by a launch of their own
     assert attend_plan(lib, cache(heads=8, dim=128, size=64), batch(sequences=64), 32, 64)[1].workspace_bytes == 0
