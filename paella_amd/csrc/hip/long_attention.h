@@ -180,7 +180,7 @@ struct WeighArgs {
     int64_t q_stride;  // bytes
     int sequences, max_new, tokens, max_pages, prefix_len, prefix_pages, num_pages, page_size, heads;
     Divisor kv_heads, per_kv, page_blocks, splits, own_splits, chunks;  // chunks: of a sequence's rows
-    float scale_log2;
+    float scale_log2, rise;  // rise: of scores that are not yet scaled
     f32x2* ml;         // [splits][tokens * heads]: maximum and sum of each part
     float* scores;     // q . k: [sequences][kv_heads][score_rows][max_pages * page_size], -inf where a row does not see the token
     int score_rows;
@@ -189,10 +189,16 @@ struct WeighArgs {
 };
 
 constexpr float kRise = 8.f;  // how far scores may be above the running maximum before it moves
+constexpr float kLowest = -3.4028234663852886e38f;  // the maximum of no scores: what is not seen, -inf, is below it
 
 // Rows that a workgroup has in LDS: 32 KB of queries.
 template <typename T, int D>
 constexpr int weigh_tiles() { return 32768 / (16 * D * T::bytes) > 8 ? 8 : 32768 / (16 * D * T::bytes); }
+
+// Tiles of 16 rows that a wave takes through at once: the products and exponentials of one go on while those of the other are waited for.  (The sums of 128 rows, as below, one by
+// one / two by two 33.4 / 31.3 us.)
+template <int TILES>
+constexpr int side_by_side() { return TILES % 2 ? 1 : 2; }
 
 // The keys of one key head, step by step: the prefix's pages, then the sequence's own.  Places count along those pages, the prefix's last one to its end.
 template <typename T, int D>
@@ -207,7 +213,8 @@ struct KeyWalk {
     size_t page_bytes;
     Divisor page_blocks;
 
-    u32x4 keys[NT][KC];
+    u32x4 keys[NT][KC];  // of the step that is worked on next
+    bool absent;         // the lane group's lie in no page
 
     // Where the blocks of a wave's steps lie, some steps ahead: lane i has block i % BLOCKS of step i / BLOCKS.  A request that follows keys' requests is answered after them: looked up
     // step by step, pages would have each step's keys wait for those of the one before.
@@ -227,7 +234,7 @@ struct KeyWalk {
         look(step + STEPS * 4, lane, &page_behind, &in_behind);
         left = STEPS;
     }
-    // Asks for the keys of `step`, the steps in turn; gone: the lane group's lie in no page.
+    // Asks for the keys of `step`, the steps in turn.
     __device__ __forceinline__ void request(u32x4 (&to)[NT][KC], bool& gone, int step, int lane) {
         if (left == 0) {
             page = page_behind;
@@ -246,23 +253,34 @@ struct KeyWalk {
             for (int c = 0; c < KC; ++c) to[t][c] = *reinterpret_cast<const u32x4*>(from + t * 4 * ROW + c * 64);
     }
 
-    // x = K q^T for 16 rows, whose pieces lie in LDS in the order of the lanes
-    __device__ __forceinline__ void scores(f32x4 (&x)[NT], const u32x4* q, int lane) const {
+    // Asks for a wave's first step, ahead of all else that a workgroup has to fetch: any step may be asked for.
+    __device__ __forceinline__ void start(int step, int lane) {
+        begin(step, lane);
+        request(keys, absent, step, lane);
+    }
+
+    // x = K q^T for SIDE tiles of 16 rows, whose pieces lie in LDS in the order of the lanes
+    template <int SIDE>
+    __device__ __forceinline__ void scores(f32x4 (&x)[SIDE][NT], const u32x4* q, int lane) const {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) x[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < SIDE; ++i)
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            const u32x4 piece = q[c * 64 + lane];
+            for (int t = 0; t < NT; ++t) x[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                if constexpr (F) {
+        for (int c = 0; c < KC; ++c)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[t] = mfma_f32(as_float(keys[t][c][e]), as_float(piece[e]), x[t]);
-                } else {
-                    x[t] = Mfma<T>::go(keys[t][c], piece, x[t]);
+            for (int i = 0; i < SIDE; ++i) {
+                const u32x4 piece = q[(i * KC + c) * 64 + lane];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if constexpr (F) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[i][t] = mfma_f32(as_float(keys[t][c][e]), as_float(piece[e]), x[i][t]);
+                    } else {
+                        x[i][t] = Mfma<T>::go(keys[t][c], piece, x[i][t]);
+                    }
                 }
             }
-        }
     }
 };
 
@@ -280,21 +298,31 @@ __device__ __forceinline__ KeyWalk<T, D> key_walk(const WeighArgs& a, int seq, i
     return k;
 }
 
-// Queries of the rows from `first` on to LDS, piece by piece as the lanes want them; behind the sequence's last row the last one again.
+// Queries of a workgroup's rows from `first` on, piece by piece as the lanes want them in LDS; behind the sequence's last row the last one again.  All are requested before any is put
+// there (4 sequences, 128 rows over 17000 bf16 keys of 8 heads of 128: the sums 31.3 us one after the other, 28.9 so).
 template <typename T, int D, int TILES>
-__device__ __forceinline__ void stage_queries(const WeighArgs& a, int token, int h, int first, int rows, u32x4* to) {
-    constexpr int KC = D * T::bytes / 64;
-    for (int i = threadIdx.x; i < TILES * KC * 64; i += 256) {
-        const int lane = i & 63, c = i / 64 % KC, tile = i / 64 / KC;
-        if (first + tile * 16 >= rows) break;
-        const Quotient at = divide((unsigned)min(first + tile * 16 + (lane & 15), rows - 1), a.per_kv);
-        to[i] = *reinterpret_cast<const u32x4*>(a.q + (token + (int)at.q) * a.q_stride + (size_t)(h * (int)a.per_kv.d + (int)at.r) * D * T::bytes + c * 64 + (lane >> 4) * 16);
+struct StagedQueries {
+    static constexpr int KC = D * T::bytes / 64, PIECES = TILES * KC * 64, EACH = (PIECES + 255) / 256;
+    u32x4 piece[EACH];
+
+    __device__ __forceinline__ void request(const WeighArgs& a, int token, int h, int first, int rows) {
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) {
+            const int i = min(u * 256 + (int)threadIdx.x, PIECES - 1), lane = i & 63, c = i / 64 % KC, tile = i / 64 / KC;
+            const Quotient at = divide((unsigned)min(first + tile * 16 + (lane & 15), rows - 1), a.per_kv);
+            piece[u] = *reinterpret_cast<const u32x4*>(a.q + (token + (int)at.q) * a.q_stride + (size_t)(h * (int)a.per_kv.d + (int)at.r) * D * T::bytes + c * 64 + (lane >> 4) * 16);
+        }
     }
-}
+    __device__ __forceinline__ void put(u32x4* to) const {
+#pragma unroll
+        for (int u = 0; u < EACH; ++u)
+            if (PIECES % 256 == 0 || u * 256 + (int)threadIdx.x < PIECES) to[u * 256 + threadIdx.x] = piece[u];
+    }
+};
 
 // Steps over the keys [begin, end) of `walk`, every fourth one for each wave.  each(x, tile, first): scores of a tile for the step's keys, those of keys that a row does not see
 // -inf; close(first): behind a step's last tile; open(): ahead of a step's requests.
-template <typename T, int D, int TILES, typename Open, typename Each, typename Close>
+template <typename T, int D, int TILES, int SIDE, typename Open, typename Each, typename Close>
 __device__ __forceinline__ void walk_keys(const WeighArgs& a, KeyWalk<T, D>& walk, const u32x4* q, int first_row, int rows, int past, int begin, int end, int wave, int lane, Open open,
                                           Each each, Close close) {
     using Walk = KeyWalk<T, D>;
@@ -307,18 +335,21 @@ __device__ __forceinline__ void walk_keys(const WeighArgs& a, KeyWalk<T, D>& wal
         const int first = at * Walk::STEP, mine = first + (lane >> 4) * Walk::TPL;
         const bool whole = (first + Walk::STEP <= a.prefix_len || (first >= behind && first + Walk::STEP <= least)) && !__any(absent);
 #pragma unroll
-        for (int tile = 0; tile < TILES; ++tile) {
+        for (int tile = 0; tile < TILES; tile += SIDE) {
             if (first_row + tile * 16 >= rows) break;
-            f32x4 x[Walk::NT];
+            f32x4 x[SIDE][Walk::NT];
             walk.scores(x, q + tile * Walk::KC * 64, lane);
             if (!whole) {
-                const int row = min(first_row + tile * 16 + (lane & 15), rows - 1);
-                const int limit = mine < behind ? a.prefix_len : behind + min(past + (int)divide((unsigned)row, a.per_kv).q + 1, places);
 #pragma unroll
-                for (int t = 0; t < Walk::NT; ++t)
+                for (int i = 0; i < SIDE; ++i) {
+                    const int row = min(first_row + (tile + i) * 16 + (lane & 15), rows - 1);
+                    const int limit = mine < behind ? a.prefix_len : behind + min(past + (int)divide((unsigned)row, a.per_kv).q + 1, places);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (absent || mine + t * 4 + e >= limit) x[t][e] = -INFINITY;
+                    for (int t = 0; t < Walk::NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (absent || mine + t * 4 + e >= limit) x[i][t][e] = -INFINITY;
+                }
             }
             each(x, tile, first);
         }
@@ -334,25 +365,24 @@ __device__ __forceinline__ void walk_keys(const WeighArgs& a, KeyWalk<T, D>& wal
     // A step's keys are requested one step ahead.  Not under a condition: a request that may not have been made turns every wait for older ones into one for all.  (Two steps ahead: no faster, 180 us
     // for 32 sequences of up to 16384 tokens of 8 heads of 128 in bf16 in 16 parts either way.)
     Held next;
-    bool absent, absent_next;
-    walk.begin(at, lane);
-    walk.request(walk.keys, absent, at, lane);
+    bool absent_next;
     for (; at + 4 < end; at += 4) {
         open();
         walk.request(next, absent_next, at + 4, lane);
-        work(absent);
+        work(walk.absent);
         move(walk.keys, next);
-        absent = absent_next;
+        walk.absent = absent_next;
     }
     open();
-    work(absent);
+    work(walk.absent);
 }
 
 template <typename T, int D, int TILES>
-__global__ __launch_bounds__(256) void key_sums_kernel(WeighArgs a) {
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void key_sums_kernel(WeighArgs a) {
     hook_entry(a.notifier, a.job_id);
     using Walk = KeyWalk<T, D>;
     __shared__ u32x4 q[TILES * Walk::KC * 64];
+    constexpr int SIDE = side_by_side<TILES>();
     __shared__ f32x2 sums[4][TILES * 16];
     __shared__ __attribute__((aligned(16))) float stored[TILES == 1 ? 4 * 16 * Walk::STEP : 4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -361,20 +391,24 @@ __global__ __launch_bounds__(256) void key_sums_kernel(WeighArgs a) {
     const NewTokens its = new_tokens(a.starts, a.past, seq, a.max_new, a.tokens);
     const int rows = its.count * (int)a.per_kv.d;
     if (first_row < rows) {
-        stage_queries<T, D, TILES>(a, its.first, h, first_row, rows, q);
-        float m[TILES], l[TILES];
-#pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-            m[i] = -INFINITY;
-            l[i] = 0.f;
-        }
-        __syncthreads();
         const int last_row = min(first_row + TILES * 16, rows) - 1;
         const int places = min(a.max_pages * a.page_size, 1 << 30), past = min(its.past, places);
         const int keys = a.prefix_pages * a.page_size + min(past + (int)divide((unsigned)last_row, a.per_kv).q + 1, places);
         const int steps = (keys + Walk::STEP - 1) / Walk::STEP, per = (int)divide((unsigned)steps + a.splits.d - 1, a.splits).q;
         const int begin = min(split * per, steps), end = min(begin + per, steps);
         Walk walk = key_walk<T, D>(a, seq, h);
+        walk.start(begin + wave, lane);
+        StagedQueries<T, D, TILES> staged;
+        staged.request(a, its.first, h, first_row, rows);
+        staged.put(q);
+        float m[TILES], l[TILES], limit[TILES];  // limit: what scores, not yet scaled, may rise to
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            m[i] = kLowest;
+            limit[i] = -INFINITY;
+            l[i] = 0.f;
+        }
+        __syncthreads();
         const int behind = a.prefix_pages * a.page_size, places_all = a.max_pages * a.page_size;
         const __amdgpu_buffer_rsrc_t to_scores = descriptor(TILES == 1 ? a.scores + ((size_t)seq * a.kv_heads.d + h) * a.score_rows * (size_t)places_all : nullptr);
         // Scores leave through LDS, so that whole lines do, 16 bytes of a row's per lane, and a step late, ahead of the requests of the next: a wait for keys waits for the stores ahead of them as well.
@@ -394,28 +428,38 @@ __global__ __launch_bounds__(256) void key_sums_kernel(WeighArgs a) {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
         };
-        walk_keys<T, D, TILES>(
+        walk_keys<T, D, TILES, SIDE>(
             a, walk, q, first_row, rows, past, begin, end, wave, lane, put_scores,
-            [&](const f32x4 (&x)[Walk::NT], int tile, int first) {
-                float top = x[0][0];
+            [&](const f32x4 (&x)[SIDE][Walk::NT], int tile, int first) {
+                float top[SIDE];
+                bool rises = false;
 #pragma unroll
-                for (int t = 0; t < Walk::NT; ++t)
+                for (int i = 0; i < SIDE; ++i) {
+                    top[i] = x[i][0][0];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top = fmaxf(top, x[t][e]);
-                top *= a.scale_log2;
-                if (__any(top > m[tile] + kRise)) {  // (until then the exponentials have room above 1)
-                    const float now = fmaxf(m[tile], top);
-                    l[tile] *= m[tile] == now ? 1.f : __builtin_amdgcn_exp2f(m[tile] - now);
-                    m[tile] = now;
+                    for (int t = 0; t < Walk::NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) top[i] = fmaxf(top[i], x[i][t][e]);
+                    rises |= top[i] > limit[tile + i];
                 }
-                const float base = m[tile] == -INFINITY ? 0.f : m[tile];
+                if (__any(rises)) {  // (until then the exponentials have room above 1)
 #pragma unroll
-                for (int t = 0; t < Walk::NT; ++t)
+                    for (int i = 0; i < SIDE; ++i) {
+                        const float now = fmaxf(m[tile + i], top[i] * a.scale_log2);
+                        l[tile + i] *= m[tile + i] == now ? 1.f : __builtin_amdgcn_exp2f(m[tile + i] - now);
+                        m[tile + i] = now;
+                        limit[tile + i] = fmaxf(limit[tile + i], top[i] + a.rise);
+                    }
+                }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) l[tile] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][e], a.scale_log2, -base));
+                for (int i = 0; i < SIDE; ++i)
+#pragma unroll
+                    for (int t = 0; t < Walk::NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) l[tile + i] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][t][e], a.scale_log2, -m[tile + i]));
                 if constexpr (TILES == 1) {
 #pragma unroll
-                    for (int t = 0; t < Walk::NT; ++t) *reinterpret_cast<f32x4*>(mine + (lane & 15) * Walk::STEP + (lane >> 4) * Walk::TPL + t * 4) = x[t];
+                    for (int t = 0; t < Walk::NT; ++t) *reinterpret_cast<f32x4*>(mine + (lane & 15) * Walk::STEP + (lane >> 4) * Walk::TPL + t * 4) = x[0][t];
                     waiting = first;
                 }
             },
@@ -480,10 +524,11 @@ __device__ __forceinline__ void join_rows(const WeighArgs& a, int token, int h, 
 }
 
 template <typename T, int D, int TILES>
-__global__ __launch_bounds__(256) void key_weights_kernel(WeighArgs a) {
+__global__ __launch_bounds__(256, D > 128 ? 1 : 3) void key_weights_kernel(WeighArgs a) {
     hook_entry(a.notifier, a.job_id);
     using Walk = KeyWalk<T, D>;
     __shared__ u32x4 q[TILES * Walk::KC * 64];
+    constexpr int SIDE = side_by_side<TILES>();
     __shared__ f32x2 whole[TILES * 16];  // of each row: maximum and one over the sum
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, a.own_splits);
@@ -498,21 +543,28 @@ __global__ __launch_bounds__(256) void key_weights_kernel(WeighArgs a) {
         float* const weights = a.weights + ((size_t)seq * a.kv_heads.d + h) * ((size_t)a.max_pages * a.page_size);
         Walk walk = key_walk<T, D>(a, seq, h);
         for (int first_row = 0; first_row < rows && begin < end; first_row += TILES * 16) {
+            walk.start(begin + wave, lane);
+            StagedQueries<T, D, TILES> staged;
+            staged.request(a, its.first, h, first_row, rows);
             __syncthreads();
-            stage_queries<T, D, TILES>(a, its.first, h, first_row, rows, q);
             join_rows<TILES * 16>(a, its.first, h, first_row, rows, whole);
+            staged.put(q);
             __syncthreads();
             float w[Walk::TPL];
 #pragma unroll
             for (int e = 0; e < Walk::TPL; ++e) w[e] = 0.f;
-            walk_keys<T, D, TILES>(
+            walk_keys<T, D, TILES, SIDE>(
                 a, walk, q, first_row, rows, past, begin, end, wave, lane, [] {},
-                [&](const f32x4 (&x)[Walk::NT], int tile, int) {
-                    const f32x2 row = whole[tile * 16 + (lane & 15)];
+                [&](const f32x4 (&x)[SIDE][Walk::NT], int tile, int) {
+                    f32x2 row[SIDE];
 #pragma unroll
-                    for (int t = 0; t < Walk::NT; ++t)
+                    for (int i = 0; i < SIDE; ++i) row[i] = whole[(tile + i) * 16 + (lane & 15)];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) w[t * 4 + e] += row.y * __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][e], a.scale_log2, -row.x));
+                    for (int i = 0; i < SIDE; ++i)
+#pragma unroll
+                        for (int t = 0; t < Walk::NT; ++t)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[t * 4 + e] += row[i].y * __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][t][e], a.scale_log2, -row[i].x));
                 },
                 [&](int first) {
                     float mine = 0.f;

@@ -211,7 +211,7 @@ int paella_key_weights_launch_stage(const paella_key_weights_plan* p, int stage,
     a.prefix_pages = (int)ceil_div(b->prefix_len, c->page_size); a.num_pages = c->num_pages; a.page_size = c->page_size; a.heads = p->heads;
     a.kv_heads = divisor((unsigned)p->kv_heads); a.per_kv = divisor((unsigned)(p->heads / p->kv_heads)); a.page_blocks = divisor((unsigned)c->page_size / 8);
     a.splits = divisor((unsigned)p->splits); a.own_splits = divisor((unsigned)p->own_splits); a.chunks = divisor((unsigned)chunks_of(p));
-    a.scale_log2 = p->scale * 1.44269504088896340736f; a.ml = (f32x2*)workspace;
+    a.scale_log2 = p->scale * 1.44269504088896340736f; a.rise = kRise / a.scale_log2; a.ml = (f32x2*)workspace;
     a.scores = (float*)((char*)workspace + parts_of(p)); a.score_rows = score_rows(p);
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
     launch(kernel_of(p, stage), dim3((unsigned)grid_of(p, stage)), dim3(256), 0, (hipStream_t)stream, a);
