@@ -212,9 +212,10 @@ struct Screened {
     }
 };
 
-// A turn's bounds go to registers while the ones before are worked on, and the numbers of the pages behind them.
-template <typename T, int D>
-__device__ __forceinline__ void screen_pages(const SelectArgs& a, const Screened& w) {
+// A turn's bounds go to registers while the ones before are worked on, and the numbers of the pages behind them.  entry(j, e, key) and error(j, slot, worst) take what is left of page e for the tile's
+// token j, and of all of a wave's.
+template <typename T, int D, typename Entry, typename Error>
+__device__ __forceinline__ void screen_pages(const SelectArgs& a, const Screened& w, Entry entry, Error error_of) {
     constexpr int ROW = D * T::bytes, KC = ROW / 64;
     const int lane = threadIdx.x & 63, mm = lane & 15, group = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int h = w.h, seq = w.seq, heads = (int)a.per_kv.d, j0 = w.j0, n = w.n;
@@ -302,8 +303,7 @@ __device__ __forceinline__ void screen_pages(const SelectArgs& a, const Screened
                 unsigned key = mine.y < INFINITY ? number_key(mine.x, kUnknown) : kUnknown;
                 if (e < (unsigned)a.first || e + a.last >= seen) key = kForced;
                 if ((unsigned)page >= (unsigned)a.num_pages) key = kNoPage;
-                const size_t at = (size_t)(its.first + j0 + j) * a.kv_heads.d + h;
-                if (group == 0 && e < seen) __hip_atomic_store(a.entries + at * a.pitch + e, key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (group == 0 && e < seen) entry(j, e, key);
             }
         };
         // (The next turn's bounds are requested whatever comes, or not at all: a request that may not have been made turns every wait for older ones into one for all.)
@@ -327,7 +327,7 @@ __device__ __forceinline__ void screen_pages(const SelectArgs& a, const Screened
         work();
     }
     worst = wave_max_f(worst);  // of all rows of the tile
-    if (lane < n) store_out(a.errors + ((size_t)(its.first + j0 + lane) * a.kv_heads.d + h) * step + (unsigned)w.split * 4 + wave, worst);
+    if (lane < n) error_of(lane, (unsigned)w.split * 4 + wave, worst);
 }
 
 // A page's worth in 64 bits, by a whole wave: 16 bytes of a row per lane, the bounds and four heads' queries requested together.
@@ -387,20 +387,15 @@ struct PageSpace {
     unsigned long long worth[kOpen];
 };
 
-// The row's pages by their entries, which read(address) reads, as it does the errors.  KEYS as in Span.
-template <int WAVES, int KEYS, typename Read>
-__device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, int h, unsigned pages, PageSpace<WAVES>& s, Read read) {
+// The row's pages by their entries, load(i).  error: this thread's share of the screen's.  KEYS as in Span.
+template <int WAVES, int KEYS, typename Load>
+__device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, int h, unsigned pages, float error, PageSpace<WAVES>& s, Load load) {
     const size_t row = (size_t)t * a.kv_heads.d + h;
-    const unsigned* const entries = a.entries + row * a.pitch;
-    const float* const errors = a.errors + row * 4 * a.splits.d;
     unsigned long long* const worths = a.worths + row * a.pitch;
     int* const to = a.pages + row * a.count;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const Span<WAVES, KEYS> span(pages);
     unsigned held[KEYS ? KEYS : 1];
-    auto load = [&](unsigned i) { return read(entries + i); };
-    unsigned each = threadIdx.x;  // (the last error again behind it)
-    float error = read(errors + min(each, 4 * a.splits.d - 1));
     span.hold(held, load, [](unsigned k) { return k; });
     auto get = [&](int u, unsigned i) { return KEYS ? held[u] : load(i); };
     auto known = [](unsigned k) { return k - (kUnknown + 1) < kForced - (kUnknown + 1) ? k : 0u; };
@@ -411,7 +406,6 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
         unknown += wave_count(k == kUnknown);
         range.add(known(k));
     });
-    while ((each += WAVES * 64) < 4 * a.splits.d) error = fmaxf(error, read(errors + each));
     error = wave_max_f(error);
     if (lane == 0) {
         s.forced[wave] = forced;
@@ -514,7 +508,11 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
 template <typename T, int D>
 __global__ __launch_bounds__(256) void page_screen_kernel(SelectArgs a) {
     hook_entry(a.notifier, a.job_id);
-    screen_pages<T, D>(a, Screened(a));
+    const Screened w(a);
+    auto row = [&](int j) { return (size_t)(w.its.first + w.j0 + j) * a.kv_heads.d + w.h; };
+    screen_pages<T, D>(
+        a, w, [&](int j, unsigned e, unsigned key) { __hip_atomic_store(a.entries + row(j) * a.pitch + e, key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); },
+        [&](int j, unsigned slot, float worst) { store_out(a.errors + row(j) * 4 * a.splits.d + slot, worst); });
     hook_exit(a.notifier, a.job_id);
 }
 
@@ -528,37 +526,69 @@ __global__ __launch_bounds__(WAVES * 64) void page_pick_kernel(SelectArgs a) {
     int seq, j;
     if (row_owner(a.starts, a.sequences, a.max_new, t, lane, &seq, &j)) {
         const unsigned pages = (unsigned)a.prefix_pages + (unsigned)own_pages(__builtin_amdgcn_readfirstlane(a.past[seq]), j, a.page_size, a.max_pages);
-        pick_pages<WAVES, KEYS>(a, t, seq, h, pages, space, [](auto* p) { return *p; });
+        const size_t row = (size_t)t * a.kv_heads.d + h;
+        const unsigned* const entries = a.entries + row * a.pitch;
+        const float* const errors = a.errors + row * 4 * a.splits.d;
+        float error = errors[min(threadIdx.x, 4 * a.splits.d - 1)];  // (the last one again behind it)
+        for (unsigned i = threadIdx.x + WAVES * 64; i < 4 * a.splits.d; i += WAVES * 64) error = fmaxf(error, errors[i]);
+        pick_pages<WAVES, KEYS>(a, t, seq, h, pages, error, space, [&](unsigned i) { return entries[i]; });
     }
     hook_exit(a.notifier, a.job_id);
 }
 
 // One launch for both: the workgroup that arrives last at a row picks its pages, while others are still screening.  (Entries are written through ahead of the count, and read past this XCD's
-// caches.)
+// caches.)  Where a row has one workgroup, its entries stay in LDS.
 constexpr int kSelectKeys = 8;  // of a thread: up to 2048 pages
 
 template <typename T, int D>
 __global__ __launch_bounds__(256) void page_select_kernel(SelectArgs a) {
     hook_entry(a.notifier, a.job_id);
     __shared__ PageSpace<4> space;
+    __shared__ unsigned entries[256 * kSelectKeys];
+    __shared__ float errors[4];
     __shared__ unsigned arrived;
     const Screened w(a);
-    if (w.n > 0) {
-        screen_pages<T, D>(a, w);
-        if (a.splits.d > 1) {
+    if (w.n > 0) {  // (a tile is one token's)
+        const bool alone = a.splits.d == 1;
+        const size_t row = (size_t)(w.its.first + w.j0) * a.kv_heads.d + w.h;
+        unsigned* const entries_of = a.entries + row * a.pitch;
+        float* const errors_of = a.errors + row * 4 * a.splits.d;
+        screen_pages<T, D>(
+            a, w,
+            [&](int, unsigned e, unsigned key) {
+                if (alone) entries[e] = key;
+                else __hip_atomic_store(entries_of + e, key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            },
+            [&](int, unsigned slot, float worst) {
+                if (alone) errors[slot] = worst;
+                else store_out(errors_of + slot, worst);
+            });
+        if (!alone) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (threadIdx.x == 0) {  // (a tile is one token's)
-                unsigned* const counter = a.counters + ((size_t)(w.its.first + w.j0) * a.kv_heads.d + w.h) * kCounterStride;
+            if (threadIdx.x == 0) {
+                unsigned* const counter = a.counters + row * kCounterStride;
                 arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 if (arrived == a.splits.d - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
         __syncthreads();
-        if (a.splits.d == 1 || arrived == a.splits.d - 1) {
-            pick_pages<4, kSelectKeys>(a, w.its.first + w.j0, w.seq, w.h, w.pages(a, 0), space, [](auto* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
+        if (alone || arrived == a.splits.d - 1) {
+            const unsigned pages = w.pages(a, 0);
+            float error = 0.f;
+            if (alone) {
+                error = errors[threadIdx.x & 3];
+            } else {
+                unsigned held[kSelectKeys];
+                auto read = [](auto* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+#pragma unroll
+                for (int u = 0; u < kSelectKeys; ++u) held[u] = read(entries_of + min(threadIdx.x + u * 256, pages - 1));
+                for (unsigned i = threadIdx.x; i < 4 * a.splits.d; i += 256) error = fmaxf(error, read(errors_of + i));
+#pragma unroll
+                for (int u = 0; u < kSelectKeys; ++u) entries[threadIdx.x + u * 256] = held[u];
+                __syncthreads();
+            }
+            pick_pages<4, kSelectKeys>(a, w.its.first + w.j0, w.seq, w.h, pages, error, space, [&](unsigned i) { return entries[i]; });
         }
     }
     hook_exit(a.notifier, a.job_id);
