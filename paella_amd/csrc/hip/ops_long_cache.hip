@@ -337,8 +337,8 @@ __device__ __forceinline__ unsigned long long exact_worth_of(const SelectArgs& a
     const int lane = threadIdx.x & 63, heads = (int)a.per_kv.d, row = a.dim * T::bytes;
     const int at = min(lane * 16, row - 16);
     const char* const q = a.q + t * a.q_stride + (size_t)h * heads * row + at;
-    const int page = page_along(a, seq, e);  // (in the cache: others are not asked for)
-    const char* const from = a.bounds + ((size_t)page * a.kv_heads.d + h) * 2 * row + at;
+    const unsigned page = (unsigned)page_along(a, seq, e);  // (outside the cache only if entries are another call's)
+    const char* const from = a.bounds + ((size_t)(page < (unsigned)a.num_pages ? page : 0u) * a.kv_heads.d + h) * 2 * row + at;
     const u32x4 low = *reinterpret_cast<const u32x4*>(from), high = *reinterpret_cast<const u32x4*>(from + row);
     unsigned long long best = 0;
     for (int g = 0; g < heads; g += G) {
@@ -448,7 +448,9 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
     __syncthreads();
     const unsigned open_ahead = ahead_of(s.open, wave, &open);
     inside = uniform(waves_all(s.inside, Sum()));
-    auto take = [&](unsigned place, unsigned i) { put_int(to + place, (int)i); };
+    auto take = [&](unsigned place, unsigned i) {
+        if (place < (unsigned)a.count) put_int(to + place, (int)i);  // (more only if entries are another call's)
+    };
     auto none = [](auto) { return false; };
     unsigned taken;
     if (inside + open <= (unsigned)a.count) {
@@ -677,7 +679,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const unsigned i = first + u * 256 + threadIdx.x;
-                    if (i < keep) store_out(w + i, x[u]);
+                    if (i < min(keep, a.places)) store_out(w + i, x[u]);
                 }
             }
             if (h == 0 && threadIdx.x == 0) put_int(a.past_out + seq, a.keep);

@@ -271,3 +271,31 @@ def test_pages_behind_32_bits(cuda):
     for got, want in zip(*made):
         same(got, want)
     assert made[0][4].tolist() == [100, 100]
+
+
+def test_second_stages_over_what_no_first_stage_left(cuda):
+    """A workspace or a list that is not this call's: results are of no use, but nothing beside the outputs is written."""
+    for name in ("select in two", "evict"):
+        use = Use(name, cuda)
+        s = use.fresh()
+        torch.cuda.synchronize()
+        if use.kind == "select":
+            for poison in (-1, 0x7F7F7F7F, 1):
+                space = use.plan.new_workspace()
+                space.fill_(poison)
+                wide = torch.full((3,) + s["out"].shape, -9, dtype=torch.int32, device=cuda)
+                use.plan(use.q, use.bounds, use.cache, use.batch, out=wide[1], stage=1, workspace=space)
+                torch.cuda.synchronize()
+                assert (wide[0] == -9).all() and (wide[2] == -9).all()
+        else:
+            from paella_amd import long_cache
+            places = use.old.shape[2]
+            for keep, poison in ((100, 2 ** 31 - 1), (places + 50, 2 ** 31 - 1), (places + 50, -5)):
+                plan = long_cache.Evict(use.cache, len(use.case.past), use.case.tables.shape[1], keep)
+                kept = torch.full((len(use.case.past), use.case.kv_heads, keep), poison, dtype=torch.int32, device=cuda)
+                wide = torch.full((3,) + use.old.shape, 0.5, device=cuda)
+                plan(s["cache"], wide[1], s["past"], use.batch.tables, past_out=s["past"], kept=kept, stage=1)
+                torch.cuda.synchronize()
+                assert (wide[0] == 0.5).all() and (wide[2] == 0.5).all()
+                same(s["k"], use.cache.k)
+                same(s["v"], use.cache.v)
