@@ -330,10 +330,10 @@ __device__ __forceinline__ void screen_pages(const SelectArgs& a, const Screened
     if (lane < n) error_of(lane, (unsigned)w.split * 4 + wave, worst);
 }
 
-// A page's worth in 64 bits, by a whole wave: 16 bytes of a row per lane, the bounds and four heads' queries requested together.
-template <typename T>
+// A page's worth in 64 bits, by a whole wave: 16 bytes of a row per lane, the bounds and G heads' queries requested together.
+template <typename T, int G>
 __device__ __forceinline__ unsigned long long exact_worth_of(const SelectArgs& a, int t, int seq, int h, unsigned e) {
-    constexpr int G = 4, V = 16 / T::bytes;
+    constexpr int V = 16 / T::bytes;
     const int lane = threadIdx.x & 63, heads = (int)a.per_kv.d, row = a.dim * T::bytes;
     const int at = min(lane * 16, row - 16);
     const char* const q = a.q + t * a.q_stride + (size_t)h * heads * row + at;
@@ -370,8 +370,9 @@ __device__ __forceinline__ unsigned long long exact_worth_of(const SelectArgs& a
     }
     return best;
 }
+template <int G>
 __device__ __forceinline__ unsigned long long exact_worth(const SelectArgs& a, int t, int seq, int h, unsigned e) {
-    return a.dtype == PAELLA_F32 ? exact_worth_of<F32>(a, t, seq, h, e) : a.dtype == PAELLA_BF16 ? exact_worth_of<Bf16>(a, t, seq, h, e) : exact_worth_of<F16>(a, t, seq, h, e);
+    return a.dtype == PAELLA_F32 ? exact_worth_of<F32, G>(a, t, seq, h, e) : a.dtype == PAELLA_BF16 ? exact_worth_of<Bf16, G>(a, t, seq, h, e) : exact_worth_of<F16, G>(a, t, seq, h, e);
 }
 
 __device__ __forceinline__ void put_int(int* p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -472,7 +473,7 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
             each_open([&](int, unsigned i, unsigned at) { s.list[at] = i; });
             __syncthreads();
             for (unsigned k = wave; k < n; k += WAVES) {
-                const unsigned long long worth = exact_worth(a, t, seq, h, uniform(s.list[k]));
+                const unsigned long long worth = exact_worth<WAVES == 16 ? 2 : 4>(a, t, seq, h, uniform(s.list[k]));  // (sixteen waves have 128 registers each)
                 if (lane == 0) s.worth[k] = worth;
             }
             __syncthreads();

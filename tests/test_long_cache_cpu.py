@@ -46,6 +46,15 @@ def test_header_and_table_and_library_agree(lib):
     assert declared == sorted(_abi_long.LONG_SYMBOLS) and all(hasattr(lib, n) for n in declared)
 
 
+def test_no_kernel_needs_scratch_memory(lib):
+    """Direct-dispatch queues have none to give: by what the library's code objects say of their kernels."""
+    built = open(lib._name, "rb").read()
+    said = re.findall(rb"\.name[\xa0-\xbf\xd9\xda]..?.?([\w$.]{8,200}?)\xbb\.private_segment_fixed_size(.)", built, flags=re.S)
+    kernels = {name.decode(): size for name, size in said if re.search(rb"page_(bounds|screen|pick|select|attention)_kernel|evict_\w+_kernel|key_(sums|weights)_kernel|stored_weights_kernel", name)}
+    assert len(kernels) == 6 + 9 + 9 + 5 + 9 + 4 + 1 + 18 + 9 + 1, sorted(kernels)
+    assert [name for name, size in kernels.items() if size != b"\0"] == []
+
+
 # ------------------------------------------------------------------ bounds
 
 def bounds(lib, c=None, b=None, at=BOUNDS):

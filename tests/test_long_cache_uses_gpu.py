@@ -299,3 +299,40 @@ def test_second_stages_over_what_no_first_stage_left(cuda):
                 assert (wide[0] == 0.5).all() and (wide[2] == 0.5).all()
                 same(s["k"], use.cache.k)
                 same(s["v"], use.cache.v)
+
+
+@pytest.mark.parametrize("pages", [100, 1500, 3000, 10000, 20000])
+def test_every_form_of_picking_on_direct_queues(cuda, pages):
+    from paella_amd import decode, long_cache, ops
+    c = Case(pages, BF16, 1, 64, 8, [8 * pages - 5, 100], 3)
+    cache, batch = c.to(cuda)
+    q, bounds = c.queries(2).to(cuda), bounds_like(c).to(cuda)
+    select = long_cache.PageSelect(2, cache, batch, 50)
+    weights = torch.rand((2, 1, pages), generator=c.gen).to(cuda)   # an eviction from as many tokens
+    tokens = decode.KVCache(*(torch.rand((2 * pages // 4, 1, 8, 8), generator=c.gen).to(cuda) for _ in range(2))) if pages % 8 == 0 else None
+    want = select(q, bounds, cache, batch)
+    with ops.DirectQueue() as queue:
+        out = torch.zeros_like(want)
+        torch.cuda.synchronize()
+        assert select.plan.stages == 2
+        for stage in range(2):
+            select(q, bounds, cache, batch, out=out, stage=stage, stream=queue.handle)
+            queue.wait()
+        same(out, want)
+        if tokens is not None:
+            evict = long_cache.Evict(tokens, 2, pages // 8, pages // 3, first=2, recent=3)
+            past = torch.tensor([pages, pages // 4], dtype=torch.int32, device=cuda)
+            tables = torch.randperm(2 * pages // 8, generator=c.gen).to(torch.int32).view(2, pages // 8).to(cuda)
+            made = []
+            for direct in (False, True):
+                k, v, w = tokens.k.clone(), tokens.v.clone(), weights.clone()
+                lengths, kept = torch.zeros_like(past), torch.zeros((2, 1, pages // 3), dtype=torch.int32, device=cuda)
+                torch.cuda.synchronize()
+                for stage in range(2):
+                    evict(decode.KVCache(k, v), w, past, tables, past_out=lengths, kept=kept, stage=stage, stream=queue.handle if direct else None)
+                    if direct:
+                        queue.wait()
+                torch.cuda.synchronize()
+                made.append((k, v, w, lengths, kept))
+            for got, expected in zip(*made):
+                same(got, expected)
