@@ -188,6 +188,7 @@ struct WeighArgs {
     Notifier* notifier;
 };
 
+constexpr int kOnce = 2;  // for stores: not to be kept in the caches (the scores of 32 sequences of up to 16384 tokens: 174.6 us without, 170.6 with)
 constexpr float kRise = 8.f;  // how far scores may be above the running maximum before it moves
 constexpr float kLowest = -3.4028234663852886e38f;  // the maximum of no scores: what is not seen, -inf, is below it
 
@@ -423,7 +424,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void key_sums_kernel(WeighArg
                 for (int u = 0; u < 16 * PIECES / 64; ++u) {
                     const int i = u * 64 + lane, row = i / PIECES, at = waiting + i % PIECES * 4 - behind;
                     if (row < rows && at >= 0 && at < places_all)
-                        __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u32x4*>(mine + i * 4), to_scores, (row * places_all + at) * 4, 0, kThrough);
+                        __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u32x4*>(mine + i * 4), to_scores, (row * places_all + at) * 4, 0, kThrough | kOnce);
                 }
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
