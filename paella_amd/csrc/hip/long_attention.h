@@ -114,7 +114,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void page_attention_kernel(Pa
     using Fm = Form<1, false>;
     __shared__ __attribute__((aligned(16))) char lds[attention_lds<T, D, Fm>()];
     __shared__ u32x2 list[kListed];
-    __shared__ int row_id[16], done[16];
+    __shared__ int row_id[16], done[16], ends[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int head_bytes = D * T::bytes;
     const Quotient by_head = divide(blockIdx.x, a.kv_heads), by_split = divide(by_head.q, p.splits), by_tile = divide(by_split.q, p.tiles);
@@ -140,6 +140,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void page_attention_kernel(Pa
         for (int first = split * p.per; first < end; first += kListed) {
             const int n = min(end - first, kListed);
             __syncthreads();
+            int last = 0;  // lane 0: behind the wave's last entry of which something is seen
             for (int i = threadIdx.x; i < n; i += 256) {
                 const int e = entries[first + i], o = e < 0 ? e : e - a.prefix_pages;
                 int page = 0, seen = 0;
@@ -152,9 +153,13 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void page_attention_kernel(Pa
                 }
                 if ((unsigned)page >= (unsigned)a.num_pages) seen = 0;
                 list[i] = u32x2{(unsigned)page, (unsigned)max(min(seen, a.page_size), 0)};
+                const unsigned long long who = __ballot(seen > 0);
+                if (who) last = i - lane + 64 - __clzll(who);
             }
+            if (lane == 0) ends[wave] = last;
             __syncthreads();
-            walk_list<T, D>(rows, s, list, n, a.scale_log2, __builtin_amdgcn_readfirstlane(wave), lane);
+            const int some = __builtin_amdgcn_readfirstlane(max(max(ends[0], ends[1]), max(ends[2], ends[3])));  // (lists of short sequences end in entries of no page)
+            walk_list<T, D>(rows, s, list, some, a.scale_log2, __builtin_amdgcn_readfirstlane(wave), lane);
         }
         leave<T, D, Fm>(a, rows, split, row_id, lds);
         if (a.counters) join_last<T, D, 16>(a, row_id, (unsigned)(((size_t)t * p.tiles.d + tile) * a.kv_heads.d + h) * 32, min(per_kv - first_row, 16), done);
