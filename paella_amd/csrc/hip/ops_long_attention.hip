@@ -92,10 +92,12 @@ int paella_page_attention_plan_make(const paella_kv_cache* c, const paella_kv_ba
     p->scale = scale > 0.f ? scale : 1.f / std::sqrt((float)c->head_dim);
     p->splits = 1;
     if (!plan_ok(p)) return PAELLA_ENOSUP;
-    const int64_t undivided = grid_of(p), keys = (int64_t)count * c->page_size;
-    // Lists are equally long: no more parts than the device holds at once, three workgroups to a compute unit, and of 256 keys at least.  (8 key heads of 128 in bf16: 512 lists of 4096 tokens in 1 / 2 / 3
-    // parts 178 / 187 / 199 us, 120 of 1600 in 6 / 7 18.4 / 20.7, 64 of 4096 in 12 / 16 26.0 / 27.9.)
-    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({768 / undivided, ceil_div(keys, 256), (int64_t)count, 64}));
+    const int64_t undivided = grid_of(p), keys = (int64_t)count * c->page_size, pages = std::min<int64_t>(count, ceil_div(b->prefix_len, c->page_size) + b->max_pages);
+    // Lists are equally long, and have no more pages than the sequence: no more parts than the device holds at once, three workgroups to a compute unit or, of heads of 256, one, and of 256 keys at least.
+    // (8 key heads of 128 in bf16: 512 lists of 4096 tokens in 1 / 2 / 3 parts 178 / 187 / 199 us, 120 of 1600 in 6 / 7 18.4 / 20.7, 64 of 4096 in 12 / 16 26.0 / 27.9; of 256: 64 of 4096 in 4 / 8 / 12
+    // 43 / 48 / 52, 192 in 1 / 4 135 / 147; 122 fp32 lists of 44 entries, of which sequences of 3 pages fill 3, in 1 / 6 7.2 / 15.2.)
+    const int64_t resident = c->head_dim > 128 ? 256 : 768;
+    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({resident / undivided, ceil_div(pages * c->page_size, 256), pages, 64}));
     if (!plan_ok(p)) return PAELLA_ENOSUP;
     p->stages = stages_of(p);
     p->workspace_bytes = workspace_of(p);

@@ -127,9 +127,10 @@ def test_what_plans_plan(lib):
     assert select_plan(lib, cache(pages=9000), batch(sequences=1, max_pages=5000))[1].stages == 2
     # lists that fill the device are not shared out; one of many pages is, and a wide one's parts are joined by a launch of their own
     assert attend_plan(lib, cache(heads=8, dim=128, size=64), batch(sequences=64), 32, 64)[1].workspace_bytes == 0
-    rc, p = attend_plan(lib, cache(heads=1, dim=128, size=64), batch(sequences=1), 4, 64)
+    rc, p = attend_plan(lib, cache(heads=1, dim=128, size=64), batch(sequences=1, max_pages=64), 4, 64)
     assert rc == 0 and (p.splits, p.stages) == (16, 1) and p.dims.grid == 16
-    rc, p = attend_plan(lib, cache(heads=1, dim=256, size=64), batch(sequences=1), 16, 64)
+    assert attend_plan(lib, cache(heads=1, dim=128, size=64), batch(sequences=1, max_pages=4), 4, 64)[1].splits == 1   # (there are no more pages than that)
+    rc, p = attend_plan(lib, cache(heads=1, dim=256, size=64), batch(sequences=1, max_pages=64), 16, 64)
     assert rc == 0 and p.stages == 2
     join = _abi.LaunchDims()
     assert lib.paella_page_attention_dims(ctypes.byref(p), 1, ctypes.byref(join)) == 0 and join.grid >= 1
@@ -150,9 +151,9 @@ def test_what_plans_plan(lib):
 class Call:
     """One planned operator's launch with every operand replaceable."""
 
-    def __init__(self, lib, name, make, operands, **kw):
-        self.lib, self.name, self.operands = lib, "paella_%s_launch" % name, operands
-        self.c, self.b = cache(), batch(prefix=40)
+    def __init__(self, lib, name, make, operands, width=4, **kw):
+        self.lib, self.name, self.operands, self.width = lib, "paella_%s_launch" % name, operands, width
+        self.c, self.b = cache(), batch(prefix=40, max_pages=width)
         rc, self.plan = make(lib, self.c, self.b, **kw)
         assert rc == 0
         self.fresh = lambda: make(lib, self.c, self.b, **kw)[1]
@@ -165,7 +166,7 @@ class Call:
 
 CALLS = {
     "select": lambda lib: Call(lib, "page_select", select_plan, dict(q=Q, bounds=BOUNDS, pages=PAGES)),
-    "attend": lambda lib: Call(lib, "page_attention", attend_plan, dict(q=Q, pages=PAGES, out=OUT), count=100),
+    "attend": lambda lib: Call(lib, "page_attention", attend_plan, dict(q=Q, pages=PAGES, out=OUT), width=100, count=100),
     "weigh": lambda lib: Call(lib, "key_weights", weigh_plan, dict(q=Q, weights=WEIGHTS)),
 }
 
@@ -183,8 +184,8 @@ def test_launches_refuse(lib, which):
     for kw in (dict(dtype=2), dict(heads=4), dict(size=8), dict(dim=128), dict(k=None), dict(v=V + 8)):
         assert call(c=cache(**kw)) == EINVAL, kw
     for kw in (dict(prefix=41), dict(prefix=0), dict(sequences=4), dict(max_pages=5), dict(past=None), dict(tables=None), dict(max_new=2, tokens=3)):
-        assert call(b=batch(**{"prefix": 40, **kw})) == EINVAL, kw
-    broken = batch(prefix=40)
+        assert call(b=batch(**{"prefix": 40, "max_pages": call.width, **kw})) == EINVAL, kw
+    broken = batch(prefix=40, max_pages=call.width)
     broken.prefix_table = None
     assert call(b=broken) == EINVAL
     fields = [("splits", 0), ("heads", 7), ("dtype", 5), ("head_dim", 96), ("page_size", 12), ("sequences", 0), ("max_pages", 0), ("tokens", 0)]
@@ -201,8 +202,8 @@ def test_outputs_over_what_is_read(lib, which):
     call = CALLS[which](lib)
     need = call.plan.workspace_bytes
     result = list(call.operands)[-1]
-    sizes = {"q": 3 * 512 * 2, "bounds": 10 * 2 * 2 * 64 * 2, "pages": 3 * 2 * call.plan.count * 4 if which != "weigh" else 0, "out": 3 * 512 * 2, "weights": 3 * 2 * 64 * 4}
-    inputs = [(call.operands[n], sizes[n]) for n in call.operands if n != result] + [(PAST, 12), (TABLES, 48), (PREFIX, 12)]
+    sizes = {"q": 3 * 512 * 2, "bounds": 10 * 2 * 2 * 64 * 2, "pages": 3 * 2 * call.plan.count * 4 if which != "weigh" else 0, "out": 3 * 512 * 2, "weights": 3 * 2 * 16 * call.width * 4}
+    inputs = [(call.operands[n], sizes[n]) for n in call.operands if n != result] + [(PAST, 12), (TABLES, 12 * call.width), (PREFIX, 12)]
     if which != "select":
         inputs += [(K, CACHE_BYTES), (V, CACHE_BYTES)]
     for at, size in inputs:
@@ -213,7 +214,7 @@ def test_outputs_over_what_is_read(lib, which):
     last = call.operands[result] + (sizes[result] - 1) // 16 * 16
     assert call(space=call.operands[result]) == EINVAL and call(space=last) == EINVAL and call(space=call.operands[result] - (need + 15) // 16 * 16 + 16) == EINVAL
     assert call(stride=1 << 20, space=Q + (4 << 20) + 256) == EINVAL                       # over the last of rows that lie far apart
-    ragged = batch(prefix=40, starts=STARTS)
+    ragged = batch(prefix=40, starts=STARTS, max_pages=call.width)
     assert call(b=ragged, space=STARTS) == EINVAL
 
 
