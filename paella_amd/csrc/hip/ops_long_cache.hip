@@ -787,6 +787,8 @@ SelectKernel screen_kernel(const paella_page_select_plan* p, bool whole) {
 }
 
 // A kernel of one of these forms, by how many there are to pick from at most: with their keys in registers, or, beyond what the registers of 16 waves hold, read again for every pass.
+// (Pages of 96 rows: 1001 by 4 / 16 waves 9.2 / 9.4 us, 4001 by 4 / 16 14.3 / 11.1; 1001 of 1536 rows 18.4 / 41.2; 15626 of 32 rows from registers / read again 19.4 / 42. Tokens of 8 to 192 heads: 4000 by
+// 4 / 16 waves 11.1 / 8.2, 4000 from registers / read again 8.3 / 10.9, 16384 15.4 / 20.7, 49285 in 64 registers a thread, more than there are, / read again 90 / 46.)
 template <typename Kernel>
 struct PickForm {
     Kernel kernel;
