@@ -427,7 +427,7 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
         any_unknown = unknown > 0;
         out = 0;
         if (range.some >= want) {
-            const float border = key_number(range.some == want ? range.least : find_bound<WAVES, KEYS, unsigned>(span, range, want, s.pick, [&](int u, unsigned i) { return known(get(u, i)); }).bound);
+            const float border = key_number(range.some == want ? range.least : find_bound<WAVES, KEYS, unsigned>(span, range, want, s.pick, get).bound);
             const float off = 2.f * (error * (float)(2 * a.dim + 8) * 0x1p-24f + 0x1p-110f);  // (products below the least number of 32 bits are lost, too)
             out = number_key(border - off, 1u);
             if (!unknown) in = number_key(border + off, 1u);  // (a page that nothing is known of may be worth more)
@@ -448,14 +448,15 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
     }
     __syncthreads();
     const unsigned open_ahead = ahead_of(s.open, wave, &open);
-    inside = uniform(waves_all(s.inside, Sum()));
+    const unsigned inside_ahead = ahead_of(s.inside, wave, &inside);
     auto take = [&](unsigned place, unsigned i) {
         if (place < (unsigned)a.count) put_int(to + place, (int)i);  // (more only if entries are another call's)
     };
     auto none = [](auto) { return false; };
     unsigned taken;
     if (inside + open <= (unsigned)a.count) {
-        taken = emit(span, s.pick, get, [&](unsigned k) { return is_in(k) || is_open(k); }, none, 0u, take);
+        emit_from(span, inside_ahead + open_ahead, get, [&](unsigned k) { return is_in(k) || is_open(k); }, take);
+        taken = inside + open;
     } else {
         // The open pages, in order, a list at a time, whose worths the waves share out.
         for (unsigned first = 0; first < open; first += kOpen) {
@@ -834,11 +835,12 @@ size_t select_errors(const paella_page_select_plan* p) { return up256((size_t)p-
 size_t select_entries(const paella_page_select_plan* p) { return up256((size_t)p->tokens * p->kv_heads * select_pitch(p) * 4); }
 size_t select_workspace(const paella_page_select_plan* p) { return select_counters(p) + select_errors(p) + 3 * select_entries(p); }  // (worths of 64 bits: twice the entries)
 
-// Bytes of a row that a workgroup moves: 128, which memory likes best, where that still makes a workgroup for each compute unit, else 64, or 32 where even those leave half of the device idle.  (bf16
-// heads of 128, 4096 tokens kept of 8 heads: 24 sequences by 128 / 64 bytes 193 / 247 us, 8 91 / 94, 4 57 / 48; one by 64 / 32 40 / 26.)
+// Bytes of a row that a workgroup moves: 128, which memory likes best, where that still makes a workgroup for each compute unit, else 64, or 32 where even those leave half of the device idle, or 16 where
+// three quarters.  (bf16 heads of 128, 4096 tokens kept of 8 heads: 24 sequences by 128 / 64 bytes 193 / 247 us, 8 91 / 94, 4 57 / 48; one by 64 / 32 / 16 40 / 26 / 44; 20000 tokens of 2 heads by 32 / 16
+// 111 / 85.)
 int evict_slice_log2(int sequences, const paella_kv_cache* c) {
     const int64_t heads = (int64_t)sequences * c->kv_heads, row = (int64_t)c->head_dim * element_bytes(c->dtype);
-    return 2 * heads * ceil_div(row, 128) >= 256 ? 7 : 2 * heads * ceil_div(row, 64) >= 128 ? 6 : 5;
+    return 2 * heads * ceil_div(row, 128) >= 256 ? 7 : 2 * heads * ceil_div(row, 64) >= 128 ? 6 : 2 * heads * ceil_div(row, 32) >= 64 ? 5 : 4;
 }
 int64_t evict_slices(int sequences, const paella_kv_cache* c) {
     return 2 * ceil_div((int64_t)c->head_dim * element_bytes(c->dtype), 1 << evict_slice_log2(sequences, c)) + 1;

@@ -144,6 +144,8 @@ struct Range {
         most = (Key)uniform(waves_all(s.high, Most()));
         some = uniform(waves_all(s.count[0], Sum()));
     }
+    // Of joined ranges: whether k is among the keys, or beyond them all.
+    __device__ __forceinline__ bool holds(Key k) const { return k - least <= most - least; }
 };
 
 // What is taken: keys above `bound`, and the first `left` of those equal to it (all of them where left is ~0).
@@ -153,7 +155,7 @@ struct Bound {
     unsigned left;
 };
 
-// Of the keys get(u, i) (0 is none), `range` of which is known: the `want` largest.  Digit by digit from the highest one in which the keys differ, by a histogram of the
+// Of the keys get(u, i) within `range`, which is theirs (others may lie below and above it): the `want` largest.  Digit by digit from the highest one in which the keys differ, by a histogram of the
 // keys that agree with the bound so far, until they are so few that each is ranked against all others.  Called by all threads.
 template <int WAVES, int KEYS, typename Key, typename Get>
 __device__ __forceinline__ Bound<Key> find_bound(const Span<WAVES, KEYS>& span, const Range<Key>& range, unsigned want, PickSpace<WAVES>& s, Get get) {
@@ -170,7 +172,7 @@ __device__ __forceinline__ Bound<Key> find_bound(const Span<WAVES, KEYS>& span, 
         for (unsigned b = threadIdx.x; b < 1u << kDigit; b += WAVES * 64) s.bins[b] = 0;
         __syncthreads();
         span.visit(get, [&](int, unsigned, Key k) {
-            if (k && (k & known) == bound) atomicAdd(&s.bins[(unsigned)(k >> shift) & ((1u << kDigit) - 1)], 1u);
+            if (range.holds(k) && (k & known) == bound) atomicAdd(&s.bins[(unsigned)(k >> shift) & ((1u << kDigit) - 1)], 1u);
         });
         __syncthreads();
         if (threadIdx.x < 64) {  // some digits a lane, the highest first
@@ -215,7 +217,7 @@ __device__ __forceinline__ Bound<Key> find_bound(const Span<WAVES, KEYS>& span, 
     if (threadIdx.x == 0) s.found = 0;
     __syncthreads();
     span.visit(get, [&](int, unsigned, Key k) {
-        if (k && (k & known) == bound) s.list[atomicAdd(&s.found, 1u)] = k;
+        if (range.holds(k) && (k & known) == bound) s.list[atomicAdd(&s.found, 1u)] = k;
     });
     __syncthreads();
     if (threadIdx.x < size) {
@@ -255,6 +257,20 @@ __device__ __forceinline__ unsigned ahead_of(const unsigned (&of)[WAVES], int wa
     return uniform(ahead);
 }
 
+// take(place, i) for the places whose value is mine(value), in order, the wave's from `place` on.
+template <int WAVES, int KEYS, typename Get, typename Mine, typename Take>
+__device__ __forceinline__ void emit_from(const Span<WAVES, KEYS>& span, unsigned place, Get get, Mine mine, Take take) {
+    const unsigned long long before = (1ull << (threadIdx.x & 63)) - 1;
+    span.visit(get, [&](int, unsigned i, auto k) {
+        const bool is = mine(k);
+        const unsigned long long who = __ballot(is);
+        if (who) {
+            if (is) take(place + (unsigned)__popcll(who & before), i);
+            place += (unsigned)__popcll(who);
+        }
+    });
+}
+
 // take(place, i) for every place whose value above(value), and for the first `left` of those whose value is tied(value), in order; returns how many.
 template <int WAVES, int KEYS, typename Get, typename Above, typename Tied, typename Take>
 __device__ __forceinline__ unsigned emit(const Span<WAVES, KEYS>& span, PickSpace<WAVES>& s, Get get, Above above, Tied tied, unsigned left, Take take) {
@@ -276,19 +292,15 @@ __device__ __forceinline__ unsigned emit(const Span<WAVES, KEYS>& span, PickSpac
     place += min(ties, left);
     all += min(ties_all, left);
     const unsigned long long before = (1ull << lane) - 1;
-    span.visit(get, [&](int, unsigned i, auto k) {
+    emit_from(span, place, get, [&](auto k) {
         bool mine = above(k);
         if (left) {
             const unsigned long long who = __ballot(tied(k));
             mine |= tied(k) && ties + (unsigned)__popcll(who & before) < left;
             ties += (unsigned)__popcll(who);
         }
-        const unsigned long long who = __ballot(mine);
-        if (who) {
-            if (mine) take(place + (unsigned)__popcll(who & before), i);
-            place += (unsigned)__popcll(who);
-        }
-    });
+        return mine;
+    }, take);
     return all;
 }
 
