@@ -16,14 +16,15 @@ namespace {
 using namespace paella;
 
 // ------------------------------------------------------------------------------------------ bounds of a page's keys
-// A wave per page and key head: 16 bytes of a key per lane, as many keys side by side as fit the wave, all of the page's requested eight at a time.  Bound by memory:
+// A wave per page and key head, or some of its key heads: 16 bytes of a key per lane, as many keys side by side as fit the wave, four or eight requests at a time.  Bound by memory:
 // each key of the pages is read once.
 struct BoundsArgs {
     const char* k_cache;
     char* bounds;
     const int *starts, *past, *tables;
     int sequences, max_new, tokens, max_pages, num_pages, page_size, row_bytes, pieces, group_log2;  // pieces: 16 bytes of a key each; 2^group_log2 lanes side by side for a key
-    Divisor kv_heads, touched;  // touched: most pages that a sequence's new tokens lie in
+    int kv_heads;
+    Divisor groups, touched;  // groups: of a page's key heads; touched: most pages that a sequence's new tokens lie in
     unsigned items;
     uint32_t job_id;
     Notifier* notifier;
@@ -90,15 +91,15 @@ __device__ __forceinline__ void lanes_apart(float (&low)[V], float (&high)[V], i
     if (log2 <= 5) swapped([](unsigned v) { return __builtin_amdgcn_permlane32_swap(v, v, false, false); });  // both halves
 }
 
-// AHEAD: requests of a lane that go out together.
-template <typename T, int AHEAD>
-__global__ __launch_bounds__(256, AHEAD == 4 ? 8 : 1) void page_bounds_kernel(BoundsArgs a) {
+// AHEAD: requests of a lane for a head that go out together; HEADS: key heads of a wave, which lie side by side in the page.
+template <typename T, int AHEAD, int HEADS>
+__global__ __launch_bounds__(256, AHEAD * HEADS == 4 && HEADS < 4 ? 8 : 1) void page_bounds_kernel(BoundsArgs a) {
     hook_entry(a.notifier, a.job_id);
     constexpr int V = 16 / T::bytes;
     const int lane = threadIdx.x & 63;
     const unsigned item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if (item < a.items) {
-        const Quotient by_head = divide(item, a.kv_heads), by_page = divide(by_head.q, a.touched);
+        const Quotient by_head = divide(item, a.groups), by_page = divide(by_head.q, a.touched);
         const int seq = (int)by_page.q;
         const NewTokens its = new_tokens(a.starts, a.past, seq, a.max_new, a.tokens);
         const unsigned page = (unsigned)its.past / (unsigned)a.page_size + by_page.r;  // along the sequence
@@ -107,30 +108,42 @@ __global__ __launch_bounds__(256, AHEAD == 4 ? 8 : 1) void page_bounds_kernel(Bo
         if (its.count > 0 && first < end && page < (unsigned)a.max_pages) physical = __builtin_amdgcn_readfirstlane(a.tables[(size_t)seq * a.max_pages + page]);
         if ((unsigned)physical < (unsigned)a.num_pages) {
             const int held = (int)min((int64_t)a.page_size, end - first);
-            const size_t head_at = (size_t)physical * a.kv_heads.d + by_head.r;
+            const int heads = min(a.kv_heads - (int)by_head.r * HEADS, HEADS);
+            const size_t head_at = (size_t)physical * a.kv_heads + by_head.r * HEADS;
             const char* const keys = a.k_cache + head_at * a.page_size * a.row_bytes;
             const __amdgpu_buffer_rsrc_t to = descriptor(a.bounds + head_at * 2 * a.row_bytes);
+            const size_t head_bytes = (size_t)a.page_size * a.row_bytes;
             const int group = 1 << a.group_log2, each = 64 >> a.group_log2;
             for (int piece = lane & (group - 1); piece < (a.pieces + group - 1) / group * group; piece += group) {  // (whole waves: lanes of all groups meet below)
                 const bool in = piece < a.pieces;
-                float low[V], high[V];
+                float low[HEADS][V], high[HEADS][V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    low[e] = INFINITY;
-                    high[e] = -INFINITY;
-                }
+                for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        low[h][e] = INFINITY;
+                        high[h][e] = -INFINITY;
+                    }
                 for (int key = lane >> a.group_log2; key < held; key += AHEAD * each) {
-                    u32x4 w[AHEAD];
+                    u32x4 w[HEADS][AHEAD];
 #pragma unroll
-                    for (int u = 0; u < AHEAD; ++u)  // behind the last key: the last one again
-                        w[u] = *reinterpret_cast<const u32x4*>(keys + (size_t)min(key + u * each, held - 1) * a.row_bytes + (in ? piece : 0) * 16);
+                    for (int h = 0; h < HEADS; ++h)
 #pragma unroll
-                    for (int u = 0; u < AHEAD; ++u) widen<T>(w[u], low, high);
+                        for (int u = 0; u < AHEAD; ++u)  // behind the last key, and the last head: the last one again
+                            w[h][u] = *reinterpret_cast<const u32x4*>(keys + min(h, heads - 1) * head_bytes + (size_t)min(key + u * each, held - 1) * a.row_bytes + (in ? piece : 0) * 16);
+#pragma unroll
+                    for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+                        for (int u = 0; u < AHEAD; ++u) widen<T>(w[h][u], low[h], high[h]);
                 }
-                lanes_apart<V>(low, high, a.group_log2);
-                if (lane < group && in) {
-                    __builtin_amdgcn_raw_buffer_store_b128(packed<T>(low), to, piece * 16, 0, kThrough);
-                    __builtin_amdgcn_raw_buffer_store_b128(packed<T>(high), to, a.row_bytes + piece * 16, 0, kThrough);
+#pragma unroll
+                for (int h = 0; h < HEADS; ++h) {
+                    if (h >= heads) break;
+                    lanes_apart<V>(low[h], high[h], a.group_log2);
+                    if (lane < group && in) {
+                        __builtin_amdgcn_raw_buffer_store_b128(packed<T>(low[h]), to, 2 * h * a.row_bytes + piece * 16, 0, kThrough);
+                        __builtin_amdgcn_raw_buffer_store_b128(packed<T>(high[h]), to, (2 * h + 1) * a.row_bytes + piece * 16, 0, kThrough);
+                    }
                 }
             }
         }
@@ -745,9 +758,9 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
 // ------------------------------------------------------------------------------------------ host
 
 using BoundsKernel = void (*)(BoundsArgs);
-template <int AHEAD>
+template <int AHEAD, int HEADS>
 BoundsKernel bounds_kernel_of(int dtype) {
-    return dtype == PAELLA_F32 ? page_bounds_kernel<F32, AHEAD> : dtype == PAELLA_BF16 ? page_bounds_kernel<Bf16, AHEAD> : page_bounds_kernel<F16, AHEAD>;
+    return dtype == PAELLA_F32 ? page_bounds_kernel<F32, AHEAD, HEADS> : dtype == PAELLA_BF16 ? page_bounds_kernel<Bf16, AHEAD, HEADS> : page_bounds_kernel<F16, AHEAD, HEADS>;
 }
 // 2^n lanes side by side have a key's 16-byte pieces.
 int bounds_group_log2(const paella_kv_cache* c) {
@@ -755,18 +768,26 @@ int bounds_group_log2(const paella_kv_cache* c) {
     while ((16 << n) < c->head_dim * element_bytes(c->dtype) && n < 6) ++n;
     return n;
 }
-// A page's keys in one go of four requests a lane where they fit that: with half the registers twice as many waves are there.
-BoundsKernel bounds_kernel(const paella_kv_cache* c) { return c->page_size <= 4 * (64 >> bounds_group_log2(c)) ? bounds_kernel_of<4>(c->dtype) : bounds_kernel_of<8>(c->dtype); }
+// Requests that a lane needs for a head's keys: four together where they fit that (with half the registers of eight twice as many waves are there), and where two or one do, two or four heads of a page by one
+// wave (fp16 heads of 64: 32 MB in pages of 16 tokens of 4 heads by one / two heads a wave
+// 15.0 / 12.9 us, 42 MB in pages of 8 of 8 heads by one / four 33 / 26).
+int bounds_requests(const paella_kv_cache* c) { return (int)ceil_div(c->page_size, 64 >> bounds_group_log2(c)); }
 
 struct BoundsGrid {
-    int64_t touched, items;
+    int64_t touched, groups, items;
     unsigned grid() const { return (unsigned)((items + 3) / 4); }
 };
 BoundsGrid bounds_grid(const paella_kv_cache* c, const paella_kv_batch* b) {
+    const int requests = bounds_requests(c);
     BoundsGrid g;
     g.touched = std::min<int64_t>(ceil_div(std::min(b->max_new, b->tokens) - 1, c->page_size) + 1, b->max_pages);
-    g.items = (int64_t)b->sequences * g.touched * c->kv_heads;
+    g.groups = ceil_div(c->kv_heads, requests > 2 ? 1 : 4 / requests);
+    g.items = (int64_t)b->sequences * g.touched * g.groups;
     return g;
+}
+BoundsKernel bounds_kernel(const paella_kv_cache* c) {
+    const int requests = bounds_requests(c);
+    return requests == 1 ? bounds_kernel_of<1, 4>(c->dtype) : requests == 2 ? bounds_kernel_of<2, 2>(c->dtype) : requests <= 4 ? bounds_kernel_of<4, 1>(c->dtype) : bounds_kernel_of<8, 1>(c->dtype);
 }
 
 int bounds_check(const paella_kv_cache* c, const paella_kv_batch* b) {
@@ -899,7 +920,8 @@ extern "C" {
 int paella_page_bounds_dims(const paella_kv_cache* c, const paella_kv_batch* b, paella_launch_dims* dims) {
     if (int rc = bounds_check(c, b)) return rc;
     if (!dims) return PAELLA_EINVAL;
-    set_launch_dims(dims, bounds_grid(c, b).grid(), 256, 0, 64);
+    const BoundsGrid g = bounds_grid(c, b);
+    set_launch_dims(dims, g.grid(), 256, 0, 64);
     loaded_dims((const void*)bounds_kernel(c), dims);
     return 0;
 }
@@ -915,7 +937,7 @@ int paella_page_bounds_launch(const paella_kv_cache* c, const paella_kv_batch* b
     a.starts = b->starts; a.past = b->past; a.tables = b->tables;
     a.sequences = b->sequences; a.max_new = b->max_new; a.tokens = b->tokens; a.max_pages = b->max_pages; a.num_pages = c->num_pages; a.page_size = c->page_size;
     a.row_bytes = c->head_dim * element_bytes(c->dtype); a.pieces = a.row_bytes / 16; a.group_log2 = bounds_group_log2(c);
-    a.kv_heads = divisor((unsigned)c->kv_heads); a.touched = divisor((unsigned)g.touched); a.items = (unsigned)g.items;
+    a.kv_heads = c->kv_heads; a.groups = divisor((unsigned)g.groups); a.touched = divisor((unsigned)g.touched); a.items = (unsigned)g.items;
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
     launch(bounds_kernel(c), dim3(g.grid()), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();

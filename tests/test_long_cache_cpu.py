@@ -51,7 +51,7 @@ def test_no_kernel_needs_scratch_memory(lib):
     built = open(lib._name, "rb").read()
     said = re.findall(rb"\.name[\xa0-\xbf\xd9\xda]..?.?([\w$.]{8,200}?)\xbb\.private_segment_fixed_size(.)", built, flags=re.S)
     kernels = {name.decode(): size for name, size in said if re.search(rb"page_(bounds|screen|pick|select|attention)_kernel|evict_\w+_kernel|key_(sums|weights)_kernel|stored_weights_kernel", name)}
-    assert len(kernels) == 6 + 9 + 9 + 5 + 9 + 4 + 1 + 18 + 9 + 1, sorted(kernels)
+    assert len(kernels) == 12 + 9 + 9 + 5 + 9 + 4 + 1 + 18 + 9 + 1, sorted(kernels)
     assert [name for name, size in kernels.items() if size != b"\0"] == []
 
 
@@ -71,7 +71,8 @@ def test_bounds_refuse(lib):
         assert bounds(lib, at=at) == EINVAL, at
     assert bounds(lib, b=batch(starts=STARTS, tokens=3), at=STARTS) == EINVAL
     d = _abi.LaunchDims()
-    assert lib.paella_page_bounds_dims(*refs(cache(), batch(sequences=5)), ctypes.byref(d)) == 0 and (d.grid, d.block) == (3, 256)   # a wave per page and key head
+    assert lib.paella_page_bounds_dims(*refs(cache(), batch(sequences=5)), ctypes.byref(d)) == 0 and (d.grid, d.block) == (2, 256)   # a wave for both key heads of a small page
+    assert lib.paella_page_bounds_dims(*refs(cache(size=64), batch(sequences=5)), ctypes.byref(d)) == 0 and (d.grid, d.block) == (3, 256)   # a wave per page and key head
     assert lib.paella_page_bounds_dims(*refs(cache(), batch()), None) == EINVAL and lib.paella_page_bounds_dims(None, ctypes.byref(batch()), ctypes.byref(d)) == EINVAL
 
 

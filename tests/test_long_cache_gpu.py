@@ -66,6 +66,9 @@ BOUNDS = [
     (F32, 2, 512, 8, [1, 6], 9, None),                         # a row of more pieces than a wave has lanes
     (F16, 2, 8, 8, [0, 70], 3, None),                          # one lane a key
     (F32, 1, 96, 128, [100, 0], 300, [0, 1, 301]),
+    (F16, 7, 64, 8, [0, 50, 7], 20, None),                     # four heads a wave, and a group of three
+    (BF16, 5, 64, 16, [3, 0, 9], 30, [0, 30, 30, 47]),         # two, and one that is left over
+    (F32, 1, 32, 8, [5, 20], 3, None),                         # no other head
 ]
 
 
