@@ -10,7 +10,7 @@
  * holds such a token.
  *
  * Device data that the host cannot check is checked where it is used, as there: pages outside the cache take no part, tokens beyond the
- * table are none, a negative length counts as 0, no access leaves the tensors whatever the numbers are.  What `starts` has to hold to is said there.
+ * table are none, a negative length counts as 0, no access leaves the tensors whatever the numbers are; tables of 2^30 tokens and more are refused (PAELLA_ENOSUP).  What `starts` has to hold to is said there.
  */
 #ifndef PAELLA_LONG_CACHE_H
 #define PAELLA_LONG_CACHE_H

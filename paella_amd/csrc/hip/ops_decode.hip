@@ -75,7 +75,8 @@ __device__ __forceinline__ u32x4 load_unaligned(const char* p) {
     return v;
 }
 
-template <typename T>
+// AT: at given positions (a kernel of its own: asking for them or not in the one cost every call 1%).
+template <typename T, bool AT>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     hook_entry(a.notifier, a.job_id);
     // (cos, sin) of each pair's angle and the norms' weights, the same for every head.  In LDS rather than in registers: with them there five
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
         };
         fetch(0);
         // Trips to memory that do not wait for one another go out together: heads, length, weights and frequencies, then the page.
-        const int past = a.past[seq], position = a.positions ? a.positions[seq] : 0;
+        const int past = a.past[seq], position = AT ? a.positions[seq] : 0;
         float wq[2], wk[2], freq = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
         // The angle in revolutions, reduced to half a turn in 64 bits: in 32 bits a position of 100000 would be off by 0.006 radians.  Each pair once per
         // token, by one lane.
         if ((int)threadIdx.x < a.rotary / 2) {
-            const double turns = (a.positions ? (double)position + (double)j : (double)a.prefix_len + (double)own) * (double)freq * 0.15915494309189533577;
+            const double turns = (AT ? (double)position + (double)j : (double)a.prefix_len + (double)own) * (double)freq * 0.15915494309189533577;
             float s, c;
             sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
             turn[threadIdx.x] = f32x2{c, s};
@@ -726,8 +727,9 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
 }
 
 using AppendKernel = void (*)(AppendArgs);
+template <bool AT>
 AppendKernel append_kernel(int dtype) {
-    return dtype == PAELLA_F32 ? kv_append_kernel<F32> : dtype == PAELLA_BF16 ? kv_append_kernel<Bf16> : kv_append_kernel<F16>;
+    return dtype == PAELLA_F32 ? kv_append_kernel<F32, AT> : dtype == PAELLA_BF16 ? kv_append_kernel<Bf16, AT> : kv_append_kernel<F16, AT>;
 }
 
 using SelectKernel = void (*)(SelectArgs);
@@ -773,7 +775,7 @@ int paella_kv_append_dims(const paella_kv_append_desc* desc, const paella_kv_cac
     if (int rc = append_check(desc, cache, batch)) return rc;
     if (!dims) return PAELLA_EINVAL;
     set_launch_dims(dims, (unsigned)batch->tokens, 256, 0, 64);
-    loaded_dims((const void*)append_kernel(cache->dtype), dims);
+    loaded_dims((const void*)append_kernel<false>(cache->dtype), dims);
     return 0;
 }
 
@@ -815,7 +817,7 @@ int paella_kv_append_at_launch(const paella_kv_append_desc* d, const paella_kv_c
     a.group_log2 = 0;
     while ((8 << a.group_log2) < c->head_dim) ++a.group_log2;
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
-    launch(append_kernel(c->dtype), dim3(b->tokens), dim3(256), 0, (hipStream_t)stream, a);
+    launch(positions ? append_kernel<true>(c->dtype) : append_kernel<false>(c->dtype), dim3(b->tokens), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 

@@ -172,8 +172,8 @@ int paella_key_weights_plan_make(const paella_kv_cache* c, const paella_kv_batch
     if (!plan_ok(p)) return PAELLA_ENOSUP;
     const int64_t own = (int64_t)c->page_size * b->max_pages, keys = own + b->prefix_len;
     const int64_t sums = grid_of(p, 0), weights = grid_of(p, 1);
-    // Few rows: memory bounds it, and parts are as many as even out the sequences' lengths (32 sequences of 8192 to 16384 tokens of 8 heads of 128 in bf16 in 4 / 8 / 16 / 32 parts 204 / 187 / 180 / 173 us).
-    // Many rows: as many workgroups as the device holds at once, two to a compute unit in the first stage (4 sequences, 128 rows over 17000 keys of 8 heads, in 12 / 16 / 24 parts 41 / 34 / 52 us) and three
+    // Few rows: memory bounds it, and parts are as many as even out the sequences' lengths (32 sequences of 8192 to 16384 tokens of 8 heads of 128 in bf16 in 16 / 32 / 48 / 64 parts 181 / 174 / 177 / 182 us).
+    // Many rows: as many workgroups as the device holds at once, two to a compute unit in the first stage (4 sequences, 128 rows over 17000 keys of 8 heads, in 12 / 16 / 24 parts 35 / 29 / 45 us) and three
     // in the second.
     const bool few = few_rows(p);
     p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(few ? 8192 : 512, sums), ceil_div(keys, 256), 64}));

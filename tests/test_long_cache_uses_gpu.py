@@ -336,3 +336,23 @@ def test_every_form_of_picking_on_direct_queues(cuda, pages):
                 made.append((k, v, w, lengths, kept))
             for got, expected in zip(*made):
                 same(got, expected)
+
+
+def test_append_at_positions_on_direct_queues(cuda):
+    from paella_amd import decode, ops
+    c = Case(12, BF16, 2, 64, 16, [5, 30, 0], 3)
+    k, v = (randn(c.gen, c.tokens, 2, 64, dtype=BF16).to(cuda) for _ in range(2))
+    q, freq = c.queries(4).to(cuda), torch.rand(32, generator=c.gen).to(cuda)
+    positions = torch.tensor([77, 3, 1000], dtype=torch.int32, device=cuda)
+    made = []
+    with ops.DirectQueue() as queue:
+        for direct in (False, True):
+            cache, batch = c.to(cuda)
+            out = torch.zeros_like(q)
+            torch.cuda.synchronize()
+            decode.kv_append(cache, batch, k, v, q=q, inv_freq=freq, positions=positions, out=out, stream=queue.handle if direct else None)
+            queue.wait()
+            torch.cuda.synchronize()
+            made.append((out, cache.k, cache.v))
+    for got, want in zip(*made):
+        same(got, want)
