@@ -75,8 +75,8 @@ typedef struct paella_page_attention_plan {
 } paella_page_attention_plan;
 
 /* out[t][h] = sum_i softmax_i(scale * q[t][h] . k_i) v_i over the tokens that row t sees of the pages in pages[t][h / (heads / kv_heads)] (int32 [tokens][kv_heads][count], as
- * paella_page_select writes it; entries outside the sequence's pages, and pages outside the cache, are passed over wherever they stand, and a page listed twice counts twice).  Precision as for paella_prefix_attention;
- * a row without any token gives zeros, and what lies in places that a row does not see may be anything.  head_dim 64, 128 or 256. */
+ * paella_page_select writes it; entries outside the sequence's pages, and pages outside the cache, are passed over wherever they stand, and a page listed twice counts twice).  Scores, maxima, sums and outputs are kept in 32 bits;
+ * of 16-bit types a weight is taken as the sum of two numbers of the type, divided by the sum of those, so that a result is off by little more than its own rounding; a row without any token gives zeros, and what lies in places that a row does not see may be anything.  head_dim 64, 128 or 256. */
 int paella_page_attention_plan_make(const paella_kv_cache* cache, const paella_kv_batch* batch, int heads, int count, float scale, paella_page_attention_plan* plan);
 int paella_page_attention_dims(const paella_page_attention_plan* plan, int stage, paella_launch_dims* dims);
 int paella_page_attention_launch(const paella_page_attention_plan* plan, const paella_kv_cache* cache, const paella_kv_batch* batch, const void* q, int64_t q_stride,

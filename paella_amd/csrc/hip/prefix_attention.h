@@ -169,8 +169,9 @@ struct AttentionRows {
                     if (absent || first + t * 4 + e >= limit[r]) x[r][t][e] = -INFINITY;
     }
 
-    // Scores to probabilities, as operands of the second product.
-    __device__ __forceinline__ void weigh(const f32x4 (&x)[R][NT], float scale, unsigned (&p)[R][4]) {
+    // Scores to probabilities, as operands of the second product: each the sum of PARTS numbers of its type.
+    template <int PARTS>
+    __device__ __forceinline__ void weigh(const f32x4 (&x)[R][NT], float scale, unsigned (&p)[PARTS][R][4]) {
         // Until a score is above the running maximum by 2^SLACK, neither the lanes' exchange nor the rescaling is needed.
         bool grown = false;
         float top[R];
@@ -207,38 +208,52 @@ struct AttentionRows {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[t * 4 + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r][t][e], scale, -base));
             if constexpr (F) {
+                static_assert(PARTS == 1);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    p[r][e] = as_word(y[e]);
+                    p[0][r][e] = as_word(y[e]);
                     total[r][0] += y[e];
                 }
             } else {
                 // Probabilities to the products' type, since both of a product's operands have one: half a step of relative error each (a weight that BELOW has not kept from
-                // fp16's subnormals: half of their step), as much as the values they weigh have.
-#pragma unroll
-                for (int e = 0; e < 4; ++e) p[r][e] = pack2<T>(y[2 * e], y[2 * e + 1]);
+                // fp16's subnormals: half of their step), as much as the values they weigh have.  A second part has what the first leaves, and leaves half a step of half a step.
                 constexpr unsigned one = __is_same(T, Bf16) ? 0x3F803F80u : 0x3C003C00u;
-                total[r] = Mfma<T>::go(u32x4{one, one, one, one}, u32x4{p[r][0], p[r][1], p[r][2], p[r][3]}, total[r]);  // every row of it the same sum
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        p[part][r][e] = pack2<T>(y[2 * e], y[2 * e + 1]);
+                        if (part + 1 < PARTS) {
+                            const f32x2 had = unpack2<T>(p[part][r][e]);
+                            y[2 * e] -= had.x;
+                            y[2 * e + 1] -= had.y;
+                        }
+                    }
+                    total[r] = Mfma<T>::go(u32x4{one, one, one, one}, u32x4{p[part][r][0], p[part][r][1], p[part][r][2], p[part][r][3]}, total[r]);  // every row of it the same sum
+                }
             }
         }
     }
 
     // out += V^T p; v: the lane group's keys, PER dimensions of each in every group of 16 PER
-    __device__ __forceinline__ void add_values(const unsigned (&v)[TPL][GRP * VW], const unsigned (&p)[R][4]) {
+    template <int PARTS>
+    __device__ __forceinline__ void add_values(const unsigned (&v)[TPL][GRP * VW], const unsigned (&p)[PARTS][R][4]) {
 #pragma unroll
         for (int d = 0; d < GRP * PER; ++d) {
             if constexpr (F) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
-                    for (int r = 0; r < R; ++r) acc[r][d] = mfma_f32(as_float(v[e][d]), as_float(p[r][e]), acc[r][d]);
+                    for (int r = 0; r < R; ++r) acc[r][d] = mfma_f32(as_float(v[e][d]), as_float(p[0][r][e]), acc[r][d]);
             } else {
                 u32x4 a;
                 const int w = d / 2;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) a[e] = __builtin_amdgcn_perm(v[2 * e + 1][w], v[2 * e][w], d & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                for (int r = 0; r < R; ++r) acc[r][d] = Mfma<T>::go(a, u32x4{p[r][0], p[r][1], p[r][2], p[r][3]}, acc[r][d]);
+                for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) acc[r][d] = Mfma<T>::go(a, u32x4{p[part][r][0], p[part][r][1], p[part][r][2], p[part][r][3]}, acc[r][d]);
             }
         }
     }
@@ -360,7 +375,7 @@ struct NarrowWalk {
                     for (int w = 0; w < Rows::GRP * Rows::VW; ++w) v[u][w] = 0;
                 }
         }
-        unsigned p[1][4];
+        unsigned p[1][1][4];
         rows.weigh(x, scale, p);
         rows.add_values(v, p);
         next(false);
@@ -562,10 +577,10 @@ struct WideWalk {
             }
             const bool gone = gone_blocks >> (group * TPL / 8) & 1;
             if (first + STEP > least || gone_blocks) Rows::mask(x, first + group * TPL, gone, limit);
-            unsigned p[R][4];
+            unsigned p[1][R][4];
             rows.weigh(x, scale, p);
             if constexpr (F) rows.add_values(w, p);
-            else rows.add_straight(straight, p);
+            else rows.add_straight(straight, p[0]);
             buffer = buffer == BUFFERS - 1 ? 0 : buffer + 1;
         }
     }
