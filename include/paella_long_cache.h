@@ -53,7 +53,7 @@ typedef struct paella_page_select_plan {
  * Bounds have to be those of the keys (paella_page_bounds_launch).  head_dim 64, 128 or 256 (PAELLA_ENOSUP otherwise). */
 int paella_page_select_plan_make(const paella_kv_cache* cache, const paella_kv_batch* batch, int heads, int count, int first, int last, paella_page_select_plan* plan);
 int paella_page_select_dims(const paella_page_select_plan* plan, int stage, paella_launch_dims* dims);
-/* q as for attention; of the cache only the extents are looked at.  pages must not overlap q, bounds or the workspace.  Workspace, stages and queues as for
+/* q as for attention; of the cache only the extents are read.  pages and the workspace must not overlap q, bounds, the cache, the batch's tensors or each other.  Workspace, stages and queues as for
  * paella_prefix_attention_launch. */
 int paella_page_select_launch(const paella_page_select_plan* plan, const paella_kv_cache* cache, const paella_kv_batch* batch, const void* q, int64_t q_stride,
                               const void* bounds, int32_t* pages, void* workspace, void* stream, uint32_t job_id, void* notifier);

@@ -982,7 +982,9 @@ int paella_page_select_launch_stage(const paella_page_select_plan* p, int stage,
     const double bound_bytes = 2.0 * c->num_pages * c->kv_heads * c->head_dim * size;
     const struct { const void* at; double bytes; } outs[2] = {{pages, out_bytes}, {workspace, space}};
     for (const auto& o : outs)
-        if (rows_overlap(q, p->tokens, q_stride * size, row * size, o.at, o.bytes) || overlap(bounds, bound_bytes, o.at, o.bytes) || over_batch(b, c->page_size, o.at, o.bytes)) return PAELLA_EINVAL;
+        if (rows_overlap(q, p->tokens, q_stride * size, row * size, o.at, o.bytes) || overlap(bounds, bound_bytes, o.at, o.bytes) || over_cache(c, o.at, o.bytes) ||
+            over_batch(b, c->page_size, o.at, o.bytes))
+            return PAELLA_EINVAL;
     if (overlap(pages, out_bytes, workspace, space)) return PAELLA_EINVAL;
     SelectArgs a;
     a.q = (const char*)q; a.bounds = (const char*)bounds;
