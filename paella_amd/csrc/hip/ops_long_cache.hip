@@ -869,8 +869,9 @@ int64_t evict_slices(int sequences, const paella_kv_cache* c) {
 int evict_check(const paella_kv_evict_desc* d, const paella_kv_cache* c) {
     if (!d || !cache_extents_ok(c) || d->sequences <= 0 || d->max_pages <= 0 || d->keep <= 0 || d->first < 0 || d->recent < 0 || (int64_t)d->first + d->recent > d->keep) return PAELLA_EINVAL;
     const double heads = (double)d->sequences * c->kv_heads;
-    if ((double)d->max_pages * c->page_size >= 1073741824.0 || heads * evict_slices(d->sequences, c) > kMostWorkgroups || (double)d->sequences * d->max_pages >= 2147483648.0) return PAELLA_ENOSUP;
-    return 0;
+    if ((double)d->max_pages * c->page_size >= 1073741824.0 || (double)d->sequences * d->max_pages >= 2147483648.0) return PAELLA_ENOSUP;
+    const double picking = heads * evict_pick((int64_t)d->max_pages * c->page_size).threads / 256, moving = heads * evict_slices(d->sequences, c);
+    return picking <= kMostWorkgroups && moving <= kMostWorkgroups ? 0 : PAELLA_ENOSUP;
 }
 
 // ------------------------------------------------------------------------------------------ the weights of stored scores (long_attention.h)

@@ -1,5 +1,7 @@
 """What the entry points over long caches refuse, beyond test_long_cache_cpu.py: nothing here is launched."""
-from test_long_cache_cpu import CACHE_BYTES, CALLS, EINVAL, K, V, lib  # noqa: F401  (lib: a fixture)
+import ctypes
+
+from test_long_cache_cpu import AT, CACHE_BYTES, CALLS, EINVAL, ENOSUP, K, V, cache, evict, lib, refs  # noqa: F401  (lib: a fixture)
 
 
 def test_selections_over_the_cache(lib):  # noqa: F811
@@ -10,3 +12,18 @@ def test_selections_over_the_cache(lib):  # noqa: F811
         for name, extent in sizes.items():
             for over in (base, base + CACHE_BYTES - 16, base - (extent + 15) // 16 * 16 + 16):
                 assert call(**{name: over}) == EINVAL, (name, base // AT)
+
+
+def test_evictions_of_more_threads_than_a_launch_has(lib):  # noqa: F811
+    """Histories of thousands of tokens are picked from by 1024 threads a head, of which 2^32 are more than the runtime counts; the same heads with short ones are not."""
+    from paella_amd import _abi
+    from paella_amd._abi_long import KvEvictDesc
+    c, d = cache(heads=8), _abi.LaunchDims()
+    for tokens, most in ((1024, 16777215 // 3 // 8), (1040, 16777215 // 4 // 8), (2400, 16777215 // 4 // 8), (20000, 16777215 // 4 // 8)):
+        for sequences, want in ((most, 0), (most + 1, ENOSUP), (550000, 0 if most >= 550000 else ENOSUP)):
+            for stage in (0, 1):
+                desc = KvEvictDesc(sequences, tokens // 16, 100, 0, 0)
+                got = lib.paella_kv_evict_dims(*refs(desc, c), stage, ctypes.byref(d))
+                assert got == want and (got or d.grid * d.block < 2 ** 32), (tokens, sequences, stage, d.grid, d.block)
+            if want:
+                assert evict(lib, c=c, sequences=sequences, max_pages=tokens // 16, keep=100) == ENOSUP
