@@ -792,6 +792,7 @@ BoundsKernel bounds_kernel(const paella_kv_cache* c) {
 
 int bounds_check(const paella_kv_cache* c, const paella_kv_batch* b) {
     if (!cache_extents_ok(c) || !batch_extents_ok(b)) return PAELLA_EINVAL;
+    if ((double)b->max_pages * c->page_size >= 1073741824.0) return PAELLA_ENOSUP;
     return (double)b->sequences * bounds_grid(c, b).touched * c->kv_heads / 4 <= kMostWorkgroups - 1 ? 0 : PAELLA_ENOSUP;
 }
 

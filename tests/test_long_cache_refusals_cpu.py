@@ -1,7 +1,7 @@
 """What the entry points over long caches refuse, beyond test_long_cache_cpu.py: nothing here is launched."""
 import ctypes
 
-from test_long_cache_cpu import AT, CACHE_BYTES, CALLS, EINVAL, ENOSUP, K, V, cache, evict, lib, refs  # noqa: F401  (lib: a fixture)
+from test_long_cache_cpu import AT, CACHE_BYTES, CALLS, EINVAL, ENOSUP, K, V, batch, bounds, cache, evict, lib, refs  # noqa: F401  (lib: a fixture)
 
 
 def test_selections_over_the_cache(lib):  # noqa: F811
@@ -27,3 +27,14 @@ def test_evictions_of_more_threads_than_a_launch_has(lib):  # noqa: F811
                 assert got == want and (got or d.grid * d.block < 2 ** 32), (tokens, sequences, stage, d.grid, d.block)
             if want:
                 assert evict(lib, c=c, sequences=sequences, max_pages=tokens // 16, keep=100) == ENOSUP
+
+
+def test_bounds_of_tables_of_2_to_the_30_tokens(lib):  # noqa: F811
+    """Refused as by the other operators that work on the same batch."""
+    from paella_amd import _abi
+    d = _abi.LaunchDims()
+    for size, pages, want in ((8, (1 << 27) - 1, 0), (8, 1 << 27, ENOSUP), (8, 1 << 28, ENOSUP), (16, (1 << 26) - 1, 0), (16, 1 << 26, ENOSUP)):
+        c, b = cache(size=size), batch(sequences=1, max_pages=pages)
+        assert lib.paella_page_bounds_dims(*refs(c, b), ctypes.byref(d)) == want, (size, pages)
+        if want:
+            assert bounds(lib, c=c, b=b) == want
