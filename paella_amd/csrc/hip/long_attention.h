@@ -191,6 +191,7 @@ struct WeighArgs {
     f32x2* ml;         // [splits][tokens * heads]: maximum and sum of each part
     float* scores;     // q . k: [sequences][kv_heads][score_rows][max_pages * page_size], -inf where a row does not see the token
     int score_rows;
+    float* sums;       // what a call's rows so far give each token, where a workgroup takes them through in several chunks: [sequences][kv_heads][max_pages * page_size]
     uint32_t job_id;
     Notifier* notifier;
 };
@@ -548,7 +549,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 3) void key_weights_kernel(Weigh
         const int before = a.prefix_pages * a.page_size / Walk::STEP, steps = (a.prefix_pages * a.page_size + held + Walk::STEP - 1) / Walk::STEP - before;
         const int per = (int)divide((unsigned)steps + a.own_splits.d - 1, a.own_splits).q;
         const int begin = before + min(split * per, steps), end = min(begin + per, before + steps);
-        float* const weights = a.weights + ((size_t)seq * a.kv_heads.d + h) * ((size_t)a.max_pages * a.page_size);
+        const size_t head_at = ((size_t)seq * a.kv_heads.d + h) * ((size_t)a.max_pages * a.page_size);
+        float *const weights = a.weights + head_at, *const sums = a.sums + head_at;
         Walk walk = key_walk<T, D>(a, seq, h);
         for (int first_row = 0; first_row < rows && begin < end; first_row += TILES * 16) {
             walk.start(begin + wave, lane);
@@ -583,9 +585,12 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 3) void key_weights_kernel(Weigh
                         w[e] = 0.f;
                     }
                     const int i = first + (lane >> 4) * Walk::TPL + (lane & 15) - a.prefix_pages * a.page_size;
+                    // The call's sum by itself until it is whole: a heavy old weight would take a rounding of its own size from each part of it.
                     if ((lane & 15) < Walk::TPL && i >= 0 && i < held) {
-                        const float old = first_row || i < past ? __hip_atomic_load(weights + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.f;
-                        store_out(weights + i, old + mine);
+                        auto at = [](const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+                        const float sum = first_row ? at(sums + i) + mine : mine;
+                        if (first_row + TILES * 16 < rows) store_out(sums + i, sum);
+                        else store_out(weights + i, i < past ? at(weights + i) + sum : sum);
                     }
                 });
         }

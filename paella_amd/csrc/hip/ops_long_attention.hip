@@ -78,7 +78,9 @@ bool plan_ok(const WeighPlan* p) {
 
 size_t parts_of(const WeighPlan* p) { return up256((size_t)p->splits * p->tokens * p->heads * 8); }
 int score_rows(const WeighPlan* p) { return few_rows(p) ? std::min(p->max_new, p->tokens) * (p->heads / p->kv_heads) : 0; }
-size_t workspace_of(const WeighPlan* p) { return parts_of(p) + (size_t)p->sequences * p->kv_heads * score_rows(p) * p->max_pages * p->page_size * 4; }
+// Floats that are kept of an own token: its scores, or the sum over the rows so far.
+int kept_of(const WeighPlan* p) { return few_rows(p) ? score_rows(p) : chunks_of(p) > 1 ? 1 : 0; }
+size_t workspace_of(const WeighPlan* p) { return parts_of(p) + (size_t)p->sequences * p->kv_heads * kept_of(p) * p->max_pages * p->page_size * 4; }
 
 }  // namespace
 
@@ -214,7 +216,7 @@ int paella_key_weights_launch_stage(const paella_key_weights_plan* p, int stage,
     a.kv_heads = divisor((unsigned)p->kv_heads); a.per_kv = divisor((unsigned)(p->heads / p->kv_heads)); a.page_blocks = divisor((unsigned)c->page_size / 8);
     a.splits = divisor((unsigned)p->splits); a.own_splits = divisor((unsigned)p->own_splits); a.chunks = divisor((unsigned)chunks_of(p));
     a.scale_log2 = p->scale * 1.44269504088896340736f; a.rise = kRise / a.scale_log2; a.ml = (f32x2*)workspace;
-    a.scores = (float*)((char*)workspace + parts_of(p)); a.score_rows = score_rows(p);
+    a.scores = a.sums = (float*)((char*)workspace + parts_of(p)); a.score_rows = score_rows(p);
     a.job_id = job_id; a.notifier = (Notifier*)notifier;
     launch(kernel_of(p, stage), dim3((unsigned)grid_of(p, stage)), dim3(256), 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();

@@ -6,7 +6,7 @@ import torch
 
 import _decode_ref as ref
 import _long_ref as long_ref
-from test_decode_gpu import BF16, F16, within
+from test_decode_gpu import BF16, F16, F32, within
 from test_long_cache_gpu import Case, lists
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +28,24 @@ def test_attention_over_pages_is_off_by_its_own_rounding(cuda, dtype, dim):
     largest = c.v[~c.v.isnan()].abs().max().item()
     tiny = 2.0 ** -25 + 2.0 ** -36 * most * largest if dtype == F16 else 0.0
     within(out, want, half * want.abs() + (2 * half ** 2 + 2.0 ** -24 * (2 * dim * products[..., None] + 2 * most + 64)) * weight * 1.01 + tiny)
+
+
+@pytest.mark.parametrize("case", [(F32, 4, 256, 64), (BF16, 8, 128, 70), (F16, 8, 64, 40)], ids=lambda c: str(c[0])[6:])
+def test_a_heavy_old_weight_is_rounded_once(cuda, case):
+    """Many rows, which are taken through in several chunks, each of which gives a token less than half a step of what it weighs already: half a step of the result, and the error of the call's own sum."""
+    from paella_amd import long_cache
+    dtype, heads, dim, new = case
+    c = Case(dim + 1, dtype, 1, dim, 16, [100, 70], new, prefix=20)
+    cache, batch = c.to(cuda)
+    q = c.queries(heads, scale=0.3)
+    places = c.tables.shape[1] * 16
+    nothing = torch.zeros((2, 1, places))
+    old = nothing + 2.0 ** 24
+    weights = old.to(cuda)
+    long_cache.KeyWeights(heads, cache, batch)(q.to(cuda), cache, batch, weights)
+    want, error = long_ref.weigh(c.host, q, c.k, nothing, 1 / math.sqrt(dim))
+    for b, past in enumerate(c.past):
+        assert want[b, :, :past].min() > 1.0   # half a step of the old weight
+        want[b, :, :past] += old[b, :, :past]
+        want[b, :, past + new:] = old[b, :, past + new:]
+    within(weights, want, error + 2.0 ** -24 * want.abs())
