@@ -43,6 +43,7 @@ typedef struct paella_page_select_plan {
     int splits;                  /* workgroups that share a row's pages */
     int stages;                  /* launches of a call */
     size_t workspace_bytes;
+    size_t zero_bytes;           /* the first bytes of the workspace that have to be 0 ahead of its first call; what the others hold does not matter */
     paella_launch_dims dims;
     double flops, bytes;         /* algorithmic, every sequence as long as its table */
 } paella_page_select_plan;
@@ -53,8 +54,8 @@ typedef struct paella_page_select_plan {
  * Bounds have to be those of the keys (paella_page_bounds_launch).  head_dim 64, 128 or 256 (PAELLA_ENOSUP otherwise). */
 int paella_page_select_plan_make(const paella_kv_cache* cache, const paella_kv_batch* batch, int heads, int count, int first, int last, paella_page_select_plan* plan);
 int paella_page_select_dims(const paella_page_select_plan* plan, int stage, paella_launch_dims* dims);
-/* q as for attention; of the cache only the extents are read.  pages and the workspace must not overlap q, bounds, the cache, the batch's tensors or each other.  Workspace, stages and queues as for
- * paella_prefix_attention_launch. */
+/* q as for attention; of the cache only the extents are read.  pages and the workspace must not overlap q, bounds, the cache, the batch's tensors or each other.  Stages and queues as for
+ * paella_prefix_attention_launch, and the workspace but for the plan's zero_bytes, here and below. */
 int paella_page_select_launch(const paella_page_select_plan* plan, const paella_kv_cache* cache, const paella_kv_batch* batch, const void* q, int64_t q_stride,
                               const void* bounds, int32_t* pages, void* workspace, void* stream, uint32_t job_id, void* notifier);
 int paella_page_select_launch_stage(const paella_page_select_plan* plan, int stage, const paella_kv_cache* cache, const paella_kv_batch* batch, const void* q,
@@ -70,6 +71,7 @@ typedef struct paella_page_attention_plan {
     int splits;                  /* workgroups that share a list */
     int stages;                  /* 2 where their parts are joined by a launch of its own */
     size_t workspace_bytes;      /* 0 where one workgroup does a list */
+    size_t zero_bytes;
     paella_launch_dims dims;
     double flops, bytes;         /* algorithmic, lists full and of different pages */
 } paella_page_attention_plan;
@@ -93,6 +95,7 @@ typedef struct paella_key_weights_plan {
     int splits, own_splits;      /* workgroups that share a sequence's keys in the first and in the second stage */
     int stages;
     size_t workspace_bytes;
+    size_t zero_bytes;
     paella_launch_dims dims;
     double flops, bytes;
 } paella_key_weights_plan;

@@ -8,7 +8,7 @@ c_int, c_float, c_double, c_void_p, c_size_t, c_u32, c_i64 = (ctypes.c_int, ctyp
                                                               ctypes.c_uint32, ctypes.c_int64)
 
 _EXTENTS = [(n, c_int) for n in ("dtype", "heads", "kv_heads", "head_dim", "page_size", "sequences", "max_new", "tokens", "max_pages", "prefix_len")]
-_COSTS = [("workspace_bytes", c_size_t), ("dims", LaunchDims), ("flops", c_double), ("bytes", c_double)]
+_COSTS = [("workspace_bytes", c_size_t), ("zero_bytes", c_size_t), ("dims", LaunchDims), ("flops", c_double), ("bytes", c_double)]
 
 
 class PageSelectPlan(ctypes.Structure):

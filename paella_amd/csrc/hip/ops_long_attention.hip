@@ -103,6 +103,7 @@ int paella_page_attention_plan_make(const paella_kv_cache* c, const paella_kv_ba
     if (!plan_ok(p)) return PAELLA_ENOSUP;
     p->stages = stages_of(p);
     p->workspace_bytes = workspace_of(p);
+    p->zero_bytes = p->workspace_bytes ? counters_of(p) : 0;
     set_launch_dims(&p->dims, (unsigned)grid_of(p), 256, 0, 256);
     const double size = element_bytes(c->dtype), rows = (double)p->tokens * p->kv_heads;
     p->flops = 4.0 * p->head_dim * p->tokens * heads * (double)keys;

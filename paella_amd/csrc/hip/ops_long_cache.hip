@@ -959,6 +959,7 @@ int paella_page_select_plan_make(const paella_kv_cache* c, const paella_kv_batch
     if (!select_plan_ok(p)) return PAELLA_ENOSUP;
     p->stages = select_stages(p);
     p->workspace_bytes = select_workspace(p);
+    p->zero_bytes = select_counters(p);
     set_launch_dims(&p->dims, (unsigned)screen_grid(p), 256, 0, 128);
     const double size = element_bytes(c->dtype);
     p->flops = 4.0 * p->tokens * p->heads * pages * p->head_dim;

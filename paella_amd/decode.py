@@ -97,13 +97,14 @@ def _unpark(stream):
 
 
 class _Workspaces:
-    """Scratch memory of a plan that starts out zeroed, one per stream, so that calls on different streams do not meet in it.  On a queue that keeps no order, a call that
+    """Scratch memory of a plan whose first `zeroed` bytes (all of them unless said) start out zeroed, one per stream, so that calls on different streams do not meet in it.  On a queue that keeps no order, a call that
     finds it in use waits for the queue first.  A call under graph capture gets one of its own in the graph's memory: graphs that were captured from one plan may run at once.
     The stages of a call that is issued stage by stage meet in the workspace of their stream.  Where there is none that both would find, or none that a captured call may have,
     calls are refused without one of the caller's."""
 
-    def __init__(self, nbytes, stages=1):
+    def __init__(self, nbytes, stages=1, zeroed=None):
         self.nbytes = nbytes
+        self.zeroed = zeroed  # (under graph capture each fill is a launch of every replay, by as many bytes as it fills)
         self.stages = stages
         self.of_stream = {}
         self.foreign = {}   # what those streams are that torch did not allocate the workspace for
@@ -112,7 +113,12 @@ class _Workspaces:
         self.lock = threading.RLock()  # held over a call of two launches: another thread's on the same stream would come between them
 
     def new(self, device):
-        return torch.zeros(self.nbytes // 4 + 1, dtype=torch.int32, device=device)
+        if self.zeroed is None:
+            return torch.zeros(self.nbytes // 4 + 1, dtype=torch.int32, device=device)
+        w = torch.empty(self.nbytes // 4 + 1, dtype=torch.int32, device=device)
+        if self.zeroed:
+            w[:self.zeroed // 4].zero_()
+        return w
 
     def given(self, workspace):
         """Address of a caller's workspace."""

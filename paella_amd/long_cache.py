@@ -67,10 +67,10 @@ class _Planned:
         check(getattr(self.lib, "paella_%s_plan_make" % name)(cache.ref, batch.ref, *args, self._ref), "paella_%s_plan_make" % name)
         self._dims = getattr(self.lib, "paella_%s_dims" % name)
         self._whole, self._stage = getattr(self.lib, self._name), getattr(self.lib, self._name + "_stage")
-        self.workspaces = _Workspaces(plan.workspace_bytes, plan.stages)
+        self.workspaces = _Workspaces(plan.workspace_bytes, plan.stages, plan.zero_bytes)
 
     def new_workspace(self, device="cuda"):
-        """Scratch memory for one call at a time, zero-filled on the current torch stream; a call leaves it ready for the next."""
+        """Scratch memory for one call at a time of this plan, made ready (plan.zero_bytes of it zeroed) on the current torch stream; a call leaves it ready for the next."""
         return self.workspaces.new(device)
 
     def dims(self, stage=0):
