@@ -103,7 +103,8 @@ typedef struct paella_key_weights_plan {
 /* weights [sequences][kv_heads][max_pages * page_size], float, on a 16-byte boundary: to each own token i of a sequence is added sum softmax_i(scale * q[t][h] . k) over the sequence's new tokens t that
  * see it and the query heads h of the key head, the softmax taken over the prefix and the own tokens that t sees.  The sequence's new tokens (i >= past) start from 0 whatever was there; places behind them, and all of a sequence
  * without new tokens, are left as they were.  Everything is kept in 32 bits; sums are taken in the same order in every run, and
- * the old weight is added once, to the sum of the call's.  The workspace holds the scores of a sequence's own tokens where it has 16 rows (new tokens by heads of a key head) at most, and those sums where it has many.  head_dim 64, 128 or 256. */
+ * the old weight is added once, to the sum of the call's.  The workspace holds the scores of all own tokens where a sequence has 16 rows (new tokens by heads of a key head)
+ * at most and they are 1 GB at most by the tables' width, and those sums, 4 bytes a place, where it has many.  head_dim 64, 128 or 256. */
 int paella_key_weights_plan_make(const paella_kv_cache* cache, const paella_kv_batch* batch, int heads, float scale, paella_key_weights_plan* plan);
 int paella_key_weights_dims(const paella_key_weights_plan* plan, int stage, paella_launch_dims* dims);
 int paella_key_weights_launch(const paella_key_weights_plan* plan, const paella_kv_cache* cache, const paella_kv_batch* batch, const void* q, int64_t q_stride,

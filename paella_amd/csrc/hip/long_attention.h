@@ -179,7 +179,7 @@ PageAttentionKernel page_attention_kernel_of(int dim) {
 // ------------------------------------------------------------------------------------------ the weight that tokens gather
 // weights[i] += sum over rows r of exp2(x_ri - m_r) / l_r, x = scale q . k in powers of two.  A first launch leaves each row's maximum and sum over its part of the keys, a second one
 // puts the parts together and adds the rows' weights up, key by key.  A wave has a step's keys in registers and takes the rows through, 16 at a time, from LDS.  Where a key head has 16 rows at most, as
-// in a step of single tokens, memory bounds both: the first launch leaves the scores, too, a sixteenth of what the keys are, and the second reads those instead of the keys.
+// in a step of single tokens, memory bounds both: the first launch leaves the scores, too, 4 bytes a row and key, and the second reads those instead of the keys.
 struct WeighArgs {
     const char *q, *k_cache;
     float* weights;

@@ -50,10 +50,14 @@ size_t workspace_of(const PagePlan* p) {
 
 using WeighPlan = paella_key_weights_plan;
 
-// Scores are stored by 32-bit offsets.
+// Few rows: the first pass stores the scores, which the second one reads in place of the keys.  That pays while a token's scores, written and read, 8 bytes a row, are less than its key, and costs nothing where they
+// are as much: a tile of 16 rows and a key of 128 bytes.  (32 sequences of 4096 to 8192 tokens, 8 key heads, stored / keys read again, us: bf16 heads of 64, 4 / 8 / 16 rows 48 / 56 / 77, 77; of 128 99 / 105 / 119,
+// 147; of 256 180 / 185 / 200, 309; fp32 heads of 64 95 / 103 / 124, 187; of 256 322 / 337 / 357, 653.  A small call, 4 bf16 sequences of 4096 tokens of 2 heads of 64, 16 rows, 12.0 / 11.5.)  Scores go by the
+// tables' width, the plan not knowing the lengths, and each stream that the plan is used on has its own: up to 1 GB in all, where 32 sequences of 65536 tokens, 16 rows of bf16 heads of 128, take 970 / 1252.
+constexpr double kMostScores = 1073741824.0;
 bool few_rows(const WeighPlan* p) {
     const int64_t rows = (int64_t)std::min(p->max_new, p->tokens) * (p->heads / p->kv_heads);
-    return rows <= 16 && (double)rows * p->max_pages * p->page_size < 1073741824.0 / 2;
+    return rows <= 16 && 4.0 * p->sequences * p->kv_heads * (double)rows * p->max_pages * p->page_size <= kMostScores;
 }
 int chunk_rows(const WeighPlan* p) {
     if (few_rows(p)) return 16;
@@ -78,7 +82,7 @@ bool plan_ok(const WeighPlan* p) {
 
 size_t parts_of(const WeighPlan* p) { return up256((size_t)p->splits * p->tokens * p->heads * 8); }
 int score_rows(const WeighPlan* p) { return few_rows(p) ? std::min(p->max_new, p->tokens) * (p->heads / p->kv_heads) : 0; }
-// Floats that are kept of an own token: its scores, or the sum over the rows so far.
+// Floats that are kept of an own token: its scores, or the sum over the rows so far (as much memory as the weights themselves).
 int kept_of(const WeighPlan* p) { return few_rows(p) ? score_rows(p) : chunks_of(p) > 1 ? 1 : 0; }
 size_t workspace_of(const WeighPlan* p) { return parts_of(p) + (size_t)p->sequences * p->kv_heads * kept_of(p) * p->max_pages * p->page_size * 4; }
 
@@ -178,6 +182,8 @@ int paella_key_weights_plan_make(const paella_kv_cache* c, const paella_kv_batch
     // Few rows: memory bounds it, and parts are as many as even out the sequences' lengths (32 sequences of 8192 to 16384 tokens of 8 heads of 128 in bf16 in 16 / 32 / 48 / 64 parts 181 / 174 / 177 / 182 us).
     // Many rows: as many workgroups as the device holds at once, two to a compute unit in the first stage (4 sequences, 128 rows over 17000 keys of 8 heads, in 12 / 16 / 24 parts 35 / 29 / 45 us) and three
     // in the second.
+    // The second pass over stored scores: eight workgroups to a compute unit, of 1024 tokens at least (64 sequences of 2048 to 4096 tokens, 16 rows, 8 heads by 1024 / 2048 / 4096 workgroups 80.2 / 77.4 / 77.5 us for
+    // the call; 2 of 60000 tokens, 8 rows, one head, by 512 / 1024 / 2048 tokens 19.9 / 20.2 / 21.7, 3 of 900 9.8 / 9.4 / 9.6).
     const bool few = few_rows(p);
     p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(few ? 8192 : 512, sums), ceil_div(keys, 256), 64}));
     p->own_splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(few ? 2048 : 768, weights), ceil_div(own, few ? 1024 : 256)));

@@ -46,3 +46,14 @@ def test_plans_say_what_has_to_be_zero(lib, dtype):  # noqa: F811
         assert p.zero_bytes % 4 == 0
     whole = attend_plan(lib, c, batch(sequences=500, max_pages=4), count=4)[1]
     assert (whole.workspace_bytes, whole.zero_bytes) == (0, 0)
+
+
+@pytest.mark.parametrize("dtype, dim", [(1, 64), (2, 128), (0, 256)])
+def test_key_weights_of_wide_tables_keep_a_bounded_workspace(lib, dtype, dim):  # noqa: F811
+    """Scores are stored for few rows up to 1 GB by the tables' width; beyond it a call keeps each row's sums alone, as with many rows."""
+    c = cache(dtype=dtype, heads=8, dim=dim, size=64, pages=100)
+    for sequences, rows, pages in ((32, 16, 1024), (32, 16, 2048), (32, 4, 1024), (1, 16, 1 << 15), (500, 1, 4096), (2, 8, 200000)):
+        rc, p = weigh_plan(lib, c, batch(sequences=sequences, max_new=1, max_pages=pages), 8 * rows)
+        scores = sequences * 8 * rows * pages * 64 * 4
+        sums = p.splits * sequences * 8 * rows * 8
+        assert rc == 0 and p.workspace_bytes == -(-sums // 256) * 256 + (scores if scores <= 1 << 30 else 0), (sequences, rows, pages)
