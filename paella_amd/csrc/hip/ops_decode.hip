@@ -789,7 +789,7 @@ int paella_kv_append_at_launch(const paella_kv_append_desc* d, const paella_kv_c
                                const void* v, const float* q_weight, const float* k_weight, const float* inv_freq, void* q_out, void* stream,
                                uint32_t job_id, void* notifier) {
     if (int rc = append_check(d, c, b)) return rc;
-    if (!cache_ok(c) || !batch_ok(b) || !k || !v || (d->heads > 0) != (q != nullptr) || (d->heads > 0) != (q_out != nullptr)) return PAELLA_EINVAL;
+    if (!cache_ok(c) || !batch_ok(b) || !k || !v || (d->heads > 0) != (q != nullptr) || (d->heads > 0) != (q_out != nullptr) || ((uintptr_t)positions & 3)) return PAELLA_EINVAL;
     if (d->rotary_dim && !inv_freq) return PAELLA_EINVAL;
     const int64_t size = element_bytes(c->dtype), kv_row = (int64_t)c->kv_heads * c->head_dim, q_row = (int64_t)d->heads * c->head_dim;
     if (d->k_stride < kv_row || d->v_stride < kv_row || d->k_stride % 8 || d->v_stride % 8) return PAELLA_EINVAL;

@@ -1033,6 +1033,7 @@ int paella_kv_evict_launch_stage(const paella_kv_evict_desc* d, int stage, const
                                  int32_t* past_out, void* stream, uint32_t job_id, void* notifier) {
     if (int rc = evict_check(d, c)) return rc;
     if (stage < 0 || stage > 1 || !cache_ok(c) || !weights || !past || !tables || !kept || !past_out) return PAELLA_EINVAL;
+    if (((uintptr_t)weights | (uintptr_t)past | (uintptr_t)tables | (uintptr_t)kept | (uintptr_t)past_out) & 3) return PAELLA_EINVAL;
     const double heads = (double)d->sequences * c->kv_heads, kept_bytes = heads * d->keep * 4, weight_bytes = heads * d->max_pages * c->page_size * 4;
     const double table_bytes = (double)d->sequences * d->max_pages * 4, past_bytes = (double)d->sequences * 4;
     const struct { const void* at; double bytes; } outs[3] = {{kept, kept_bytes}, {past_out, past_bytes}, {weights, weight_bytes}};

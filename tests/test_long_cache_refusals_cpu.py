@@ -1,7 +1,8 @@
 """What the entry points over long caches refuse, beyond test_long_cache_cpu.py: nothing here is launched."""
 import ctypes
 
-from test_long_cache_cpu import AT, CACHE_BYTES, CALLS, EINVAL, ENOSUP, K, V, batch, bounds, cache, evict, lib, refs  # noqa: F401  (lib: a fixture)
+from test_long_cache_cpu import (AT, CACHE_BYTES, CALLS, EINVAL, ENOSUP, K, KEPT, LENGTHS, OUT, PAGES, PAST, Q, TABLES, V, WEIGHTS, batch, bounds, cache, evict, lib,  # noqa: F401  (lib: a fixture)
+                                 refs)
 
 
 def test_selections_over_the_cache(lib):  # noqa: F811
@@ -38,3 +39,15 @@ def test_bounds_of_tables_of_2_to_the_30_tokens(lib):  # noqa: F811
         assert lib.paella_page_bounds_dims(*refs(c, b), ctypes.byref(d)) == want, (size, pages)
         if want:
             assert bounds(lib, c=c, b=b) == want
+
+
+def test_numbers_that_begin_inside_a_word(lib):  # noqa: F811
+    """Lengths, tables, lists, weights and positions are read and written by words."""
+    from paella_amd._abi_decode import KvAppendDesc
+    for name, at in (("weights", WEIGHTS), ("past", PAST), ("tables", TABLES), ("kept", KEPT), ("past_out", LENGTHS)):
+        for off in (1, 2, 3):
+            for stage in (None, 0, 1):
+                assert evict(lib, **{name: at + off}, stage=stage) == EINVAL, (name, off, stage)
+    d = KvAppendDesc(4, 64, 0, 1e-6, 256, 128, 128)
+    for off in (1, 2, 3):
+        assert lib.paella_kv_append_at_launch(ctypes.byref(d), *refs(cache(), batch()), KEPT + off, Q, OUT, OUT + AT // 2, None, None, WEIGHTS, PAGES, None, 0, None) == EINVAL, off
