@@ -73,7 +73,7 @@ struct ListWalk : NarrowWalk<T, D> {
                 }
         }
         // In two parts, so that results are off by little more than their own rounding: memory bounds the walk, and the second product's units have room.  (One / two parts: 64 bf16 lists of 4096 tokens of 8
-        // heads of 128 179.8 / 179.9 us, 30 fp16 ones of 1600 20.2 / 20.3.)
+        // heads of 128 179.8 / 179.9 us, 30 fp16 ones of 1600 20.2 / 20.3, 3 of 256 tokens of 2 heads of 256 8.6 / 9.0.)
         unsigned p[F ? 1 : 2][1][4];
         rows.weigh(x, scale, p);
         rows.add_values(this->v, p);
@@ -560,6 +560,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 3) void key_weights_kernel(Weigh
             join_rows<TILES * 16>(a, its.first, h, first_row, rows, whole);
             staged.put(q);
             __syncthreads();
+            const bool whole_call = first_row + TILES * 16 >= rows;
+            float* const to = whole_call ? weights : sums;
             float w[Walk::TPL];
 #pragma unroll
             for (int e = 0; e < Walk::TPL; ++e) w[e] = 0.f;
@@ -585,12 +587,12 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 3) void key_weights_kernel(Weigh
                         w[e] = 0.f;
                     }
                     const int i = first + (lane >> 4) * Walk::TPL + (lane & 15) - a.prefix_pages * a.page_size;
-                    // The call's sum by itself until it is whole: a heavy old weight would take a rounding of its own size from each part of it.
+                    // The call's sum by itself until it is whole: a heavy old weight would take a rounding of its own size from each part of it.  (A prompt of 2000 tokens, 8000 rows of 8 bf16 heads of 128,
+                    // in 63 chunks: each added to the weight itself / so 542 / 546 us.)
                     if ((lane & 15) < Walk::TPL && i >= 0 && i < held) {
                         auto at = [](const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-                        const float sum = first_row ? at(sums + i) + mine : mine;
-                        if (first_row + TILES * 16 < rows) store_out(sums + i, sum);
-                        else store_out(weights + i, i < past ? at(weights + i) + sum : sum);
+                        const float before = first_row ? at(sums + i) : 0.f, old = whole_call && i < past ? at(weights + i) : 0.f;
+                        store_out(to + i, old + (before + mine));
                     }
                 });
         }
