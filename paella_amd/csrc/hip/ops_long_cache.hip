@@ -501,7 +501,8 @@ __device__ __forceinline__ void pick_pages(const SelectArgs& a, int t, int seq, 
                 __syncthreads();
                 each_open([&](int u, unsigned, unsigned at) { held[u] = s.list[at]; });
             } else {
-                for (unsigned k = threadIdx.x; k < n; k += WAVES * 64) worths[s.list[k]] = s.worth[k];
+                // (through to memory, as all that a kernel here writes: on a direct queue nothing writes a cache back behind it, and the workspace may be another tensor's by the time a line leaves the cache)
+                for (unsigned k = threadIdx.x; k < n; k += WAVES * 64) __hip_atomic_store(worths + s.list[k], s.worth[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 __syncthreads();
             }
         }
